@@ -409,6 +409,66 @@ int moss_advance_step(const void *next_ids, void *ids, void *position, void *aud
                       void *history, void *status, int step, int width, long long audio_start_id,
                       long long gen_slot_id, long long delay_slot_id, void *stream);
 
+/* One index per row of logits (dtype 0 bf16, 1 fp16, 2 fp32; rows `stride` values apart, the first
+ * `vocab` <= 2^19 used) from the row's uniform number u in [0, 1) (uniform fp32 [rows]).  With M the row's
+ * largest logit, w_i = exp((x_i - M) / T) and entries ordered by falling x (ties: lower index first), kept are
+ * the first top_k (<= 0 or >= vocab: all), of those the ones whose predecessors' sum of w is at most top_p times
+ * the sum over those (>= 1: all), and w_i >= min_p (at most 1 is used); drawn is the first kept index i, in
+ * index order, with sum_{j <= i, kept} w_j > u sum_kept w_j.  T <= 0 gives the first of the largest logits; NaN
+ * counts as -inf; a row with nothing above -inf gives -1.  temperature, top_p, min_p (fp32 [rows]) and top_k
+ * (int32 [rows]) are device buffers, or NULL for the value behind each, one for all rows.  out int64 [rows].
+ * Sums are integers (w in units of 2^-44): results do not depend on any order.
+ * A batch's counterpart of moss_sample_topk: any vocabulary, per-row settings, the caller's random numbers. */
+int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, int vocab, const void *uniform,
+                     const void *temperature, float temperature_value, const void *top_k, int top_k_value,
+                     const void *top_p, float top_p_value, const void *min_p, float min_p_value, void *out,
+                     void *stream);
+
+/* ------------------------------------------- a batch over a paged cache */
+/* The single-request operators' counterparts for B sequences whose keys and values lie in pages that they
+ * are handed one by one.  dtype 0 bf16, 1 fp16; head dim d 64 or 128; qh query heads, kh KV heads (qh % kh == 0,
+ * qh <= 1024; query head h reads KV head h / (qh / kh)).
+ *   k, v      [pages, kh, page_rows, d], pages k_stride / v_stride elements apart (a multiple of 8), the rest
+ *             contiguous, 16-byte aligned; page_rows a power of two in [16, 4096]
+ *   table     int32 [B, W], rows table_stride entries apart (W * page_rows <= 2^30): row r of sequence b is row
+ *             r % page_rows of page table[b][r / page_rows]; an entry outside [0, pages) is no page, and its rows
+ *             take no part
+ *   lengths   int32 [B]: rows of each sequence, the new tokens' included (clamped to [0, W * page_rows])
+ *   starts    int32 [B + 1], rising: the packed tokens starts[b] .. starts[b + 1] - 1 are sequence b's newest n, at
+ *             positions lengths[b] - n ..; packed rows from starts[B] on are padding and left alone
+ * Table, lengths and starts are read on the device when the kernels run, so a captured graph follows them; their
+ * contents cannot lead an access outside the cache or the packed rows.  */
+
+/* q/k head RMSNorm (weights [d], or both NULL: no norm) + rotary embedding + page write of T packed tokens:
+ * qkv [T, (qh + 2 kh) d] (q | k | v), rows qkv_stride elements apart; cos / sin [table_rows, d] by position, of the
+ * given dtype or fp32 (table_f32); q_out [T, qh, d].  starts NULL: one token a sequence (T == B).  fp32 from the
+ * inputs to one rounding.  A token whose position is negative, or has no page, is written to no cache row.
+ * Counterpart of moss_qk_norm_rope_kv. */
+int moss_paged_qk_rope(const void *qkv, long long qkv_stride, const void *q_weight, const void *k_weight,
+                       const void *cos, const void *sin, int table_f32, int table_rows, void *q_out, void *k, void *v,
+                       long long k_stride, long long v_stride, int pages, int page_rows, const void *table,
+                       long long table_stride, const void *lengths, const void *starts, int B, int W, int T, int qh,
+                       int kh, int d, float eps, int dtype, void *stream);
+
+/* Attention of one query token per sequence, q [B, qh, d] (rows q_stride elements apart), over its lengths[b] rows:
+ * softmax(scale q k^T) v, out [B, qh * d]; a sequence without rows gives zeros.  The work is shared out evenly
+ * over the device whatever the lengths; the workspace (moss_paged_decode_workspace_bytes, 16-byte aligned) holds
+ * the shares' partial results, and calls that overlap must not share one.  Counterpart of moss_decode_attention. */
+long long moss_paged_decode_workspace_bytes(int B, int W, int page_rows, int qh, int kh, int d);
+int moss_paged_decode_attention(const void *q, long long q_stride, const void *k, const void *v, long long k_stride,
+                                long long v_stride, int pages, int page_rows, const void *table,
+                                long long table_stride, const void *lengths, int B, int W, int qh, int kh, int d,
+                                float scale, void *out, void *workspace, long long workspace_bytes, int dtype,
+                                void *stream);
+
+/* Causal attention of T packed tokens, q [T, qh, d] (rows q_stride elements apart), whose K / V rows are in the pages:
+ * a token attends its sequence's rows up to its own position; out [T, qh * d].  Tokens without a visible row give
+ * zeros.  Counterpart of moss_prefill_attention. */
+int moss_paged_prompt_attention(const void *q, long long q_stride, const void *k, const void *v, long long k_stride,
+                                long long v_stride, int pages, int page_rows, const void *table,
+                                long long table_stride, const void *lengths, const void *starts, int B, int W, int T,
+                                int qh, int kh, int d, float scale, void *out, int dtype, void *stream);
+
 /* ------------------------------------------------------- measurement */
 /* No counterpart in the reference: a streaming read for bench.py, which times it on the bytes of a
  * decode GEMV to measure the ceiling of one launch that only reads those bytes.  Reads `bytes` (a

@@ -1,0 +1,61 @@
+// Where the rows of a paged cache are and how decode work is shared out: the arithmetic of every index that the kernels
+// of the paged operators take from device data, in one place and free of the device, so that it also runs on a host.
+#pragma once
+
+#include <stddef.h>
+
+#if defined(__HIP__)
+#define MOSS_HD __host__ __device__ __forceinline__
+#else
+#define MOSS_HD inline
+#endif
+
+namespace moss {
+
+MOSS_HD int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// Rows of a sequence that the table can hold, whatever the length says (W << shift <= 2^30).
+MOSS_HD int clamp_length(int length, int W, int shift) { return clamp_int(length, 0, W << shift); }
+
+// A table entry as a page, or -1 for none.
+MOSS_HD int page_or_none(int entry, int pages) { return entry >= 0 && entry < pages ? entry : -1; }
+
+// The page of row `row` of a sequence with table row `trow`, or -1: no such row, or no page.
+MOSS_HD int page_of_row(const int* trow, int row, int W, int shift, int pages) {
+    if (row < 0 || (row >> shift) >= W) return -1;
+    return page_or_none(trow[row >> shift], pages);
+}
+
+// Elements from the cache's start to row `row` of a KV head in a page (-1 reads as page 0: its values are not used).
+MOSS_HD size_t row_offset(int page, long long page_stride, int kvh, int row, int shift, int D) {
+    return (size_t)(page < 0 ? 0 : page) * (size_t)page_stride +
+           (((size_t)kvh << shift) + (size_t)(row & ((1 << shift) - 1))) * (size_t)D;
+}
+
+// First packed token and number of tokens of a sequence, inside [0, T] whatever `starts` holds.
+MOSS_HD void clamp_tokens(int s0, int s1, int T, int& first, int& count) {
+    first = clamp_int(s0, 0, T);
+    count = clamp_int(s1, first, T) - first;
+}
+
+// Decode work: rows in units, the units of all sequences in shares of `share` units, at most `shares` of them and one
+// more per sequence; a sequence's units are spread evenly over its own shares.
+constexpr int kUnit = 128;
+MOSS_HD int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
+MOSS_HD int share_of_units(long long total, int shares) {
+    const long long share = total <= shares ? 1 : (total + shares - 1) / shares;
+    return share < (1 << 24) ? (int)share : 1 << 24;  // no sequence has more units
+}
+MOSS_HD int shares_of(int units, int share) { return (units + share - 1) / share; }
+MOSS_HD void share_rows(int rows, int count, int index, int& r0, int& r1) {
+    const int per = (units_of(rows) + count - 1) / count;
+    const long long from = (long long)index * per * kUnit, to = from + (long long)per * kUnit;
+    r0 = from < rows ? (int)from : rows;
+    r1 = to < rows ? (int)to : rows;
+}
+inline long long decode_slots(int B, int W, int shift, int shares) {
+    const long long most = (long long)B * ((((long long)W << shift) + kUnit - 1) / kUnit);
+    return (long long)B + shares < most ? (long long)B + shares : most;
+}
+
+}  // namespace moss

@@ -21,6 +21,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_L = ctypes.c_longlong
 
 # name -> argtypes; every function returns int (hipError_t) unless listed in _RESTYPES.
 SIGNATURES: dict[str, list] = {
@@ -73,12 +74,21 @@ SIGNATURES: dict[str, list] = {
     "moss_compose_next_ids": [_P, _P, _P, _P, _P, ctypes.c_longlong, ctypes.c_longlong, _I, ctypes.c_longlong, _P, _P],
     "moss_advance_step": [_P, _P, _P, _P, _P, _P, _P, _I, _I, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong,
                           _P],
+    "moss_sample_rows": [_P, _I, _I, _L, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P],
+    "moss_paged_qk_rope": [_P, _L, _P, _P, _P, _P, _I, _I, _P, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I,
+                           _I, _F, _I, _P],
+    "moss_paged_decode_workspace_bytes": [_I, _I, _I, _I, _I, _I],
+    "moss_paged_decode_attention": [_P, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _F, _P, _P, _L, _I,
+                                    _P],
+    "moss_paged_prompt_attention": [_P, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _I,
+                                    _P],
     "moss_stream_read_words": [ctypes.c_longlong],
     "moss_stream_read": [_P, ctypes.c_longlong, _P, _P],
 }
 _RESTYPES = {"moss_error_string": ctypes.c_char_p, "moss_gemm_workspace_bytes": ctypes.c_longlong,
              "moss_gemm_silu_workspace_bytes": ctypes.c_longlong,
              "moss_gemm_qk_rope_workspace_bytes": ctypes.c_longlong,
+             "moss_paged_decode_workspace_bytes": ctypes.c_longlong,
              "moss_stream_read_words": ctypes.c_longlong}
 
 
@@ -111,6 +121,17 @@ def check(code: int, what: str) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """:func:`call` with ``t``'s device current and its current stream as the last argument: a kernel
+    starts on the device that is current, whatever device its stream and pointers belong to."""
+    index = t.get_device()
+    if torch._C._cuda_getDevice() == index:
+        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
+        return
+    with torch.cuda.device(index):
+        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
 
 
 def gemm_workspace(m: int, k: int, n: int, device) -> tuple:

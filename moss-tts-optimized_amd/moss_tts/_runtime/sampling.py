@@ -97,6 +97,63 @@ def sample_topk_pair(a: dict, b: dict, *, seed: torch.Tensor, position: torch.Te
                 native.stream_of(a["logits"]))
 
 
+_SAMPLE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_SAMPLE_VOCAB = 1 << 19
+
+
+def _setting(name: str, value, rows: int, dtype: torch.dtype, device):
+    """(pointer, value) of one sampling setting: a device tensor with one value a row, or a number for all."""
+    if isinstance(value, torch.Tensor):
+        _cuda_contig(name, value, dtype, device)
+        _require(value.numel() == rows, f"{name} must hold one value a row")
+        return value.data_ptr(), 0
+    _require(isinstance(value, (int, float)) and not isinstance(value, bool) and value == value,
+             f"{name} must be a number or a tensor")
+    return None, value
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
+           top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+           vocab: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 / fp16 / fp32 logits ``[rows, entries]`` (rows any stride apart) -> int64 indices ``[rows]`` into the
+    first ``vocab`` entries, drawn by the given numbers ``uniform`` fp32 ``[rows]`` in [0, 1).
+
+    Kept are the ``top_k`` largest (0: all; of equal logits the lower index first), of those the ones whose
+    predecessors hold at most the share ``top_p`` of the kept probability (1: all), and those at least
+    ``min_p`` times as probable as the largest.  The draw inverts the cumulative distribution of the kept entries
+    in index order.  ``temperature`` <= 0 takes the first of the largest logits.  NaN counts as ``-inf``; a row
+    with nothing above ``-inf`` gives -1.  Each setting is a number, or a device tensor with one value a row
+    (fp32; ``top_k`` int32) that is read when the kernel runs, so a captured graph serves rows with settings of
+    their own.  Where :func:`sample_topk` draws its own numbers over at most 2048 entries, this takes the
+    caller's, over up to 2^19."""
+    _require(isinstance(logits, torch.Tensor) and logits.dtype in _SAMPLE_TYPES, "logits must be a bf16, fp16 or fp32 tensor")
+    _require(logits.is_cuda, "logits must be a CUDA (HIP) tensor")
+    _require(logits.dim() == 2 and logits.shape[0] > 0 and logits.shape[1] > 0, "logits must be [rows, entries]")
+    rows, entries = logits.shape
+    _require(entries == 1 or logits.stride(1) == 1, "a row's logits must be contiguous")
+    stride = logits.stride(0) if rows > 1 else entries
+    _require(stride >= entries, "rows must not overlap")
+    vocab = entries if vocab is None else int(vocab)
+    _require(0 < vocab <= min(entries, MAX_SAMPLE_VOCAB), f"vocab must be in [1, min(entries, {MAX_SAMPLE_VOCAB})]")
+    dev = logits.device
+    _cuda_contig("uniform", uniform, torch.float32, dev)
+    _require(uniform.numel() == rows, "uniform must hold one number a row")
+    t_ptr, t = _setting("temperature", temperature, rows, torch.float32, dev)
+    k_ptr, k = _setting("top_k", top_k, rows, torch.int32, dev)
+    p_ptr, p = _setting("top_p", top_p, rows, torch.float32, dev)
+    m_ptr, m = _setting("min_p", min_p, rows, torch.float32, dev)
+    _require(int(k) == k and 0 <= k < 1 << 31, "top_k must be a non-negative integer")
+    _require(0 <= p and 0 <= m <= 1, "top_p must not be negative, min_p must lie in [0, 1]")
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+    else:
+        _cuda_contig("out", out, torch.int64, dev)
+        _require(out.numel() == rows, f"out must hold {rows} indices")
+    native.call_on(logits, "moss_sample_rows", logits.data_ptr(), _SAMPLE_TYPES[logits.dtype], rows, stride, vocab,
+                   uniform.data_ptr(), t_ptr, float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m), out.data_ptr())
+    return out
+
+
 def compose_next_ids(text_index: torch.Tensor, audio_index: torch.Tensor, text_ids: torch.Tensor,
                      audio_length: torch.Tensor, delay_length: torch.Tensor, *, delay_slot_id: int,
                      audio_end_id: int, pad_code: int = 1024, out: torch.Tensor | None = None) -> torch.Tensor:
