@@ -417,12 +417,14 @@ int moss_advance_step(const void *next_ids, void *ids, void *position, void *aud
  * index order, with sum_{j <= i, kept} w_j > u sum_kept w_j.  T <= 0 gives the first of the largest logits; NaN
  * counts as -inf; a row with nothing above -inf gives -1.  temperature, top_p, min_p (fp32 [rows]) and top_k
  * (int32 [rows]) are device buffers, or NULL for the value behind each, one for all rows.  out int64 [rows].
- * Sums are integers (w in units of 2^-44): results do not depend on any order.
+ * Sums are integers (w in units of 2^-44): results do not depend on any order.  The workspace
+ * (moss_sample_rows_workspace_bytes, 0 for vocab <= 2048; 16-byte aligned) must not be shared by calls that overlap.
  * A batch's counterpart of moss_sample_topk: any vocabulary, per-row settings, the caller's random numbers. */
+long long moss_sample_rows_workspace_bytes(int rows, int vocab);
 int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, int vocab, const void *uniform,
                      const void *temperature, float temperature_value, const void *top_k, int top_k_value,
                      const void *top_p, float top_p_value, const void *min_p, float min_p_value, void *out,
-                     void *stream);
+                     void *workspace, long long workspace_bytes, void *stream);
 
 /* ------------------------------------------- a batch over a paged cache */
 /* The single-request operators' counterparts for B sequences whose keys and values lie in pages that they

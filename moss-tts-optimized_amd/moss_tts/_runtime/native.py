@@ -74,7 +74,8 @@ SIGNATURES: dict[str, list] = {
     "moss_compose_next_ids": [_P, _P, _P, _P, _P, ctypes.c_longlong, ctypes.c_longlong, _I, ctypes.c_longlong, _P, _P],
     "moss_advance_step": [_P, _P, _P, _P, _P, _P, _P, _I, _I, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong,
                           _P],
-    "moss_sample_rows": [_P, _I, _I, _L, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P],
+    "moss_sample_rows_workspace_bytes": [_I, _I],
+    "moss_sample_rows": [_P, _I, _I, _L, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _L, _P],
     "moss_paged_qk_rope": [_P, _L, _P, _P, _P, _P, _I, _I, _P, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I,
                            _I, _F, _I, _P],
     "moss_paged_decode_workspace_bytes": [_I, _I, _I, _I, _I, _I],
@@ -89,6 +90,7 @@ _RESTYPES = {"moss_error_string": ctypes.c_char_p, "moss_gemm_workspace_bytes": 
              "moss_gemm_silu_workspace_bytes": ctypes.c_longlong,
              "moss_gemm_qk_rope_workspace_bytes": ctypes.c_longlong,
              "moss_paged_decode_workspace_bytes": ctypes.c_longlong,
+             "moss_sample_rows_workspace_bytes": ctypes.c_longlong,
              "moss_stream_read_words": ctypes.c_longlong}
 
 

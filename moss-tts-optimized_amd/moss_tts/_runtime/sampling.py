@@ -112,9 +112,16 @@ def _setting(name: str, value, rows: int, dtype: torch.dtype, device):
     return None, value
 
 
+def sample_workspace(rows: int, vocab: int, device) -> torch.Tensor | None:
+    """A workspace for :func:`sample` calls of up to these sizes (None: none needed); calls that may overlap need one
+    each."""
+    nbytes = native.lib().moss_sample_rows_workspace_bytes(rows, vocab)
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+
+
 def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
            top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
-           vocab: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+           vocab: int | None = None, out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 / fp16 / fp32 logits ``[rows, entries]`` (rows any stride apart) -> int64 indices ``[rows]`` into the
     first ``vocab`` entries, drawn by the given numbers ``uniform`` fp32 ``[rows]`` in [0, 1).
 
@@ -125,7 +132,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     with nothing above ``-inf`` gives -1.  Each setting is a number, or a device tensor with one value a row
     (fp32; ``top_k`` int32) that is read when the kernel runs, so a captured graph serves rows with settings of
     their own.  Where :func:`sample_topk` draws its own numbers over at most 2048 entries, this takes the
-    caller's, over up to 2^19."""
+    caller's, over up to 2^19.  ``ws``: a :func:`sample_workspace`, for callers that keep one."""
     _require(isinstance(logits, torch.Tensor) and logits.dtype in _SAMPLE_TYPES, "logits must be a bf16, fp16 or fp32 tensor")
     _require(logits.is_cuda, "logits must be a CUDA (HIP) tensor")
     _require(logits.dim() == 2 and logits.shape[0] > 0 and logits.shape[1] > 0, "logits must be [rows, entries]")
@@ -149,8 +156,15 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     else:
         _cuda_contig("out", out, torch.int64, dev)
         _require(out.numel() == rows, f"out must hold {rows} indices")
+    if ws is None:
+        ws = sample_workspace(rows, vocab, dev)
+    else:
+        _cuda_contig("ws", ws, torch.float32, dev)
+        _require(4 * ws.numel() >= native.lib().moss_sample_rows_workspace_bytes(rows, vocab) and ws.data_ptr() % 16 == 0,
+                 "workspace too small or not 16-byte aligned")
     native.call_on(logits, "moss_sample_rows", logits.data_ptr(), _SAMPLE_TYPES[logits.dtype], rows, stride, vocab,
-                   uniform.data_ptr(), t_ptr, float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m), out.data_ptr())
+                   uniform.data_ptr(), t_ptr, float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m), out.data_ptr(), None if ws is None else ws.data_ptr(),
+                   0 if ws is None else 4 * ws.numel())
     return out
 
 

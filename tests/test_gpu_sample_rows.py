@@ -70,7 +70,7 @@ def _mixed(rows, g):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [1, 2, 63, 513, 1024, 8191, 9000])
+@pytest.mark.parametrize("vocab", [1, 2, 63, 512, 513, 1024, 2041, 2048, 2049, 4096, 8191, 9000])
 def test_sizes(dev, dtype, vocab):
     g = torch.Generator().manual_seed(vocab)
     _check(_logits(24, vocab, g, dtype, "plain"), torch.rand(24, generator=g), _mixed(24, g), dev)
@@ -78,7 +78,7 @@ def test_sizes(dev, dtype, vocab):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["ties", "equal", "near_zero", "masked"])
-@pytest.mark.parametrize("vocab", [300, 4100])
+@pytest.mark.parametrize("vocab", [300, 1000, 2000, 4100, 30000])
 def test_hard_rows(dev, dtype, kind, vocab):
     g = torch.Generator().manual_seed(1)
     _check(_logits(40, vocab, g, dtype, kind), torch.rand(40, generator=g), _mixed(40, g), dev)
