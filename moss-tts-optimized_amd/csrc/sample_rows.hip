@@ -18,22 +18,22 @@
 // What bounds it: the arithmetic of w in 64 bits for every entry, and, for few rows, the chain of steps.  So a row is
 // read by several workgroups, in five launches (largest logit; histogram; border; weight of each segment of 512 entries;
 // draw), of which the histogram, or the segments' weights, is the one that forms w for every entry: a row without top-k
-// and top-p has no histogram, a row with them few weights in its segments.  w takes one table of 2^(-j / 1024), a
-// cubic and one fma that also rounds: 16 operations.  A row of up to 2048 entries is one wave's: it holds them and their weights in
-// registers, and needs no barrier.
+// and top-p has no histogram, a row with them few weights in its segments.  w takes 14 operations in 64
+// bits, of 8 cycles each for a wave: with a series of ten terms and no table the histograms of 128 rows took 33 us, and
+// with a table of 1024 entries, whose reads the bins' atomics wait for, 27.  A
+// row of up to 2048 entries is one wave's: it holds them and their weights in registers, and needs no barrier.
 #include "common.h"
 
 namespace moss {
 namespace {
 
 constexpr double kOne = 17592186044416.0;  // 2^44: 2^19 entries sum below 2^63
-constexpr int kSteps = 1024;               // steps of z in an octave of w
 constexpr int kSpan = 46;                  // octaves: smaller weights are 0
-constexpr int kBinShift = 5;               // 32 steps a bin
-constexpr int kBins = kSpan * kSteps >> kBinShift;
+constexpr int kBins = 32 * kSpan;          // 32 an octave
 constexpr int kSegment = 512;              // entries
 constexpr int kSmall = 2048;               // entries of a row that one wave takes
 constexpr int kMaxVocab = 1 << 19;
+constexpr int kMaxChunks = 16;             // workgroups that read a row together
 
 struct SampleArgs {
     const void* logits;
@@ -51,47 +51,67 @@ struct SampleArgs {
 
 __device__ __forceinline__ float half_value(uint32_t bits) { return (float)__builtin_bit_cast(_Float16, (uint16_t)bits); }
 
-// Eight logits from index i on, as they are compared: NaN below everything, -0 equal to 0, -inf behind the row's end.
+// Eight logits as they are compared: NaN below everything, -0 equal to 0 (CLEAN false: as they are).
+template <int TYPE, bool CLEAN = true>
+__device__ __forceinline__ void unpack8(const u32x4_t* w, float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (TYPE == 2) {
+            const uint32_t a = w[j / 2][2 * (j & 1)], b = w[j / 2][2 * (j & 1) + 1];
+            x[2 * j] = __uint_as_float(a);
+            x[2 * j + 1] = __uint_as_float(b);
+        } else {
+            const uint32_t word = w[0][j];
+            x[2 * j] = TYPE == 0 ? bf16_lo(word) : half_value(word & 0xffffu);
+            x[2 * j + 1] = TYPE == 0 ? bf16_hi(word) : half_value(word >> 16);
+        }
+    }
+    if constexpr (CLEAN)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = x[j] != x[j] ? -INFINITY : x[j] + 0.0f;
+}
+
+// The ones from index i on; -inf behind the row's end.
 template <int TYPE>
 __device__ __forceinline__ void load8(const void* row, int i, int vocab, bool aligned, float (&x)[8]) {
     if (aligned && i + 8 <= vocab) {
-        if constexpr (TYPE == 2) {
-            const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + i);
-            const float4 a = p[0], b = p[1];
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-            const u32x4_t w = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(row) + i);
+        constexpr int W = TYPE == 2 ? 2 : 1;
+        u32x4_t w[W];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t word = w[j];
-                x[2 * j] = TYPE == 0 ? bf16_lo(word) : half_value(word & 0xffffu);
-                x[2 * j + 1] = TYPE == 0 ? bf16_hi(word) : half_value(word >> 16);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (i + j >= vocab)
-                x[j] = -INFINITY;
-            else if constexpr (TYPE == 0)
-                x[j] = bf16_bits(reinterpret_cast<const uint16_t*>(row)[i + j]);
-            else if constexpr (TYPE == 1)
-                x[j] = (float)reinterpret_cast<const _Float16*>(row)[i + j];
-            else
-                x[j] = reinterpret_cast<const float*>(row)[i + j];
-        }
+        for (int k = 0; k < W; ++k) w[k] = reinterpret_cast<const u32x4_t*>(row)[(size_t)(i / 8) * W + k];
+        unpack8<TYPE>(w, x);
+        return;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = x[j] != x[j] ? -INFINITY : x[j] + 0.0f;
+    for (int j = 0; j < 8; ++j) {
+        if (i + j >= vocab)
+            x[j] = -INFINITY;
+        else if constexpr (TYPE == 0)
+            x[j] = bf16_bits(reinterpret_cast<const uint16_t*>(row)[i + j]);
+        else if constexpr (TYPE == 1)
+            x[j] = (float)reinterpret_cast<const _Float16*>(row)[i + j];
+        else
+            x[j] = reinterpret_cast<const float*>(row)[i + j];
+        x[j] = x[j] != x[j] ? -INFINITY : x[j] + 0.0f;
+    }
 }
 
-// Order-preserving key of a logit.
+// Order-preserving key of a logit; neighbouring values of the type are neighbours (the low bits of an fp32 number that a
+// 16-bit type does not have are left out).
+template <int TYPE>
+constexpr int kLowBits = TYPE == 0 ? 16 : TYPE == 1 ? 13 : 0;
+template <int TYPE>
+constexpr uint32_t kLowest = 0x007fffffu >> kLowBits<TYPE>;  // the key of -inf
+template <int TYPE>
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t b = __float_as_uint(x);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return (b & 0x80000000u ? ~b : b | 0x80000000u) >> kLowBits<TYPE>;
 }
-__device__ __forceinline__ float logit_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-constexpr uint32_t kLowest = 0x007fffffu;  // the key of -inf
+template <int TYPE>
+__device__ __forceinline__ float logit_of(uint32_t k) {
+    const uint32_t b = k << kLowBits<TYPE>;
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~(b | ((1u << kLowBits<TYPE>) - 1)));
+}
 
 // One row's settings, and its largest logit once it is known.
 struct Row {
@@ -102,7 +122,7 @@ struct Row {
     int top_k;
     bool by_k, by_p;
     float top;
-    double rate;  // steps of z per unit of a logit: kSteps log2(e) / T
+    double rate;  // parts of 1/32 octave of w per unit of a logit: 32 log2(e) / T
 };
 
 template <int TYPE>
@@ -111,7 +131,8 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int i) {
     r.at = reinterpret_cast<const unsigned char*>(a.logits) + (size_t)i * a.stride * (TYPE == 2 ? 4 : 2);
     r.vocab = a.vocab;
     r.aligned = MOSS_ALIGNED(r.at, 16);
-    r.temperature = a.temperature ? a.temperature[i] : a.temperature_v;
+    const float t = a.temperature ? a.temperature[i] : a.temperature_v;
+    r.temperature = t > 3.4e38f ? 3.4e38f : t;  // times the distance of an entry of -inf it stays infinite
     r.top_k = a.top_k ? a.top_k[i] : a.top_k_v;
     r.top_p = a.top_p ? a.top_p[i] : a.top_p_v;
     r.min_p = fminf(a.min_p ? a.min_p[i] : a.min_p_v, 1.f);
@@ -121,61 +142,103 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int i) {
 }
 
 // The largest logit with its first index, as one number whose maximum is looked for (0: none).
+template <int TYPE>
 __device__ __forceinline__ unsigned long long top_code(float x, int i) {
-    return ((unsigned long long)key_of(x) << 32) | (uint32_t)~i;
+    return ((unsigned long long)key_of<TYPE>(x) << 32) | (uint32_t)~i;
 }
 // Sets the row's largest logit; false when there is nothing to draw (then `index` is the answer).
+template <int TYPE>
 __device__ __forceinline__ bool take_top(Row& r, unsigned long long code, int& index) {
     const uint32_t k = (uint32_t)(code >> 32);
-    r.top = logit_of(k);
-    index = k > kLowest ? (int)~(uint32_t)code : -1;
-    r.rate = (kSteps * 1.4426950408889634) / (double)r.temperature;
-    return k > kLowest && r.temperature > 0.f;
+    r.top = logit_of<TYPE>(k);
+    index = k > kLowest<TYPE> ? (int)~(uint32_t)code : -1;
+    r.rate = 32.0 * 1.4426950408889634 / (double)r.temperature;
+    return k > kLowest<TYPE> && r.temperature > 0.f;
 }
 
-// How far a logit lies under the largest one, in steps of w (kSpan octaves or more: no weight).
-__device__ __forceinline__ double steps_of(const Row& r, float x) {
-    return x == r.top ? 0.0 : ((double)r.top - (double)x) * r.rate;
+// Eight entries at a time from `begin` to `end`, `step` apart: fn(i, x).  N loads are on their way together.
+template <int TYPE, int N, bool CLEAN = true, typename Fn>
+__device__ __forceinline__ void walk(const Row& r, int begin, int end, int step, Fn fn) {
+    float x[8];
+    if (!r.aligned || r.vocab < 8) {
+        for (int i = begin; i < end; i += step) {
+            load8<TYPE>(r.at, i, r.vocab, false, x);
+            fn(i, x);
+        }
+        return;
+    }
+    constexpr int W = TYPE == 2 ? 2 : 1;
+    const u32x4_t* at = reinterpret_cast<const u32x4_t*>(r.at);
+    const int last = r.vocab / 8 - 1;  // the last whole eight
+    for (int i0 = begin; i0 < end; i0 += N * step) {
+        u32x4_t raw[N][W];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int k = 0; k < W; ++k) raw[n][k] = at[(size_t)min((i0 + n * step) / 8, last) * W + k];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = i0 + n * step;
+            if (i >= end) break;
+            if (i + 8 <= r.vocab) {
+                unpack8<TYPE, CLEAN>(raw[n], x);
+            } else {
+                load8<TYPE>(r.at, i, r.vocab, false, x);
+            }
+            fn(i, x);
+        }
+    }
 }
-__device__ __forceinline__ int bin_of(const Row& r, float x) {
-    const double z = steps_of(r, x);
-    return z < (double)(kSpan * kSteps) ? (int)z >> kBinShift : kBins;
+
+// How far a logit lies under the largest one, in parts of 1/32 octave of w: at most all of them, where the weight is 0.
+// (A largest logit of +inf less itself is a NaN, which the maximum makes 0.)
+__device__ __forceinline__ double parts_of(const Row& r, float x) {
+    return fmin(fmax(((double)r.top - (double)x) * r.rate, 0.0), (double)kBins);
 }
-// w 2^44, to the nearest integer: table[j] = 2^(44 - j / kSteps); the cubic is off by 10^-14.
+__device__ __forceinline__ int bin_of(double parts) { return (int)__builtin_rint(parts); }
+// w 2^44, to the nearest integer: 2^(44 - q / 32) for the nearest whole q from a table of 32 and the exponent's bits, times
+// the series of exp for the rest of at most 1/64 octave, off by less than 2 10^-12; adding 2^52 rounds to an integer.
+__device__ __forceinline__ unsigned long long weight_at(double parts, const double* table) {
+    const double n = __builtin_rint(parts), y = (n - parts) * (0.6931471805599453 / 32.0);
+    const int q = (int)n;
+    double p = 1.0 / 24.0;
+    p = fma(p, y, 1.0 / 6.0);
+    p = fma(p, y, 0.5);
+    p = fma(p, y, 1.0);
+    p = fma(p, y, 1.0);
+    const double t = table[q & 31];
+    const double power = __hiloint2double(__double2hiint(t) - ((q >> 5) << 20), __double2loint(t));
+    return (unsigned long long)__double_as_longlong(fma(p, power, 4503599627370496.0)) & 0xfffffffffffffull;
+}
 __device__ __forceinline__ unsigned long long weight_of(const Row& r, float x, const double* table) {
-    const double z = steps_of(r, x);
-    if (!(z < (double)(kSpan * kSteps))) return 0;
-    const int zi = (int)z;
-    constexpr double c = -0.6931471805599453 / kSteps;
-    const double f = (z - (double)zi) * c;
-    const double p = table[zi & (kSteps - 1)] * fma(f, fma(f, fma(f, 1.0 / 6.0, 0.5), 1.0), 1.0);
-    const double octave = __hiloint2double((1023 - zi / kSteps) << 20, 0);
-    return (unsigned long long)__double_as_longlong(fma(p, octave, 4503599627370496.0)) & 0xfffffffffffffull;
+    return weight_at(parts_of(r, x), table);
 }
-__device__ __forceinline__ void fill_table(double* table, int tid, int threads) {
-    for (int j = tid; j < kSteps; j += threads) table[j] = exp2((double)-j / kSteps) * kOne;
+__device__ __forceinline__ void fill_table(double* table, int tid) {
+    if (tid < 32) table[tid] = exp2(44.0 - tid / 32.0);
 }
 
 // The smallest key up to the largest logit's that fulfils a condition which the largest one does and, once it holds,
 // holds for every larger key.  64 keys a turn; every lane gets the answer.
-template <typename Fn>
+template <int TYPE, typename Fn>
 __device__ __forceinline__ uint32_t first_key(uint32_t top, int lane, Fn holds) {
-    uint32_t lo = kLowest, hi = top;  // it fails at lo
+    uint32_t lo = kLowest<TYPE>, hi = top;  // it fails at lo
     while (hi - lo > 1) {
         const uint32_t step = (hi - lo + kWave - 1) / kWave;
         const uint32_t k = min(hi - lo, step * (uint32_t)(lane + 1)) + lo;
-        const unsigned long long mask = __ballot(k == hi || holds(logit_of(k)));
+        const unsigned long long mask = __ballot(k == hi || holds(logit_of<TYPE>(k)));
         const uint32_t l = (uint32_t)__builtin_ctzll(mask);
         hi = min(hi - lo, step * (l + 1)) + lo;
         lo += l ? min(hi - lo - 1, step * l) : 0;
     }
     return hi;
 }
+template <int TYPE>
 __device__ __forceinline__ uint32_t first_key_of_bins(const Row& r, int bin, int lane) {  // of bins 0 .. bin
-    return first_key(key_of(r.top), lane, [&](float x) { return bin_of(r, x) <= bin; });
+    return first_key<TYPE>(key_of<TYPE>(r.top), lane, [&](float x) { return bin_of(parts_of(r, x)) <= bin; });
 }
+template <int TYPE>
 __device__ __forceinline__ uint32_t first_key_of_min_p(const Row& r, int lane) {
-    return first_key(key_of(r.top), lane, [&](float x) { return exp2(-steps_of(r, x) / kSteps) >= (double)r.min_p; });
+    return first_key<TYPE>(key_of<TYPE>(r.top), lane, [&](float x) { return exp2(parts_of(r, x) / -32.0) >= (double)r.min_p; });
 }
 
 // The border of the prefix: entries with a key above `key` are inside, and the first `ties` with that key.
@@ -212,20 +275,41 @@ __device__ __forceinline__ unsigned long long target_of(float u, unsigned long l
     return goal > 0.0 ? min((unsigned long long)fmin(goal, 9.2e18), total - 1) : 0;
 }
 
-template <typename V>
-__device__ __forceinline__ V wave_prefix(V v, int lane) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const V o = __shfl_up(v, d);
-        if (lane >= d) v += o;
+// Lane l - d's value within its 16 lanes, or lane 15's / 31's for the lanes behind; 0 where there is none.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V dpp_before(V v) {
+    if constexpr (sizeof(V) == 4) {
+        return (V)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+    } else {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+        return ((V)hi << 32) | lo;
     }
+}
+// Inclusive sum over the wave's lanes (all of them active).
+template <typename V>
+__device__ __forceinline__ V wave_prefix(V v) {
+    v += dpp_before<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_before<0x112, 0xf>(v);
+    v += dpp_before<0x114, 0xf>(v);
+    v += dpp_before<0x118, 0xf>(v);
+    v += dpp_before<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to the rows behind them
+    v += dpp_before<0x143, 0xc>(v);  // lane 31 to the upper half
     return v;
 }
 template <typename V>
+__device__ __forceinline__ V lane_value(V v, int lane) {
+    if constexpr (sizeof(V) == 4) {
+        return (V)__builtin_amdgcn_readlane((int)v, lane);
+    } else {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+        return ((V)hi << 32) | lo;
+    }
+}
+template <typename V>
 __device__ __forceinline__ V wave_total(V v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+    return lane_value(wave_prefix(v), kWave - 1);
 }
 __device__ __forceinline__ unsigned long long wave_largest(unsigned long long v) {
 #pragma unroll
@@ -238,12 +322,12 @@ __device__ __forceinline__ unsigned long long wave_largest(unsigned long long v)
 // Inclusive sum over the workgroup's threads; `parts` holds one value a wave and is free again afterwards.
 template <typename V>
 __device__ __forceinline__ V block_prefix(V v, V* parts, int lane, int wave) {
-    v = wave_prefix(v, lane);
+    v = wave_prefix(v);
     if (lane == kWave - 1) parts[wave] = v;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) v += parts[w];
+    const V before = wave_prefix(lane < wave ? parts[lane] : (V)0);
     __syncthreads();
-    return v;
+    return v + lane_value(before, kWave - 1);
 }
 
 // ---------------------------------------------------------------- long rows: several workgroups a row
@@ -257,10 +341,11 @@ struct Work {
     int chunks, chunk, segments;  // chunk: entries, whole segments
 };
 
+template <int TYPE>
 __device__ __forceinline__ bool load_top(Row& r, const Work& w, int row, int lane, int& index) {
     unsigned long long c = 0;
     for (int i = lane; i < w.chunks; i += kWave) c = max(c, w.top[(size_t)row * w.chunks + i]);
-    return take_top(r, wave_largest(c), index);
+    return take_top<TYPE>(r, wave_largest(c), index);
 }
 
 template <int TYPE>
@@ -270,16 +355,14 @@ __global__ __launch_bounds__(512) void sample_top_kernel(SampleArgs a, Work w) {
     const Row r = row_of<TYPE>(a, row);
     const int end = min(r.vocab, (chunk + 1) * w.chunk);
     unsigned long long best = 0;
-    for (int i = chunk * w.chunk + 8 * tid; i < end; i += 8 * 512) {
-        float x[8];
-        load8<TYPE>(r.at, i, r.vocab, r.aligned, x);
+    walk<TYPE, 4>(r, chunk * w.chunk + 8 * tid, end, 8 * 512, [&](int i, const float(&x)[8]) {
         float m = x[0];
         int at = 0;
 #pragma unroll
         for (int j = 1; j < 8; ++j)
             if (x[j] > m) m = x[j], at = j;
-        best = max(best, top_code(m, i + at));
-    }
+        best = max(best, top_code<TYPE>(m, i + at));
+    });
     best = wave_largest(best);
     if (lane == 0) parts[tid / kWave] = best;
     __syncthreads();
@@ -291,148 +374,113 @@ __global__ __launch_bounds__(512) void sample_top_kernel(SampleArgs a, Work w) {
 
 template <int TYPE>
 __global__ __launch_bounds__(512) void sample_bins_kernel(SampleArgs a, Work w) {
-    __shared__ double table[kSteps];
+    __shared__ double table[32];
     __shared__ unsigned long long sum[kBins];
     __shared__ uint32_t count[kBins];
     const int row = blockIdx.x / w.chunks, chunk = blockIdx.x % w.chunks, tid = threadIdx.x, lane = tid & (kWave - 1);
     Row r = row_of<TYPE>(a, row);
     int index;
-    if (!(r.by_k || r.by_p) || !load_top(r, w, row, lane, index)) return;  // uniform
-    if (r.by_p) fill_table(table, tid, 512);
+    if (!(r.by_k || r.by_p) || !load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
+    fill_table(table, tid);
     for (int b = tid; b < kBins; b += 512) {
         sum[b] = 0;
         count[b] = 0;
     }
     __syncthreads();
     const int end = min(r.vocab, (chunk + 1) * w.chunk);
-    for (int i = chunk * w.chunk + 8 * tid; i < end; i += 8 * 512) {
-        float x[8];
-        load8<TYPE>(r.at, i, r.vocab, r.aligned, x);
+    walk<TYPE, 4>(r, chunk * w.chunk + 8 * tid, end, 8 * 512, [&](int, const float(&x)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int b = bin_of(r, x[j]);
+            const double o = parts_of(r, x[j]);
+            const unsigned long long v = r.by_p ? weight_at(o, table) : 0;
+            const int b = bin_of(o);
             if (b >= kBins) continue;
-            atomicAdd(&count[b], 1u);
-            if (r.by_p) atomicAdd(&sum[b], weight_of(r, x[j], table));
+            if (r.by_k) atomicAdd(&count[b], 1u);
+            if (r.by_p) atomicAdd(&sum[b], v);
         }
-    }
+    });
     __syncthreads();
     const size_t at = ((size_t)row * w.chunks + chunk) * kBins;
     for (int b = tid; b < kBins; b += 512) {
-        w.count[at + b] = count[b];
-        w.sum[at + b] = sum[b];
+        if (r.by_k) w.count[at + b] = count[b];
+        if (r.by_p) w.sum[at + b] = sum[b];
     }
 }
 
 constexpr int kBorderThreads = 1024, kBorderWaves = kBorderThreads / kWave;
-constexpr int kList = 2048;
+constexpr int kList = 4096;
 
-struct BorderShared {
-    double table[kSteps];
-    unsigned long long sum[2048];
-    uint32_t count[2048];
-    unsigned long long list_w[kList];
-    uint32_t list[kList];
-    unsigned long long part_sum[kBorderWaves];
-    uint32_t part_count[kBorderWaves], part_min[kBorderWaves], part_max[kBorderWaves];
-    unsigned long long before_sum;
-    uint32_t before_count, listed, lowest, equal;
-    int found;
+// A bin's entries and weight, and those of everything above it.
+struct Bin {
+    int bin;  // -1: none
+    uint32_t count, before_count;
+    unsigned long long sum, before_sum;
 };
 
-// The last of the 2048 bins in sh whose first entry is inside, given what lies above them; -1: none.  Leaves what lies
-// above that bin in sh.before_*.
-__device__ __forceinline__ int border_bin(BorderShared& sh, const Goal& goal, uint32_t base_count, unsigned long long base_sum) {
+struct BorderShared {
+    double table[32];
+    unsigned long long sum[2048];
+    uint32_t count[2048];
+    float list[kList];
+    unsigned long long part_sum[kBorderWaves];
+    uint32_t part_count[kBorderWaves];
+    Bin found[kBorderWaves];
+    uint32_t listed;
+};
+
+// The last bin whose first entry is inside; thread t holds bins 2 t and 2 t + 1.  Two barriers, the first behind all that
+// the caller has read of sh's bins.
+__device__ __forceinline__ Bin border_bin(BorderShared& sh, const Goal& goal, uint32_t c0, uint32_t c1, unsigned long long s0,
+                                          unsigned long long s1, uint32_t base_count, unsigned long long base_sum) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const uint32_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1];
-    const unsigned long long s0 = sh.sum[2 * tid], s1 = sh.sum[2 * tid + 1];
-    if (tid == 0) sh.found = -1;
-    const uint32_t cb = base_count + block_prefix<uint32_t>(c0 + c1, sh.part_count, lane, wave) - c0 - c1;
-    const unsigned long long sb = base_sum + block_prefix<unsigned long long>(s0 + s1, sh.part_sum, lane, wave) - s0 - s1;
-    if (c1 && goal.inside(cb + c0, sb + s0))
-        atomicMax(&sh.found, 2 * tid + 1);
-    else if (c0 && goal.inside(cb, sb))
-        atomicMax(&sh.found, 2 * tid);
-    __syncthreads();
-    const int bin = sh.found;
-    if (bin >= 0 && bin / 2 == tid) {
-        sh.before_count = bin & 1 ? cb + c0 : cb;
-        sh.before_sum = bin & 1 ? sb + s0 : sb;
+    const uint32_t c = wave_prefix(c0 + c1);
+    const unsigned long long s = wave_prefix(s0 + s1);
+    if (lane == kWave - 1) {
+        sh.part_count[wave] = c;
+        sh.part_sum[wave] = s;
     }
     __syncthreads();
-    return bin;
+    const uint32_t cb = base_count + wave_total(lane < wave ? sh.part_count[lane] : 0u) + c - c0 - c1;
+    const unsigned long long sb = base_sum + wave_total(lane < wave ? sh.part_sum[lane] : 0ull) + s - s0 - s1;
+    Bin mine{-1, 0, 0, 0, 0};
+    if ((c0 || s0) && goal.inside(cb, sb)) mine = Bin{2 * tid, c0, cb, s0, sb};
+    if ((c1 || s1) && goal.inside(cb + c0, sb + s0)) mine = Bin{2 * tid + 1, c1, cb + c0, s1, sb + s0};
+    const unsigned long long any = __ballot(mine.bin >= 0);
+    if (any ? lane == 63 - __builtin_clzll(any) : lane == 0) sh.found[wave] = mine;
+    __syncthreads();
+    const unsigned long long waves = __ballot(lane < kBorderWaves && sh.found[lane < kBorderWaves ? lane : 0].bin >= 0);
+    return waves ? sh.found[63 - __builtin_clzll(waves)] : Bin{-1, 0, 0, 0, 0};
 }
 
-// The border inside the keys lo .. hi, which n entries have, behind the given ones.  (Entries that an earlier border left
-// out weigh on no decision: what lies before them already exceeds the limit.)
+// The border inside the keys lo .. hi, which n entries have (0: not known, more than one key), behind the given ones.  (Entries that an earlier border left
+// out weigh on no decision: what lies before them already exceeds the limit.)  Up to kList entries are collected first;
+// then bins over equal parts of the keys' range, until a bin is one key.
 template <int TYPE>
 __device__ Border border_among(BorderShared& sh, const Row& r, const Goal& goal, uint32_t lo, uint32_t hi, uint32_t n,
                                uint32_t base_count, unsigned long long base_sum) {
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    if (n <= kList) {
-        // few: collect them; an entry knows what lies above it by looking at all of them
+    const int tid = threadIdx.x;
+    bool listed = n <= kList && lo != hi;
+    if (listed) {
+        const float xlo = logit_of<TYPE>(lo), xhi = logit_of<TYPE>(hi);
         if (tid == 0) sh.listed = 0;
-        if (tid == 0) sh.lowest = 0xffffffffu;
-        if (tid == 0) sh.equal = 0;
         __syncthreads();
-        for (int i = 8 * tid; i < r.vocab; i += 8 * kBorderThreads) {
-            float x[8];
-            load8<TYPE>(r.at, i, r.vocab, r.aligned, x);
+        walk<TYPE, TYPE == 2 ? 5 : 10, false>(r, 8 * tid, r.vocab, 8 * kBorderThreads, [&](int, const float(&x)[8]) {
+            uint32_t hits = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t k = key_of(x[j]);
-                if (k - lo > hi - lo) continue;
-                const uint32_t at = atomicAdd(&sh.listed, 1u);
-                if (at >= kList) continue;
-                sh.list[at] = k;
-                sh.list_w[at] = r.by_p ? weight_of(r, x[j], sh.table) : 0;
-            }
-        }
-        __syncthreads();
-        const uint32_t m = min(sh.listed, (uint32_t)kList);
-        for (uint32_t e = tid; e < m; e += kBorderThreads) {
-            const uint32_t k = sh.list[e];
-            uint32_t c = base_count;
-            unsigned long long s = base_sum;
-            for (uint32_t o = 0; o < m; ++o)
-                if (sh.list[o] > k) {
-                    ++c;
-                    s += sh.list_w[o];
+            for (int j = 0; j < 8; ++j) hits |= __builtin_amdgcn_fmed3f(x[j], xlo, xhi) == x[j] ? 1u << j : 0u;
+            if (!hits) return;
+            uint32_t at = atomicAdd(&sh.listed, (uint32_t)__popc(hits));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (hits >> j & 1) {
+                    if (at < kList) sh.list[at] = x[j] + 0.0f;
+                    ++at;
                 }
-            if (goal.inside(c, s)) atomicMin(&sh.lowest, k);
-        }
+        });
         __syncthreads();
-        const uint32_t key = sh.lowest;
-        for (uint32_t e = tid; e < m; e += kBorderThreads) {
-            if (sh.list[e] == key) atomicAdd(&sh.equal, 1u);
-        }
-        // what lies above the border's key
-        uint32_t c = 0;
-        unsigned long long s = 0;
-        for (uint32_t e = tid; e < m; e += kBorderThreads)
-            if (sh.list[e] > key) {
-                ++c;
-                s += sh.list_w[e];
-            }
-        c = wave_total(c);
-        s = wave_total(s);
-        if (lane == 0) {
-            sh.part_count[wave] = c;
-            sh.part_sum[wave] = s;
-        }
-        __syncthreads();
-        c = base_count;
-        s = base_sum;
-        for (int v = 0; v < kBorderWaves; ++v) {
-            c += sh.part_count[v];
-            s += sh.part_sum[v];
-        }
-        const uint32_t equal = sh.equal;
-        __syncthreads();
-        if (equal == 0) return Border{kLowest + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
-        return goal.end(key, equal, !r.by_p ? 0 : weight_of(r, logit_of(key), sh.table), c, s);
+        listed = sh.listed <= kList;
     }
-    // many: bins over equal parts of the keys' range, until a bin is one key
+    const int entries = listed ? (int)sh.listed : r.vocab;
     while (lo != hi) {
         const uint32_t range = hi - lo;
         const int shift = max(0, 32 - __builtin_clz(range) - 11);
@@ -441,30 +489,32 @@ __device__ Border border_among(BorderShared& sh, const Row& r, const Goal& goal,
             sh.count[b] = 0;
         }
         __syncthreads();
-        for (int i = 8 * tid; i < r.vocab; i += 8 * kBorderThreads) {
-            float x[8];
-            load8<TYPE>(r.at, i, r.vocab, r.aligned, x);
+        auto add = [&](float x) {
+            const uint32_t k = key_of<TYPE>(x);
+            if (k - lo > range) return;
+            atomicAdd(&sh.count[(hi - k) >> shift], 1u);
+            if (r.by_p) atomicAdd(&sh.sum[(hi - k) >> shift], weight_of(r, x, sh.table));
+        };
+        if (listed) {
+            for (int i = tid; i < entries; i += kBorderThreads) add(sh.list[i]);
+        } else {
+            walk<TYPE, 4>(r, 8 * tid, entries, 8 * kBorderThreads, [&](int, const float(&x)[8]) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t k = key_of(x[j]);
-                if (k - lo > range) continue;
-                atomicAdd(&sh.count[(hi - k) >> shift], 1u);
-                if (r.by_p) atomicAdd(&sh.sum[(hi - k) >> shift], weight_of(r, x[j], sh.table));
-            }
+                for (int j = 0; j < 8; ++j) add(x[j]);
+            });
         }
         __syncthreads();
-        const int bin = border_bin(sh, goal, base_count, base_sum);
-        if (bin < 0) return Border{kLowest + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
-        base_count = sh.before_count;
-        base_sum = sh.before_sum;
-        n = sh.count[bin];
-        hi -= (uint32_t)bin << shift;
-        lo = max(lo, hi - ((1u << shift) - 1));  // keys of numbers lie above 2^22, so this does not wrap
-        __syncthreads();
-        if (shift == 0) break;
+        const Bin f = border_bin(sh, goal, sh.count[2 * tid], sh.count[2 * tid + 1], sh.sum[2 * tid], sh.sum[2 * tid + 1],
+                                 base_count, base_sum);
+        if (f.bin < 0) return Border{kLowest<TYPE> + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
+        base_count = f.before_count;
+        base_sum = f.before_sum;
+        n = f.count;
+        hi -= (uint32_t)f.bin << shift;
+        const uint32_t width = (1u << shift) - 1;
+        lo = hi - lo > width ? hi - width : lo;
     }
-    lo = hi;
-    return goal.end(lo, n, !r.by_p ? 0 : weight_of(r, logit_of(lo), sh.table), base_count, base_sum);
+    return goal.end(lo, n, r.by_p ? weight_of(r, logit_of<TYPE>(lo), sh.table) : 0, base_count, base_sum);
 }
 
 template <int TYPE>
@@ -473,80 +523,82 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(SampleArg
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     Row r = row_of<TYPE>(a, row);
     int index;
-    if (!load_top(r, w, row, lane, index)) return;  // uniform
-    Border border{kLowest + 1, 0xffffffffu, 0};     // everything above -inf
-    unsigned long long total = 0;
-    auto load_bins = [&]() {
-        unsigned long long all = 0;
-        for (int b = tid; b < 2048; b += kBorderThreads) {
-            uint32_t c = 0;
-            unsigned long long s = 0;
-            if (b < kBins)
-                for (int i = 0; i < w.chunks; ++i) {
-                    const size_t at = ((size_t)row * w.chunks + i) * kBins + b;
-                    c += w.count[at];
-                    s += w.sum[at];
-                }
-            sh.count[b] = c;
-            sh.sum[b] = s;
-            all += s;
-        }
-        __syncthreads();
-        return all;
-    };
-    auto find = [&](const Goal& goal) {
-        const int bin = border_bin(sh, goal, 0, 0);
-        if (bin < 0) return Border{kLowest + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
-        const uint32_t n = sh.count[bin], count = sh.before_count;
-        const unsigned long long sum = sh.before_sum;
-        const uint32_t lo = first_key_of_bins(r, bin, lane);
-        const uint32_t hi = bin ? first_key_of_bins(r, bin - 1, lane) - 1 : key_of(r.top);
-        __syncthreads();
-        return border_among<TYPE>(sh, r, goal, lo, hi, n, count, sum);
-    };
+    if (!load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
+    Border border{kLowest<TYPE> + 1, 0xffffffffu, 0};     // everything above -inf
     if (r.by_k || r.by_p) {
-        if (r.by_p) fill_table(sh.table, tid, kBorderThreads);
-        total = load_bins();
+        fill_table(sh.table, tid);
+        // bins 2 tid and 2 tid + 1 of all chunks; the loads go out together (a chunk behind the last is the last one)
+        uint32_t c0 = 0, c1 = 0;
+        unsigned long long s0 = 0, s1 = 0;
+        if (2 * tid < kBins) {
+            uint2 cs[kMaxChunks];
+            ulonglong2 ss[kMaxChunks];
+            const size_t at = (size_t)row * w.chunks * kBins + 2 * tid;
+#pragma unroll
+            for (int i = 0; i < kMaxChunks; ++i) {
+                const size_t k = at + (size_t)min(i, w.chunks - 1) * kBins;
+                cs[i] = r.by_k ? *reinterpret_cast<const uint2*>(w.count + k) : make_uint2(0, 0);
+                ss[i] = r.by_p ? *reinterpret_cast<const ulonglong2*>(w.sum + k) : make_ulonglong2(0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kMaxChunks; ++i)
+                if (i < w.chunks) {
+                    c0 += cs[i].x;
+                    c1 += cs[i].y;
+                    s0 += ss[i].x;
+                    s1 += ss[i].y;
+                }
+        }
+        auto find = [&](const Goal& goal) {
+            const Bin f = border_bin(sh, goal, c0, c1, s0, s1, 0, 0);
+            if (f.bin < 0) return Border{kLowest<TYPE> + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
+            const uint32_t lo = first_key_of_bins<TYPE>(r, f.bin, lane);
+            const uint32_t hi = f.bin ? first_key_of_bins<TYPE>(r, f.bin - 1, lane) - 1 : key_of<TYPE>(r.top);
+            uint32_t n = f.count;  // counted for top_k only
+            if (!r.by_k && lo == hi) n = (uint32_t)(f.sum / weight_of(r, logit_of<TYPE>(lo), sh.table));
+            return border_among<TYPE>(sh, r, goal, lo, hi, n, f.before_count, f.before_sum);
+        };
+        unsigned long long total = 0;
         if (r.by_k) {
             border = find(Goal{true, (uint32_t)r.top_k, 0});
             total = border.sum;
-            if (r.by_p) {
-                __syncthreads();
-                load_bins();
-            }
-        } else {
-            total = wave_total(total);
-            if (lane == 0) sh.part_sum[wave] = total;
-            __syncthreads();
-            total = 0;
-            for (int v = 0; v < kBorderWaves; ++v) total += sh.part_sum[v];
-            __syncthreads();
         }
-        if (r.by_p) border = find(Goal{false, 0, share_limit(r, total)});
+        __syncthreads();  // the slots of the search
+        if (r.by_p) {
+            if (!r.by_k) {
+                total = wave_total(s0 + s1);
+                if (lane == 0) sh.part_sum[wave] = total;
+                __syncthreads();
+                total = wave_total(lane < kBorderWaves ? sh.part_sum[lane] : 0ull);
+                __syncthreads();
+            }
+            border = find(Goal{false, 0, share_limit(r, total)});
+        }
     }
     if (r.min_p > 0.f) {
-        const uint32_t k = first_key_of_min_p(r, lane);
+        const uint32_t k = first_key_of_min_p<TYPE>(r, lane);
         if (k > border.key) border = Border{k, 0xffffffffu, 0};
     }
     if (tid == 0) w.border[row] = make_uint2(border.key, border.ties);
 }
 
 // The weight of an entry above the border's key; `tie`: it has that key.
+template <int TYPE>
 __device__ __forceinline__ unsigned long long kept_weight(const Row& r, float x, uint32_t border, const double* table, bool& tie) {
-    const uint32_t k = key_of(x);
+    const uint32_t k = key_of<TYPE>(x);
     tie = k == border;
     return k > border ? weight_of(r, x, table) : 0;
 }
 
 template <int TYPE>
 __global__ __launch_bounds__(512) void sample_segments_kernel(SampleArgs a, Work w) {
-    __shared__ double table[kSteps];
     const int row = blockIdx.x / w.chunks, chunk = blockIdx.x % w.chunks, tid = threadIdx.x, lane = tid & (kWave - 1);
     Row r = row_of<TYPE>(a, row);
     int index;
-    if (!load_top(r, w, row, lane, index)) return;  // uniform
+    if (!load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
+    __shared__ double table[32];
     const uint32_t border = w.border[row].x;
-    fill_table(table, tid, 512);
+    fill_table(table, tid);
     __syncthreads();
     const int per = w.chunk / kSegment, last = min(w.segments, (chunk + 1) * per);
     for (int s = chunk * per + tid / kWave; s < last; s += 512 / kWave) {
@@ -557,11 +609,11 @@ __global__ __launch_bounds__(512) void sample_segments_kernel(SampleArgs a, Work
         float m = x[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) m = fmaxf(m, x[j]);
-        if (__any(key_of(m) >= border)) {  // else nothing of the segment is kept
+        if (__any(key_of<TYPE>(m) >= border)) {  // else nothing of the segment is kept
             bool tie;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                sum += kept_weight(r, x[j], border, table, tie);
+                sum += kept_weight<TYPE>(r, x[j], border, table, tie);
                 ties += tie;
             }
             sum = wave_total(sum);
@@ -580,19 +632,19 @@ __device__ __forceinline__ uint32_t ties_kept(uint32_t ties, uint32_t before, ui
 
 template <int TYPE>
 __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a, Work w) {
-    __shared__ double table[kSteps];
+    __shared__ double table[32];
     __shared__ unsigned long long part_sum[16], before_sum, all;
     __shared__ uint32_t part_count[16], before_ties;
     __shared__ int found;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     Row r = row_of<TYPE>(a, row);
     int index;
-    if (!load_top(r, w, row, lane, index)) {  // uniform
+    if (!load_top<TYPE>(r, w, row, lane, index)) {  // uniform
         if (tid == 0) a.out[row] = index;
         return;
     }
     const uint2 border = w.border[row];
-    fill_table(table, tid, 1024);
+    fill_table(table, tid);
     const size_t at = (size_t)row * w.segments + tid;
     const unsigned long long s = tid < w.segments ? w.seg[at] : 0;
     const uint32_t n = tid < w.segments ? w.tie[at] : 0;
@@ -601,8 +653,8 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a, Work w)
         before_sum = 0;
         before_ties = 0;
     }
-    const uint32_t before = block_prefix<uint32_t>(n, part_count, lane, wave) - n;  // also the table's barrier
-    const unsigned long long border_w = weight_of(r, logit_of(border.x), table);
+    const uint32_t before = block_prefix<uint32_t>(n, part_count, lane, wave) - n;  // and the table is there
+    const unsigned long long border_w = weight_of(r, logit_of<TYPE>(border.x), table);
     const unsigned long long mine = s + ties_kept(border.y, before, n) * border_w;
     const unsigned long long through = block_prefix<unsigned long long>(mine, part_sum, lane, wave);
     if (tid == 1023) all = through;
@@ -623,16 +675,16 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a, Work w)
     uint32_t ties = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        wj[j] = kept_weight(r, x[j], border.x, table, tie[j]);
+        wj[j] = kept_weight<TYPE>(r, x[j], border.x, table, tie[j]);
         ties += tie[j];
     }
-    uint32_t rank = before_ties + wave_prefix<uint32_t>(ties, lane) - ties;
+    uint32_t rank = before_ties + wave_prefix<uint32_t>(ties) - ties;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (tie[j]) wj[j] = rank++ < border.y ? border_w : 0;
         sum += wj[j];
     }
-    unsigned long long cum = before_sum + wave_prefix<unsigned long long>(sum, lane) - sum;
+    unsigned long long cum = before_sum + wave_prefix<unsigned long long>(sum) - sum;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (cum <= target && cum + wj[j] > target) a.out[row] = i0 + j;  // one entry's
@@ -641,12 +693,11 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a, Work w)
 }
 
 // ---------------------------------------------------------------- short rows: one wave a row
-constexpr int kWaveBinShift = 7, kWaveBins = 384;  // 46 octaves of 8 bins, 6 bins a lane
-static_assert((kSpan * kSteps >> kWaveBinShift) <= kWaveBins && kWaveBins % kWave == 0, "bins");
+constexpr int kWaveBins = kBins / 4, kWaveBinsPerLane = (kWaveBins + kWave - 1) / kWave;  // 8 an octave
 
 struct WaveBins {
-    unsigned long long sum[kWaveBins];
-    uint32_t count[kWaveBins];
+    unsigned long long sum[kWaveBinsPerLane * kWave];
+    uint32_t count[kWaveBinsPerLane * kWave];
 };
 
 // Other lanes' LDS writes before this point are seen behind it (a wave's LDS accesses are carried out in order).
@@ -655,11 +706,11 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-template <int E>
+template <int TYPE, int E>
 __device__ Border wave_border(WaveBins& sh, const Row& r, const float (&x)[E], const unsigned long long (&weight)[E],
                               const Goal& goal, int lane) {
-    constexpr int PER = kWaveBins / kWave;
-    uint32_t lo = kLowest + 1, hi = key_of(r.top), base_count = 0;
+    constexpr int PER = kWaveBinsPerLane;
+    uint32_t lo = kLowest<TYPE> + 1, hi = key_of<TYPE>(r.top), base_count = 0;
     unsigned long long base_sum = 0;
     int shift = -1;  // -1: bins linear in log w
     for (;;) {
@@ -670,11 +721,10 @@ __device__ Border wave_border(WaveBins& sh, const Row& r, const float (&x)[E], c
         }
         wave_sync();
         auto bin_at = [&](float v) {
-            const uint32_t k = key_of(v);
+            const uint32_t k = key_of<TYPE>(v);
             if (k - lo > hi - lo) return kWaveBins;
             if (shift >= 0) return (int)((hi - k) >> shift);
-            const int b = bin_of(r, v);
-            return b >= kBins ? kWaveBins : b >> (kWaveBinShift - kBinShift);
+            return bin_of(parts_of(r, v)) / (kBins / kWaveBins);  // the entries without weight: the last
         };
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -693,8 +743,8 @@ __device__ Border wave_border(WaveBins& sh, const Row& r, const float (&x)[E], c
             ct += c[b];
             st += s[b];
         }
-        uint32_t cb = base_count + wave_prefix<uint32_t>(ct, lane) - ct, found_c = 0, found_n = 0;
-        unsigned long long sb = base_sum + wave_prefix<unsigned long long>(st, lane) - st, found_s = 0;
+        uint32_t cb = base_count + wave_prefix<uint32_t>(ct) - ct, found_c = 0, found_n = 0;
+        unsigned long long sb = base_sum + wave_prefix<unsigned long long>(st) - st, found_s = 0;
         int found = -1;
 #pragma unroll
         for (int b = 0; b < PER; ++b) {
@@ -708,18 +758,18 @@ __device__ Border wave_border(WaveBins& sh, const Row& r, const float (&x)[E], c
             sb += s[b];
         }
         const unsigned long long mask = __ballot(found >= 0);
-        if (!mask) return Border{kLowest + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
+        if (!mask) return Border{kLowest<TYPE> + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
         const int l = 63 - __builtin_clzll(mask);
-        const int bin = __shfl(found, l);
-        base_count = __shfl(found_c, l);
-        base_sum = __shfl(found_s, l);
-        const uint32_t n = __shfl(found_n, l);
+        const int bin = __builtin_amdgcn_readlane(found, l);
+        base_count = lane_value(found_c, l);
+        base_sum = lane_value(found_s, l);
+        const uint32_t n = lane_value(found_n, l);
         uint32_t kmin = 0xffffffffu, kmax = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (bin_at(x[e]) == bin) {
-                kmin = min(kmin, key_of(x[e]));
-                kmax = max(kmax, key_of(x[e]));
+                kmin = min(kmin, key_of<TYPE>(x[e]));
+                kmax = max(kmax, key_of<TYPE>(x[e]));
             }
 #pragma unroll
         for (int d = 1; d < kWave; d <<= 1) {
@@ -732,7 +782,7 @@ __device__ Border wave_border(WaveBins& sh, const Row& r, const float (&x)[E], c
             unsigned long long w = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (key_of(x[e]) == lo) w = weight[e];
+                if (key_of<TYPE>(x[e]) == lo) w = weight[e];
             return goal.end(lo, n, wave_largest(w), base_count, base_sum);
         }
         shift = max(0, 32 - __builtin_clz(hi - lo) - 8);
@@ -743,10 +793,10 @@ __device__ Border wave_border(WaveBins& sh, const Row& r, const float (&x)[E], c
 template <int TYPE, int J>
 __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs a, int rows) {
     constexpr int E = 8 * J;
-    __shared__ double table[kSteps];
+    __shared__ double table[32];
     __shared__ WaveBins bins[4];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, row = 4 * blockIdx.x + wave;
-    fill_table(table, tid, 256);
+    fill_table(table, tid);
     __syncthreads();
     if (row >= rows) return;
     Row r = row_of<TYPE>(a, row);
@@ -760,19 +810,19 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs a, int rows
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             x[8 * j + e] = v[e];
-            if (i + e < r.vocab) code = max(code, top_code(v[e], i + e));
+            if (i + e < r.vocab) code = max(code, top_code<TYPE>(v[e], i + e));
         }
     }
     int index;
-    if (!take_top(r, wave_largest(code), index)) {
+    if (!take_top<TYPE>(r, wave_largest(code), index)) {
         if (lane == 0) a.out[row] = index;
         return;
     }
     unsigned long long weight[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) weight[e] = weight_of(r, x[e], table);
-    Border border{kLowest + 1, 0xffffffffu, 0};
-    if (r.by_k) border = wave_border<E>(bins[wave], r, x, weight, Goal{true, (uint32_t)r.top_k, 0}, lane);
+    Border border{kLowest<TYPE> + 1, 0xffffffffu, 0};
+    if (r.by_k) border = wave_border<TYPE, E>(bins[wave], r, x, weight, Goal{true, (uint32_t)r.top_k, 0}, lane);
     if (r.by_p) {
         unsigned long long total = border.sum;
         if (!r.by_k) {
@@ -780,10 +830,10 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs a, int rows
             for (int e = 0; e < E; ++e) total += weight[e];
             total = wave_total(total);
         }
-        border = wave_border<E>(bins[wave], r, x, weight, Goal{false, 0, share_limit(r, total)}, lane);
+        border = wave_border<TYPE, E>(bins[wave], r, x, weight, Goal{false, 0, share_limit(r, total)}, lane);
     }
     if (r.min_p > 0.f) {
-        const uint32_t k = first_key_of_min_p(r, lane);
+        const uint32_t k = first_key_of_min_p<TYPE>(r, lane);
         if (k > border.key) border = Border{k, 0xffffffffu, 0};
     }
     // the kept weights in index order
@@ -793,21 +843,21 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs a, int rows
     for (int j = 0; j < J; ++j) {
         uint32_t ties = 0;
 #pragma unroll
-        for (int e = 8 * j; e < 8 * j + 8; ++e) ties += key_of(x[e]) == border.key;
-        const uint32_t all = wave_prefix<uint32_t>(ties, lane);
+        for (int e = 8 * j; e < 8 * j + 8; ++e) ties += key_of<TYPE>(x[e]) == border.key;
+        const uint32_t all = wave_prefix<uint32_t>(ties);
         uint32_t mine = rank + all - ties;
-        rank += __shfl(all, kWave - 1);
+        rank += lane_value(all, kWave - 1);
         unsigned long long s = 0;
 #pragma unroll
         for (int e = 8 * j; e < 8 * j + 8; ++e) {
-            const uint32_t k = key_of(x[e]);
+            const uint32_t k = key_of<TYPE>(x[e]);
             const bool tie = k == border.key, kept = k > border.key || (tie && mine < border.ties);
             mine += tie;
             weight[e] = kept ? weight[e] : 0;
             s += weight[e];
         }
-        through[j] = total + wave_prefix<unsigned long long>(s, lane);
-        total = __shfl(through[j], kWave - 1);
+        through[j] = total + wave_prefix<unsigned long long>(s);
+        total = lane_value(through[j], kWave - 1);
         through[j] -= s;
     }
     const unsigned long long target = target_of(a.uniform[row], total);
@@ -834,14 +884,14 @@ SamplePlan sample_plan(int rows, int vocab) {
     p.segments = (vocab + kSegment - 1) / kSegment;
     // about 1024 workgroups, of at least 8 segments each and at most 16 a row
     int chunks = 1024 / rows;
-    if (chunks > 16) chunks = 16;
+    if (chunks > kMaxChunks) chunks = kMaxChunks;
     if (chunks > p.segments / 8) chunks = p.segments / 8;
     if (chunks < 1) chunks = 1;
     p.chunk = (p.segments + chunks - 1) / chunks * kSegment;
     p.chunks = (vocab + p.chunk - 1) / p.chunk;
     const long long bins = (long long)rows * p.chunks * kBins, segs = (long long)rows * p.segments;
     p.top = 0;
-    p.sum = p.top + 8ll * rows * p.chunks;
+    p.sum = p.top + (8ll * rows * p.chunks + 15) / 16 * 16;  // read 16 bytes at a time
     p.seg = p.sum + 8 * bins;
     p.border = p.seg + 8 * segs;
     p.count = p.border + 8ll * rows;
