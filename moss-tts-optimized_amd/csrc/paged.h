@@ -79,16 +79,6 @@ __device__ __forceinline__ int2 paged_tokens(const PagedBatch& bt, int b, int T)
     return r;
 }
 
-// Sum over the lanes before this one, and its own (inclusive); the last lane holds the wave's total.
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int o = __shfl_up(v, d);
-        v += lane >= d ? o : 0;
-    }
-    return v;
-}
-
 // A sequence of the batch and what the caller looks for in it.
 struct Place {
     int b;      // -1: the index lies behind the last item
@@ -104,7 +94,7 @@ __device__ __forceinline__ Place find_item(int B, int item, int lane, Count coun
     int before = 0;
     for (int b0 = 0; b0 < B; b0 += kWave) {
         const int n = b0 + lane < B ? count(b0 + lane) : 0;
-        const int through = wave_scan(n, lane);
+        const int through = wave_prefix(n);
         const unsigned long long past = __ballot(before + through > item);
         if (past) {
             const int l = __builtin_ctzll(past);

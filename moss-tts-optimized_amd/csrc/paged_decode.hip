@@ -10,7 +10,9 @@
 // sequence of one share writes its output; the others write (m, l, O) per share and a second launch joins them, which
 // also writes the zeros of the empty ones.
 //
-// A wave takes every fourth 32-row tile of its workgroup's share and reads it from the pages straight into registers:
+// A wave takes every fourth 32-row tile of its workgroup's share and reads it from the pages straight into registers
+// (K of the next tile once the scores are formed, V of it once this one's is used: half the registers of two whole
+// tiles, three workgroups a CU for two; 16 sequences of 17 to 8000 rows 23.5 -> 17.0 us with the join's loads together):
 // K as the A operand of the 16x16x32 matrix instruction (S^T[row][head], up to 16 heads of a KV head in one tile), V
 // with a full row over 16 lanes, so a lane holds 8 rows x D / 16 dims.  S^T leaves lane (g, head) with rows 4 g + i and
 // 16 + 4 g + i, which is the K order that the V rows are loaded in: P goes from the softmax into the B operand of
@@ -22,7 +24,12 @@
 namespace moss {
 namespace {
 
-constexpr int kTarget = 2048;  // workgroups that the work is shared out over
+// Workgroups that the work is shared out over.  512 / 1024 / 1536 / 2048: 300 / 298 / 296 / 299 us for 64 sequences of 4 to 8
+// thousand rows of 8 heads, 23.3 / 22.3 / 21.7 / 21.8 for 48 of up to 2000 rows of 12 heads of 64, no difference for fewer.
+constexpr int kTarget = 1536;
+// A cache that the last-level cache (256 MB) cannot hold is read past it: 296 -> 272 us for those 64 sequences (1.6 GB),
+// but 17.0 -> 18.4 for 16 sequences whose 58 MB stay there from call to call.
+constexpr long long kCached = 256ll << 20;
 
 struct DecodeArgs {
     const uint16_t* q;
@@ -38,43 +45,64 @@ struct DecodeArgs {
 __device__ __forceinline__ int share_units(const PagedBatch& bt, int shift, int shares, int lane) {
     long long total = 0;
     for (int b = lane; b < bt.B; b += kWave) total += units_of(paged_length(bt, b, shift));
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m);
-    return __builtin_amdgcn_readfirstlane(share_of_units(total, shares));
+    return share_of_units(wave_total(total), shares);
+}
+
+// The sequence and share of a slot.  A batch of up to 64 is one load and two sums over the wave.
+__device__ __forceinline__ Place find_share(const PagedBatch& bt, int shift, int shares, int slot, int lane) {
+    if (bt.B <= kWave) {
+        const int units = lane < bt.B ? units_of(paged_length(bt, lane, shift)) : 0;
+        const int share = share_of_units(wave_total((long long)units), shares), n = shares_of(units, share);
+        const int through = wave_prefix(n);
+        const unsigned long long past = __ballot(through > slot);
+        if (!past) return Place{-1, 0, 0, 0};
+        const int l = __builtin_ctzll(past), c = __builtin_amdgcn_readlane(n, l);
+        const int first = __builtin_amdgcn_readlane(through, l) - c;
+        return Place{l, slot - first, c, first};
+    }
+    const int share = share_units(bt, shift, shares, lane);
+    return find_item(bt.B, slot, lane, [&](int b) { return shares_of(units_of(paged_length(bt, b, shift)), share); });
 }
 
 template <int D>
 struct KvTile {  // 32 rows: lane (g, r = lane % 16)
     static constexpr int NC = D / 32, VW = D / 32;  // K chunks of 32 dims; words of a lane's D / 16 values of a V row
-    u32x4_t k[2][NC];    // row 16 h + r, dims 32 c + 8 g ..
-    uint32_t v[8][VW];   // row 16 (e / 4) + 4 g + e % 4, dims (D / 16) r ..
+    u32x4_t k[2][NC];   // row 16 h + r, dims 32 c + 8 g ..
+    uint32_t v[8][VW];  // row 16 (e / 4) + 4 g + e % 4, dims (D / 16) r ..
 };
 
-// One half tile's rows: from row `row` (a multiple of 16) of page `page` (-1: of some page, unused).
-template <int D>
-__device__ __forceinline__ void load_half(KvTile<D>& t, int h, const PagedCache& c, int page, int kvh, int row, int g, int r) {
-    using T = KvTile<D>;
+// K or V of one half tile: from row `row` (a multiple of 16) of page `page` (-1: of some page, unused) on.
+template <bool NT, typename V>
+__device__ __forceinline__ V load_row(const uint16_t* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    return *reinterpret_cast<const V*>(p);
+}
+template <bool NT, int D>
+__device__ __forceinline__ void load_k(KvTile<D>& t, int h, const PagedCache& c, int page, int kvh, int row, int g, int r) {
     const uint16_t* kr = c.k + row_offset(page, c.k_stride, kvh, row, c.shift, D);
+#pragma unroll
+    for (int i = 0; i < KvTile<D>::NC; ++i) t.k[h][i] = load_row<NT, u32x4_t>(kr + r * D + 32 * i + 8 * g);
+}
+template <bool NT, int D>
+__device__ __forceinline__ void load_v(KvTile<D>& t, int h, const PagedCache& c, int page, int kvh, int row, int g, int r) {
     const uint16_t* vr = c.v + row_offset(page, c.v_stride, kvh, row, c.shift, D);
 #pragma unroll
-    for (int i = 0; i < T::NC; ++i) t.k[h][i] = *reinterpret_cast<const u32x4_t*>(kr + (size_t)r * D + 32 * i + 8 * g);
-#pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint16_t* p = vr + (size_t)(4 * g + e) * D + (D / 16) * r;
-        if constexpr (T::VW == 4) {
-            const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p);
+        const uint16_t* p = vr + (4 * g + e) * D + (D / 16) * r;
+        if constexpr (KvTile<D>::VW == 4) {
+            const u32x4_t w = load_row<NT, u32x4_t>(p);
 #pragma unroll
             for (int i = 0; i < 4; ++i) t.v[4 * h + e][i] = w[i];
         } else {
-            const u32x2_v w = *reinterpret_cast<const u32x2_v*>(p);
+            const u32x2_v w = load_row<NT, u32x2_v>(p);
             t.v[4 * h + e][0] = w[0];
             t.v[4 * h + e][1] = w[1];
         }
     }
 }
 
-template <typename E, int D>
-__global__ __launch_bounds__(256, 2) void paged_decode_split(DecodeArgs a, PagedCache c, PagedBatch bt) {
+template <typename E, int D, bool NT>
+__global__ __launch_bounds__(256, 3) void paged_decode_split(DecodeArgs a, PagedCache c, PagedBatch bt) {
     using T = KvTile<D>;
     constexpr int NJ = D / 16;
     __shared__ __attribute__((aligned(16))) float ow[4][16][D];
@@ -84,8 +112,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_split(DecodeArgs a, Paged
     const int tiles = (a.group + 15) / 16;  // head tiles of a KV head
     const int slot = blockIdx.x / a.xdim, x = blockIdx.x % a.xdim;
     const int kvh = x / tiles, h0 = 16 * (x % tiles), heads = min(16, a.group - h0);
-    const int su = share_units(bt, c.shift, a.shares, lane);
-    const Place pl = find_item(bt.B, slot, lane, [&](int b) { return shares_of(units_of(paged_length(bt, b, c.shift)), su); });
+    const Place pl = find_share(bt, c.shift, a.shares, slot, lane);
     if (pl.b < 0) return;
     int r0, r1;  // may be empty
     share_rows(paged_length(bt, pl.b, c.shift), pl.count, pl.index, r0, r1);
@@ -106,32 +133,45 @@ __global__ __launch_bounds__(256, 2) void paged_decode_split(DecodeArgs a, Paged
 
     const int* trow = bt.table + (size_t)pl.b * bt.table_stride;
     const int ntile = r1 > r0 ? ((r1 - r0 + 31) / 32 - w + 3) / 4 : 0;  // this wave's tiles w, w + 4, ..
-    int pages = -1;  // lane i: the page of half tile i of the 32 tiles from `fetched` on
+    // lane i: the page of half tile i of 32 tiles; those of the next 32 replace them when tile 32 k is loaded
+    auto row_of = [&](int i, int h) { return r0 + 32 * (w + 4 * i) + 16 * h; };
+    int pages = -1;
     auto fetch_pages = [&](int first) {
-        const int row = r0 + 32 * (w + 4 * (first + lane / 2)) + 16 * (lane & 1);
+        const int row = row_of(first + lane / 2, lane & 1);
         int p = -1;
         if (row < r1) p = page_or_none(trow[row >> c.shift], c.pages);
         pages = p;
     };
-    auto load = [&](KvTile<D>& t, int i) {
+    // K of tile i + 1 is loaded as soon as the scores of tile i are formed, V of it once tile i's is consumed: one set
+    // of registers for each, and loads on their way all the time
+    KvTile<D> t;
+    int p0 = -1, p1 = -1;  // the pages of the tile whose K was loaded last
+    auto next_k = [&](int i) {
         if ((i & 31) == 0) fetch_pages(i);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = r0 + 32 * (w + 4 * i) + 16 * h;
-            const int page = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + h);
-            load_half<D>(t, h, c, page, kvh, row, g, r);
-        }
+        p0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31));
+        p1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
+        load_k<NT, D>(t, 0, c, p0, kvh, row_of(i, 0), g, r);
+        load_k<NT, D>(t, 1, c, p1, kvh, row_of(i, 1), g, r);
     };
-    // rows of half tile h of tile i that take part: 16, fewer at the end, none without a page
-    auto rows_of = [&](int i, int h, int page) { return page < 0 ? 0 : min(16, max(0, r1 - (r0 + 32 * (w + 4 * i) + 16 * h))); };
-    auto compute = [&](KvTile<D>& t, int n0, int n1) {
+    auto next_v = [&](int i) {
+        load_v<NT, D>(t, 0, c, p0, kvh, row_of(i, 0), g, r);
+        load_v<NT, D>(t, 1, c, p1, kvh, row_of(i, 1), g, r);
+    };
+    if (ntile > 0) {
+        next_k(0);
+        next_v(0);
+    }
+    for (int i = 0; i < ntile; ++i) {
+        // rows of the halves that take part: 16, fewer at the end, none without a page
+        const int n0 = p0 < 0 ? 0 : min(16, max(0, r1 - row_of(i, 0))), n1 = p1 < 0 ? 0 : min(16, max(0, r1 - row_of(i, 1)));
         f32x4_v s[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             s[h] = f32x4_v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < T::NC; ++i) s[h] = E::mfma16(t.k[h][i], qf[i], s[h]);
+            for (int k = 0; k < T::NC; ++k) s[h] = E::mfma16(t.k[h][k], qf[k], s[h]);
         }
+        if (i + 1 < ntile) next_k(i + 1);
         float sv[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) sv[e] = s[e >> 2][e & 3] * a.scale;
@@ -141,7 +181,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_split(DecodeArgs a, Paged
                 const bool live = 4 * g + (e & 3) < (e < 4 ? n0 : n1);
                 sv[e] = live ? sv[e] : -INFINITY;
 #pragma unroll
-                for (int i = 0; i < T::VW; ++i) t.v[e][i] = live ? t.v[e][i] : 0u;
+                for (int k = 0; k < T::VW; ++k) t.v[e][k] = live ? t.v[e][k] : 0u;
             }
         }
         float mx = sv[0];
@@ -156,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_split(DecodeArgs a, Paged
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[j][i] *= f;
+                for (int k = 0; k < 4; ++k) o[j][k] *= f;
         }
         const float mr = m == -INFINITY ? 0.f : m;
         float p[8];
@@ -167,40 +207,24 @@ __global__ __launch_bounds__(256, 2) void paged_decode_split(DecodeArgs a, Paged
         }
         u32x4_t ph, plo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ph[i] = E::pack(p[2 * i], p[2 * i + 1]);
-            plo[i] = E::pack(p[2 * i] - E::lo(ph[i]), p[2 * i + 1] - E::hi(ph[i]));
+        for (int k = 0; k < 4; ++k) {
+            ph[k] = E::pack(p[2 * k], p[2 * k + 1]);
+            plo[k] = E::pack(p[2 * k] - E::lo(ph[k]), p[2 * k + 1] - E::hi(ph[k]));
         }
 #pragma unroll
         for (int jw = 0; jw < T::VW; ++jw) {
             u32x4_t even, odd;  // V^T rows (D / 16) r + 2 jw and + 1, the lane's 8 rows as K
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                even[i] = __builtin_amdgcn_perm(t.v[2 * i + 1][jw], t.v[2 * i][jw], 0x05040100u);
-                odd[i] = __builtin_amdgcn_perm(t.v[2 * i + 1][jw], t.v[2 * i][jw], 0x07060302u);
+            for (int k = 0; k < 4; ++k) {
+                even[k] = __builtin_amdgcn_perm(t.v[2 * k + 1][jw], t.v[2 * k][jw], 0x05040100u);
+                odd[k] = __builtin_amdgcn_perm(t.v[2 * k + 1][jw], t.v[2 * k][jw], 0x07060302u);
             }
             o[2 * jw] = E::mfma16(even, ph, o[2 * jw]);
             o[2 * jw + 1] = E::mfma16(odd, ph, o[2 * jw + 1]);
             o[2 * jw] = E::mfma16(even, plo, o[2 * jw]);
             o[2 * jw + 1] = E::mfma16(odd, plo, o[2 * jw + 1]);
         }
-    };
-    // tile i + 1 is on its way while tile i is consumed
-    KvTile<D> ta, tb;
-    int na0 = 0, na1 = 0, nb0 = 0, nb1 = 0;
-    auto load_counted = [&](KvTile<D>& t, int i, int& n0, int& n1) {
-        load(t, i);
-        n0 = rows_of(i, 0, __builtin_amdgcn_readlane(pages, 2 * (i & 31)));
-        n1 = rows_of(i, 1, __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1));
-    };
-    if (ntile > 0) load_counted(ta, 0, na0, na1);
-    for (int i = 0; i < ntile; i += 2) {
-        if (i + 1 < ntile) load_counted(tb, i + 1, nb0, nb1);
-        compute(ta, na0, na1);
-        if (i + 1 < ntile) {
-            if (i + 2 < ntile) load_counted(ta, i + 2, na0, na1);
-            compute(tb, nb0, nb1);
-        }
+        if (i + 1 < ntile) next_v(i + 1);
     }
 
     // the waves' parts, each against its own m, meet in LDS
@@ -259,27 +283,45 @@ __global__ __launch_bounds__(256) void paged_decode_join(DecodeArgs a, PagedCach
     }
     int first = 0;
     for (int s = lane; s < b; s += kWave) first += shares_of(units_of(paged_length(bt, s, c.shift)), su);
-#pragma unroll
-    for (int k = 1; k < kWave; k <<= 1) first += __shfl_xor(first, k);
+    first = wave_total(first);
+    // m and l of share 64 i + lane; a share's weight is 2^(m - largest m)
     const float2* st = a.stat + (size_t)first * a.qh + h;
-    float mx = -INFINITY;
-    for (int s = lane; s < count; s += kWave) mx = fmaxf(mx, st[(size_t)s * a.qh].x);
+    const float2 own = lane < count ? st[(size_t)lane * a.qh] : make_float2(-INFINITY, 0.f);
+    const float* part = a.part + ((size_t)first * a.qh + h) * D + VPL * lane;
+    const size_t step = (size_t)a.qh * D;
+    float mx = own.x;
+    for (int s = kWave + lane; s < count; s += kWave) mx = fmaxf(mx, st[(size_t)s * a.qh].x);
     mx = wave_max(mx);
-    float den = 0.f;
-    for (int s = lane; s < count; s += kWave) {
+    auto weight = [&](float m) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx); };
+    const float f0 = weight(own.x);
+    float den = f0 * own.y;
+    for (int s = kWave + lane; s < count; s += kWave) {
         const float2 v = st[(size_t)s * a.qh];
-        den += v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - mx) * v.y;
+        den += weight(v.x) * v.y;
     }
     den = wave_sum(den);
     float acc[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
-    for (int s = w; s < count; s += 4) {
-        const size_t at = (size_t)(first + s) * a.qh + h;
-        const float ms = a.stat[at].x;
-        const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mx);
+    constexpr int N = 8;  // parts on their way together: shares w, w + 4, ..
+    for (int s0 = w; s0 < count; s0 += 4 * N) {
+        float x[N][VPL], f[N];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) acc[i] = fmaf(f, a.part[at * D + VPL * lane + i], acc[i]);
+        for (int n = 0; n < N; ++n) {
+            const int s = min(s0 + 4 * n, count - 1);
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) x[n][i] = part[s * step + i];
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int s = min(s0 + 4 * n, count - 1);
+            f[n] = s < kWave ? __uint_as_float(lane_value(__float_as_uint(f0), s)) : weight(st[(size_t)s * a.qh].x);
+            if (s0 + 4 * n >= count) f[n] = 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) acc[i] = f[n] == 0.f ? acc[i] : fmaf(f[n], x[n][i], acc[i]);
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i) acc_s[w][VPL * lane + i] = acc[i];
@@ -311,7 +353,12 @@ DecodePlan decode_plan(int B, int W, int shift, int qh, int kh) {
 
 template <typename E, int D>
 void launch_decode(const DecodeArgs& a, const PagedCache& c, const PagedBatch& bt, const DecodePlan& p, hipStream_t st) {
-    hipLaunchKernelGGL((paged_decode_split<E, D>), dim3((unsigned)(p.xdim * p.slots)), dim3(256), 0, st, a, c, bt);
+    const long long page = ((long long)c.kh << c.shift) * D * 2, named = (long long)bt.B * bt.W;
+    const dim3 grid((unsigned)(p.xdim * p.slots));
+    if ((named < c.pages ? named : c.pages) * page * 2 > kCached)
+        hipLaunchKernelGGL((paged_decode_split<E, D, true>), grid, dim3(256), 0, st, a, c, bt);
+    else
+        hipLaunchKernelGGL((paged_decode_split<E, D, false>), grid, dim3(256), 0, st, a, c, bt);
     hipLaunchKernelGGL((paged_decode_join<E, D>), dim3((unsigned)a.qh, (unsigned)bt.B), dim3(256), 0, st, a, c, bt);
 }
 

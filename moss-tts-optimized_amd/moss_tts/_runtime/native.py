@@ -129,11 +129,14 @@ def call_on(t: torch.Tensor, name: str, *args) -> None:
     """:func:`call` with ``t``'s device current and its current stream as the last argument: a kernel
     starts on the device that is current, whatever device its stream and pointers belong to."""
     index = t.get_device()
+    fn = getattr(lib(), name)
     if torch._C._cuda_getDevice() == index:
-        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
-        return
-    with torch.cuda.device(index):
-        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)), name)
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        check(code, name)
 
 
 def gemm_workspace(m: int, k: int, n: int, device) -> tuple:

@@ -24,81 +24,144 @@ from .w4g32 import _aligned, _cuda_contig, _require
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _PAGE_ROWS = tuple(1 << s for s in range(4, 13))
+_HEAD_DIMS = (64, 128)
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    def end(t):
-        return t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
-
-
-def _pages(keys: torch.Tensor, values: torch.Tensor, dtype: torch.dtype, dev):
-    """(KV heads, page rows, head dim) of a checked cache."""
+# The checks below read a tensor's shape and strides once and compare plain integers: a call of these operators takes
+# the host longer than most of their kernels take the device (28 us with a torch view or a generator per check, of
+# which 8 are the launches).  What a check finds wrong is named by the slower functions that end in _refuse.
+def _cache_refuse(keys, values, dtype, index):
     for name, t in (("keys", keys), ("values", values)):
         _require(isinstance(t, torch.Tensor) and t.dtype == dtype, f"{name} must be a {dtype} tensor")
-        _require(t.is_cuda and t.device == dev, f"{name} must be on {dev}")
+        _require(t.is_cuda and t.get_device() == index, f"{name} must be on cuda:{index}")
         _require(t.dim() == 4 and t.shape == keys.shape and t.numel() > 0,
                  "matching [pages, KV heads, page rows, head dim] keys and values required")
         n, kh, rows, d = t.shape
-        _require(t.stride(3) == 1 and (rows == 1 or t.stride(2) == d) and (kh == 1 or t.stride(1) == rows * d),
+        _require(rows in _PAGE_ROWS, "page rows must be a power of two from 16 to 4096")
+        _require(d in _HEAD_DIMS, "head dim must be 64 or 128")
+        _require(t.stride(3) == 1 and t.stride(2) == d and (kh == 1 or t.stride(1) == rows * d),
                  f"a page of {name} must be contiguous")
         _require(_aligned(t, 16) and (n == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= kh * rows * d)),
                  f"{name}: pages must be 16-byte aligned and must not overlap")
-    _require(rows in _PAGE_ROWS, "page rows must be a power of two from 16 to 4096")
-    _require(d in (64, 128), "head dim must be 64 or 128")
-    return kh, rows, d
 
 
-def _page_strides(keys: torch.Tensor, values: torch.Tensor):
-    page = keys.shape[1] * keys.shape[2] * keys.shape[3]
-    return tuple(t.stride(0) if t.shape[0] > 1 else page for t in (keys, values))
+class _Cache:
+    """A checked cache as numbers: pages, KV heads, page rows, head dim, pointers and page strides, ends."""
+
+    __slots__ = ("pages", "kh", "rows", "d", "k", "v", "ks", "vs", "kend", "vend")
+
+    def __init__(self, keys, values, dtype, index):
+        try:
+            n, kh, rows, d = shape = keys.shape
+            ks, k2, k1, k0 = keys.stride()
+            vs, v2, v1, v0 = values.stride()
+            k, v = keys.data_ptr(), values.data_ptr()
+            page = kh * rows * d
+            if n == 1:
+                ks = vs = page
+            if kh == 1:
+                k2 = v2 = rows * d
+            ok = (keys.dtype is dtype and values.dtype is dtype and values.shape == shape and page
+                  and keys.get_device() == index and values.get_device() == index and rows in _PAGE_ROWS
+                  and d in _HEAD_DIMS and k0 == 1 and v0 == 1 and k1 == d and v1 == d and k2 == v2 == rows * d
+                  and not ((ks | vs) & 7 or (k | v) & 15) and ks >= page and vs >= page)
+        except (AttributeError, ValueError, TypeError):
+            ok = False
+        if not ok:
+            _cache_refuse(keys, values, dtype, index)
+            raise ValueError("keys and values are not a paged cache")
+        self.pages, self.kh, self.rows, self.d, self.k, self.v, self.ks, self.vs = n, kh, rows, d, k, v, ks, vs
+        self.kend, self.vend = k + 2 * ((n - 1) * ks + page), v + 2 * ((n - 1) * vs + page)
 
 
-def _batch(table: torch.Tensor, lengths: torch.Tensor, starts, rows: int, dev):
-    """(B, W, table stride) of a checked batch."""
+def _batch_refuse(table, lengths, starts, rows, index):
     _require(isinstance(table, torch.Tensor) and table.dtype == torch.int32 and table.dim() == 2 and table.numel() > 0,
              "table must be an int32 [B, W] tensor")
-    _require(table.is_cuda and table.device == dev, f"table must be on {dev}")
+    _require(table.is_cuda and table.get_device() == index, f"table must be on cuda:{index}")
     b, w = table.shape
-    stride = table.stride(0) if b > 1 else w
-    _require((w == 1 or table.stride(1) == 1) and stride >= w, "a row of table must be contiguous")
+    _require((w == 1 or table.stride(1) == 1) and (b == 1 or table.stride(0) >= w), "a row of table must be contiguous")
     _require(b <= 65535 and w * rows <= 1 << 30, "at most 65535 sequences of 2^30 rows")
-    _cuda_contig("lengths", lengths, torch.int32, dev)
+    _cuda_contig("lengths", lengths, torch.int32, table.device)
     _require(lengths.numel() == b, "one length a sequence required")
     if starts is not None:
-        _cuda_contig("starts", starts, torch.int32, dev)
+        _cuda_contig("starts", starts, torch.int32, table.device)
         _require(starts.numel() == b + 1, "starts must hold one value a sequence and the end")
-    return b, w, stride
 
 
-def _heads(name: str, t: torch.Tensor):
-    """Row stride of ``[rows, heads, d]`` (or ``[rows, width]``) whose rows are contiguous, 16-byte aligned and apart."""
-    width = t[0].numel()
-    _require(t[0].is_contiguous(), f"a row of {name} must be contiguous")
-    stride = t.stride(0) if t.shape[0] > 1 else width
-    _require(stride >= width and stride % 8 == 0 and _aligned(t, 16), f"{name}: rows must be 16-byte aligned and must not overlap")
-    return stride
+def _batch(table, lengths, starts, rows, index):
+    """(B, W, table stride) of a checked batch."""
+    try:
+        b, w = table.shape
+        ts, t1 = table.stride()
+        if b == 1:
+            ts = w
+        ok = (table.dtype is torch.int32 and lengths.dtype is torch.int32 and table.get_device() == index
+              and lengths.get_device() == index and (t1 == 1 or w == 1) and ts >= w > 0 and 0 < b <= 65535
+              and w * rows <= 1 << 30 and lengths.numel() == b and lengths.is_contiguous()
+              and (starts is None or (starts.dtype is torch.int32 and starts.get_device() == index
+                                      and starts.numel() == b + 1 and starts.is_contiguous())))
+    except (AttributeError, ValueError):
+        ok = False
+    if not ok:
+        _batch_refuse(table, lengths, starts, rows, index)
+        raise ValueError("table, lengths and starts do not describe a batch")
+    return b, w, ts
 
 
-def _query(q: torch.Tensor):
+def _query(q):
+    """(tokens, heads, head dim, row stride, device index) of checked queries."""
     _require(isinstance(q, torch.Tensor) and q.dtype in _TYPES, "q must be a bf16 or fp16 tensor")
-    _require(q.is_cuda and q.dim() == 3 and q.numel() > 0, "q must be a CUDA (HIP) tensor [tokens, heads, head dim]")
-    return _heads("q", q)
+    index = q.get_device()
+    _require(index >= 0 and q.dim() == 3 and q.numel() > 0, "q must be a CUDA (HIP) tensor [tokens, heads, head dim]")
+    n, h, d = q.shape
+    stride, s1, s0 = q.stride()
+    if n == 1:
+        stride = h * d
+    _require((s0 == 1 or d == 1) and (s1 == d or h == 1), "a row of q must be contiguous")
+    _require(stride >= h * d and not (stride & 7 or q.data_ptr() & 15),
+             "q: rows must be 16-byte aligned and must not overlap")
+    return n, h, d, stride, index
+
+
+def _vector(name, t, n: int, dtype, index) -> int:
+    """The pointer of ``n`` checked values."""
+    _require(isinstance(t, torch.Tensor) and t.dtype is dtype, f"{name} must be a {dtype} tensor")
+    at = t.data_ptr()
+    _require(t.get_device() == index and t.numel() == n and t.is_contiguous() and not at & 15,
+             f"{name} must hold {n} values on cuda:{index}, contiguous and 16-byte aligned")
+    return at
+
+
+def _table(name, t, d: int, dtype, index):
+    """(pointer, rows) of a checked ``[positions, d]`` table."""
+    _require(isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 2 and t.shape[1] == d and t.shape[0] > 0,
+             f"{name} must be a {dtype} (cos and sin: or float32) [positions, {d}] table")
+    return _vector(name, t, t.numel(), dtype, index), t.shape[0]
 
 
 def _scale(scale, d: int) -> float:
-    scale = d ** -0.5 if scale is None else float(scale)
+    if scale is None:
+        return d ** -0.5
+    scale = float(scale)
     _require(scale == scale and abs(scale) != float("inf"), "scale must be finite")
     return scale
 
 
-def _output(out, shape, like: torch.Tensor, *others) -> torch.Tensor:
+def _apart(name: str, t: torch.Tensor, *spans) -> None:
+    """Raise when the contiguous tensor ``t`` shares memory with one of the (first, end) spans."""
+    at = t.data_ptr()
+    end = at + t.numel() * t.element_size()
+    for first, last in spans:
+        _require(end <= first or last <= at, f"{name} must not overlap the other tensors")
+
+
+def _output(out, rows: int, width: int, like: torch.Tensor, *spans) -> torch.Tensor:
+    """A new output (which shares no memory with anything), or the caller's, checked."""
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return like.new_empty((rows, width))
     _cuda_contig("out", out, like.dtype, like.device)
-    _require(out.numel() == shape[0] * shape[1] and _aligned(out, 16), f"out must hold {shape[0]} x {shape[1]} values, 16-byte aligned")
-    _require(not any(_overlap(out, t) for t in (like, *others)), "out must not overlap an input")
+    _require(out.numel() == rows * width and not out.data_ptr() & 15, f"out must hold {rows} x {width} values, 16-byte aligned")
+    _apart("out", out, *spans)
     return out
 
 
@@ -113,36 +176,40 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     to one rounding, where ``pointwise.qk_rope`` rounds after every step.  A token at a negative position (more tokens
     than its length) or without a page is written to no row; a position behind the tables takes their last row."""
     _require(isinstance(qkv, torch.Tensor) and qkv.dtype in _TYPES, "qkv must be a bf16 or fp16 tensor")
-    _require(qkv.is_cuda and qkv.dim() == 2 and qkv.numel() > 0, "qkv must be a CUDA (HIP) tensor [tokens, width]")
-    dev, dtype = qkv.device, qkv.dtype
-    qkv_stride = _heads("qkv", qkv)
-    kh, rows, d = _pages(keys, values, dtype, dev)
-    b, w, table_stride = _batch(table, lengths, starts, rows, dev)
+    index, dtype = qkv.get_device(), qkv.dtype
+    _require(index >= 0 and qkv.dim() == 2 and qkv.numel() > 0, "qkv must be a CUDA (HIP) tensor [tokens, width]")
     tokens, width = qkv.shape
+    stride, s0 = qkv.stride()
+    if tokens == 1:
+        stride = width
+    at = qkv.data_ptr()
+    _require(s0 == 1 or width == 1, "a row of qkv must be contiguous")
+    _require(stride >= width and not (stride & 7 or at & 15), "qkv: rows must be 16-byte aligned and must not overlap")
+    c = _Cache(keys, values, dtype, index)
+    kh, d = c.kh, c.d
+    b, w, table_stride = _batch(table, lengths, starts, c.rows, index)
     qh = width // d - 2 * kh
-    _require(width % d == 0 and qh > 0 and qh % kh == 0 and qh <= 1024,
+    _require(width % d == 0 and 0 < qh <= 1024 and qh % kh == 0,
              "qkv must hold a multiple of the KV heads as query heads, then the keys and the values")
     _require(starts is not None or tokens == b, "without starts, one token a sequence required")
-    _require((q_weight is None) == (k_weight is None), "both head-norm weights or none")
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None:
-            _cuda_contig(name, t, dtype, dev)
-            _require(t.numel() == d and _aligned(t, 16), f"{name} must hold {d} values, 16-byte aligned")
-    _require(isinstance(cos, torch.Tensor) and cos.dtype in (dtype, torch.float32), f"cos must be {dtype} or float32")
-    for name, t in (("cos", cos), ("sin", sin)):
-        _cuda_contig(name, t, cos.dtype, dev)
-        _require(t.dim() == 2 and t.shape == cos.shape and t.shape[0] > 0 and t.shape[1] == d and _aligned(t, 16),
-                 f"{name} must be a [positions, {d}] table, 16-byte aligned")
+    if q_weight is None or k_weight is None:
+        _require(q_weight is k_weight, "both head-norm weights or none")
+        qw = kw = None
+    else:
+        qw, kw = _vector("q_weight", q_weight, d, dtype, index), _vector("k_weight", k_weight, d, dtype, index)
+    f32 = isinstance(cos, torch.Tensor) and cos.dtype is torch.float32
+    cos_at, positions = _table("cos", cos, d, torch.float32 if f32 else dtype, index)
+    sin_at, others = _table("sin", sin, d, torch.float32 if f32 else dtype, index)
+    _require(positions == others, "cos and sin must hold the same positions")
     _require(eps >= 0, "eps must not be negative")
-    _require(tokens < 1 << 31 and cos.shape[0] < 1 << 31, "too many tokens or positions")
-    q = _output(out, (tokens, qh * d), qkv, keys, values).view(tokens, qh, d)
-    for t in (keys, values):
-        _require(not _overlap(t, qkv), "qkv must not overlap the cache")
-    native.call_on(qkv, "moss_paged_qk_rope", qkv.data_ptr(), qkv_stride, None if q_weight is None else q_weight.data_ptr(),
-                   None if k_weight is None else k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                   int(cos.dtype == torch.float32), cos.shape[0], q.data_ptr(), keys.data_ptr(), values.data_ptr(),
-                   *_page_strides(keys, values), keys.shape[0], rows, table.data_ptr(), table_stride, lengths.data_ptr(),
-                   None if starts is None else starts.data_ptr(), b, w, tokens, qh, kh, d, float(eps), _TYPES[dtype])
+    _require(tokens < 1 << 31, "too many tokens")
+    span = (at, at + 2 * ((tokens - 1) * stride + width))
+    _require((c.kend <= span[0] or span[1] <= c.k) and (c.vend <= span[0] or span[1] <= c.v),
+             "qkv must not overlap the cache")
+    q = _output(out, tokens, qh * d, qkv, span, (c.k, c.kend), (c.v, c.vend)).view(tokens, qh, d)
+    native.call_on(qkv, "moss_paged_qk_rope", at, stride, qw, kw, cos_at, sin_at, int(f32), positions, q.data_ptr(), c.k, c.v, c.ks, c.vs, c.pages, c.rows,
+                   table.data_ptr(), table_stride, lengths.data_ptr(), None if starts is None else starts.data_ptr(), b,
+                   w, tokens, qh, kh, d, eps, _TYPES[dtype])
     return q
 
 
@@ -160,25 +227,25 @@ def decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     """One new token per sequence: ``q`` ``[B, query heads, head dim]`` (rows may lie apart) against the
     ``lengths[b]`` rows of each sequence, the new token's own among them; ``scale`` defaults to head dim ** -0.5.
     Returns ``[B, query heads * head dim]``; a sequence without rows gives zeros."""
-    q_stride = _query(q)
-    dev = q.device
-    kh, rows, d = _pages(keys, values, q.dtype, dev)
-    b, w, table_stride = _batch(table, lengths, None, rows, dev)
-    qh = q.shape[1]
-    _require(q.shape[0] == b and q.shape[2] == d and qh % kh == 0 and qh <= 1024,
-             "q must be [B, a multiple of the KV heads, head dim]")
-    scale = _scale(scale, d)
+    n, qh, hd, stride, index = _query(q)
+    c = _Cache(keys, values, q.dtype, index)
+    kh, d = c.kh, c.d
+    b, w, table_stride = _batch(table, lengths, None, c.rows, index)
+    _require(n == b and hd == d and qh % kh == 0 and qh <= 1024, "q must be [B, a multiple of the KV heads, head dim]")
+    at = q.data_ptr()
+    spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
+    out = _output(out, b, qh * d, q, *spans)
+    nbytes = native.lib().moss_paged_decode_workspace_bytes(b, w, c.rows, qh, kh, d)
     if ws is None:
-        ws = decode_workspace(q, keys, table)
+        ws = q.new_empty(nbytes // 4, dtype=torch.float32)
     else:
-        _cuda_contig("ws", ws, torch.float32, dev)
-        _require(_aligned(ws, 16), "ws must be 16-byte aligned")
-    out = _output(out, (b, qh * d), q, keys, values)
-    _require(4 * ws.numel() >= native.lib().moss_paged_decode_workspace_bytes(b, w, rows, qh, kh, d), "workspace too small")
-    _require(not any(_overlap(ws, t) for t in (q, out, keys, values)), "the workspace must not overlap the tensors")
-    native.call_on(q, "moss_paged_decode_attention", q.data_ptr(), q_stride, keys.data_ptr(), values.data_ptr(),
-                   *_page_strides(keys, values), keys.shape[0], rows, table.data_ptr(), table_stride, lengths.data_ptr(),
-                   b, w, qh, kh, d, scale, out.data_ptr(), ws.data_ptr(), 4 * ws.numel(), _TYPES[q.dtype])
+        _cuda_contig("ws", ws, torch.float32, q.device)
+        _require(4 * ws.numel() >= nbytes and not ws.data_ptr() & 15, "workspace too small or not 16-byte aligned")
+        o = out.data_ptr()
+        _apart("ws", ws, (o, o + 2 * out.numel()), *spans)
+    native.call_on(q, "moss_paged_decode_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),
+                   table_stride, lengths.data_ptr(), b, w, qh, kh, d, _scale(scale, d), out.data_ptr(), ws.data_ptr(),
+                   nbytes, _TYPES[q.dtype])
     return out
 
 
@@ -189,17 +256,16 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     head dim]`` (rows may lie apart); each token attends its sequence's rows up to its own position, the cached
     ones before the new among them.  ``scale`` defaults to head dim ** -0.5.  Returns ``[T, query heads * head
     dim]``; a token without a visible row gives zeros."""
-    q_stride = _query(q)
-    dev = q.device
-    kh, rows, d = _pages(keys, values, q.dtype, dev)
+    n, qh, hd, stride, index = _query(q)
+    c = _Cache(keys, values, q.dtype, index)
+    kh, d = c.kh, c.d
     _require(starts is not None, "starts required")
-    b, w, table_stride = _batch(table, lengths, starts, rows, dev)
-    tokens, qh = q.shape[:2]
-    _require(q.shape[2] == d and qh % kh == 0 and qh <= 1024, "q must be [tokens, a multiple of the KV heads, head dim]")
-    _require(tokens <= 1 << 20, "at most 2^20 packed tokens")
-    scale = _scale(scale, d)
-    out = _output(out, (tokens, qh * d), q, keys, values)
-    native.call_on(q, "moss_paged_prompt_attention", q.data_ptr(), q_stride, keys.data_ptr(), values.data_ptr(),
-                   *_page_strides(keys, values), keys.shape[0], rows, table.data_ptr(), table_stride, lengths.data_ptr(),
-                   starts.data_ptr(), b, w, tokens, qh, kh, d, scale, out.data_ptr(), _TYPES[q.dtype])
+    b, w, table_stride = _batch(table, lengths, starts, c.rows, index)
+    _require(hd == d and qh % kh == 0 and qh <= 1024, "q must be [tokens, a multiple of the KV heads, head dim]")
+    _require(n <= 1 << 20, "at most 2^20 packed tokens")
+    at = q.data_ptr()
+    out = _output(out, n, qh * d, q, (at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
+    native.call_on(q, "moss_paged_prompt_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),
+                   table_stride, lengths.data_ptr(), starts.data_ptr(), b, w, n, qh, kh, d, _scale(scale, d),
+                   out.data_ptr(), _TYPES[q.dtype])
     return out
