@@ -465,11 +465,15 @@ int moss_paged_decode_attention(const void *q, long long q_stride, const void *k
 
 /* Causal attention of T packed tokens, q [T, qh, d] (rows q_stride elements apart), whose K / V rows are in the pages:
  * a token attends its sequence's rows up to its own position; out [T, qh * d].  Tokens without a visible row give
- * zeros.  Counterpart of moss_prefill_attention. */
+ * zeros.  A tile of tokens that sees far more rows than its share of the call's work is cut into parts, whose results
+ * the workspace holds (moss_paged_prompt_workspace_bytes, 0 for tables of up to 512 rows; 16-byte aligned; calls that
+ * overlap must not share one).  Counterpart of moss_prefill_attention. */
+long long moss_paged_prompt_workspace_bytes(int B, int W, int page_rows, int T, int qh, int kh, int d);
 int moss_paged_prompt_attention(const void *q, long long q_stride, const void *k, const void *v, long long k_stride,
                                 long long v_stride, int pages, int page_rows, const void *table,
                                 long long table_stride, const void *lengths, const void *starts, int B, int W, int T,
-                                int qh, int kh, int d, float scale, void *out, int dtype, void *stream);
+                                int qh, int kh, int d, float scale, void *out, void *workspace,
+                                long long workspace_bytes, int dtype, void *stream);
 
 /* ------------------------------------------------------- measurement */
 /* No counterpart in the reference: a streaming read for bench.py, which times it on the bytes of a

@@ -53,6 +53,72 @@ MOSS_HD void share_rows(int rows, int count, int index, int& r0, int& r1) {
     r0 = from < rows ? (int)from : rows;
     r1 = to < rows ? (int)to : rows;
 }
+
+// Prompt work: tiles of kPromptRows (token, head) rows, which see keys up to their last row's position, in blocks of
+// kPromptBlock keys; a tile of more than `share` blocks is cut into parts of that many.  The sum of all tiles' blocks is
+// at most `shares` times the share, so at most `shares` parts come on top of the tiles and the parts of the cut tiles are at
+// most twice as many.
+constexpr int kPromptRows = 128, kPromptBlock = 64, kPromptShare = 8;
+struct PromptTiles {
+    int tokens, group, pos0;  // new tokens of a sequence, query heads per KV head, position of the first one
+    MOSS_HD int rows() const { return tokens * group; }
+    MOSS_HD int tiles() const { return (rows() + kPromptRows - 1) / kPromptRows; }
+    MOSS_HD int last_key(int tile) const {  // -1 and below: none
+        const int row = (tile + 1) * kPromptRows - 1;
+        return pos0 + (row < rows() - 1 ? row : rows() - 1) / group;
+    }
+    MOSS_HD int blocks(int tile) const {
+        const int last = last_key(tile);
+        return last < 0 ? 0 : last / kPromptBlock + 1;
+    }
+    // tiles, the last ones, of more than `blocks` (> 0) blocks
+    MOSS_HD int tiles_over(int blocks) const {
+        const long long y = (long long)blocks * kPromptBlock - pos0;  // tokens before the first that sees so many
+        const int n = tiles();
+        if (y <= 0) return n;
+        if (y > tokens - 1) return 0;
+        const int first = (int)((y * group + kPromptRows) / kPromptRows) - 1;  // ceil((y group + 1) / rows) - 1
+        return (first < n - 1 ? n - 1 - first : 0) + 1;
+    }
+    // no less than the sum of blocks() over the tiles
+    MOSS_HD long long blocks_bound() const {
+        const int n = tiles();
+        if (n == 0) return 0;
+        const long long end = (long long)pos0 + ((long long)n * kPromptRows - 1) / group;
+        return ((long long)n * (blocks(0) + (end < 0 ? 0 : end / kPromptBlock + 1) + 2) + 1) / 2;
+    }
+    MOSS_HD int items(int share) const {
+        int n = tiles();
+        for (int k = 1, c = 1; c > 0; ++k) n += c = tiles_over(k * share);
+        return n;
+    }
+    MOSS_HD int parts(int share) const {
+        int n = tiles_over(share);
+        for (int k = 1, c = 1; c > 0; ++k) n += c = tiles_over(k * share);
+        return n;
+    }
+};
+MOSS_HD int prompt_share(long long blocks, int shares) {
+    const long long share = (blocks + shares - 1) / shares;
+    return share < kPromptShare ? kPromptShare : share < (1 << 24) ? (int)share : 1 << 24;
+}
+// A sequence's item: part `part` of `count` of tile `tile`, whose first partial result is number `slot` (of the
+// sequence's; its parts are tiles_over(share) apart at part 0 and then as the parts are listed).
+struct PromptItem {
+    int tile, part, slot;
+};
+MOSS_HD PromptItem prompt_item(const PromptTiles& t, int share, int index) {
+    const int n = t.tiles();
+    if (index < n) return PromptItem{n - 1 - index, 0, index};  // parts 0: of the cut tiles the first numbers
+    int slot = t.tiles_over(share);
+    index -= n;
+    for (int k = 1;; ++k) {
+        const int c = t.tiles_over(k * share);
+        if (index < c || c == 0) return PromptItem{n - 1 - index, k, slot + index};
+        index -= c;
+        slot += c;
+    }
+}
 inline long long decode_slots(int B, int W, int shift, int shares) {
     const long long most = (long long)B * ((((long long)W << shift) + kUnit - 1) / kUnit);
     return (long long)B + shares < most ? (long long)B + shares : most;

@@ -5,17 +5,20 @@
 // the new ones up to itself (all written).  o_h = sum_t softmax_t(scale q_h . k_t) v_t with query head h reading KV head
 // h / (QH / KH); a token without a visible row gives zeros; tokens behind the last sequence are left alone.
 //
-// Tiling: the rows of a tile are (token, query head of the KV head's group) pairs, token first, so any group size fills
-// them.  A workgroup takes 32 RW rows of one sequence and KV head; a wave takes 32 rows and, of every block of keys, the
-// 32-key tiles ks, ks + KS, .. (SUB of them).  Which sequence and rows a workgroup has follows from starts on the device;
-// the last rows, which see the most keys, go first.
+// Work: the rows of a tile are (token, query head of the KV head's group) pairs, token first, so any group size fills
+// them.  A workgroup takes 128 rows of one sequence and KV head, a wave 32 of them, over all keys or, where a tile sees
+// many more than a workgroup's fair share of the whole call (a few new tokens behind a long prefix), over a part of them:
+// such parts leave (m, l, O) in a workspace, and a second launch joins them.  Who takes what follows from starts and lengths
+// on the device (paged_index.h).
 //   S^T = K Q^T: 32 keys x 32 rows per matrix instruction, so a lane holds one row and 16 of its keys, and the row's
 //   maximum needs one exchange with the lane 32 away; the running maximum and sum are fp32, base 2.
-//   O^T += V^T P^T: P, rounded to 16 bits, is the B operand as S^T left it; V^T is read from LDS in the same K order.
-// P's rounding is the one step with fewer bits before the output: the largest P of a tile is exactly 1 or its
+//   O^T += V^T P^T: P, rounded to 16 bits, is the B operand as S^T left it.
+// P's rounding is the one step with fewer bits before the output: the largest P of a block is exactly 1 or its
 // share of the running maximum, and the sum adds up the unrounded values.
-// K / V blocks go from the pages through registers into two LDS stages (V transposed); block b + 2 is on its way while
-// block b is consumed and b + 1 waits: one barrier per block.  The KS waves of the same rows are joined in LDS at the end.
+// Blocks of 64 keys go from the pages straight into LDS (buffer loads, 16 rows of K and of V a wave, which lie in one page;
+// rows that nobody sees or that have no page are read as zeros: past the buffer's end), into one of two stages while the
+// other is consumed: one barrier per block, no registers.  V is read transposed (ds_read_b64_tr_b16: a lane gets one
+// dim of 4 rows).  16-byte chunk c of row r lies at c ^ f(r), which spreads the rows of one read over the banks.
 #include "paged.h"
 
 namespace moss {
@@ -25,69 +28,89 @@ struct PromptArgs {
     const uint16_t* q;
     long long q_stride;
     uint16_t* out;
-    int T, qh, group;
+    float* part;   // [slots, KH, D / 4, 128 rows] of 4: O of each part
+    float2* stat;  // [slots, KH, 128]: its m and l
+    int T, qh, group, shares;
+    long long slots;
     float scale;    // |scale| log2(e), not 0: a masked score stays -inf
     uint32_t flip;  // its sign, for the two values of a word of q
 };
 
-template <int D, int RW, int KS, int SUB>
-struct PromptTile {
-    static constexpr int kRows = 32 * RW, kThreads = 64 * RW * KS;
-    static constexpr int kBK = 32 * SUB * KS;                // keys per block
-    static constexpr int kDC = D / 8;                        // 16-byte pieces of a row
-    static constexpr int kKPT = kBK * kDC / kThreads;        // keys per thread in the copy
-    static constexpr int kKPad = D + 8, kVPad = kBK + 4;     // LDS rows (16-bit values), padded
-    static constexpr int kKBytes = kBK * kKPad * 2;
-    static constexpr int kFlags = kKBytes + D * kVPad * 2;   // one byte per 16 keys: they have a page
-    static constexpr int kStage = kFlags + 16;
-    static constexpr int kXo = RW * (D / 32) * (KS - 1) * 4 * 64 * 16;  // O^T tiles handed over
-    static constexpr int kMl = RW * KS * 2 * 64 * 4;
-    static constexpr int kJoin = KS > 1 ? kXo + kMl : 0;
-    static constexpr int kLds = 2 * kStage > kJoin ? 2 * kStage : kJoin;
-    static_assert(kKPT == 1 || kKPT == 2 || kKPT == 4, "keys per thread in the copy");
-    static_assert(kBK / 16 <= 16 && kKBytes % 16 == 0 && kStage % 16 == 0 && kXo % 16 == 0, "LDS layout");
-    static_assert(kLds <= 160 * 1024, "LDS");
-};
+__device__ __forceinline__ PromptTiles prompt_tiles(const PagedBatch& bt, int b, int T, int group, int shift) {
+    const int n = paged_tokens(bt, b, T).y;
+    return PromptTiles{n, group, paged_length(bt, b, shift) - n};
+}
 
-__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
-__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+// Blocks in a part: from all sequences' tiles, over the KV head's fair shares.
+__device__ __forceinline__ int prompt_share_of(const PagedBatch& bt, int T, int group, int shift, int shares, int lane) {
+    long long blocks = 0;
+    for (int b = lane; b < bt.B; b += kWave) blocks += prompt_tiles(bt, b, T, group, shift).blocks_bound();
+    return __builtin_amdgcn_readfirstlane(prompt_share(wave_total(blocks), shares));
+}
 
-// V^T column of key `key` in row d: 8-key groups are swapped by XOR with 8 (d / 32), so the 16 rows that one store writes
-// land in different banks; 4-key groups stay whole, and the rows of one read share d / 32.
-__device__ __forceinline__ int vt_column(int d, int key) { return key ^ (8 * ((d >> 5) & 3)); }
+// Partial results of the sequences before b.
+__device__ __forceinline__ int parts_before(const PagedBatch& bt, int b, int T, int group, int shift, int share, int lane) {
+    int n = 0;
+    for (int s = lane; s < b; s += kWave) {
+        const PromptTiles t = prompt_tiles(bt, s, T, group, shift);
+        if (t.tiles_over(share)) n += t.parts(share);
+    }
+    return wave_total(n);
+}
 
-template <typename E, int D, int RW, int KS, int SUB>
-__global__ __launch_bounds__(64 * RW * KS, (RW * KS > 4 ? 1 : 2)) void paged_prompt_kernel(PromptArgs a, PagedCache c,
-                                                                                           PagedBatch bt) {
-    using T = PromptTile<D, RW, KS, SUB>;
-    constexpr int KPT = T::kKPT, BK = T::kBK, KPAD = T::kKPad, VPAD = T::kVPad, DT = D / 32, DK = D / 16;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[T::kLds];
+// Where 16-byte chunk c of key row r lies in its LDS row: c ^ f(r).
+template <int D>
+__device__ __forceinline__ int k_swizzle(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+template <int D>
+__device__ __forceinline__ int v_swizzle(int r) {
+    return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r >> 1 & 1) << 2) | ((r >> 2) & 3);
+}
+
+// 16 bytes per lane straight to lds + 16 lane.  (In a function of its own: the host's pass drops a kernel that names a
+// builtin it does not know.)
+__device__ __forceinline__ void copy16(const Span& s, unsigned char* lds, uint32_t voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(span_rsrc(s), lds, 16, voff, 0, 0, 0);
+}
+
+typedef short s16x4_v __attribute__((ext_vector_type(4)));
+// 4 rows of one dim: a 16-lane group reads 4 rows of 16 dims, lane i the 8 bytes of row i / 4 from dim 4 (i % 4) on.
+__device__ __forceinline__ u32x2_v read_transposed(const unsigned char* p) {
+    return __builtin_bit_cast(u32x2_v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_v*)p));
+}
+
+template <typename E, int D>
+__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PromptArgs a, PagedCache c, PagedBatch bt) {
+    constexpr int BK = kPromptBlock, DT = D / 32, DK = D / 16, RB = 2 * D;  // RB: bytes of a row
+    constexpr int KB = BK * RB, NL = 16 * RB / 1024, RPL = 1024 / RB, CPR = D / 8;  // loads of 16 rows, rows of a load
+    // two stages of K | V: two variables, so that reading one does not wait for the loads into the other
+    __shared__ __attribute__((aligned(1024))) unsigned char even[2 * KB], odd[2 * KB];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, rl = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, kq = wave / RW;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x % c.kh, G = a.group;  // neighbours in the grid, which lie on different XCDs, differ in it
-    const Place pl = find_item(bt.B, (int)((gridDim.x - 1 - blockIdx.x) / c.kh), lane, [&](int b) {
-        return (int)(((long long)paged_tokens(bt, b, a.T).y * G + T::kRows - 1) / T::kRows);
-    });
+    const int share = prompt_share_of(bt, a.T, G, c.shift, a.shares, lane);
+    const Place pl = find_item(bt.B, (int)(blockIdx.x / c.kh), lane,
+                               [&](int b) { return prompt_tiles(bt, b, a.T, G, c.shift).items(share); });
     if (pl.b < 0) return;
-    const int2 tk = paged_tokens(bt, pl.b, a.T);
-    const int len = paged_length(bt, pl.b, c.shift);
-    const int pos0 = len - tk.y;  // position of the sequence's first new token (negative: it has none)
-    const int row0 = pl.index * T::kRows, nrows = tk.y * G;
-    const int row = min(row0 + 32 * rw + rl, nrows - 1);  // this lane's row (clamped: stores are guarded)
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // it is; this puts it into a scalar
+    const int sequence = uniform(pl.b), tok0 = uniform(paged_tokens(bt, sequence, a.T).x);
+    const PromptTiles all = prompt_tiles(bt, sequence, a.T, G, c.shift);
+    const PromptTiles tiles{uniform(all.tokens), G, uniform(all.pos0)};
+    const PromptItem found = prompt_item(tiles, share, uniform(pl.index));
+    const PromptItem item{uniform(found.tile), uniform(found.part), uniform(found.slot)};
+    const int pos0 = tiles.pos0;
+    const int row0 = item.tile * kPromptRows, nrows = tiles.rows();
+    const int row = min(row0 + 32 * wave + rl, nrows - 1);  // this lane's row (clamped: stores are guarded)
     const int token = row / G, head = kvh * G + row % G;
     const int qpos = pos0 + token;  // sees keys 0 .. qpos
-    const int last = pos0 + min(row0 + T::kRows - 1, nrows - 1) / G;         // the workgroup's last key
-    const int wave_last = pos0 + min(row0 + 32 * rw + 31, nrows - 1) / G;    // this wave's
-    const int wave_first = pos0 + min(row0 + 32 * rw, nrows - 1) / G;        // keys up to it are seen by all its rows
-    const int nblk = last / BK + (last >= 0 ? 1 : 0);
-
-    auto stage_k = [&](int s) { return reinterpret_cast<uint16_t(*)[KPAD]>(smem + s * T::kStage); };
-    auto stage_v = [&](int s) { return reinterpret_cast<uint16_t(*)[VPAD]>(smem + s * T::kStage + T::kKBytes); };
-    auto stage_f = [&](int s) { return smem + s * T::kStage + T::kFlags; };
+    const int last = uniform(tiles.last_key(item.tile)), blocks = uniform(tiles.blocks(item.tile));  // the workgroup's last key
+    const bool cut = blocks > share, idle = row0 + 32 * wave >= nrows;             // idle: no row of this wave's exists
+    const int wave_last = uniform(pos0 + min(row0 + 32 * wave + 31, nrows - 1) / G);
+    const int wave_first = uniform(pos0 + min(row0 + 32 * wave, nrows - 1) / G);  // keys up to it are seen by all its rows
+    const int b0 = uniform(item.part * share), b1 = uniform(min(blocks, b0 + share));
 
     u32x4_t qf[DK];  // lane: row rl, dims 16 kk + 8 half .. + 7
     {
-        const uint16_t* qr = a.q + (size_t)(tk.x + token) * a.q_stride + (size_t)head * D + 8 * half;
+        const uint16_t* qr = a.q + (size_t)(tok0 + token) * a.q_stride + (size_t)head * D + 8 * half;
 #pragma unroll
         for (int kk = 0; kk < DK; ++kk) qf[kk] = *reinterpret_cast<const u32x4_t*>(qr + 16 * kk) ^ a.flip;
     }
@@ -96,243 +119,224 @@ __global__ __launch_bounds__(64 * RW * KS, (RW * KS > 4 ? 1 : 2)) void paged_pro
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // l: this lane's keys only
 
-    // the copy: thread (kg, dc) holds keys KPT kg .. of a block (all in one 16-row group) at dims 8 dc .. + 7
-    const int dc = tid % T::kDC, kg = tid / T::kDC;
-    const int* trow = bt.table + (size_t)pl.b * bt.table_stride;
-    auto page_of = [&](int b) {
-        const int key = BK * b + KPT * kg;
-        return key <= last ? page_or_none(trow[key >> c.shift], c.pages) : -1;
+    // pages: lane i holds that of 16-row group i of 16 blocks (-1: none, or behind the last key); bit i of `there` says
+    // that the group's rows up to the last key exist
+    const int* trow = bt.table + (size_t)sequence * bt.table_stride;
+    int pages = -1;
+    unsigned long long there = 0, there_next = 0;
+    auto fetch_pages = [&](int b) {
+        const int key = BK * b + 16 * lane;
+        pages = key <= last ? page_or_none(trow[key >> c.shift], c.pages) : -1;
+        there_next = __ballot(pages >= 0 || key > last);
     };
-    u32x4_t kr[KPT], vr[KPT];
-    bool have = false;
-    auto load = [&](int b, int page) {
-        const int key = BK * b + KPT * kg;
-        have = page >= 0;
-        const uint16_t* kp = c.k + row_offset(page, c.k_stride, kvh, key, c.shift, D) + 8 * dc;
-        const uint16_t* vp = c.v + row_offset(page, c.v_stride, kvh, key, c.shift, D) + 8 * dc;
+    // LDS offsets: this lane's part of a load, and what it reads
+    uint32_t kload[NL], vload[NL];
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            kr[i] = *reinterpret_cast<const u32x4_t*>(kp + (size_t)i * D);
-            vr[i] = *reinterpret_cast<const u32x4_t*>(vp + (size_t)i * D);
-        }
-    };
-    auto store = [&](int b) {
-        uint16_t(*ks)[KPAD] = stage_k(b & 1);
-        uint16_t(*vt)[VPAD] = stage_v(b & 1);
-        const int key = BK * b + KPT * kg;
-#pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            *reinterpret_cast<u32x4_t*>(&ks[KPT * kg + i][8 * dc]) = kr[i];
-            // rows that nobody sees may hold anything, and 0 times a NaN is one
-            if (!have || key + i > last) vr[i] = u32x4_t{0u, 0u, 0u, 0u};
-        }
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            uint16_t* even = &vt[8 * dc + 2 * p][vt_column(8 * dc, KPT * kg)];
-            uint16_t* odd = &vt[8 * dc + 2 * p + 1][vt_column(8 * dc, KPT * kg)];
-            if constexpr (KPT == 4) {
-                *reinterpret_cast<uint2*>(even) = make_uint2(low_halves(vr[0][p], vr[1][p]), low_halves(vr[2][p], vr[3][p]));
-                *reinterpret_cast<uint2*>(odd) = make_uint2(high_halves(vr[0][p], vr[1][p]), high_halves(vr[2][p], vr[3][p]));
-            } else if constexpr (KPT == 2) {
-                *reinterpret_cast<uint32_t*>(even) = low_halves(vr[0][p], vr[1][p]);
-                *reinterpret_cast<uint32_t*>(odd) = high_halves(vr[0][p], vr[1][p]);
-            } else {
-                *even = (uint16_t)vr[0][p];
-                *odd = (uint16_t)(vr[0][p] >> 16);
-            }
-        }
-        if (dc == 0 && (KPT * kg) % 16 == 0) stage_f(b & 1)[KPT * kg / 16] = have ? 1 : 0;
-    };
-
-    int page = -1;
-    if (nblk > 0) {
-        load(0, page_of(0));
-        page = page_of(1);
-        store(0);
-        if (nblk > 1) {
-            load(1, page);
-            page = page_of(2);
-        }
+    for (int j = 0; j < NL; ++j) {
+        const int r = j * RPL + lane / CPR, slot = lane % CPR;
+        kload[j] = (uint32_t)(r * RB + 16 * (slot ^ k_swizzle<D>(r)));
+        vload[j] = (uint32_t)(r * RB + 16 * (slot ^ v_swizzle<D>(r)));
     }
-    for (int b = 0; b < nblk; ++b) {
-        // block b is staged by every wave, and every wave is done with block b - 1's stage
+    auto copy = [&](unsigned char* stage, int b) {  // block b's rows 16 wave .. + 15
+        if (((b - b0) & 15) == 0) fetch_pages(b);
+        const int page = __builtin_amdgcn_readlane(pages, 4 * ((b - b0) & 15) + wave), key = BK * b + 16 * wave;
+        const uint32_t bytes = (uint32_t)uniform(page < 0 ? 0 : min(max(last + 1 - key, 0), 16) * RB);
+        const Span ks{c.k + row_offset(page, c.k_stride, kvh, key, c.shift, D), bytes};
+        const Span vs{c.v + row_offset(page, c.v_stride, kvh, key, c.shift, D), bytes};
+        unsigned char* at = stage + 16 * RB * wave;
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            copy16(ks, at + 1024 * j, kload[j]);
+            copy16(vs, at + KB + 1024 * j, vload[j]);
+        }
+    };
+    uint32_t kread[DK], vread[2][DT];
+#pragma unroll
+    for (int kk = 0; kk < DK; ++kk) kread[kk] = (uint32_t)(rl * RB + 16 * ((2 * kk + half) ^ k_swizzle<D>(rl)));
+    {
+        const int i = lane & 15, r = 4 * half + (i >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                vread[s2][dt] = (uint32_t)((r + 8 * s2) * RB + 16 * ((4 * dt + chunk) ^ v_swizzle<D>(r + 8 * s2)) + 8 * (i & 1));
+    }
+
+    auto block = [&](const unsigned char* ks, unsigned char* next, int b) {
+        // this wave's rows of block b are there, then everyone's; and everyone is done with block b - 1's stage
+        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0)
         __syncthreads();
-        const uint16_t(*ks)[KPAD] = stage_k(b & 1);
-        const uint16_t(*vt)[VPAD] = stage_v(b & 1);
-        const unsigned char* flags = stage_f(b & 1);
-        const int part = 32 * kq;
-        if (BK * b + part <= wave_last) {  // else none of its rows sees any of its keys
-            f32x16_v s[SUB];
+        if (((b - b0) & 15) == 0) there = there_next;
+        const unsigned int groups = (unsigned int)(there >> (4 * ((b - b0) & 15))) & 15u;
+        if (b + 1 < b1) copy(next, b + 1);
+        if (idle || BK * b > wave_last) return;  // none of its rows sees any of its keys
+        const unsigned char* vs = ks + KB;
+        f32x16_v s[2];
+        s[0] = f32x16_v{};
+        s[1] = f32x16_v{};
 #pragma unroll
-            for (int i = 0; i < SUB; ++i) s[i] = f32x16_v{};
+        for (int kk = 0; kk < DK; ++kk)
 #pragma unroll
-            for (int kk = 0; kk < DK; ++kk)
+            for (int i = 0; i < 2; ++i)
+                s[i] = E::mfma32(*reinterpret_cast<const u32x4_t*>(ks + kread[kk] + 32 * RB * i), qf[kk], s[i]);
+        // element e of tile i: key BK b + 32 i + 8 (e / 4) + 4 half + e % 4, row rl
+        if (groups != 15u || BK * b + BK - 1 > wave_first) {
 #pragma unroll
-                for (int i = 0; i < SUB; ++i) {
-                    const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(&ks[part + 32 * KS * i + rl][16 * kk + 8 * half]);
-                    s[i] = E::mfma32(kf, qf[kk], s[i]);
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = BK * b + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3);
+                    s[i][e] = key <= qpos && (groups >> (2 * i + (e >> 3)) & 1) ? s[i][e] : -INFINITY;
                 }
-            // element e of tile i: key BK b + part + 32 KS i + 8 (e / 4) + 4 half + e % 4, row rl
-            bool holes = false;
-#pragma unroll
-            for (int i = 0; i < SUB; ++i) {
-                const int f = (part + 32 * KS * i) / 16;
-                holes |= !(flags[f] & flags[f + 1]);
-            }
-            if (__any(holes) || BK * b + BK - 1 > wave_first) {
-#pragma unroll
-                for (int i = 0; i < SUB; ++i) {
-                    const int tile = part + 32 * KS * i;
-                    const bool f0 = flags[tile / 16], f1 = flags[tile / 16 + 1];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = BK * b + tile + 8 * (e >> 2) + 4 * half + (e & 3);
-                        s[i][e] = key <= qpos && (e < 8 ? f0 : f1) ? s[i][e] : -INFINITY;
-                    }
-                }
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < SUB; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[i][e]);
-            mx = max_xor32(mx) * a.scale;
-            if (__any(mx > m)) {
-                const float mn = fmaxf(m, mx);
-                const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[d][e] *= f;
-            }
-            const float mr = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int i = 0; i < SUB; ++i) {
-                u32x4_t pf[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * v], a.scale, -mr));
-                        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * v + 1], a.scale, -mr));
-                        l += p0 + p1;
-                        pf[u][v] = E::pack(p0, p1);
-                    }
-                // K step u: keys 16 u + {4 half + 0..3, 8 + 4 half + 0..3} of the tile
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int key = part + 32 * KS * i + 16 * u + 4 * half;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const uint16_t* vrow = vt[32 * dt + rl];
-                        const uint2 a0 = *reinterpret_cast<const uint2*>(vrow + vt_column(32 * dt, key));
-                        const uint2 a1 = *reinterpret_cast<const uint2*>(vrow + vt_column(32 * dt, key + 8));
-                        o[dt] = E::mfma32(u32x4_t{a0.x, a0.y, a1.x, a1.y}, pf[u], o[dt]);
-                    }
-                }
-            }
         }
-        if (b + 1 < nblk) {  // block b + 1's stage was last read for block b - 1
-            store(b + 1);
-            if (b + 2 < nblk) {
-                load(b + 2, page);
-                page = page_of(b + 3);
-            }
+        float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(fmaxf(mx, s[0][e]), s[1][e]);
+        mx = max_xor32(mx) * a.scale;
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= f;
         }
+        const float mr = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u32x4_t pf[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * v], a.scale, -mr));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * v + 1], a.scale, -mr));
+                    l += p0 + p1;
+                    pf[u][v] = E::pack(p0, p1);
+                }
+            // K step u: keys 16 u + {4 half + 0..3, 8 + 4 half + 0..3} of the tile
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const u32x2_v a0 = read_transposed(vs + vread[0][dt] + (32 * i + 16 * u) * RB);
+                    const u32x2_v a1 = read_transposed(vs + vread[1][dt] + (32 * i + 16 * u) * RB);
+                    o[dt] = E::mfma32(u32x4_t{a0[0], a0[1], a1[0], a1[1]}, pf[u], o[dt]);
+                }
+        }
+    };
+    if (b0 < b1) copy(even, b0);
+    for (int b = b0; b < b1; b += 2) {
+        block(even, odd, b);
+        if (b + 1 < b1) block(odd, even, b + 1);
     }
     l = sum_xor32(l);
-    float inv;
-    if constexpr (KS == 1) {
-        inv = l == 0.f ? 0.f : 1.0f / l;
-    } else {
-        // each of a row's KS waves finishes the d tiles dt with dt % KS == kq from all of them
-        __syncthreads();
-        float4* xo = reinterpret_cast<float4*>(smem);  // [RW][dt][KS - 1 slots][e / 4][lane]
-        float* ml = reinterpret_cast<float*>(smem + T::kXo);
-        ml[((rw * KS + kq) * 2) * 64 + lane] = m;
-        ml[((rw * KS + kq) * 2 + 1) * 64 + lane] = l;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const int owner = dt % KS;
-            if (owner == kq) continue;
-            const int slot = kq < owner ? kq : kq - 1;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                xo[(((rw * DT + dt) * (KS - 1) + slot) * 4 + j) * 64 + lane] =
-                    make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
-        }
-        __syncthreads();
-        float f[KS], mx = -INFINITY, den = 0.f;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            f[j] = ml[((rw * KS + j) * 2) * 64 + lane];
-            mx = fmaxf(mx, f[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            f[j] = f[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(f[j] - mx);
-            den = fmaf(ml[((rw * KS + j) * 2 + 1) * 64 + lane], f[j], den);
-        }
-        inv = den == 0.f ? 0.f : 1.0f / den;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const int owner = dt % KS;
-            if (owner != kq) continue;
-#pragma unroll
-            for (int j4 = 0; j4 < 4; ++j4) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    float4 w;
-                    if (j == kq) {
-                        w = make_float4(o[dt][4 * j4], o[dt][4 * j4 + 1], o[dt][4 * j4 + 2], o[dt][4 * j4 + 3]);
-                    } else {
-                        const int slot = j < owner ? j : j - 1;
-                        w = xo[(((rw * DT + dt) * (KS - 1) + slot) * 4 + j4) * 64 + lane];
-                    }
-                    acc[0] = fmaf(w.x, f[j], acc[0]);
-                    acc[1] = fmaf(w.y, f[j], acc[1]);
-                    acc[2] = fmaf(w.z, f[j], acc[2]);
-                    acc[3] = fmaf(w.w, f[j], acc[3]);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[dt][4 * j4 + i] = acc[i];
-            }
-        }
-    }
-    if (row0 + 32 * rw + rl >= nrows) return;
-    uint16_t* dst = a.out + ((size_t)(tk.x + token) * a.qh + head) * D;
     // O^T element e of d tile dt: d = 32 dt + 8 (e / 4) + 4 half + e % 4
+    if (cut) {
+        const int before = parts_before(bt, sequence, a.T, G, c.shift, share, lane);
+        // (starts that do not rise can name more parts than there are tokens for: they have no slot)
+        if (row0 + 32 * wave + rl >= nrows || before + item.slot >= a.slots) return;
+        const size_t at = (size_t)(before + item.slot) * c.kh + kvh;
+        float4* part = reinterpret_cast<float4*>(a.part) + at * (D / 4) * kPromptRows + 32 * wave + rl;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-        if (dt % KS != kq) continue;
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                part[(8 * dt + 2 * q4 + half) * kPromptRows] =
+                    make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
+        if (half == 0) a.stat[at * kPromptRows + 32 * wave + rl] = make_float2(m, l);
+        return;
+    }
+    if (row0 + 32 * wave + rl >= nrows) return;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t* dst = a.out + ((size_t)(tok0 + token) * a.qh + head) * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
             *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * q4 + 4 * half) =
                 make_uint2(E::pack(o[dt][4 * q4] * inv, o[dt][4 * q4 + 1] * inv),
                            E::pack(o[dt][4 * q4 + 2] * inv, o[dt][4 * q4 + 3] * inv));
-    }
 }
 
-template <typename E, int D, int RW, int KS, int SUB>
-int launch_prompt_tile(const PromptArgs& a, const PagedCache& c, const PagedBatch& bt, hipStream_t st) {
-    using T = PromptTile<D, RW, KS, SUB>;
-    const long long groups = (((long long)a.T * a.group + T::kRows - 1) / T::kRows + bt.B) * c.kh;
-    MOSS_CHECK_ARG(groups * T::kThreads < (1ll << 32));
-    hipLaunchKernelGGL((paged_prompt_kernel<E, D, RW, KS, SUB>), dim3((unsigned)groups), dim3(T::kThreads), 0, st, a, c,
-                       bt);
-    return moss_launch_status();
+// The parts of one cut tile and KV head, 256 threads: thread (row, h) takes the 4-dim pieces h, h + 2, .. of the row.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void paged_prompt_join(PromptArgs a, PagedCache c, PagedBatch bt) {
+    const int lane = threadIdx.x & 63, r = threadIdx.x & 127, h = threadIdx.x >> 7, kvh = blockIdx.x % c.kh, G = a.group;
+    const int share = prompt_share_of(bt, a.T, G, c.shift, a.shares, lane);
+    const Place pl = find_item(bt.B, (int)(blockIdx.x / c.kh), lane,
+                               [&](int b) { return prompt_tiles(bt, b, a.T, G, c.shift).tiles_over(share); });
+    if (pl.b < 0) return;
+    const PromptTiles tiles = prompt_tiles(bt, pl.b, a.T, G, c.shift);
+    const int tile = tiles.tiles() - 1 - pl.index, row = tile * kPromptRows + r;
+    const int count = (tiles.blocks(tile) + share - 1) / share;
+    const int before = parts_before(bt, pl.b, a.T, G, c.shift, share, lane);
+    // part k's slot: the cut tiles' parts 0, then the tiles' of more than k shares
+    auto number_of = [&](int k) {
+        int slot = before + pl.index;
+        for (int i = 0; i < k; ++i) slot += tiles.tiles_over(i ? i * share : share);
+        return slot;
+    };
+    auto slot_of = [&](int k) { return ((size_t)number_of(k) * c.kh + kvh) * kPromptRows; };
+    if (row >= tiles.rows() || number_of(count - 1) >= a.slots) return;
+    float mx = -INFINITY, den = 0.f;
+    for (int k = 0; k < count; ++k) mx = fmaxf(mx, a.stat[slot_of(k) + r].x);
+    float4 acc[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < count; ++k) {
+        const size_t at = slot_of(k);
+        const float2 st = a.stat[at + r];
+        const float f = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - mx);
+        den = fmaf(f, st.y, den);
+        const float4* part = reinterpret_cast<const float4*>(a.part) + at * (D / 4) + r;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            const float4 v = part[(2 * i + h) * kPromptRows];
+            acc[i].x = fmaf(f, v.x, acc[i].x);
+            acc[i].y = fmaf(f, v.y, acc[i].y);
+            acc[i].z = fmaf(f, v.z, acc[i].z);
+            acc[i].w = fmaf(f, v.w, acc[i].w);
+        }
+    }
+    const float inv = den == 0.f ? 0.f : 1.0f / den;
+    uint16_t* dst = a.out + ((size_t)(paged_tokens(bt, pl.b, a.T).x + row / G) * a.qh + kvh * G + row % G) * D;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<uint2*>(dst + 4 * (2 * i + h)) =
+            make_uint2(E::pack(acc[i].x * inv, acc[i].y * inv), E::pack(acc[i].z * inv, acc[i].w * inv));
+}
+
+// Tiles at most, shares of a KV head, partial results at most (0: no tile can see more than a share's least blocks).
+struct PromptPlan {
+    long long tiles, slots;
+    int shares;
+};
+constexpr int kShares = 512;  // workgroups of all KV heads that the work is shared out over: two a CU
+
+PromptPlan prompt_plan(int B, int W, int shift, int T, int qh, int kh) {
+    PromptPlan p;
+    p.tiles = ((long long)T * (qh / kh) + kPromptRows - 1) / kPromptRows + (B < T ? B : T);
+    p.shares = kShares / kh > 1 ? kShares / kh : 1;
+    const long long parts = (((long long)W << shift) + kPromptShare * kPromptBlock - 1) / (kPromptShare * kPromptBlock);
+    p.slots = parts <= 1 ? 0 : p.tiles * parts < 2 * p.shares ? p.tiles * parts : 2 * p.shares;
+    return p;
 }
 
 template <typename E, int D>
-int launch_prompt(const PromptArgs& a, const PagedCache& c, const PagedBatch& bt, hipStream_t st) {
-    const long long rows = (long long)a.T * a.group * c.kh;  // rows over all KV heads
-    if (rows <= 32 * 512) return launch_prompt_tile<E, D, 2, 2, 1>(a, c, bt, st);
-    return launch_prompt_tile<E, D, 4, 1, 2>(a, c, bt, st);
+int launch_prompt(const PromptArgs& a, const PagedCache& c, const PagedBatch& bt, const PromptPlan& p, hipStream_t st) {
+    const long long groups = (p.tiles + (p.slots ? p.shares : 0)) * c.kh;
+    MOSS_CHECK_ARG(groups * 256 < (1ll << 32));
+    hipLaunchKernelGGL((paged_prompt_kernel<E, D>), dim3((unsigned)groups), dim3(256), 0, st, a, c, bt);
+    if (p.slots) {
+        const long long cut = (p.tiles < p.shares ? p.tiles : p.shares) * c.kh;
+        hipLaunchKernelGGL((paged_prompt_join<E, D>), dim3((unsigned)cut), dim3(256), 0, st, a, c, bt);
+    }
+    return moss_launch_status();
 }
 
 }  // namespace
@@ -340,20 +344,33 @@ int launch_prompt(const PromptArgs& a, const PagedCache& c, const PagedBatch& bt
 
 using namespace moss;
 
+MOSS_API long long moss_paged_prompt_workspace_bytes(int B, int W, int page_rows, int T, int qh, int kh, int d) {
+    const int shift = page_shift(page_rows);
+    if (B <= 0 || W <= 0 || shift < 0 || ((long long)W << shift) > (1ll << 30) || T <= 0 || kh <= 0 || qh <= 0 || qh % kh ||
+        (d != 64 && d != 128))
+        return 0;
+    return prompt_plan(B, W, shift, T, qh, kh).slots * kh * kPromptRows * (d + 2) * 4;
+}
+
 MOSS_API int moss_paged_prompt_attention(const void* q, long long q_stride, const void* k, const void* v,
                                          long long k_stride, long long v_stride, int pages, int page_rows,
                                          const void* table, long long table_stride, const void* lengths,
                                          const void* starts, int B, int W, int T, int qh, int kh, int d, float scale,
-                                         void* out, int dtype, void* stream) {
+                                         void* out, void* workspace, long long workspace_bytes, int dtype, void* stream) {
     const PagedCache c = paged_cache(k, v, k_stride, v_stride, pages, kh, page_rows);
     const PagedBatch bt{(const int*)table, (const int*)lengths, (const int*)starts, B, W, table_stride};
     MOSS_CHECK_ARG(q && out && starts && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, qh, d));
     MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && T > 0 && T <= (1 << 20) && q_stride % 8 == 0 &&
                    q_stride >= (long long)qh * d && scale == scale);
-    MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16));
-    const PromptArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, T, qh, qh / kh, fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f),
-                       scale < 0.f ? 0x80008000u : 0u};
+    MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16) && MOSS_ALIGNED(workspace, 16));
+    const PromptPlan p = prompt_plan(B, W, c.shift, T, qh, kh);
+    const long long values = p.slots * kh * kPromptRows;
+    MOSS_CHECK_ARG(p.slots == 0 || (workspace && workspace_bytes >= values * (d + 2) * 4));
+    const PromptArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, (float*)workspace,
+                       reinterpret_cast<float2*>((float*)workspace + values * d), T, qh, qh / kh, p.shares,
+                       p.slots, fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f), scale < 0.f ? 0x80008000u : 0u};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == 0) return d == 128 ? launch_prompt<Bf16, 128>(a, c, bt, st) : launch_prompt<Bf16, 64>(a, c, bt, st);
-    return d == 128 ? launch_prompt<F16, 128>(a, c, bt, st) : launch_prompt<F16, 64>(a, c, bt, st);
+    if (dtype == 0)
+        return d == 128 ? launch_prompt<Bf16, 128>(a, c, bt, p, st) : launch_prompt<Bf16, 64>(a, c, bt, p, st);
+    return d == 128 ? launch_prompt<F16, 128>(a, c, bt, p, st) : launch_prompt<F16, 64>(a, c, bt, p, st);
 }

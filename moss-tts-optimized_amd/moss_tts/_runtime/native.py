@@ -81,8 +81,9 @@ SIGNATURES: dict[str, list] = {
     "moss_paged_decode_workspace_bytes": [_I, _I, _I, _I, _I, _I],
     "moss_paged_decode_attention": [_P, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _F, _P, _P, _L, _I,
                                     _P],
-    "moss_paged_prompt_attention": [_P, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _I,
-                                    _P],
+    "moss_paged_prompt_attention": [_P, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P,
+                                    _L, _I, _P],
+    "moss_paged_prompt_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I],
     "moss_stream_read_words": [ctypes.c_longlong],
     "moss_stream_read": [_P, ctypes.c_longlong, _P, _P],
 }
@@ -90,6 +91,7 @@ _RESTYPES = {"moss_error_string": ctypes.c_char_p, "moss_gemm_workspace_bytes": 
              "moss_gemm_silu_workspace_bytes": ctypes.c_longlong,
              "moss_gemm_qk_rope_workspace_bytes": ctypes.c_longlong,
              "moss_paged_decode_workspace_bytes": ctypes.c_longlong,
+             "moss_paged_prompt_workspace_bytes": ctypes.c_longlong,
              "moss_sample_rows_workspace_bytes": ctypes.c_longlong,
              "moss_stream_read_words": ctypes.c_longlong}
 

@@ -155,6 +155,17 @@ def _apart(name: str, t: torch.Tensor, *spans) -> None:
         _require(end <= first or last <= at, f"{name} must not overlap the other tensors")
 
 
+def _workspace(ws, nbytes: int, like: torch.Tensor, out: torch.Tensor, spans):
+    """A new workspace of ``nbytes`` (None for none), or the caller's, checked."""
+    if ws is None:
+        return like.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
+    _cuda_contig("ws", ws, torch.float32, like.device)
+    _require(4 * ws.numel() >= nbytes and not ws.data_ptr() & 15, "workspace too small or not 16-byte aligned")
+    at = out.data_ptr()
+    _apart("ws", ws, (at, at + 2 * out.numel()), *spans)
+    return ws
+
+
 def _output(out, rows: int, width: int, like: torch.Tensor, *spans) -> torch.Tensor:
     """A new output (which shares no memory with anything), or the caller's, checked."""
     if out is None:
@@ -236,22 +247,24 @@ def decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
     out = _output(out, b, qh * d, q, *spans)
     nbytes = native.lib().moss_paged_decode_workspace_bytes(b, w, c.rows, qh, kh, d)
-    if ws is None:
-        ws = q.new_empty(nbytes // 4, dtype=torch.float32)
-    else:
-        _cuda_contig("ws", ws, torch.float32, q.device)
-        _require(4 * ws.numel() >= nbytes and not ws.data_ptr() & 15, "workspace too small or not 16-byte aligned")
-        o = out.data_ptr()
-        _apart("ws", ws, (o, o + 2 * out.numel()), *spans)
+    ws = _workspace(ws, nbytes, q, out, spans)
     native.call_on(q, "moss_paged_decode_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),
                    table_stride, lengths.data_ptr(), b, w, qh, kh, d, _scale(scale, d), out.data_ptr(), ws.data_ptr(),
                    nbytes, _TYPES[q.dtype])
     return out
 
 
+def prompt_workspace(q: torch.Tensor, keys: torch.Tensor, table: torch.Tensor) -> torch.Tensor | None:
+    """A workspace for :func:`prompt_attention` calls of these shapes (None: none needed); calls that may overlap need
+    one each."""
+    nbytes = native.lib().moss_paged_prompt_workspace_bytes(table.shape[0], table.shape[1], keys.shape[2], q.shape[0],
+                                                            q.shape[1], keys.shape[1], keys.shape[3])
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
+
+
 def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor,
                      lengths: torch.Tensor, starts: torch.Tensor, *, scale: float | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed new tokens whose K and V rows are in the pages already: ``q`` ``[T, query heads,
     head dim]`` (rows may lie apart); each token attends its sequence's rows up to its own position, the cached
     ones before the new among them.  ``scale`` defaults to head dim ** -0.5.  Returns ``[T, query heads * head
@@ -264,8 +277,11 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     _require(hd == d and qh % kh == 0 and qh <= 1024, "q must be [tokens, a multiple of the KV heads, head dim]")
     _require(n <= 1 << 20, "at most 2^20 packed tokens")
     at = q.data_ptr()
-    out = _output(out, n, qh * d, q, (at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
+    spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
+    out = _output(out, n, qh * d, q, *spans)
+    nbytes = native.lib().moss_paged_prompt_workspace_bytes(b, w, c.rows, n, qh, kh, d)
+    ws = _workspace(ws, nbytes, q, out, spans)
     native.call_on(q, "moss_paged_prompt_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),
                    table_stride, lengths.data_ptr(), starts.data_ptr(), b, w, n, qh, kh, d, _scale(scale, d),
-                   out.data_ptr(), _TYPES[q.dtype])
+                   out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _TYPES[q.dtype])
     return out

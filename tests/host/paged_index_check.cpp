@@ -75,6 +75,50 @@ int main() {
         }
         REQUIRE(slots <= decode_slots(B, W, shift, shares));
     }
+    // tiles of prompts and their parts
+    for (int round = 0; round < 4000; ++round) {
+        const int B = 1 + rng() % 12, group = any({1, 2, 3, 4, 7, 8, 16, 40, 128, 200}), shares = any({1, 2, 64, 512});
+        std::vector<PromptTiles> seqs(B);
+        long long bound = 0, blocks = 0;
+        for (auto& t : seqs) {
+            t = PromptTiles{rng() % 4 ? (int)(rng() % 900) : 0, group, (rng() % 3 ? (int)(rng() % 3000) : (int)(rng() % 40) - 700)};
+            long long sum = 0;
+            for (int i = 0; i < t.tiles(); ++i) sum += t.blocks(i);
+            REQUIRE(sum <= t.blocks_bound());
+            for (int x : {1, 2, 5, 8, 13, 40}) {
+                int over = 0;
+                for (int i = 0; i < t.tiles(); ++i) over += t.blocks(i) > x;
+                REQUIRE(over == t.tiles_over(x));
+            }
+            bound += t.blocks_bound();
+            blocks += sum;
+        }
+        const int share = prompt_share(bound, shares);
+        long long items = 0, tiles = 0, parts = 0, cut = 0;
+        for (const auto& t : seqs) {
+            std::vector<int> seen(t.tiles(), 0), slot(t.parts(share) + 1, 0);
+            for (int i = 0; i < t.items(share); ++i) {
+                const PromptItem it = prompt_item(t, share, i);
+                REQUIRE(it.tile >= 0 && it.tile < t.tiles());
+                REQUIRE(it.part == 0 || it.part * share < t.blocks(it.tile));
+                seen[it.tile] |= 1 << it.part;
+                if (t.blocks(it.tile) > share) {
+                    REQUIRE(it.slot >= 0 && it.slot < t.parts(share) && !slot[it.slot]);
+                    slot[it.slot] = 1;
+                }
+            }
+            for (int i = 0; i < t.tiles(); ++i) {
+                const int n = std::max(1, (t.blocks(i) + share - 1) / share);
+                REQUIRE(n < 31 && seen[i] == (1 << n) - 1);
+            }
+            items += t.items(share);
+            tiles += t.tiles();
+            if (t.tiles_over(share)) parts += t.parts(share);
+            else REQUIRE(t.parts(share) == 0);
+            cut += t.tiles_over(share);
+        }
+        REQUIRE(items <= tiles + shares && parts <= 2 * shares && cut <= shares);
+    }
     REQUIRE(share_of_units(65535ll << 23, 1) == 1 << 24 && shares_of(1 << 23, 1 << 24) == 1);
     printf("ok\n");
     return 0;

@@ -389,3 +389,29 @@ def test_refusals(dev):
     refused("sin must be", r, qkv, None, None, cos, cos.bfloat16(), keys, vals, table, lens, 1e-6)
     refused("eps", r, qkv, None, None, cos, cos, keys, vals, table, lens, -1.0)
     refused("16-byte", r, qkv.view(-1)[4:4 + 512].view(1, 512), None, None, cos, cos, keys, vals, table[:1], lens[:1], 1e-6)
+
+
+@pytest.mark.parametrize("new, old", [([1], [2500]), ([3, 40], [1500, 0]), ([150], [1900]), ([1, 1, 1, 300], [4000, 30, 1200, 700])])
+@pytest.mark.parametrize("layout", [(8, 2, 128), (16, 1, 128), (4, 4, 64)])
+def test_prompt_cut_tiles(dev, new, old, layout):
+    """A few new tokens behind a long prefix: tiles that are cut into parts and joined."""
+    _prompt(dev, new, old, layout, torch.bfloat16, 16, pad=2)
+
+
+def test_prompt_starts_that_do_not_rise(dev):
+    """Starts that name the same tokens many times over, fall or lie outside: no write past the output or the workspace,
+    whose end is watched."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(3)
+    n = 40
+    keys, vals, table, lens = cache(dev, g, [1500] * n, kh=2, d=128, page=64, dtype=torch.bfloat16)
+    q = torch.randn((2, 8, 128), generator=g).bfloat16().to(dev)
+    need = paged.prompt_workspace(q, keys, table).numel()
+    ws = torch.full((need + 4096,), 3.0, device=dev)
+    buffer = torch.full((4, 1024), 3.0, dtype=torch.bfloat16, device=dev)
+    for starts in ([0, 1] * (n // 2) + [0], [2] * n + [-5], [-2 ** 31, 2 ** 31 - 1] * (n // 2) + [7], list(range(n, -1, -1))):
+        paged.prompt_attention(q, keys, vals, table, lens, torch.tensor(starts, dtype=torch.int32, device=dev),
+                               out=buffer[1:3], ws=ws[:need])
+        torch.cuda.synchronize()
+        assert (ws[need:] == 3.0).all() and (buffer[[0, 3]] == 3.0).all()
