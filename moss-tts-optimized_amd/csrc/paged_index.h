@@ -54,18 +54,19 @@ MOSS_HD void share_rows(int rows, int count, int index, int& r0, int& r1) {
     r1 = to < rows ? (int)to : rows;
 }
 
-// Prompt work: tiles of kPromptRows (token, head) rows, which see keys up to their last row's position, in blocks of
+// Prompt work: tiles of `height` (128 or 64) (token, head) rows, which see keys up to their last row's position, in blocks of
 // kPromptBlock keys; a tile of more than `share` blocks is cut into parts of that many.  The sum of all tiles' blocks is
 // at most `shares` times the share, so at most `shares` parts come on top of the tiles and the parts of the cut tiles are at
 // most twice as many.
-constexpr int kPromptRows = 128, kPromptBlock = 64, kPromptShare = 8;
+constexpr int kPromptBlock = 64, kPromptShare = 8;
 struct PromptTiles {
-    int tokens, group, pos0;  // new tokens of a sequence, query heads per KV head, position of the first one
+    int tokens, group, pos0, height;  // new tokens of a sequence, query heads per KV head, position of the first one
     MOSS_HD int rows() const { return tokens * group; }
-    MOSS_HD int tiles() const { return (rows() + kPromptRows - 1) / kPromptRows; }
+    MOSS_HD int tiles() const { return (rows() + height - 1) / height; }
+    MOSS_HD int token_of(int row) const { return (int)((unsigned)row / (unsigned)group); }
     MOSS_HD int last_key(int tile) const {  // -1 and below: none
-        const int row = (tile + 1) * kPromptRows - 1;
-        return pos0 + (row < rows() - 1 ? row : rows() - 1) / group;
+        const int row = (tile + 1) * height - 1;
+        return pos0 + token_of(row < rows() - 1 ? row : rows() - 1);
     }
     MOSS_HD int blocks(int tile) const {
         const int last = last_key(tile);
@@ -77,14 +78,14 @@ struct PromptTiles {
         const int n = tiles();
         if (y <= 0) return n;
         if (y > tokens - 1) return 0;
-        const int first = (int)((y * group + kPromptRows) / kPromptRows) - 1;  // ceil((y group + 1) / rows) - 1
+        const int first = ((int)y * group + height) / height - 1;  // ceil((y group + 1) / rows) - 1
         return (first < n - 1 ? n - 1 - first : 0) + 1;
     }
-    // no less than the sum of blocks() over the tiles
+    // no less than the sum of blocks() over the tiles: they rise no faster than a line (rows are at most 2^30)
     MOSS_HD long long blocks_bound() const {
         const int n = tiles();
         if (n == 0) return 0;
-        const long long end = (long long)pos0 + ((long long)n * kPromptRows - 1) / group;
+        const int end = pos0 + token_of(n * height - 1);
         return ((long long)n * (blocks(0) + (end < 0 ? 0 : end / kPromptBlock + 1) + 2) + 1) / 2;
     }
     MOSS_HD int items(int share) const {

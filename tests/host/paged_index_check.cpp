@@ -77,11 +77,11 @@ int main() {
     }
     // tiles of prompts and their parts
     for (int round = 0; round < 4000; ++round) {
-        const int B = 1 + rng() % 12, group = any({1, 2, 3, 4, 7, 8, 16, 40, 128, 200}), shares = any({1, 2, 64, 512});
+        const int B = 1 + rng() % 12, group = any({1, 2, 3, 4, 7, 8, 16, 40, 128, 200}), shares = any({1, 2, 64, 512}), height = any({64, 128});
         std::vector<PromptTiles> seqs(B);
         long long bound = 0, blocks = 0;
         for (auto& t : seqs) {
-            t = PromptTiles{rng() % 4 ? (int)(rng() % 900) : 0, group, (rng() % 3 ? (int)(rng() % 3000) : (int)(rng() % 40) - 700)};
+            t = PromptTiles{rng() % 4 ? (int)(rng() % 900) : 0, group, (rng() % 3 ? (int)(rng() % 3000) : (int)(rng() % 40) - 700), height};
             long long sum = 0;
             for (int i = 0; i < t.tiles(); ++i) sum += t.blocks(i);
             REQUIRE(sum <= t.blocks_bound());

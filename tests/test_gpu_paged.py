@@ -415,3 +415,33 @@ def test_prompt_starts_that_do_not_rise(dev):
                                out=buffer[1:3], ws=ws[:need])
         torch.cuda.synchronize()
         assert (ws[need:] == 3.0).all() and (buffer[[0, 3]] == 3.0).all()
+
+
+@pytest.mark.parametrize("new, old, layout", [([40, 70], [0, 30], (8, 2, 128)), ([130], [5], (4, 4, 64)), ([700], [100], (32, 8, 128))])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_prompt_values_behind_a_token(dev, new, old, layout, what):
+    """NaN and infinities in K and V of tokens that come later reach no earlier token; the later ones see them."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(11)
+    qh, kh, d = layout
+    lengths = [a + b for a, b in zip(new, old)]
+    keys, vals, table, lens = cache(dev, g, lengths, kh=kh, d=d, page=16, dtype=torch.bfloat16)
+    starts = torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device=dev)
+    q = torch.randn((sum(new), qh, d), generator=g).bfloat16().to(dev)
+    clean = paged.prompt_attention(q, keys, vals, table, lens, starts)
+    bad = [n - n // 3 for n in new]  # the new token of each sequence whose row is bad
+    for b, t in enumerate(bad):
+        row = old[b] + t
+        vals[table[b, row // 16].long(), :, row % 16, ::3] = what
+        if b:
+            keys[table[b, row // 16].long(), :, row % 16, 5] = what
+    got = paged.prompt_attention(q, keys, vals, table, lens, starts)
+    torch.cuda.synchronize()
+    for b, t in enumerate(bad):
+        at = int(starts[b])
+        x, y = values(got[at:at + t]), values(clean[at:at + t])
+        # the rows of tiles without such a key are the same; others are summed without rounding P
+        assert np.isfinite(x).all() and (np.abs(x - y) <= 2.0 ** -6 * np.abs(y) + 2.0 ** -6).all()
+        after = got[at + t:at + new[b]].view(-1, qh, d)[..., ::3]
+        assert not torch.isfinite(after).any()
