@@ -17,6 +17,8 @@ graph follows them as sequences grow.  Whatever they hold, no access leaves the 
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import native
@@ -123,20 +125,41 @@ def _query(q):
     return n, h, d, stride, index
 
 
-def _vector(name, t, n: int, dtype, index) -> int:
-    """The pointer of ``n`` checked values."""
-    _require(isinstance(t, torch.Tensor) and t.dtype is dtype, f"{name} must be a {dtype} tensor")
-    at = t.data_ptr()
-    _require(t.get_device() == index and t.numel() == n and t.is_contiguous() and not at & 15,
-             f"{name} must hold {n} values on cuda:{index}, contiguous and 16-byte aligned")
-    return at
-
-
-def _table(name, t, d: int, dtype, index):
-    """(pointer, rows) of a checked ``[positions, d]`` table."""
-    _require(isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 2 and t.shape[1] == d and t.shape[0] > 0,
-             f"{name} must be a {dtype} (cos and sin: or float32) [positions, {d}] table")
-    return _vector(name, t, t.numel(), dtype, index), t.shape[0]
+def _norms_and_tables(q_weight, k_weight, cos, sin, d: int, dtype, index):
+    """(q weight, k weight, cos, sin pointers, whether the tables are fp32, their rows), checked."""
+    try:
+        rows, width = shape = cos.shape
+        kind = cos.dtype
+        c, s = cos.data_ptr(), sin.data_ptr()
+        qw = kw = None
+        ok = ((kind is torch.float32 or kind is dtype) and sin.dtype is kind and sin.shape == shape and width == d
+              and 0 < rows < 1 << 31 and cos.get_device() == index == sin.get_device() and cos.is_contiguous()
+              and sin.is_contiguous() and not (c | s) & 15)
+        if q_weight is None or k_weight is None:
+            ok = ok and q_weight is k_weight
+        else:
+            qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
+            ok = (ok and q_weight.dtype is dtype and k_weight.dtype is dtype and q_weight.numel() == d == k_weight.numel()
+                  and q_weight.get_device() == index == k_weight.get_device() and q_weight.is_contiguous()
+                  and k_weight.is_contiguous() and not (qw | kw) & 15)
+    except (AttributeError, ValueError):
+        ok = False
+    if ok:
+        return qw, kw, c, s, int(kind is torch.float32), rows
+    _require((q_weight is None) == (k_weight is None), "both head-norm weights or none")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None:
+            _require(isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == index and t.numel() == d
+                     and t.is_contiguous() and not t.data_ptr() & 15,
+                     f"{name} must hold {d} {dtype} values on cuda:{index}, contiguous and 16-byte aligned")
+    _require(isinstance(cos, torch.Tensor) and cos.dtype in (torch.float32, dtype), f"cos must be a float32 or {dtype} tensor")
+    for name, t in (("cos", cos), ("sin", sin)):
+        _require(isinstance(t, torch.Tensor) and t.dtype == cos.dtype and t.dim() == 2 and t.shape == cos.shape
+                 and t.shape[1] == d and t.shape[0] > 0 and t.get_device() == index and t.is_contiguous()
+                 and not t.data_ptr() & 15,
+                 f"{name} must be a {cos.dtype} [positions, {d}] table on cuda:{index}, contiguous and 16-byte aligned, "
+                 "as long as the other")
+    raise ValueError("the head-norm weights and tables do not fit")
 
 
 def _scale(scale, d: int) -> float:
@@ -166,12 +189,15 @@ def _workspace(ws, nbytes: int, like: torch.Tensor, out: torch.Tensor, spans):
     return ws
 
 
-def _output(out, rows: int, width: int, like: torch.Tensor, *spans) -> torch.Tensor:
+def _output(out, shape, like: torch.Tensor, *spans) -> torch.Tensor:
     """A new output (which shares no memory with anything), or the caller's, checked."""
     if out is None:
-        return like.new_empty((rows, width))
+        return like.new_empty(shape)
     _cuda_contig("out", out, like.dtype, like.device)
-    _require(out.numel() == rows * width and not out.data_ptr() & 15, f"out must hold {rows} x {width} values, 16-byte aligned")
+    if out.shape != shape:
+        _require(out.numel() == math.prod(shape), f"out must hold {' x '.join(map(str, shape))} values")
+        out = out.view(shape)
+    _require(not out.data_ptr() & 15, "out must be 16-byte aligned")
     _apart("out", out, *spans)
     return out
 
@@ -203,22 +229,14 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     _require(width % d == 0 and 0 < qh <= 1024 and qh % kh == 0,
              "qkv must hold a multiple of the KV heads as query heads, then the keys and the values")
     _require(starts is not None or tokens == b, "without starts, one token a sequence required")
-    if q_weight is None or k_weight is None:
-        _require(q_weight is k_weight, "both head-norm weights or none")
-        qw = kw = None
-    else:
-        qw, kw = _vector("q_weight", q_weight, d, dtype, index), _vector("k_weight", k_weight, d, dtype, index)
-    f32 = isinstance(cos, torch.Tensor) and cos.dtype is torch.float32
-    cos_at, positions = _table("cos", cos, d, torch.float32 if f32 else dtype, index)
-    sin_at, others = _table("sin", sin, d, torch.float32 if f32 else dtype, index)
-    _require(positions == others, "cos and sin must hold the same positions")
+    norms = _norms_and_tables(q_weight, k_weight, cos, sin, d, dtype, index)
     _require(eps >= 0, "eps must not be negative")
     _require(tokens < 1 << 31, "too many tokens")
     span = (at, at + 2 * ((tokens - 1) * stride + width))
     _require((c.kend <= span[0] or span[1] <= c.k) and (c.vend <= span[0] or span[1] <= c.v),
              "qkv must not overlap the cache")
-    q = _output(out, tokens, qh * d, qkv, span, (c.k, c.kend), (c.v, c.vend)).view(tokens, qh, d)
-    native.call_on(qkv, "moss_paged_qk_rope", at, stride, qw, kw, cos_at, sin_at, int(f32), positions, q.data_ptr(), c.k, c.v, c.ks, c.vs, c.pages, c.rows,
+    q = _output(out, (tokens, qh, d), qkv, span, (c.k, c.kend), (c.v, c.vend))
+    native.call_on(qkv, "moss_paged_qk_rope", at, stride, *norms, q.data_ptr(), c.k, c.v, c.ks, c.vs, c.pages, c.rows,
                    table.data_ptr(), table_stride, lengths.data_ptr(), None if starts is None else starts.data_ptr(), b,
                    w, tokens, qh, kh, d, eps, _TYPES[dtype])
     return q
@@ -245,7 +263,7 @@ def decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     _require(n == b and hd == d and qh % kh == 0 and qh <= 1024, "q must be [B, a multiple of the KV heads, head dim]")
     at = q.data_ptr()
     spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
-    out = _output(out, b, qh * d, q, *spans)
+    out = _output(out, (b, qh * d), q, *spans)
     nbytes = native.lib().moss_paged_decode_workspace_bytes(b, w, c.rows, qh, kh, d)
     ws = _workspace(ws, nbytes, q, out, spans)
     native.call_on(q, "moss_paged_decode_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),
@@ -278,7 +296,7 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     _require(n <= 1 << 20, "at most 2^20 packed tokens")
     at = q.data_ptr()
     spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
-    out = _output(out, n, qh * d, q, *spans)
+    out = _output(out, (n, qh * d), q, *spans)
     nbytes = native.lib().moss_paged_prompt_workspace_bytes(b, w, c.rows, n, qh, kh, d)
     ws = _workspace(ws, nbytes, q, out, spans)
     native.call_on(q, "moss_paged_prompt_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),

@@ -134,7 +134,7 @@ def _prompt(dev, new, old, layout, dtype, page, *, seed=0, pad=0, edit=None, str
     out = torch.full((total, qh * d), 7.0, dtype=dtype, device=dev)
     before = values(out)
     print(f"prompt new={new} old={old} layout={layout} {dtype} page={page}", flush=True)
-    assert paged.prompt_attention(q, keys, vals, table, lens, starts, scale=scale, out=out) is out
+    assert paged.prompt_attention(q, keys, vals, table, lens, starts, scale=scale, out=out).data_ptr() == out.data_ptr()
     torch.cuda.synchronize()
     args = values(q), values(keys), values(vals)
     rest = table.cpu().numpy(), lens.cpu().numpy(), starts.cpu().numpy(), before, scale
