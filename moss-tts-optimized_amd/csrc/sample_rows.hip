@@ -15,13 +15,14 @@
 // The borders of the prefix are found without sorting: a histogram (count and sum of w) over bins of 1/32 octave of w,
 // then the border bin's own entries; of the entries with the border's key, the first few in index order are kept.
 //
-// What bounds it: the arithmetic of w in 64 bits for every entry, and, for few rows, the chain of steps.  So a row is
-// read by several workgroups, in five launches (largest logit; histogram; border; weight of each segment of 512 entries;
-// draw), of which the histogram, or the segments' weights, is the one that forms w for every entry: a row without top-k
-// and top-p has no histogram, a row with them few weights in its segments.  w takes 14 operations in 64
-// bits, of 8 cycles each for a wave: with a series of ten terms and no table the histograms of 128 rows took 33 us, and
-// with a table of 1024 entries, whose reads the bins' atomics wait for, 27.  A
-// row of up to 2048 entries is one wave's: it holds them and their weights in registers, and needs no barrier.
+// What bounds it: the arithmetic of w in 64 bits, and for few rows the chain of steps.  So a row is read by several
+// workgroups, in five launches (largest logit; histogram; border; weight of each segment of 512 entries; draw), of which
+// the segments form w for the kept entries, and the histogram for all of a row with top-p, unless its bins are single
+// values that need only be counted (bf16).  w takes 14 operations in 64 bits, of 8 cycles each for a wave.  128 rows of 151,936
+// bf16 logits, each with its own settings: 65 us (9 + 19 + 12 + 19 + 6); with linear bins and the border's bin collected 84,
+// of those with a series of ten terms and no table 93, and one workgroup a row 309.  One row: 30 us, 182 before.  A row of
+// up to 2048 entries is one wave's: it holds them and their weights in registers, and needs no barrier (512 rows of 1024:
+// 13.7 us, 46 before).
 #include "common.h"
 
 namespace moss {
@@ -295,10 +296,43 @@ __device__ __forceinline__ V block_prefix(V v, V* parts, int lane, int wave) {
 }
 
 // ---------------------------------------------------------------- long rows: several workgroups a row
+// A row of bf16 logits holds few different values that matter: a bin for each from the largest logit down to 2^-9 and from
+// -2^-9 down to where no weight is left, and one for what lies between.  A bin's entries weigh the same, so they need only
+// be counted.  `on`: the row's values fit the bins (a largest logit of 2^-9 to 2^7, and weights that end soon enough below 0).
+struct KeyBins {
+    bool on;
+    uint32_t top;
+    int np, all;  // bin np: what lies between
+};
+constexpr int kKeyBins = 4096;
+constexpr uint32_t kLeastPositive = 0xbb00u, kLeastNegative = 0x44ffu;  // the keys of 2^-9 and -2^-9
+template <int TYPE>
+__device__ __forceinline__ KeyBins key_bins(const Row& r) {
+    KeyBins q{false, 0, 0, 0};
+    if constexpr (TYPE == 0) {
+        q.top = key_of<TYPE>(r.top);
+        q.np = (int)(q.top - kLeastPositive) + 1;
+        const float far = (float)((double)r.top - kBins / r.rate);  // no weight is left below; two keys to be sure
+        const int kf = far > -3.3e38f ? (int)key_of<TYPE>(far) - 2 : (int)kLowest<TYPE>;
+        q.all = q.np + 1 + max((int)kLeastNegative - kf, 0);
+        q.on = q.top >= kLeastPositive && q.np <= kKeyBins / 2 && q.all <= kKeyBins;
+    }
+    return q;
+}
+__device__ __forceinline__ int bin_of_key(const KeyBins& q, uint32_t k) {  // q.all and more: no weight
+    return k >= kLeastPositive ? (int)(q.top - k) : k > kLeastNegative ? q.np : q.np + 1 + (int)(kLeastNegative - k);
+}
+__device__ __forceinline__ uint32_t key_of_bin(const KeyBins& q, int b) {
+    return b < q.np ? q.top - (uint32_t)b : kLeastNegative - (uint32_t)(b - q.np - 1);
+}
+
+// A chunk's bins in the workspace: sums and counts of the bins that are linear in log w, or the sum of the bin between
+// and the counts of the key bins.
+constexpr int kBinBytes = 12 * kBins;
+static_assert(kBinBytes % 16 == 0 && kBinBytes >= 16 + 4 * kKeyBins, "a chunk's bins");
 struct Work {
     unsigned long long* top;    // [rows, chunks]
-    unsigned long long* sum;    // [rows, chunks, kBins]
-    uint32_t* count;            // [rows, chunks, kBins]
+    unsigned char* bins;        // [rows, chunks, kBinBytes]
     unsigned long long* seg;    // [rows, segments]: weight of the entries above the border's key
     uint32_t* tie;              // [rows, segments]: entries with the border's key
     uint2* border;              // [rows]
@@ -319,7 +353,7 @@ __global__ __launch_bounds__(512) void sample_top_kernel(SampleArgs a, Work w) {
     const Row r = row_of<TYPE>(a, row);
     const int end = min(r.vocab, (chunk + 1) * w.chunk);
     unsigned long long best = 0;
-    walk<TYPE, 4>(r, chunk * w.chunk + 8 * tid, end, 8 * 512, [&](int i, const float(&x)[8]) {
+    walk<TYPE, 5>(r, chunk * w.chunk + 8 * tid, end, 8 * 512, [&](int i, const float(&x)[8]) {
         float m = x[0];
         int at = 0;
 #pragma unroll
@@ -339,36 +373,47 @@ __global__ __launch_bounds__(512) void sample_top_kernel(SampleArgs a, Work w) {
 template <int TYPE>
 __global__ __launch_bounds__(512) void sample_bins_kernel(SampleArgs a, Work w) {
     __shared__ double table[32];
-    __shared__ unsigned long long sum[kBins];
-    __shared__ uint32_t count[kBins];
+    __shared__ __attribute__((aligned(16))) unsigned char bins[kBinBytes];
     const int row = blockIdx.x / w.chunks, chunk = blockIdx.x % w.chunks, tid = threadIdx.x, lane = tid & (kWave - 1);
     Row r = row_of<TYPE>(a, row);
     int index;
     if (!(r.by_k || r.by_p) || !load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
     fill_table(table, tid);
-    for (int b = tid; b < kBins; b += 512) {
-        sum[b] = 0;
-        count[b] = 0;
-    }
+    const u32x4_t zero = {0u, 0u, 0u, 0u};
+    for (int b = tid; b < kBinBytes / 16; b += 512) reinterpret_cast<u32x4_t*>(bins)[b] = zero;
     __syncthreads();
+    unsigned long long* sum = reinterpret_cast<unsigned long long*>(bins);
     const int end = min(r.vocab, (chunk + 1) * w.chunk);
-    walk<TYPE, 4>(r, chunk * w.chunk + 8 * tid, end, 8 * 512, [&](int, const float(&x)[8]) {
+    const KeyBins q = key_bins<TYPE>(r);
+    int used = kBinBytes / 16;
+    if (q.on) {
+        uint32_t* count = reinterpret_cast<uint32_t*>(bins + 16);
+        walk<TYPE, 5>(r, chunk * w.chunk + 8 * tid, end, 8 * 512, [&](int, const float(&x)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double o = parts_of(r, x[j]);
-            const unsigned long long v = r.by_p ? weight_at(o, table) : 0;
-            const int b = bin_of(o);
-            if (b >= kBins) continue;
-            if (r.by_k) atomicAdd(&count[b], 1u);
-            if (r.by_p) atomicAdd(&sum[b], v);
-        }
-    });
-    __syncthreads();
-    const size_t at = ((size_t)row * w.chunks + chunk) * kBins;
-    for (int b = tid; b < kBins; b += 512) {
-        if (r.by_k) w.count[at + b] = count[b];
-        if (r.by_p) w.sum[at + b] = sum[b];
+            for (int j = 0; j < 8; ++j) {
+                const int b = bin_of_key(q, key_of<TYPE>(x[j]));
+                if (b < q.all) atomicAdd(&count[b], 1u);
+                if (b == q.np && r.by_p) atomicAdd(sum, weight_of(r, x[j], table));
+            }
+        });
+        used = 1 + (q.all + 3) / 4;
+    } else {
+        uint32_t* count = reinterpret_cast<uint32_t*>(bins + 8 * kBins);
+        walk<TYPE, 5>(r, chunk * w.chunk + 8 * tid, end, 8 * 512, [&](int, const float(&x)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const double o = parts_of(r, x[j]);
+                const unsigned long long v = r.by_p ? weight_at(o, table) : 0;
+                const int b = bin_of(o);
+                if (b >= kBins) continue;
+                if (r.by_k) atomicAdd(&count[b], 1u);
+                if (r.by_p) atomicAdd(&sum[b], v);
+            }
+        });
     }
+    __syncthreads();
+    u32x4_t* to = reinterpret_cast<u32x4_t*>(w.bins + ((size_t)row * w.chunks + chunk) * kBinBytes);
+    for (int b = tid; b < used; b += 512) to[b] = reinterpret_cast<const u32x4_t*>(bins)[b];
 }
 
 constexpr int kBorderThreads = 1024, kBorderWaves = kBorderThreads / kWave;
@@ -392,23 +437,35 @@ struct BorderShared {
     uint32_t listed;
 };
 
-// The last bin whose first entry is inside; thread t holds bins 2 t and 2 t + 1.  Two barriers, the first behind all that
+// The last bin whose first entry is inside; thread t holds bins N t .. + N - 1.  Two barriers, the first behind all that
 // the caller has read of sh's bins.
-__device__ __forceinline__ Bin border_bin(BorderShared& sh, const Goal& goal, uint32_t c0, uint32_t c1, unsigned long long s0,
-                                          unsigned long long s1, uint32_t base_count, unsigned long long base_sum) {
+template <int N>
+__device__ __forceinline__ Bin border_bin(BorderShared& sh, const Goal& goal, const uint32_t (&c)[N],
+                                          const unsigned long long (&s)[N], uint32_t base_count, unsigned long long base_sum) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const uint32_t c = wave_prefix(c0 + c1);
-    const unsigned long long s = wave_prefix(s0 + s1);
+    uint32_t ct = 0;
+    unsigned long long st = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        ct += c[i];
+        st += s[i];
+    }
+    const uint32_t cp = wave_prefix(ct);
+    const unsigned long long sp = wave_prefix(st);
     if (lane == kWave - 1) {
-        sh.part_count[wave] = c;
-        sh.part_sum[wave] = s;
+        sh.part_count[wave] = cp;
+        sh.part_sum[wave] = sp;
     }
     __syncthreads();
-    const uint32_t cb = base_count + wave_total(lane < wave ? sh.part_count[lane] : 0u) + c - c0 - c1;
-    const unsigned long long sb = base_sum + wave_total(lane < wave ? sh.part_sum[lane] : 0ull) + s - s0 - s1;
+    uint32_t cb = base_count + wave_total(lane < wave ? sh.part_count[lane] : 0u) + cp - ct;
+    unsigned long long sb = base_sum + wave_total(lane < wave ? sh.part_sum[lane] : 0ull) + sp - st;
     Bin mine{-1, 0, 0, 0, 0};
-    if ((c0 || s0) && goal.inside(cb, sb)) mine = Bin{2 * tid, c0, cb, s0, sb};
-    if ((c1 || s1) && goal.inside(cb + c0, sb + s0)) mine = Bin{2 * tid + 1, c1, cb + c0, s1, sb + s0};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if ((c[i] || s[i]) && goal.inside(cb, sb)) mine = Bin{N * tid + i, c[i], cb, s[i], sb};
+        cb += c[i];
+        sb += s[i];
+    }
     const unsigned long long any = __ballot(mine.bin >= 0);
     if (any ? lane == 63 - __builtin_clzll(any) : lane == 0) sh.found[wave] = mine;
     __syncthreads();
@@ -416,9 +473,9 @@ __device__ __forceinline__ Bin border_bin(BorderShared& sh, const Goal& goal, ui
     return waves ? sh.found[63 - __builtin_clzll(waves)] : Bin{-1, 0, 0, 0, 0};
 }
 
-// The border inside the keys lo .. hi, which n entries have (0: not known, more than one key), behind the given ones.  (Entries that an earlier border left
-// out weigh on no decision: what lies before them already exceeds the limit.)  Up to kList entries are collected first;
-// then bins over equal parts of the keys' range, until a bin is one key.
+// The border inside the keys lo .. hi, which n entries have (0: not known, more than one key), behind the given ones.
+// (Entries that an earlier border left out weigh on no decision: what lies before them exceeds the limit.)  Up to kList
+// entries are collected first; then bins over equal parts of the keys' range, until a bin is one key.
 template <int TYPE>
 __device__ Border border_among(BorderShared& sh, const Row& r, const Goal& goal, uint32_t lo, uint32_t hi, uint32_t n,
                                uint32_t base_count, unsigned long long base_sum) {
@@ -468,8 +525,9 @@ __device__ Border border_among(BorderShared& sh, const Row& r, const Goal& goal,
             });
         }
         __syncthreads();
-        const Bin f = border_bin(sh, goal, sh.count[2 * tid], sh.count[2 * tid + 1], sh.sum[2 * tid], sh.sum[2 * tid + 1],
-                                 base_count, base_sum);
+        const uint32_t c[2] = {sh.count[2 * tid], sh.count[2 * tid + 1]};
+        const unsigned long long s[2] = {sh.sum[2 * tid], sh.sum[2 * tid + 1]};
+        const Bin f = border_bin<2>(sh, goal, c, s, base_count, base_sum);
         if (f.bin < 0) return Border{kLowest<TYPE> + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
         base_count = f.before_count;
         base_sum = f.before_sum;
@@ -491,35 +549,71 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(SampleArg
     Border border{kLowest<TYPE> + 1, 0xffffffffu, 0};     // everything above -inf
     if (r.by_k || r.by_p) {
         fill_table(sh.table, tid);
-        // bins 2 tid and 2 tid + 1 of all chunks; the loads go out together (a chunk behind the last is the last one)
-        uint32_t c0 = 0, c1 = 0;
-        unsigned long long s0 = 0, s1 = 0;
-        if (2 * tid < kBins) {
+        const KeyBins q = key_bins<TYPE>(r);
+        const unsigned char* from = w.bins + (size_t)row * w.chunks * kBinBytes;
+        // this thread's bins, summed over the chunks; their loads go out together (a chunk behind the last is the last one)
+        uint32_t c[4] = {0u, 0u, 0u, 0u};
+        unsigned long long s[4] = {0ull, 0ull, 0ull, 0ull};
+        if (q.on) {  // bins 4 tid ..
+            __syncthreads();  // the table
+            if (4 * tid < q.all) {
+                uint4 cs[kMaxChunks];
+                unsigned long long between = 0;
+#pragma unroll
+                for (int i = 0; i < kMaxChunks; ++i)
+                    cs[i] = *reinterpret_cast<const uint4*>(from + (size_t)min(i, w.chunks - 1) * kBinBytes + 16 + 16 * tid);
+#pragma unroll
+                for (int i = 0; i < kMaxChunks; ++i)
+                    if (i < w.chunks) {
+                        c[0] += cs[i].x;
+                        c[1] += cs[i].y;
+                        c[2] += cs[i].z;
+                        c[3] += cs[i].w;
+                    }
+                if (q.np / 4 == tid)
+                    for (int i = 0; i < w.chunks; ++i)
+                        between += *reinterpret_cast<const unsigned long long*>(from + (size_t)i * kBinBytes);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int b = 4 * tid + i;
+                    if (b >= q.all) c[i] = 0;  // what the last 16 bytes hold besides
+                    if (r.by_p)
+                        s[i] = b == q.np ? between : c[i] ? c[i] * weight_of(r, logit_of<TYPE>(key_of_bin(q, b)), sh.table) : 0;
+                }
+            }
+        } else if (2 * tid < kBins) {  // bins 2 tid, 2 tid + 1
             uint2 cs[kMaxChunks];
             ulonglong2 ss[kMaxChunks];
-            const size_t at = (size_t)row * w.chunks * kBins + 2 * tid;
 #pragma unroll
             for (int i = 0; i < kMaxChunks; ++i) {
-                const size_t k = at + (size_t)min(i, w.chunks - 1) * kBins;
-                cs[i] = r.by_k ? *reinterpret_cast<const uint2*>(w.count + k) : make_uint2(0, 0);
-                ss[i] = r.by_p ? *reinterpret_cast<const ulonglong2*>(w.sum + k) : make_ulonglong2(0, 0);
+                const unsigned char* p = from + (size_t)min(i, w.chunks - 1) * kBinBytes;
+                cs[i] = r.by_k ? *reinterpret_cast<const uint2*>(p + 8 * kBins + 8 * tid) : make_uint2(0, 0);
+                ss[i] = r.by_p ? *reinterpret_cast<const ulonglong2*>(p + 16 * tid) : make_ulonglong2(0, 0);
             }
 #pragma unroll
             for (int i = 0; i < kMaxChunks; ++i)
                 if (i < w.chunks) {
-                    c0 += cs[i].x;
-                    c1 += cs[i].y;
-                    s0 += ss[i].x;
-                    s1 += ss[i].y;
+                    c[0] += cs[i].x;
+                    c[1] += cs[i].y;
+                    s[0] += ss[i].x;
+                    s[1] += ss[i].y;
                 }
         }
         auto find = [&](const Goal& goal) {
-            const Bin f = border_bin(sh, goal, c0, c1, s0, s1, 0, 0);
+            const uint32_t c2[2] = {c[0], c[1]};
+            const unsigned long long s2[2] = {s[0], s[1]};
+            const Bin f = q.on ? border_bin<4>(sh, goal, c, s, 0, 0) : border_bin<2>(sh, goal, c2, s2, 0, 0);
             if (f.bin < 0) return Border{kLowest<TYPE> + 1, 0xffffffffu, 0};  // only when the logits change under the kernel
-            const uint32_t lo = first_key_of_bins<TYPE>(r, f.bin, lane);
-            const uint32_t hi = f.bin ? first_key_of_bins<TYPE>(r, f.bin - 1, lane) - 1 : key_of<TYPE>(r.top);
-            uint32_t n = f.count;  // counted for top_k only
-            if (!r.by_k && lo == hi) n = (uint32_t)(f.sum / weight_of(r, logit_of<TYPE>(lo), sh.table));
+            uint32_t n = f.count, lo, hi;
+            if (q.on) {
+                lo = f.bin == q.np ? kLeastNegative + 1 : key_of_bin(q, f.bin);
+                hi = f.bin == q.np ? kLeastPositive - 1 : lo;
+            } else {
+                lo = first_key_of_bins<TYPE>(r, f.bin, lane);
+                hi = f.bin ? first_key_of_bins<TYPE>(r, f.bin - 1, lane) - 1 : key_of<TYPE>(r.top);
+                // entries are counted for top_k only
+                if (!r.by_k && lo == hi) n = (uint32_t)(f.sum / weight_of(r, logit_of<TYPE>(lo), sh.table));
+            }
             return border_among<TYPE>(sh, r, goal, lo, hi, n, f.before_count, f.before_sum);
         };
         unsigned long long total = 0;
@@ -530,7 +624,7 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(SampleArg
         __syncthreads();  // the slots of the search
         if (r.by_p) {
             if (!r.by_k) {
-                total = wave_total(s0 + s1);
+                total = wave_total(s[0] + s[1] + s[2] + s[3]);
                 if (lane == 0) sh.part_sum[wave] = total;
                 __syncthreads();
                 total = wave_total(lane < kBorderWaves ? sh.part_sum[lane] : 0ull);
@@ -839,7 +933,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs a, int rows
 // ---------------------------------------------------------------- launches
 struct SamplePlan {
     int chunks, chunk, segments;
-    long long top, sum, seg, border, count, tie, bytes;  // offsets
+    long long top, bins, seg, border, tie, bytes;  // offsets
 };
 
 SamplePlan sample_plan(int rows, int vocab) {
@@ -853,13 +947,12 @@ SamplePlan sample_plan(int rows, int vocab) {
     if (chunks < 1) chunks = 1;
     p.chunk = (p.segments + chunks - 1) / chunks * kSegment;
     p.chunks = (vocab + p.chunk - 1) / p.chunk;
-    const long long bins = (long long)rows * p.chunks * kBins, segs = (long long)rows * p.segments;
+    const long long segs = (long long)rows * p.segments;
     p.top = 0;
-    p.sum = p.top + (8ll * rows * p.chunks + 15) / 16 * 16;  // read 16 bytes at a time
-    p.seg = p.sum + 8 * bins;
+    p.bins = p.top + (8ll * rows * p.chunks + 15) / 16 * 16;  // read 16 bytes at a time
+    p.seg = p.bins + (long long)rows * p.chunks * kBinBytes;
     p.border = p.seg + 8 * segs;
-    p.count = p.border + 8ll * rows;
-    p.tie = p.count + 4 * bins;
+    p.tie = p.border + 8ll * rows;
     p.bytes = (p.tie + 4 * segs + 15) / 16 * 16;
     return p;
 }
@@ -877,9 +970,8 @@ int launch_sample(const SampleArgs& a, int rows, const SamplePlan& p, void* ws, 
         return moss_launch_status();
     }
     unsigned char* at = (unsigned char*)ws;
-    const Work w{(unsigned long long*)(at + p.top), (unsigned long long*)(at + p.sum), (uint32_t*)(at + p.count),
-                 (unsigned long long*)(at + p.seg), (uint32_t*)(at + p.tie),           (uint2*)(at + p.border),
-                 p.chunks,                          p.chunk,                           p.segments};
+    const Work w{(unsigned long long*)(at + p.top), at + p.bins, (unsigned long long*)(at + p.seg), (uint32_t*)(at + p.tie),
+                 (uint2*)(at + p.border), p.chunks, p.chunk, p.segments};
     const dim3 many((unsigned)(rows * p.chunks)), one((unsigned)rows);
     hipLaunchKernelGGL(sample_top_kernel<TYPE>, many, dim3(512), 0, st, a, w);
     hipLaunchKernelGGL(sample_bins_kernel<TYPE>, many, dim3(512), 0, st, a, w);

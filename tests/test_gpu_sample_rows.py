@@ -21,6 +21,14 @@ def _logits(rows, vocab, g, dtype, kind):
     if kind == "near_zero":  # many distinct keys in a narrow range
         return (torch.randn((rows, vocab), generator=g) * 1e-3).to(dtype)
     x = torch.randn((rows, vocab), generator=g) * 2
+    if kind == "negative":
+        return (x - 20).to(dtype)
+    if kind == "between":  # a few entries above, most around 0
+        x = x * 4e-3
+        x[:, ::37] += 0.05
+        return x.to(dtype)
+    if kind == "far":
+        return (x * 300).to(dtype)
     if kind == "masked":  # all but a few entries masked, by -inf or the type's lowest value
         keep = torch.rand((rows, vocab), generator=g) < 4 / vocab
         keep[:, 0] = True
@@ -77,7 +85,7 @@ def test_sizes(dev, dtype, vocab):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("kind", ["ties", "equal", "near_zero", "masked"])
+@pytest.mark.parametrize("kind", ["ties", "equal", "near_zero", "masked", "negative", "between", "far"])
 @pytest.mark.parametrize("vocab", [300, 1000, 2000, 4100, 30000])
 def test_hard_rows(dev, dtype, kind, vocab):
     g = torch.Generator().manual_seed(1)
@@ -107,6 +115,7 @@ def test_text_vocabulary(dev, dtype):
     g = torch.Generator().manual_seed(3)
     _check(_logits(16, 151936, g, dtype, "plain"), torch.rand(16, generator=g), _mixed(16, g), dev)
     _check(_logits(2, 151936, g, dtype, "equal"), torch.rand(2, generator=g), dict(top_k=1000, top_p=0.5), dev)
+    _check(_logits(4, 151936, g, dtype, "between"), torch.rand(4, generator=g), dict(top_p=0.5), dev)
 
 
 def test_strides_and_vocab(dev):
