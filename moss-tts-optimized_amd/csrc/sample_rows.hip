@@ -931,30 +931,45 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleArgs a, int rows
 }
 
 // ---------------------------------------------------------------- launches
+// Where a call's parts lie in its workspace, and what it needs in all.
 struct SamplePlan {
     int chunks, chunk, segments;
-    long long top, bins, seg, border, tie, bytes;  // offsets
+    long long bins, seg, border, tie, bytes;  // offsets; the largest logits lie at 0
 };
+
+constexpr int kReaders = 1024;  // workgroups that read rows, about, of at least 8 segments each
+
+void lay_out(SamplePlan& p, long long rows, long long chunks) {  // chunks: of all rows
+    p.bins = (8 * chunks + 15) / 16 * 16;  // read 16 bytes at a time
+    p.seg = p.bins + chunks * kBinBytes;
+    p.border = p.seg + 8 * rows * p.segments;
+    p.tie = p.border + 8 * rows;
+    p.bytes = (p.tie + 4 * rows * p.segments + 15) / 16 * 16;
+}
 
 SamplePlan sample_plan(int rows, int vocab) {
     SamplePlan p{};
     if (vocab <= kSmall) return p;
     p.segments = (vocab + kSegment - 1) / kSegment;
-    // about 1024 workgroups, of at least 8 segments each and at most 16 a row
-    int chunks = 1024 / rows;
+    int chunks = kReaders / rows;
     if (chunks > kMaxChunks) chunks = kMaxChunks;
     if (chunks > p.segments / 8) chunks = p.segments / 8;
     if (chunks < 1) chunks = 1;
     p.chunk = (p.segments + chunks - 1) / chunks * kSegment;
     p.chunks = (vocab + p.chunk - 1) / p.chunk;
-    const long long segs = (long long)rows * p.segments;
-    p.top = 0;
-    p.bins = p.top + (8ll * rows * p.chunks + 15) / 16 * 16;  // read 16 bytes at a time
-    p.seg = p.bins + (long long)rows * p.chunks * kBinBytes;
-    p.border = p.seg + 8 * segs;
-    p.tie = p.border + 8ll * rows;
-    p.bytes = (p.tie + 4 * segs + 15) / 16 * 16;
+    lay_out(p, rows, (long long)rows * p.chunks);
     return p;
+}
+
+// No call of up to `rows` rows and `vocab` entries needs more, whatever the workgroups that its rows are shared out over.
+long long most_bytes(int rows, int vocab) {
+    SamplePlan p{};
+    if (vocab <= kSmall) return 0;
+    p.segments = (vocab + kSegment - 1) / kSegment;
+    long long chunks = (long long)rows * (p.segments / 8 < 1 ? 1 : p.segments / 8 < kMaxChunks ? p.segments / 8 : kMaxChunks);
+    const long long most = rows > kReaders ? rows : kReaders;
+    lay_out(p, rows, chunks < most ? chunks : most);
+    return p.bytes;
 }
 
 template <int TYPE>
@@ -970,7 +985,7 @@ int launch_sample(const SampleArgs& a, int rows, const SamplePlan& p, void* ws, 
         return moss_launch_status();
     }
     unsigned char* at = (unsigned char*)ws;
-    const Work w{(unsigned long long*)(at + p.top), at + p.bins, (unsigned long long*)(at + p.seg), (uint32_t*)(at + p.tie),
+    const Work w{(unsigned long long*)at, at + p.bins, (unsigned long long*)(at + p.seg), (uint32_t*)(at + p.tie),
                  (uint2*)(at + p.border), p.chunks, p.chunk, p.segments};
     const dim3 many((unsigned)(rows * p.chunks)), one((unsigned)rows);
     hipLaunchKernelGGL(sample_top_kernel<TYPE>, many, dim3(512), 0, st, a, w);
@@ -986,9 +1001,10 @@ int launch_sample(const SampleArgs& a, int rows, const SamplePlan& p, void* ws, 
 
 using namespace moss;
 
+// Enough for any call of up to these sizes: fewer rows are read by more workgroups each.
 MOSS_API long long moss_sample_rows_workspace_bytes(int rows, int vocab) {
     if (rows <= 0 || rows > (1 << 21) || vocab <= 0 || vocab > kMaxVocab) return 0;
-    return sample_plan(rows, vocab).bytes;
+    return most_bytes(rows, vocab);
 }
 
 MOSS_API int moss_sample_rows(const void* logits, int dtype, int rows, long long stride, int vocab, const void* uniform,
@@ -1000,7 +1016,7 @@ MOSS_API int moss_sample_rows(const void* logits, int dtype, int rows, long long
     MOSS_CHECK_ARG(MOSS_ALIGNED(logits, dtype == 2 ? 4 : 2) && MOSS_ALIGNED(uniform, 4) && MOSS_ALIGNED(temperature, 4) &&
                    MOSS_ALIGNED(top_k, 4) && MOSS_ALIGNED(top_p, 4) && MOSS_ALIGNED(min_p, 4) && MOSS_ALIGNED(out, 8));
     const SamplePlan p = sample_plan(rows, vocab);
-    MOSS_CHECK_ARG(p.bytes == 0 || (workspace && MOSS_ALIGNED(workspace, 16) && workspace_bytes >= p.bytes));
+    MOSS_CHECK_ARG(p.bytes == 0 || (workspace && MOSS_ALIGNED(workspace, 16) && workspace_bytes >= most_bytes(rows, vocab)));
     const SampleArgs a{logits, stride, vocab, (const float*)uniform, (const float*)temperature, (const int*)top_k,
                        (const float*)top_p, (const float*)min_p, temperature_value, top_p_value, min_p_value, top_k_value,
                        (int64_t*)out};

@@ -162,9 +162,13 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
         _cuda_contig("ws", ws, torch.float32, dev)
         _require(4 * ws.numel() >= native.lib().moss_sample_rows_workspace_bytes(rows, vocab) and ws.data_ptr() % 16 == 0,
                  "workspace too small or not 16-byte aligned")
+        end = ws.data_ptr() + 4 * ws.numel()
+        for first, size in ((logits.data_ptr(), ((rows - 1) * stride + entries) * logits.element_size()),
+                            (out.data_ptr(), 8 * rows), (uniform.data_ptr(), 4 * rows)):
+            _require(end <= first or first + size <= ws.data_ptr(), "ws must not overlap the other tensors")
     native.call_on(logits, "moss_sample_rows", logits.data_ptr(), _SAMPLE_TYPES[logits.dtype], rows, stride, vocab,
-                   uniform.data_ptr(), t_ptr, float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m), out.data_ptr(), None if ws is None else ws.data_ptr(),
-                   0 if ws is None else 4 * ws.numel())
+                   uniform.data_ptr(), t_ptr, float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m), out.data_ptr(),
+                   None if ws is None else ws.data_ptr(), 0 if ws is None else 4 * ws.numel())
     return out
 
 

@@ -98,3 +98,16 @@ def test_sample_rows(lib):
     assert lib.moss_sample_rows_workspace_bytes(3, 2048) == 0
     assert lib.moss_sample_rows_workspace_bytes(0, 5000) == 0
     assert lib.moss_sample_rows_workspace_bytes(3, (1 << 19) + 1) == 0
+
+
+def test_sample_workspace_serves_smaller_calls(lib):
+    """A workspace for some rows and entries is enough for fewer of either."""
+    size = lib.moss_sample_rows_workspace_bytes
+    rows = [1, 2, 3, 17, 63, 64, 65, 100, 128, 129, 511, 512, 513, 1023, 1024, 1025, 5000]
+    vocabs = [2049, 2560, 4096, 4097, 8191, 8193, 16385, 50000, 65537, 100000, 151936, 262145, 1 << 19]
+    for n in rows:
+        sizes = [size(n, v) for v in vocabs]
+        assert sizes == sorted(sizes)
+    for v in vocabs:
+        sizes = [size(n, v) for n in rows]
+        assert sizes == sorted(sizes)

@@ -169,6 +169,69 @@ def test_graph_reads_settings_at_replay(dev):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("rows, vocab", [(2, 40000), (70, 9000), (1100, 2500)])
+def test_long_rows_graph_and_kept_workspace(dev, rows, vocab):
+    """Several launches in one graph, with a workspace of a larger call's, new logits and settings between the replays; eager
+    work and synchronizations between them too."""
+    from moss_tts._runtime import sampling
+
+    g = torch.Generator().manual_seed(6)
+    x = _logits(rows, vocab, g, torch.bfloat16, "plain").to(dev)
+    u = torch.rand(rows, generator=g).to(dev)
+    s = {k: v.to(dev) for k, v in _mixed(rows, g).items()}
+    ws = sampling.sample_workspace(rows + 3, vocab + 7000, dev).fill_(math.nan)
+    sampling.sample(x, u, **s, ws=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sampling.sample(x, u, **s, ws=ws)
+    for _ in range(4):
+        x.copy_(_logits(rows, vocab, g, torch.bfloat16, "plain"))
+        u.copy_(torch.rand(rows, generator=g))
+        for k, v in _mixed(rows, g).items():
+            s[k].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, sampling.sample(x, u, **s))
+        torch.cuda.synchronize()
+
+
+def test_kept_workspace_of_more_rows(dev):
+    """65 rows are read by fewer workgroups than 64."""
+    from moss_tts._runtime import sampling
+
+    g = torch.Generator().manual_seed(7)
+    ws = sampling.sample_workspace(65, 151936, dev)
+    x = _logits(64, 151936, g, torch.bfloat16, "plain").to(dev)
+    u = torch.rand(64, generator=g).to(dev)
+    assert torch.equal(sampling.sample(x, u, top_k=50, top_p=0.9, ws=ws), sampling.sample(x, u, top_k=50, top_p=0.9))
+
+
+def test_calls_on_two_streams(dev):
+    from moss_tts._runtime import sampling
+
+    g = torch.Generator().manual_seed(8)
+    sets = [(_logits(n, 30000, g, torch.bfloat16, "plain").to(dev), torch.rand(n, generator=g).to(dev)) for n in (3, 40)]
+    alone = [sampling.sample(*s, top_k=100, top_p=0.95) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    outs = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(sampling.sample(*sets[i], top_k=100, top_p=0.95))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, alone[i]) for y in outs[i])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_largest_vocabulary(dev, dtype):
+    g = torch.Generator().manual_seed(9)
+    _check(_logits(6, 1 << 19, g, dtype, "plain"), torch.rand(6, generator=g), _mixed(6, g), dev)
+
+
 def test_refusals(dev):
     from moss_tts._runtime import sampling
 
@@ -186,3 +249,12 @@ def test_refusals(dev):
                         ("vocab", (x, u), dict(vocab=0)), ("out must hold", (x, u), dict(out=torch.zeros(2, dtype=torch.int64, device=dev)))):
         with pytest.raises(ValueError, match=match):
             sampling.sample(*a, **k)
+    x = torch.zeros((3, 3000), dtype=torch.float32, device=dev)
+    ws = sampling.sample_workspace(3, 3000, dev)
+    for match, bad in (("workspace too small", ws[:-4]), ("16-byte", torch.zeros(ws.numel() + 4, device=dev)[1:]),
+                       ("must not overlap", torch.zeros(ws.numel() + 9000, device=dev))):
+        with pytest.raises(ValueError, match=match):
+            if match == "must not overlap":
+                sampling.sample(bad[-9000:].view(3, 3000), u, ws=bad)
+            else:
+                sampling.sample(x, u, ws=bad)
