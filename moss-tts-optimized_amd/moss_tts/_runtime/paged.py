@@ -13,7 +13,11 @@ outside ``[0, pages)`` names no page: its rows take no part and nothing is writt
 sequence ``b`` and stand at its last positions.  Packed rows from ``starts[B]`` on are padding and left as they are.
 
 Table, lengths and starts are device values, read when the kernels run and not checked by the host: a captured
-graph follows them as sequences grow.  Whatever they hold, no access leaves the cache or the packed rows.
+graph follows them as sequences grow.  Whatever they hold, no access leaves the cache or the packed rows; what they have
+to hold for results is the caller's to see to: lengths that the table's row can hold (the attention takes as many
+rows as that), starts that rise, and no two new tokens on one row of a page (sequences may share the pages that they
+only read).  A row that takes part with values that are not finite makes what it touches not finite; rows that
+take no part may hold anything.
 """
 from __future__ import annotations
 
@@ -235,6 +239,9 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     span = (at, at + 2 * ((tokens - 1) * stride + width))
     _require((c.kend <= span[0] or span[1] <= c.k) and (c.vend <= span[0] or span[1] <= c.v),
              "qkv must not overlap the cache")
+    if c.k < c.vend and c.v < c.kend:  # interleaved: the keys of a page lie between the values of two
+        page, step = 2 * kh * c.rows * d, 2 * c.ks
+        _require(c.ks == c.vs and page <= (c.v - c.k) % step <= step - page, "keys and values must not share memory")
     q = _output(out, (tokens, qh, d), qkv, span, (c.k, c.kend), (c.v, c.vend))
     native.call_on(qkv, "moss_paged_qk_rope", at, stride, *norms, q.data_ptr(), c.k, c.v, c.ks, c.vs, c.pages, c.rows,
                    table.data_ptr(), table_stride, lengths.data_ptr(), None if starts is None else starts.data_ptr(), b,

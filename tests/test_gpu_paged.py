@@ -341,6 +341,95 @@ def test_calls_on_two_streams(dev):
         assert all(torch.equal(x, alone[i]) for x in outs[i])
 
 
+def test_prompt_graph_follows_its_batch(dev):
+    """A captured prompt pass of 60 packed rows and its rope, replayed with other starts and lengths: more and fewer tokens,
+    tiles that are cut and tiles that are not, padding; eager work and synchronizations between the replays."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(12)
+    kh, qh, d, page, total = 2, 8, 128, 16, 60
+    keys, vals, table, lens = cache(dev, g, [3000, 900, 500], kh=kh, d=d, page=page, dtype=torch.bfloat16, poison=0.0)
+    starts = torch.tensor([0, 1, 20, 60], dtype=torch.int32, device=dev)
+    qkv = torch.randn((total, (qh + 2 * kh) * d), generator=g).bfloat16().to(dev)
+    cos, sin = (torch.randn((4096, d), generator=g).to(dev) for _ in range(2))
+    out = torch.zeros((total, qh * d), dtype=torch.bfloat16, device=dev)
+
+    def step(k, v, q, o):
+        paged.qk_rope(qkv, None, None, cos, sin, k, v, table, lens, 1e-6, starts=starts, out=q)
+        return paged.prompt_attention(q, k, v, table, lens, starts, out=o)
+
+    q = torch.zeros((total, qh, d), dtype=torch.bfloat16, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(keys, vals, q, out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(keys, vals, q, out)
+    k2, v2, q2, o2 = (t.clone() for t in (keys, vals, q, out))
+    for at, n in (([0, 1, 20, 60], [3000, 900, 500]), ([0, 0, 40, 41], [0, 40, 17]), ([0, 1, 2, 3], [2999, 898, 499]),
+                  ([0, 60, 60, 60], [60, 0, 3]), ([0, 0, 0, 0], [1, 2, 3]), ([0, 2, 3, 40], [2048, 64, 500])):
+        starts.copy_(torch.tensor(at, dtype=torch.int32))
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        qkv.copy_(torch.randn(qkv.shape, generator=g).to(torch.bfloat16))
+        for t in (q, out, q2, o2):
+            t.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        step(k2, v2, q2, o2)
+        torch.cuda.synchronize()
+        for a, b in ((q, q2), (out, o2), (keys, k2), (vals, v2)):
+            assert torch.equal(a, b)
+        assert (out[at[-1]:] == 9.0).all() and (q[at[-1]:] == 9.0).all()
+
+
+def test_prompt_calls_on_two_streams(dev):
+    """Prompts whose tiles are cut, on two streams, with workspaces of their own."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(13)
+    sets = []
+    for old, new in (([3000, 10], [2, 30]), ([1500, 700], [20, 1])):
+        keys, vals, table, lens = cache(dev, g, [a + b for a, b in zip(old, new)], kh=2, d=128, page=32, dtype=torch.bfloat16)
+        starts = torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device=dev)
+        sets.append((torch.randn((sum(new), 8, 128), generator=g).bfloat16().to(dev), keys, vals, table, lens, starts))
+    alone = [paged.prompt_attention(*s) for s in sets]
+    kept = [paged.prompt_workspace(s[0], s[1], s[3]) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    outs = [[], []]
+    for n in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(paged.prompt_attention(*sets[i], ws=kept[i] if n % 2 else None))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, alone[i]) for x in outs[i])
+
+
+def test_pages_that_sequences_share(dev):
+    """A prefix of whole pages that three sequences read, and one page twice in a sequence."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(14)
+    keys, vals, _, _ = cache(dev, g, [160], kh=2, d=64, page=16, dtype=torch.bfloat16)
+    rows = [int(p) for p in torch.where(torch.isfinite(keys[:, 0, 0, 0].float()))[0]]
+    table = torch.tensor([rows[:4] + [rows[4], rows[4]], rows[:4] + [rows[5], -1], rows[:4] + [rows[6], rows[7]]],
+                         dtype=torch.int32, device=dev)
+    lens = torch.tensor([96, 70, 90], dtype=torch.int32, device=dev)
+    q = torch.randn((3, 8, 64), generator=g).bfloat16().to(dev)
+    k, v = values(keys), values(vals)
+    ref = o.decode_attention(values(q), k, v, table.cpu().numpy(), lens.cpu().numpy())
+    ref_abs = o.decode_attention(values(q), k, np.abs(v), table.cpu().numpy(), lens.cpu().numpy())
+    live_k, live_v = np.nan_to_num(k), np.nan_to_num(v)
+    got = paged.decode_attention(q, keys, vals, table, lens)
+    _close(got, ref, attention_bound(values(q), live_k, live_v, ref, ref_abs, 0.125, q.dtype, False), "decode")
+    starts = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=dev)
+    got = paged.prompt_attention(q, keys, vals, table, lens, starts)
+    _close(got, ref, attention_bound(values(q), live_k, live_v, ref, ref_abs, 0.125, q.dtype, True), "prompt")
+
+
 def test_refusals(dev):
     from moss_tts._runtime import paged
 
@@ -387,6 +476,8 @@ def test_refusals(dev):
     refused("one token a sequence", r, qkv[:1], None, None, cos, cos, keys, vals, table, lens, 1e-6)
     refused("cos must be", r, qkv, None, None, cos.double(), cos.double(), keys, vals, table, lens, 1e-6)
     refused("sin must be", r, qkv, None, None, cos, cos.bfloat16(), keys, vals, table, lens, 1e-6)
+    refused("share memory", r, qkv, None, None, cos, cos, keys, keys, table, lens, 1e-6)
+    refused("share memory", r, qkv, None, None, cos, cos, keys[:2], keys[1:3], table, lens, 1e-6)
     refused("eps", r, qkv, None, None, cos, cos, keys, vals, table, lens, -1.0)
     refused("16-byte", r, qkv.view(-1)[4:4 + 512].view(1, 512), None, None, cos, cos, keys, vals, table[:1], lens[:1], 1e-6)
 
@@ -430,6 +521,7 @@ def test_prompt_values_behind_a_token(dev, new, old, layout, what):
     starts = torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device=dev)
     q = torch.randn((sum(new), qh, d), generator=g).bfloat16().to(dev)
     clean = paged.prompt_attention(q, keys, vals, table, lens, starts)
+    spread = values(paged.prompt_attention(q, keys, vals.abs(), table, lens, starts))  # sum p |v|
     bad = [n - n // 3 for n in new]  # the new token of each sequence whose row is bad
     for b, t in enumerate(bad):
         row = old[b] + t
@@ -440,8 +532,11 @@ def test_prompt_values_behind_a_token(dev, new, old, layout, what):
     torch.cuda.synchronize()
     for b, t in enumerate(bad):
         at = int(starts[b])
-        x, y = values(got[at:at + t]), values(clean[at:at + t])
-        # the rows of tiles without such a key are the same; others are summed without rounding P
-        assert np.isfinite(x).all() and (np.abs(x - y) <= 2.0 ** -6 * np.abs(y) + 2.0 ** -6).all()
+        x, y, a = values(got[at:at + t]), values(clean[at:at + t]), spread[at:at + t]
+        # The rows of tiles without such a key are the same.  The others are summed without rounding P, by which each
+        # weight differs by at most 2^-8 of itself and the output by twice that of sum p |v|; both are rounded once more,
+        # by 2^-8, and scores summed in another order move a weight by less than 2^-12.
+        assert np.isfinite(x).all()
+        assert (np.abs(x - y) <= (2.0 ** -7 + 2.0 ** -11) * a * (1 + 2.0 ** -6) + 2.0 ** -8 * (np.abs(x) + np.abs(y))).all()
         after = got[at + t:at + new[b]].view(-1, qh, d)[..., ::3]
         assert not torch.isfinite(after).any()
