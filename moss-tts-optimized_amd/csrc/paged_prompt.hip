@@ -40,7 +40,7 @@ struct PromptArgs {
 };
 
 // A workgroup's sequence and its item's number, of what count(tiles, share) counts; `first`: partial results of the
-// sequences before it.  A batch of up to 64 is one read of lengths and starts.
+// sequences taken before it.  A batch of up to 64 is one read of lengths and starts, and taken in the order of its lengths.
 struct Found {
     PromptTiles tiles;
     int b, tok0, index, share, first;  // b -1: none
@@ -59,16 +59,33 @@ __device__ __forceinline__ Found find_tile(const PromptArgs& a, const PagedCache
     int tok0 = 0;
     if (bt.B <= kWave) {
         PromptTiles t{0, a.group, 0, HEIGHT};
+        int b = lane;
         if (lane < bt.B) t = of(lane, tok0);
+        if (bt.B > 1) {
+            // longest first: its tiles see the most keys, and what is taken last ends last.  (Nine prompts that come shortest
+            // first 64 -> 48 us.)
+            const int key = lane < bt.B ? (t.pos0 + t.tokens) / kPromptBlock * kWave + kWave - 1 - lane : -1;
+            int place = 0;
+            for (int j0 = 0; j0 < bt.B; j0 += 8)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) place += __builtin_amdgcn_readlane(key, j0 + j) > key;
+            if (lane >= bt.B) place = lane;
+            auto move = [&](int v) { return __builtin_amdgcn_ds_permute(4 * place, v); };
+            b = move(b);
+            tok0 = move(tok0);
+            t = PromptTiles{move(t.tokens), a.group, move(t.pos0), HEIGHT};
+        }
         f.share = uniform(prompt_share(wave_total(t.blocks_bound()), a.shares));
         const int n = count(t, f.share), through = wave_prefix(n);
         const unsigned long long past = __ballot(through > item);
-        f.b = past ? __builtin_ctzll(past) : -1;
+        f.b = -1;
         if (!past) return f;
-        f.tiles = PromptTiles{lane_value(t.tokens, f.b), a.group, lane_value(t.pos0, f.b), HEIGHT};
-        f.tok0 = lane_value(tok0, f.b);
-        f.index = item - (lane_value(through, f.b) - lane_value(n, f.b));
-        f.first = wave_total(lane < f.b ? parts(t, f.share) : 0);
+        const int l = __builtin_ctzll(past);
+        f.b = lane_value(b, l);
+        f.tiles = PromptTiles{lane_value(t.tokens, l), a.group, lane_value(t.pos0, l), HEIGHT};
+        f.tok0 = lane_value(tok0, l);
+        f.index = item - (lane_value(through, l) - lane_value(n, l));
+        f.first = wave_total(lane < l ? parts(t, f.share) : 0);
         return f;
     }
     long long blocks = 0;
