@@ -15,14 +15,16 @@
 // The borders of the prefix are found without sorting: a histogram (count and sum of w) over bins of 1/32 octave of w,
 // then the border bin's own entries; of the entries with the border's key, the first few in index order are kept.
 //
-// What bounds it: the arithmetic of w in 64 bits, and for few rows the chain of steps.  So a row is read by several
-// workgroups, in five launches (largest logit; histogram; border; weight of each segment of 512 entries; draw), of which
-// the segments form w for the kept entries, and the histogram for all of a row with top-p, unless its bins are single
-// values that need only be counted (bf16).  w takes 14 operations in 64 bits, of 8 cycles each for a wave.  128 rows of 151,936
-// bf16 logits, each with its own settings: 65 us (9 + 19 + 12 + 19 + 6); with linear bins and the border's bin collected 84,
-// of those with a series of ten terms and no table 93, and one workgroup a row 309.  One row: 30 us, 182 before.  A row of
-// up to 2048 entries is one wave's: it holds them and their weights in registers, and needs no barrier (512 rows of 1024:
-// 13.7 us, 46 before).
+// What bounds it: the arithmetic of w in 64 bits, counting in LDS, and for few rows the chain of steps.  A row is read by
+// several workgroups, in five launches (largest logit; histogram; border; weight of each segment of 512 entries; draw), of
+// which the segments form w for the kept entries, and the histogram for all of a row with top-p, unless its bins are single
+// values that need only be counted (bf16).  Then, for more than kFewRows rows, the counts also say which part of the row the
+// drawn entry lies in, and one launch in place of the last three finds the border and reads that part alone.  w takes 14
+// operations in 64 bits, of 8 cycles each for a wave.  128 rows of 151,936 bf16 logits, each with its own settings: 53 us;
+// with the last three launches 61 (9 + 18 + 12 + 18 + 6), with linear bins besides 84, of those with a series of ten terms and
+// no table 93, and one workgroup a row 309.  One row: 28 us on the average of its settings, 182 by one workgroup.  A row of up
+// to 2048 entries is one wave's: it holds them and their weights in registers, and needs no barrier (512 rows of 1024: 13.7 us,
+// 46 before).
 #include "common.h"
 
 namespace moss {
@@ -337,6 +339,7 @@ struct Work {
     uint32_t* tie;              // [rows, segments]: entries with the border's key
     uint2* border;              // [rows]
     int chunks, chunk, segments;  // chunk: entries, whole segments
+    bool finish;                  // sample_finish_kernel draws: it wants every row's key bins
 };
 
 template <int TYPE>
@@ -377,14 +380,15 @@ __global__ __launch_bounds__(512) void sample_bins_kernel(SampleArgs a, Work w) 
     const int row = blockIdx.x / w.chunks, chunk = blockIdx.x % w.chunks, tid = threadIdx.x, lane = tid & (kWave - 1);
     Row r = row_of<TYPE>(a, row);
     int index;
-    if (!(r.by_k || r.by_p) || !load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
+    if (!load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
+    const KeyBins q = key_bins<TYPE>(r);
+    if (!(r.by_k || r.by_p || (w.finish && q.on))) return;
     fill_table(table, tid);
     const u32x4_t zero = {0u, 0u, 0u, 0u};
     for (int b = tid; b < kBinBytes / 16; b += 512) reinterpret_cast<u32x4_t*>(bins)[b] = zero;
     __syncthreads();
     unsigned long long* sum = reinterpret_cast<unsigned long long*>(bins);
     const int end = min(r.vocab, (chunk + 1) * w.chunk);
-    const KeyBins q = key_bins<TYPE>(r);
     int used = kBinBytes / 16;
     if (q.on) {
         uint32_t* count = reinterpret_cast<uint32_t*>(bins + 16);
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(512) void sample_bins_kernel(SampleArgs a, Work w) 
             for (int j = 0; j < 8; ++j) {
                 const int b = bin_of_key(q, key_of<TYPE>(x[j]));
                 if (b < q.all) atomicAdd(&count[b], 1u);
-                if (b == q.np && r.by_p) atomicAdd(sum, weight_of(r, x[j], table));
+                if (b == q.np && (r.by_p || w.finish)) atomicAdd(sum, weight_of(r, x[j], table));
             }
         });
         used = 1 + (q.all + 3) / 4;
@@ -539,23 +543,17 @@ __device__ Border border_among(BorderShared& sh, const Row& r, const Goal& goal,
     return goal.end(lo, n, r.by_p ? weight_of(r, logit_of<TYPE>(lo), sh.table) : 0, base_count, base_sum);
 }
 
+// The border of a row with the workgroup's bins in place and the table filled; `q`: its key bins.
 template <int TYPE>
-__global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(SampleArgs a, Work w) {
-    __shared__ BorderShared sh;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    Row r = row_of<TYPE>(a, row);
-    int index;
-    if (!load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
-    Border border{kLowest<TYPE> + 1, 0xffffffffu, 0};     // everything above -inf
+__device__ __forceinline__ Border row_border(BorderShared& sh, const Row& r, const KeyBins& q, const Work& w, int row) {
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    Border border{kLowest<TYPE> + 1, 0xffffffffu, 0};  // everything above -inf
     if (r.by_k || r.by_p) {
-        fill_table(sh.table, tid);
-        const KeyBins q = key_bins<TYPE>(r);
         const unsigned char* from = w.bins + (size_t)row * w.chunks * kBinBytes;
         // this thread's bins, summed over the chunks; their loads go out together (a chunk behind the last is the last one)
         uint32_t c[4] = {0u, 0u, 0u, 0u};
         unsigned long long s[4] = {0ull, 0ull, 0ull, 0ull};
         if (q.on) {  // bins 4 tid ..
-            __syncthreads();  // the table
             if (4 * tid < q.all) {
                 uint4 cs[kMaxChunks];
                 unsigned long long between = 0;
@@ -637,6 +635,19 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(SampleArg
         const uint32_t k = first_key_of_min_p<TYPE>(r, lane);
         if (k > border.key) border = Border{k, 0xffffffffu, 0};
     }
+    return border;
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(SampleArgs a, Work w) {
+    __shared__ BorderShared sh;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
+    Row r = row_of<TYPE>(a, row);
+    int index;
+    if (!load_top<TYPE>(r, w, row, lane, index)) return;  // uniform
+    fill_table(sh.table, tid);
+    __syncthreads();
+    const Border border = row_border<TYPE>(sh, r, key_bins<TYPE>(r), w, row);
     if (tid == 0) w.border[row] = make_uint2(border.key, border.ties);
 }
 
@@ -646,6 +657,26 @@ __device__ __forceinline__ unsigned long long kept_weight(const Row& r, float x,
     const uint32_t k = key_of<TYPE>(x);
     tie = k == border;
     return k > border ? weight_of(r, x, table) : 0;
+}
+
+// The weight of a segment's entries above the border's key and the number of those with it, eight entries a lane.
+template <int TYPE>
+__device__ __forceinline__ unsigned long long segment_weight(const Row& r, const float (&x)[8], uint32_t border,
+                                                             const double* table, uint32_t& ties) {
+    unsigned long long sum = 0;
+    ties = 0;
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = fmaxf(m, x[j]);
+    if (!__any(key_of<TYPE>(m) >= border)) return 0;  // nothing of the segment is kept
+    bool tie;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        sum += kept_weight<TYPE>(r, x[j], border, table, tie);
+        ties += tie;
+    }
+    ties = wave_total(ties);
+    return wave_total(sum);
 }
 
 template <int TYPE>
@@ -662,21 +693,8 @@ __global__ __launch_bounds__(512) void sample_segments_kernel(SampleArgs a, Work
     for (int s = chunk * per + tid / kWave; s < last; s += 512 / kWave) {
         float x[8];
         load8<TYPE>(r.at, kSegment * s + 8 * lane, r.vocab, r.aligned, x);
-        unsigned long long sum = 0;
-        uint32_t ties = 0;
-        float m = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) m = fmaxf(m, x[j]);
-        if (__any(key_of<TYPE>(m) >= border)) {  // else nothing of the segment is kept
-            bool tie;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sum += kept_weight<TYPE>(r, x[j], border, table, tie);
-                ties += tie;
-            }
-            sum = wave_total(sum);
-            ties = wave_total(ties);
-        }
+        uint32_t ties;
+        const unsigned long long sum = segment_weight<TYPE>(r, x, border, table, ties);
         if (lane == 0) {
             w.seg[(size_t)row * w.segments + s] = sum;
             w.tie[(size_t)row * w.segments + s] = ties;
@@ -688,44 +706,38 @@ __device__ __forceinline__ uint32_t ties_kept(uint32_t ties, uint32_t before, ui
     return ties > before ? min(ties - before, count) : 0u;
 }
 
+// The draw in segments first .. first + count - 1 of a row, whose weights s and ties n thread i holds for segment first + i.
+// Before them lie `before_sum` and `before_ties`; `total`: of the whole row (0: these segments are the whole row).
+struct DrawShared {
+    unsigned long long part_sum[kBorderWaves], before_sum, all;
+    uint32_t part_count[kBorderWaves], before_ties;
+    int found;
+};
 template <int TYPE>
-__global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a, Work w) {
-    __shared__ double table[32];
-    __shared__ unsigned long long part_sum[16], before_sum, all;
-    __shared__ uint32_t part_count[16], before_ties;
-    __shared__ int found;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    Row r = row_of<TYPE>(a, row);
-    int index;
-    if (!load_top<TYPE>(r, w, row, lane, index)) {  // uniform
-        if (tid == 0) a.out[row] = index;
-        return;
-    }
-    const uint2 border = w.border[row];
-    fill_table(table, tid);
-    const size_t at = (size_t)row * w.segments + tid;
-    const unsigned long long s = tid < w.segments ? w.seg[at] : 0;
-    const uint32_t n = tid < w.segments ? w.tie[at] : 0;
+__device__ __forceinline__ void draw_in(DrawShared& sh, const SampleArgs& a, const Row& r, int row, const double* table, uint2 border,
+                                        int first, int count, unsigned long long s, uint32_t n, unsigned long long before_sum,
+                                        uint32_t before_ties, unsigned long long total) {
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     if (tid == 0) {
-        found = w.segments - 1;
-        before_sum = 0;
-        before_ties = 0;
+        sh.found = count - 1;
+        sh.before_sum = before_sum;
+        sh.before_ties = before_ties;
     }
-    const uint32_t before = block_prefix<uint32_t>(n, part_count, lane, wave) - n;  // and the table is there
+    const uint32_t before = before_ties + block_prefix<uint32_t>(n, sh.part_count, lane, wave) - n;  // and the table is there
     const unsigned long long border_w = weight_of(r, logit_of<TYPE>(border.x), table);
     const unsigned long long mine = s + ties_kept(border.y, before, n) * border_w;
-    const unsigned long long through = block_prefix<unsigned long long>(mine, part_sum, lane, wave);
-    if (tid == 1023) all = through;
+    const unsigned long long through = before_sum + block_prefix<unsigned long long>(mine, sh.part_sum, lane, wave);
+    if (tid == kBorderThreads - 1) sh.all = through;
     __syncthreads();
-    const unsigned long long target = target_of(a.uniform[row], all);
+    const unsigned long long target = target_of(a.uniform[row], total ? total : sh.all);
     if (through > target && through - mine <= target) {
-        found = tid;
-        before_sum = through - mine;
-        before_ties = before;
+        sh.found = tid;
+        sh.before_sum = through - mine;
+        sh.before_ties = before;
     }
     __syncthreads();
     if (wave != 0) return;
-    const int i0 = kSegment * found + 8 * lane;
+    const int i0 = kSegment * (first + sh.found) + 8 * lane;
     float x[8];
     load8<TYPE>(r.at, i0, r.vocab, r.aligned, x);
     unsigned long long wj[8], sum = 0;
@@ -736,18 +748,128 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a, Work w)
         wj[j] = kept_weight<TYPE>(r, x[j], border.x, table, tie[j]);
         ties += tie[j];
     }
-    uint32_t rank = before_ties + wave_prefix<uint32_t>(ties) - ties;
+    uint32_t rank = sh.before_ties + wave_prefix<uint32_t>(ties) - ties;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (tie[j]) wj[j] = rank++ < border.y ? border_w : 0;
         sum += wj[j];
     }
-    unsigned long long cum = before_sum + wave_prefix<unsigned long long>(sum) - sum;
+    unsigned long long cum = sh.before_sum + wave_prefix<unsigned long long>(sum) - sum;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (cum <= target && cum + wj[j] > target) a.out[row] = i0 + j;  // one entry's
         cum += wj[j];
     }
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kBorderThreads) void sample_draw_kernel(SampleArgs a, Work w) {
+    __shared__ double table[32];
+    __shared__ DrawShared sh;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
+    Row r = row_of<TYPE>(a, row);
+    int index;
+    if (!load_top<TYPE>(r, w, row, lane, index)) {  // uniform
+        if (tid == 0) a.out[row] = index;
+        return;
+    }
+    fill_table(table, tid);
+    const size_t at = (size_t)row * w.segments + tid;
+    const unsigned long long s = tid < w.segments ? w.seg[at] : 0;
+    const uint32_t n = tid < w.segments ? w.tie[at] : 0;
+    draw_in<TYPE>(sh, a, r, row, table, w.border[row], 0, w.segments, s, n, 0, 0, 0);
+}
+
+// Border and draw of a row of bf16 logits.  The key bins say what each chunk's kept entries weigh, so that only the chunk
+// with the drawn entry is read again.  A row without key bins, or with its border between them, is read here as a whole.
+struct FinishShared {
+    BorderShared border;
+    DrawShared draw;
+    unsigned long long chunk_sum[kMaxChunks][kBorderWaves];
+    uint32_t chunk_ties[kMaxChunks];
+};
+__global__ __launch_bounds__(kBorderThreads) void sample_finish_kernel(SampleArgs a, Work w) {
+    constexpr int TYPE = 0;
+    __shared__ FinishShared sh;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    Row r = row_of<TYPE>(a, row);
+    int index;
+    if (!load_top<TYPE>(r, w, row, lane, index)) {  // uniform
+        if (tid == 0) a.out[row] = index;
+        return;
+    }
+    const double* table = sh.border.table;
+    fill_table(sh.border.table, tid);
+    if (tid < kMaxChunks) sh.chunk_ties[tid] = 0;
+    __syncthreads();
+    const KeyBins q = key_bins<TYPE>(r);
+    const Border border = row_border<TYPE>(sh.border, r, q, w, row);
+    int first = 0, last = w.segments;
+    unsigned long long before_sum = 0, total = 0;
+    uint32_t before_ties = 0;
+    if (q.on && (border.key >= kLeastPositive || border.key <= kLeastNegative)) {
+        const unsigned char* from = w.bins + (size_t)row * w.chunks * kBinBytes;
+        const int edge = bin_of_key(q, border.key);  // behind all bins: nothing is cut off
+        const bool some = 4 * kWave * wave <= edge && 4 * kWave * wave < q.all;  // of this wave's bins
+        uint4 c[kMaxChunks];
+        unsigned long long weight[4] = {0ull, 0ull, 0ull, 0ull};
+        const int mine = min(4 * tid, q.all - 1) & ~3;
+        if (some) {
+#pragma unroll
+            for (int i = 0; i < kMaxChunks; ++i)
+                c[i] = *reinterpret_cast<const uint4*>(from + (size_t)min(i, w.chunks - 1) * kBinBytes + 16 + 4 * mine);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = 4 * tid + i;
+                if (b < min(edge, q.all) && b != q.np) weight[i] = weight_of(r, logit_of<TYPE>(key_of_bin(q, b)), table);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kMaxChunks; ++i)
+            if (i < w.chunks) {
+                unsigned long long s = 0;
+                if (some) {
+                    s = c[i].x * weight[0] + c[i].y * weight[1] + c[i].z * weight[2] + c[i].w * weight[3];
+                    if (q.np / 4 == tid && edge > q.np) s += *reinterpret_cast<const unsigned long long*>(from + (size_t)i * kBinBytes);
+                    s = wave_total(s);
+                    if (edge / 4 == tid && edge < q.all)
+                        sh.chunk_ties[i] = edge % 4 == 0 ? c[i].x : edge % 4 == 1 ? c[i].y : edge % 4 == 2 ? c[i].z : c[i].w;
+                }
+                if (lane == 0) sh.chunk_sum[i][wave] = s;
+            }
+        __syncthreads();
+        unsigned long long s = 0;
+        uint32_t n = 0;
+        if (lane < w.chunks) {
+            for (int v = 0; v < kBorderWaves; ++v) s += sh.chunk_sum[lane][v];
+            n = sh.chunk_ties[lane];
+        }
+        const uint32_t before = wave_prefix<uint32_t>(n) - n;
+        const unsigned long long kept = s + ties_kept(border.ties, before, n) * weight_of(r, logit_of<TYPE>(border.key), table);
+        const unsigned long long through = wave_prefix<unsigned long long>(kept);
+        total = lane_value(through, kWave - 1);
+        const unsigned long long past = __ballot(through > target_of(a.uniform[row], total));
+        const int chunk = past ? __builtin_ctzll(past) : w.chunks - 1;
+        before_sum = lane_value(through, chunk) - lane_value(kept, chunk);
+        before_ties = lane_value(before, chunk);
+        const int per = w.chunk / kSegment;
+        first = chunk * per;
+        last = min(w.segments, first + per);
+    }
+    __syncthreads();
+    walk<TYPE, 5>(r, kSegment * first + 8 * tid, kSegment * last, 8 * kBorderThreads, [&](int i, const float(&x)[8]) {
+        uint32_t ties;
+        const unsigned long long sum = segment_weight<TYPE>(r, x, border.key, table, ties);  // a wave's entries are a segment
+        if (lane == 0) {
+            sh.border.sum[i / kSegment - first] = sum;
+            sh.border.count[i / kSegment - first] = ties;
+        }
+    });
+    __syncthreads();
+    const unsigned long long s = tid < last - first ? sh.border.sum[tid] : 0;
+    const uint32_t n = tid < last - first ? sh.border.count[tid] : 0;
+    draw_in<TYPE>(sh.draw, a, r, row, table, make_uint2(border.key, border.ties), first, last - first, s, n, before_sum, before_ties,
+                  total);
 }
 
 // ---------------------------------------------------------------- short rows: one wave a row
@@ -972,6 +1094,10 @@ long long most_bytes(int rows, int vocab) {
     return p.bytes;
 }
 
+// More bf16 rows than this are drawn by a workgroup each, fewer by several.  Several / one: 28 / 31 us for one row of 151,936
+// with top-p (18 / 29 without), 33.5 / 33.8 for 16, 62 / 53 for 128; 28 / 25 for 40 of 5,000, 62 / 58 for 400 of 30,000.
+constexpr int kFewRows = 16;
+
 template <int TYPE>
 int launch_sample(const SampleArgs& a, int rows, const SamplePlan& p, void* ws, hipStream_t st) {
     if (a.vocab <= kSmall) {
@@ -986,13 +1112,18 @@ int launch_sample(const SampleArgs& a, int rows, const SamplePlan& p, void* ws, 
     }
     unsigned char* at = (unsigned char*)ws;
     const Work w{(unsigned long long*)at, at + p.bins, (unsigned long long*)(at + p.seg), (uint32_t*)(at + p.tie),
-                 (uint2*)(at + p.border), p.chunks, p.chunk, p.segments};
+                 (uint2*)(at + p.border), p.chunks, p.chunk, p.segments,
+                 TYPE == 0 && rows > kFewRows};
     const dim3 many((unsigned)(rows * p.chunks)), one((unsigned)rows);
     hipLaunchKernelGGL(sample_top_kernel<TYPE>, many, dim3(512), 0, st, a, w);
     hipLaunchKernelGGL(sample_bins_kernel<TYPE>, many, dim3(512), 0, st, a, w);
-    hipLaunchKernelGGL(sample_border_kernel<TYPE>, one, dim3(kBorderThreads), 0, st, a, w);
-    hipLaunchKernelGGL(sample_segments_kernel<TYPE>, many, dim3(512), 0, st, a, w);
-    hipLaunchKernelGGL(sample_draw_kernel<TYPE>, one, dim3(1024), 0, st, a, w);
+    if (w.finish) {
+        hipLaunchKernelGGL(sample_finish_kernel, one, dim3(kBorderThreads), 0, st, a, w);
+    } else {
+        hipLaunchKernelGGL(sample_border_kernel<TYPE>, one, dim3(kBorderThreads), 0, st, a, w);
+        hipLaunchKernelGGL(sample_segments_kernel<TYPE>, many, dim3(512), 0, st, a, w);
+        hipLaunchKernelGGL(sample_draw_kernel<TYPE>, one, dim3(kBorderThreads), 0, st, a, w);
+    }
     return moss_launch_status();
 }
 

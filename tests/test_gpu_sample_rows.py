@@ -92,6 +92,15 @@ def test_hard_rows(dev, dtype, kind, vocab):
     _check(_logits(40, vocab, g, dtype, kind), torch.rand(40, generator=g), _mixed(40, g), dev)
 
 
+@pytest.mark.parametrize("kind", ["plain", "ties", "equal", "near_zero", "masked", "negative", "between", "far", "special"])
+@pytest.mark.parametrize("vocab, padded", [(2049, 0), (4100, 3), (30000, 0)])
+def test_many_long_rows(dev, kind, vocab, padded):
+    """More long rows than are drawn by several workgroups each; rows whose border lies between their key bins, rows without
+    key bins, rows without anything to cut."""
+    g = torch.Generator().manual_seed(10)
+    _check(_logits(40, vocab, g, torch.bfloat16, kind), torch.rand(40, generator=g), _mixed(40, g), dev, padded=padded)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_special_values(dev, dtype):
     g = torch.Generator().manual_seed(2)
