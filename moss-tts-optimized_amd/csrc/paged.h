@@ -8,7 +8,7 @@
 // outside the cache.
 #pragma once
 
-#include "common.h"
+#include "wave_scan.h"
 #include "paged_index.h"
 
 namespace moss {

@@ -25,7 +25,7 @@
 // no table 93, and one workgroup a row 309.  One row: 28 us on the average of its settings, 182 by one workgroup.  A row of up
 // to 2048 entries is one wave's: it holds them and their weights in registers, and needs no barrier (512 rows of 1024: 13.7 us,
 // 46 before).
-#include "common.h"
+#include "wave_scan.h"
 
 namespace moss {
 namespace {
