@@ -4,7 +4,8 @@
 // h / (QH / KH)); a sequence without rows gives zeros.  One pass with the running maximum m and sum l of each head:
 // scores in the base-2 domain (scale log2(e) in one multiplication), O = sum 2^(s - m) v, rescaled when m grows.
 //
-// What bounds it: the cache's bytes.  Work is laid out on the device from the lengths, so that it is even whatever
+// What bounds it: the cache's bytes (64 sequences of 4 to 8 thousand rows, 32 / 8 heads of 128: 261 us, 6.2 TB/s; 16 of up to
+// 8000, 58 MB that the last-level cache holds: 16.7 us; one of 509: two launches and the chain of a share, 8.2 us).  Work is laid out on the device from the lengths, so that it is even whatever
 // they are and a captured graph follows them: rows are counted in units of kUnit, every KV head's units of all
 // sequences are shared out over about kTarget workgroups, and a workgroup takes an even share of one sequence.  A
 // sequence of one share writes its output; the others write (m, l, O) per share and a second launch joins them, which

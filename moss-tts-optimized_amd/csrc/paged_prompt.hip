@@ -20,7 +20,7 @@
 // other is consumed: one barrier per block, no registers.  V is read transposed (ds_read_b64_tr_b16: a lane gets one
 // dim of 4 rows).  16-byte chunk c of row r lies at c ^ f(r), which spreads the rows of one read over the banks.
 // What bounds it: the matrix and vector pipes in turn at the clock that power holds (8000 tokens of 32 / 8 heads of 128:
-// 528 us, 993 TFLOP/s, where a matrix product of 8192^3 reaches 1180); with K and V through registers, V transposed on the
+// 530 to 550 us, 950 to 990 TFLOP/s, where a matrix product of 8192^3 reaches 1180); with K and V through registers, V transposed on the
 // way, 667 us.
 #include "paged.h"
 

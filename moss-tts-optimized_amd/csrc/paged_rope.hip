@@ -7,7 +7,8 @@
 // of the sequence's n.  The single-request form (norm_rope.hip) rounds after every step, as the modules it stands in
 // for do; here the steps are kept in fp32, which halves the error of q and k.
 //
-// What bounds it: memory.  A head is D / 16 lanes, each with 8 values of either half, so every load and store is 16
+// What bounds it: memory (2549 tokens of 32 / 8 heads of 128: 13.8 us, 4.6 TB/s, where a large copy reaches 4.9; one token:
+// the launch, 2.8 us).  A head is D / 16 lanes, each with 8 values of either half, so every load and store is 16
 // bytes; one workgroup takes 256 / (D / 16) heads of one token, and a wave finds the token's sequence with one ballot
 // per 64 sequences.
 #include "paged.h"
