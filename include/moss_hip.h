@@ -418,7 +418,8 @@ int moss_advance_step(const void *next_ids, void *ids, void *position, void *aud
  * counts as -inf; a row with nothing above -inf gives -1.  temperature, top_p, min_p (fp32 [rows]) and top_k
  * (int32 [rows]) are device buffers, or NULL for the value behind each, one for all rows.  out int64 [rows].
  * Sums are integers (w in units of 2^-44): results do not depend on any order.  The workspace
- * (moss_sample_rows_workspace_bytes, 0 for vocab <= 2048; 16-byte aligned) must not be shared by calls that overlap.
+ * (moss_sample_rows_workspace_bytes, 0 for vocab <= 2048; 16-byte aligned; one serves any call of up to its rows
+ * and vocab) must not be shared by calls that overlap.
  * A batch's counterpart of moss_sample_topk: any vocabulary, per-row settings, the caller's random numbers. */
 long long moss_sample_rows_workspace_bytes(int rows, int vocab);
 int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, int vocab, const void *uniform,
