@@ -30,7 +30,7 @@
 namespace moss {
 namespace {
 
-constexpr double kOne = 17592186044416.0;  // 2^44: 2^19 entries sum below 2^63
+constexpr double kOne = 17592186044416.0;  // 2^44: 2^19 entries sum to at most 2^63
 constexpr int kSpan = 46;                  // octaves: smaller weights are 0
 constexpr int kBins = 32 * kSpan;          // 32 an octave
 constexpr int kSegment = 512;              // entries
@@ -272,10 +272,11 @@ struct Goal {
 __device__ __forceinline__ unsigned long long share_limit(const Row& r, unsigned long long total) {
     return (unsigned long long)((double)fmaxf(r.top_p, 0.f) * (double)total);
 }
-// The number that the sums through the kept entries are held against.
+// The number that the sums through the kept entries are held against.  u outside [0, 1) draws the first or the last kept
+// entry; totals reach 2^63 (2^19 entries of full weight), and 2^64 - 2^11 is the last double that an integer holds.
 __device__ __forceinline__ unsigned long long target_of(float u, unsigned long long total) {
-    const double goal = (double)u * (double)total;  // u outside [0, 1) draws the first or the last kept entry
-    return goal > 0.0 ? min((unsigned long long)fmin(goal, 9.2e18), total - 1) : 0;
+    const double goal = (double)u * (double)total;
+    return goal > 0.0 ? min((unsigned long long)fmin(goal, 18446744073709549568.0), total - 1) : 0;
 }
 
 __device__ __forceinline__ unsigned long long wave_largest(unsigned long long v) {

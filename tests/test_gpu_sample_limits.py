@@ -1,0 +1,37 @@
+"""GPU: ``sampling.sample`` at the ends of its ranges: rows whose kept weight comes near 2^63."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+VOCAB = 1 << 19
+# above 0.9975 the draw of 2^19 entries of full weight passes 9.2 10^18 units of 2^-44
+UNIFORM = [0.0, 0.25, 0.9974, 0.998, 0.9995, 0.9999, 1.0 - 2.0 ** -24, 1.0, 1e30, math.inf]
+
+
+@pytest.mark.parametrize("rows", [3, 20])  # few rows; rows that one workgroup each draws (bf16)
+@pytest.mark.parametrize("kind", ["equal", "hot"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weights_that_sum_to_two_to_the_63(dev, dtype, kind, rows):
+    """Every entry weighs 1, so the draw is floor(u entries), and the last entry from u = 1 on: equal logits, and logits
+    whose distance a temperature of 1e30 takes away.  All numbers are exact: 2^44 an entry, u of 24 bits."""
+    from moss_tts._runtime import sampling
+
+    g = torch.Generator().manual_seed(1)
+    x = torch.full((rows, VOCAB), 1.5) if kind == "equal" else torch.randn((rows, VOCAB), generator=g)
+    x = x.to(dtype).to(dev)
+    temperature = 1.0 if kind == "equal" else 1e30
+    for first in range(0, len(UNIFORM), rows):
+        u = np.float32((UNIFORM[first:] + UNIFORM * 3)[:rows])
+        print(f"sample {kind} {dtype} rows={rows} from u={u[0]}", flush=True)
+        got = sampling.sample(x, torch.from_numpy(u).to(dev), temperature=temperature).tolist()
+        assert got == [int(min(float(v) * VOCAB, VOCAB - 1)) for v in u]
+        # half of the entries by top-p: the ones whose predecessors weigh at most half of all
+        kept = VOCAB // 2 + 1
+        if kind == "equal":
+            got = sampling.sample(x, torch.from_numpy(u).to(dev), top_p=0.5).tolist()
+            assert got == [int(min(float(v) * kept, kept - 1)) for v in u]
