@@ -419,7 +419,7 @@ int moss_advance_step(const void *next_ids, void *ids, void *position, void *aud
  * (int32 [rows]) are device buffers, or NULL for the value behind each, one for all rows.  out int64 [rows].
  * Sums are integers (w in units of 2^-44): results do not depend on any order.  The workspace
  * (moss_sample_rows_workspace_bytes, 0 for vocab <= 2048; 16-byte aligned; one serves any call of up to its rows
- * and vocab) must not be shared by calls that overlap.
+ * and vocab) must not be shared by calls that overlap; neither it nor out may overlap the inputs.
  * A batch's counterpart of moss_sample_topk: any vocabulary, per-row settings, the caller's random numbers. */
 long long moss_sample_rows_workspace_bytes(int rows, int vocab);
 int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, int vocab, const void *uniform,

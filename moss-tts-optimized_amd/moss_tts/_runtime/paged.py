@@ -26,7 +26,7 @@ import math
 import torch
 
 from . import native
-from .w4g32 import _aligned, _cuda_contig, _require
+from .w4g32 import _aligned, _apart, _cuda_contig, _require
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _PAGE_ROWS = tuple(1 << s for s in range(4, 13))
@@ -172,14 +172,6 @@ def _scale(scale, d: int) -> float:
     scale = float(scale)
     _require(scale == scale and abs(scale) != float("inf"), "scale must be finite")
     return scale
-
-
-def _apart(name: str, t: torch.Tensor, *spans) -> None:
-    """Raise when the contiguous tensor ``t`` shares memory with one of the (first, end) spans."""
-    at = t.data_ptr()
-    end = at + t.numel() * t.element_size()
-    for first, last in spans:
-        _require(end <= first or last <= at, f"{name} must not overlap the other tensors")
 
 
 def _workspace(ws, nbytes: int, like: torch.Tensor, out: torch.Tensor, spans):

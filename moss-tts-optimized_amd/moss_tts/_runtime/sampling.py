@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import native
-from .w4g32 import _cuda_contig, _require
+from .w4g32 import _apart, _cuda_contig, _require
 
 MAX_TOP_K = 64
 MAX_VOCAB = 2048
@@ -132,7 +132,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     with nothing above ``-inf`` gives -1.  Each setting is a number, or a device tensor with one value a row
     (fp32; ``top_k`` int32) that is read when the kernel runs, so a captured graph serves rows with settings of
     their own.  Where :func:`sample_topk` draws its own numbers over at most 2048 entries, this takes the
-    caller's, over up to 2^19.  ``ws``: a :func:`sample_workspace`, for callers that keep one."""
+    caller's, over up to 2^19.  ``ws``: a :func:`sample_workspace`, for callers that keep one; neither it nor ``out``
+    may share memory with another argument."""
     _require(isinstance(logits, torch.Tensor) and logits.dtype in _SAMPLE_TYPES, "logits must be a bf16, fp16 or fp32 tensor")
     _require(logits.is_cuda, "logits must be a CUDA (HIP) tensor")
     _require(logits.dim() == 2 and logits.shape[0] > 0 and logits.shape[1] > 0, "logits must be [rows, entries]")
@@ -151,21 +152,23 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     m_ptr, m = _setting("min_p", min_p, rows, torch.float32, dev)
     _require(int(k) == k and 0 <= k < 1 << 31, "top_k must be a non-negative integer")
     _require(0 <= p and 0 <= m <= 1, "top_p must not be negative, min_p must lie in [0, 1]")
+    if out is not None or ws is not None:  # memory of the caller's, which must be nobody else's: (first, end) of the rest
+        at = logits.data_ptr()
+        spans = [(first, first + 4 * rows) for first in (uniform.data_ptr(), t_ptr, k_ptr, p_ptr, m_ptr) if first is not None]
+        spans.append((at, at + ((rows - 1) * stride + entries) * logits.element_size()))
     if out is None:
         out = torch.empty(rows, dtype=torch.int64, device=dev)
     else:
         _cuda_contig("out", out, torch.int64, dev)
         _require(out.numel() == rows, f"out must hold {rows} indices")
+        _apart("out", out, *spans)
     if ws is None:
         ws = sample_workspace(rows, vocab, dev)
     else:
         _cuda_contig("ws", ws, torch.float32, dev)
         _require(4 * ws.numel() >= native.lib().moss_sample_rows_workspace_bytes(rows, vocab) and ws.data_ptr() % 16 == 0,
                  "workspace too small or not 16-byte aligned")
-        end = ws.data_ptr() + 4 * ws.numel()
-        for first, size in ((logits.data_ptr(), ((rows - 1) * stride + entries) * logits.element_size()),
-                            (out.data_ptr(), 8 * rows), (uniform.data_ptr(), 4 * rows)):
-            _require(end <= first or first + size <= ws.data_ptr(), "ws must not overlap the other tensors")
+        _apart("ws", ws, (out.data_ptr(), out.data_ptr() + 8 * rows), *spans)
     native.call_on(logits, "moss_sample_rows", logits.data_ptr(), _SAMPLE_TYPES[logits.dtype], rows, stride, vocab,
                    uniform.data_ptr(), t_ptr, float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m), out.data_ptr(),
                    None if ws is None else ws.data_ptr(), 0 if ws is None else 4 * ws.numel())

@@ -38,6 +38,14 @@ def _aligned(t: torch.Tensor, a: int) -> bool:
     return t.data_ptr() % a == 0
 
 
+def _apart(name: str, t: torch.Tensor, *spans) -> None:
+    """Raise when the contiguous tensor ``t`` shares memory with one of the (first, end) spans."""
+    at = t.data_ptr()
+    end = at + t.numel() * t.element_size()
+    for first, last in spans:
+        _require(end <= first or last <= at, f"{name} must not overlap the other tensors")
+
+
 #: Scales must lie below this bound: the decode GEMV's exact mode and the prefill GEMM form the
 #: bit-exact dequant from (128 + q) * s and (128 + z) * s in fp32, which stay finite only for
 #: s < 2^120.8 (``moss_w4g32_dequant_bf16`` is exact for every finite scale).  Real group scales

@@ -1,4 +1,4 @@
-"""GPU: ``sampling.sample`` at the ends of its ranges: rows whose kept weight comes near 2^63."""
+"""GPU: ``sampling.sample`` at the ends of its ranges: rows whose kept weight comes near 2^63, and buffers that share memory."""
 import math
 
 import numpy as np
@@ -35,3 +35,34 @@ def test_weights_that_sum_to_two_to_the_63(dev, dtype, kind, rows):
         if kind == "equal":
             got = sampling.sample(x, torch.from_numpy(u).to(dev), top_p=0.5).tolist()
             assert got == [int(min(float(v) * kept, kept - 1)) for v in u]
+
+
+def test_buffers_that_share_memory(dev):
+    """The draw of one row writes its index while others still read: an output or a workspace that lies over the logits, the
+    uniform numbers, a setting or each other is refused."""
+    from moss_tts._runtime import sampling
+
+    n, vocab = 4, 3000
+    need = sampling.sample_workspace(n, vocab, dev).numel()
+    memory = torch.zeros(need + 4096, device=dev)
+    x, u = torch.zeros((n, vocab), device=dev), torch.zeros(n, device=dev)
+    t, k = torch.ones(n, device=dev), torch.zeros(n, dtype=torch.int32, device=dev)
+    p, m = torch.ones(n, device=dev), torch.zeros(n, device=dev)
+    out = torch.zeros(n, dtype=torch.int64, device=dev)
+    plain = dict(temperature=t, top_k=k, top_p=p, min_p=m)
+    assert sampling.sample(x, u, **plain, out=out, ws=memory[:need]).tolist() == [0] * n
+    inside = memory[need - n:need]
+    for name in plain:
+        bad = dict(plain, **{name: inside.view(plain[name].dtype)})
+        with pytest.raises(ValueError, match="ws must not overlap"):
+            sampling.sample(x, u, **bad, out=out, ws=memory[:need])
+        over = inside if name == "temperature" else memory[:n]
+        with pytest.raises(ValueError, match="out must not overlap"):
+            sampling.sample(x, u, **dict(plain, **{name: over.view(plain[name].dtype)}),
+                            out=(memory[need - 2 * n:need] if name == "temperature" else memory[:2 * n]).view(torch.int64))
+    with pytest.raises(ValueError, match="out must not overlap"):
+        sampling.sample(x, inside, **plain, out=memory[need - 2 * n:need].view(torch.int64))
+    with pytest.raises(ValueError, match="out must not overlap"):
+        sampling.sample(x, u, **plain, out=x.view(torch.int64)[0, :n])
+    with pytest.raises(ValueError, match="ws must not overlap"):
+        sampling.sample(x, u, **plain, out=memory[need - 2 * n:need].view(torch.int64), ws=memory[:need])
