@@ -4,7 +4,7 @@
 //   y = x rsqrt(mean(x^2) + eps) w;   out_l = y_l cos_l - y_{l + D/2} sin_l,
 //   out_{l + D/2} = y_{l + D/2} cos_{l + D/2} + y_l sin_{l + D/2}   (l < D / 2)
 // with row p of the cos / sin tables (bf16 / fp16 / fp32 as given) for the token's position p = length - n + i, token i
-// of the sequence's n.  The single-request form (norm_rope.hip) rounds after every step, as the modules it stands in
+// of the sequence's n, the length cut to what the page table's row holds as the attentions cut it.  The single-request form (norm_rope.hip) rounds after every step, as the modules it stands in
 // for do; here the steps are kept in fp32, which halves the error of q and k.
 //
 // What bounds it: memory (2549 tokens of 32 / 8 heads of 128: 13.8 us, 4.6 TB/s, where a large copy reaches 4.9; one token:
@@ -62,9 +62,9 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, PagedCache 
         if (b < 0) return;
         const int end = min(bt.starts[b + 1], a.T);  // as the attention reads it
         if (t >= end) return;  // padding behind the last sequence
-        position = (int)min(max((long long)bt.lengths[b] - end + t, -1ll), 1ll << 30);
+        position = paged_length(bt, b, c.shift) - end + t;
     } else {
-        position = min(max(bt.lengths[b], 0), 1 << 30) - 1;
+        position = paged_length(bt, b, c.shift) - 1;
     }
     const int h = blockIdx.y * HPB + threadIdx.x / LPH, j = threadIdx.x % LPH;
     if (h >= a.qh + 2 * c.kh) return;  // whole groups of lanes

@@ -14,10 +14,10 @@ sequence ``b`` and stand at its last positions.  Packed rows from ``starts[B]`` 
 
 Table, lengths and starts are device values, read when the kernels run and not checked by the host: a captured
 graph follows them as sequences grow.  Whatever they hold, no access leaves the cache or the packed rows; what they have
-to hold for results is the caller's to see to: lengths that the table's row can hold (the attention takes as many
-rows as that), starts that rise, and no two new tokens on one row of a page (sequences may share the pages that they
-only read).  A row that takes part with values that are not finite makes what it touches not finite; rows that
-take no part may hold anything.
+to hold for results is the caller's to see to: lengths that the table's row can hold (all three operators take a
+longer one as the rows that it holds, so new tokens go to the last of them), starts that rise, and no two new tokens on
+one row of a page (sequences may share the pages that they only read).  A row that takes part with values that are not
+finite makes what it touches not finite; rows that take no part may hold anything.
 """
 from __future__ import annotations
 

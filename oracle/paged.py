@@ -77,7 +77,7 @@ def qk_rope(qkv, q_weight, k_weight, cos, sin, keys, values, table, lengths, sta
     for i in range(len(table)):
         count = starts[i + 1] - starts[i]
         for t in range(count):
-            at, position = starts[i] + t, int(lengths[i]) - count + t
+            at, position = starts[i] + t, min(max(int(lengths[i]), 0), table.shape[1] * p) - count + t
             for h in range(qh):
                 q[at, h] = rope(x[at, h], position, q_weight, cos, sin, eps)
             if position < 0 or position // p >= table.shape[1] or not 0 <= table[i, position // p] < n:

@@ -1,0 +1,45 @@
+"""GPU: paged calls at the ends of what their arguments can say."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as o
+from paged_helpers import cache, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_rope_lengths_past_the_table(dev, packed):
+    """A length that the table's row cannot hold counts as the rows that it can, in qk_rope as in the attentions: the new
+    tokens are the last of those rows, and attend themselves."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(31)
+    qh, kh, d, page = 8, 2, 64, 16
+    keys, vals, table, lens = cache(dev, g, [32, 32, 32, 32, 20], kh=kh, d=d, page=page, dtype=torch.bfloat16, width=2)
+    lens.copy_(torch.tensor([40, 33, 2 ** 31 - 1, -5, 20], dtype=torch.int32))
+    new = [8, 1, 3, 2, 4] if packed else [1] * 5
+    at = np.concatenate(([0], np.cumsum(new)))
+    starts = torch.from_numpy(at.astype(np.int32)).to(dev)
+    qkv = torch.randn((sum(new), (qh + 2 * kh) * d), generator=g).bfloat16().to(dev)
+    cos, sin = (torch.randn((64, d), generator=g).to(dev) for _ in range(2))
+    rest = table.cpu().numpy(), lens.cpu().numpy(), at
+    want = o.qk_rope(values(qkv), None, None, values(cos), values(sin), values(keys), values(vals), *rest, 1e-6,
+                     np.zeros((sum(new), qh, d)))
+    q = paged.qk_rope(qkv, None, None, cos, sin, keys, vals, table, lens, 1e-6, starts=starts if packed else None)
+    torch.cuda.synchronize()
+    # two products and a sum in fp32, each off by 2^-24 of terms of at most 20; one rounding
+    for got, ref in ((values(q), want[0]), (values(keys), want[1])):
+        assert np.array_equal(np.isnan(got), np.isnan(ref))
+        assert (np.abs(got - ref)[~np.isnan(ref)] <= (2.0 ** -8 * np.abs(ref) + 2.0 ** -18)[~np.isnan(ref)]).all()
+    assert np.array_equal(values(vals), want[2], equal_nan=True)
+    if packed:
+        out = paged.prompt_attention(q, keys, vals, table, lens, starts)
+        ref = o.prompt_attention(values(q), values(keys), values(vals), *rest, np.zeros((sum(new), qh * d)))
+    else:
+        out = paged.decode_attention(q, keys, vals, table, lens)
+        ref = o.decode_attention(values(q), values(keys), values(vals), *rest[:2])
+    # the terms of a score sum to at most 2^9 here, so fp32 moves a weight by less than (64 + 8) 2^-24 2^9 < 2^-8, and its
+    # rounding by 2^-8; an error r in every weight moves the output by at most 2 r times a value, which is at most 5
+    assert (np.abs(values(out) - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -6 * 5).all()
