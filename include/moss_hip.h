@@ -440,12 +440,14 @@ int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, 
  *   starts    int32 [B + 1], rising: the packed tokens starts[b] .. starts[b + 1] - 1 are sequence b's newest n, at
  *             positions lengths[b] - n ..; packed rows from starts[B] on are padding and left alone
  * Table, lengths and starts are read on the device when the kernels run, so a captured graph follows them; their
- * contents cannot lead an access outside the cache or the packed rows.  */
+ * contents cannot lead an access outside the cache or the packed rows.  A call whose grid would pass 2^32 - 1 threads
+ * is refused: qk_rope from 2^24 tokens on, the attentions from about 2^24 (sequences + tiles of tokens) x KV heads on. */
 
 /* q/k head RMSNorm (weights [d], or both NULL: no norm) + rotary embedding + page write of T packed tokens:
- * qkv [T, (qh + 2 kh) d] (q | k | v), rows qkv_stride elements apart; cos / sin [table_rows, d] by position, of the
- * given dtype or fp32 (table_f32); q_out [T, qh, d].  starts NULL: one token a sequence (T == B).  fp32 from the
- * inputs to one rounding.  A token whose position is negative, or has no page, is written to no cache row.
+ * qkv [T, (qh + 2 kh) d] (q | k | v), T < 2^24, rows qkv_stride elements apart; cos / sin [table_rows, d] by
+ * position, of the given dtype or fp32 (table_f32); q_out [T, qh, d].  starts NULL: one token a sequence (T == B).
+ * fp32 from the inputs to one rounding.  A token whose position is negative, or has no page, is written to no cache
+ * row.
  * Counterpart of moss_qk_norm_rope_kv. */
 int moss_paged_qk_rope(const void *qkv, long long qkv_stride, const void *q_weight, const void *k_weight,
                        const void *cos, const void *sin, int table_f32, int table_rows, void *q_out, void *k, void *v,

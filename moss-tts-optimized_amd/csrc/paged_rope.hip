@@ -150,7 +150,8 @@ MOSS_API int moss_paged_qk_rope(const void* qkv, long long qkv_stride, const voi
     const PagedCache c = paged_cache(k, v, k_stride, v_stride, pages, kh, page_rows);
     const PagedBatch bt{(const int*)table, (const int*)lengths, (const int*)starts, B, W, table_stride};
     MOSS_CHECK_ARG(qkv && cos && sin && q_out && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, qh, d));
-    MOSS_CHECK_ARG(T > 0 && (starts || T == B) && table_rows > 0 && eps >= 0.f && (dtype == 0 || dtype == 1));
+    // 256 threads a token: from 2^24 tokens on the grid would have more than 2^32 - 1
+    MOSS_CHECK_ARG(T > 0 && T < (1 << 24) && (starts || T == B) && table_rows > 0 && eps >= 0.f && (dtype == 0 || dtype == 1));
     MOSS_CHECK_ARG((q_weight == nullptr) == (k_weight == nullptr) && qkv_stride % 8 == 0 &&
                    qkv_stride >= (long long)(qh + 2 * kh) * d);
     MOSS_CHECK_ARG(MOSS_ALIGNED(qkv, 16) && MOSS_ALIGNED(q_weight, 16) && MOSS_ALIGNED(k_weight, 16) && MOSS_ALIGNED(cos, 16) &&

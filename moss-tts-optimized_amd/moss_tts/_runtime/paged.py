@@ -227,7 +227,7 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     _require(starts is not None or tokens == b, "without starts, one token a sequence required")
     norms = _norms_and_tables(q_weight, k_weight, cos, sin, d, dtype, index)
     _require(eps >= 0, "eps must not be negative")
-    _require(tokens < 1 << 31, "too many tokens")
+    _require(tokens < 1 << 24, "fewer than 2^24 packed tokens required")
     span = (at, at + 2 * ((tokens - 1) * stride + width))
     _require((c.kend <= span[0] or span[1] <= c.k) and (c.vend <= span[0] or span[1] <= c.v),
              "qkv must not overlap the cache")

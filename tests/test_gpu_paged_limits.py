@@ -43,3 +43,16 @@ def test_rope_lengths_past_the_table(dev, packed):
     # the terms of a score sum to at most 2^9 here, so fp32 moves a weight by less than (64 + 8) 2^-24 2^9 < 2^-8, and its
     # rounding by 2^-8; an error r in every weight moves the output by at most 2 r times a value, which is at most 5
     assert (np.abs(values(out) - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -6 * 5).all()
+
+
+def test_rope_refuses_more_tokens_than_a_grid_holds(dev):
+    """A launch of 256 threads a token ends at 2^32 threads."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(32)
+    keys, vals, table, lens = cache(dev, g, [20], kh=1, d=64, page=16, dtype=torch.bfloat16)
+    qkv = torch.empty((1 << 24, 3 * 64), dtype=torch.bfloat16, device=dev)
+    cos = torch.zeros((32, 64), device=dev)
+    starts = torch.tensor([0, 3], dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError, match="2\\^24"):
+        paged.qk_rope(qkv, None, None, cos, cos, keys, vals, table, lens, 1e-6, starts=starts)
