@@ -54,3 +54,37 @@ def attention_bound(q, keys, vals, ref, ref_abs, scale, dtype, rounded_p):
     # an output below the type's normal range is off by half its smallest step
     floor = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134
     return half * np.abs(ref) * (1 + 2 * r) + 2 * r * ref_abs + tiny + floor
+
+
+def attend_all(q, keys, vals, table, lengths, starts, before, scale):
+    """``oracle.paged.prompt_attention`` of whole tensors, in float64 on the device that holds them: for shapes with too
+    many tokens and heads to take one at a time."""
+    tokens, qh, d = q.shape
+    pages, kh, page, _ = keys.shape
+    group, width, dev = qh // kh, table.shape[1], q.device
+    out = before.double().reshape(tokens, qh, d).clone()
+    for b, (length, row) in enumerate(zip(lengths.tolist(), table.long())):
+        first, n = starts[b], starts[b + 1] - starts[b]
+        length = min(max(length, 0), width * page)
+        if not n:
+            continue
+        if not length:
+            out[first:first + n] = 0
+            continue
+        own = row[:-(-length // page)]
+        has_page = (own >= 0) & (own < pages)
+        there = has_page.repeat_interleave(page)[:length]
+        at = torch.where(has_page, own, torch.zeros_like(own))
+        position = length - n + torch.arange(n, device=dev)
+        seen = (there & (torch.arange(length, device=dev) <= position[:, None])).repeat_interleave(group, 0)
+        for h in range(kh):
+            k, v = (t[at, h].reshape(-1, d)[:length].double() for t in (keys, vals))
+            k, v = (torch.where(there[:, None], t, torch.zeros_like(t)) for t in (k, v))
+            x = q[first:first + n, h * group:(h + 1) * group].double().reshape(n * group, d)
+            s = torch.matmul(x, k.T.contiguous()).mul_(scale).masked_fill_(~seen, float("-inf"))
+            top = s.amax(1, keepdim=True)
+            e = s.sub_(torch.where(top == float("-inf"), torch.zeros_like(top), top)).exp_()
+            total = e.sum(1, keepdim=True)
+            y = torch.matmul(e, v) / torch.where(total == 0, torch.ones_like(total), total)
+            out[first:first + n, h * group:(h + 1) * group] = y.view(n, group, d)
+    return out.view(before.shape)
