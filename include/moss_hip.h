@@ -409,7 +409,7 @@ int moss_advance_step(const void *next_ids, void *ids, void *position, void *aud
                       void *history, void *status, int step, int width, long long audio_start_id,
                       long long gen_slot_id, long long delay_slot_id, void *stream);
 
-/* One index per row of logits (dtype 0 bf16, 1 fp16, 2 fp32; rows `stride` values apart, the first
+/* One index per row of up to 2^21 rows of logits (dtype 0 bf16, 1 fp16, 2 fp32; rows `stride` values apart, the first
  * `vocab` <= 2^19 used) from the row's uniform number u in [0, 1) (uniform fp32 [rows]).  With M the row's
  * largest logit, w_i = exp((x_i - M) / T) and entries ordered by falling x (ties: lower index first), kept are
  * the first top_k (<= 0 or >= vocab: all), of those the ones whose predecessors' sum of w is at most top_p times
@@ -417,7 +417,8 @@ int moss_advance_step(const void *next_ids, void *ids, void *position, void *aud
  * index order, with sum_{j <= i, kept} w_j > u sum_kept w_j.  T <= 0 gives the first of the largest logits; NaN
  * counts as -inf; a row with nothing above -inf gives -1.  temperature, top_p, min_p (fp32 [rows]) and top_k
  * (int32 [rows]) are device buffers, or NULL for the value behind each, one for all rows.  out int64 [rows].
- * Sums are integers (w in units of 2^-44): results do not depend on any order.  The workspace
+ * Sums are integers (w in units of 2^-44, so an entry below 2^-45 weighs nothing and is not drawn, by u = 0 neither):
+ * results do not depend on any order.  The workspace
  * (moss_sample_rows_workspace_bytes, 0 for vocab <= 2048; 16-byte aligned; one serves any call of up to its rows
  * and vocab) must not be shared by calls that overlap; neither it nor out may overlap the inputs.
  * A batch's counterpart of moss_sample_topk: any vocabulary, per-row settings, the caller's random numbers. */

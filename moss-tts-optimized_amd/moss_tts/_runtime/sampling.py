@@ -99,6 +99,7 @@ def sample_topk_pair(a: dict, b: dict, *, seed: torch.Tensor, position: torch.Te
 
 _SAMPLE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_SAMPLE_VOCAB = 1 << 19
+MAX_SAMPLE_ROWS = 1 << 21
 
 
 def _setting(name: str, value, rows: int, dtype: torch.dtype, device):
@@ -128,8 +129,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     Kept are the ``top_k`` largest (0: all; of equal logits the lower index first), of those the ones whose
     predecessors hold at most the share ``top_p`` of the kept probability (1: all), and those at least
     ``min_p`` times as probable as the largest.  The draw inverts the cumulative distribution of the kept entries
-    in index order.  ``temperature`` <= 0 takes the first of the largest logits.  NaN counts as ``-inf``; a row
-    with nothing above ``-inf`` gives -1.  Each setting is a number, or a device tensor with one value a row
+    in index order; entries less probable than 2^-45 of the largest weigh nothing.  ``temperature`` <= 0 takes the first
+    of the largest logits.  NaN counts as ``-inf``; a row with nothing above ``-inf`` gives -1.  Each setting is a number, or a device tensor with one value a row
     (fp32; ``top_k`` int32) that is read when the kernel runs, so a captured graph serves rows with settings of
     their own.  Where :func:`sample_topk` draws its own numbers over at most 2048 entries, this takes the
     caller's, over up to 2^19.  ``ws``: a :func:`sample_workspace`, for callers that keep one; neither it nor ``out``
@@ -138,6 +139,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     _require(logits.is_cuda, "logits must be a CUDA (HIP) tensor")
     _require(logits.dim() == 2 and logits.shape[0] > 0 and logits.shape[1] > 0, "logits must be [rows, entries]")
     rows, entries = logits.shape
+    _require(rows <= MAX_SAMPLE_ROWS, f"at most {MAX_SAMPLE_ROWS} rows")
     _require(entries == 1 or logits.stride(1) == 1, "a row's logits must be contiguous")
     stride = logits.stride(0) if rows > 1 else entries
     _require(stride >= entries, "rows must not overlap")

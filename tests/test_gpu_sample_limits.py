@@ -66,3 +66,23 @@ def test_buffers_that_share_memory(dev):
         sampling.sample(x, u, **plain, out=x.view(torch.int64)[0, :n])
     with pytest.raises(ValueError, match="ws must not overlap"):
         sampling.sample(x, u, **plain, out=memory[need - 2 * n:need].view(torch.int64), ws=memory[:need])
+
+
+def test_more_rows_than_a_call_takes(dev):
+    from moss_tts._runtime import sampling
+
+    rows = 1 << 21
+    x, u = torch.zeros((rows + 1, 2), dtype=torch.bfloat16, device=dev), torch.full((rows + 1,), 0.75, device=dev)
+    with pytest.raises(ValueError, match="at most 2097152 rows"):
+        sampling.sample(x, u)
+    assert (sampling.sample(x[:rows], u[:rows]) == 1).all()
+
+
+@pytest.mark.parametrize("vocab", [9, 3000])
+def test_entries_without_weight_are_not_drawn(dev, vocab):
+    """u = 0 draws the first entry that weighs anything: 2^-44 of the largest does, 2^-46 does not."""
+    from moss_tts._runtime import sampling
+
+    x = torch.full((2, vocab), -math.inf)
+    x[:, 3], x[:, 7] = torch.tensor([-44 * math.log(2.0), -46 * math.log(2.0)]), 0.0
+    assert sampling.sample(x.to(dev), torch.zeros(2, device=dev)).tolist() == [3, 7]
