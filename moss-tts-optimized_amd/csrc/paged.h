@@ -84,7 +84,6 @@ struct Place {
     int b;      // -1: the index lies behind the last item
     int index;  // the item's number within the sequence
     int count;  // the sequence's items
-    int first;  // number of the sequence's first item
 };
 
 // The sequences' items counted in order (count(b) of sequence b): whose the item `item` is.  Every wave finds it by
@@ -99,11 +98,11 @@ __device__ __forceinline__ Place find_item(int B, int item, int lane, Count coun
         if (past) {
             const int l = __builtin_ctzll(past);
             const int c = __builtin_amdgcn_readlane(n, l), t = before + __builtin_amdgcn_readlane(through, l);
-            return Place{b0 + l, item - (t - c), c, t - c};
+            return Place{b0 + l, item - (t - c), c};
         }
         before += __builtin_amdgcn_readlane(through, kWave - 1);
     }
-    return Place{-1, 0, 0, before};
+    return Place{-1, 0, 0};
 }
 
 // ---------------------------------------------------------------- host checks

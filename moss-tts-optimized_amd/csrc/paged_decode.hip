@@ -56,10 +56,10 @@ __device__ __forceinline__ Place find_share(const PagedBatch& bt, int shift, int
         const int share = share_of_units(wave_total((long long)units), shares), n = shares_of(units, share);
         const int through = wave_prefix(n);
         const unsigned long long past = __ballot(through > slot);
-        if (!past) return Place{-1, 0, 0, 0};
+        if (!past) return Place{-1, 0, 0};
         const int l = __builtin_ctzll(past), c = __builtin_amdgcn_readlane(n, l);
         const int first = __builtin_amdgcn_readlane(through, l) - c;
-        return Place{l, slot - first, c, first};
+        return Place{l, slot - first, c};
     }
     const int share = share_units(bt, shift, shares, lane);
     return find_item(bt.B, slot, lane, [&](int b) { return shares_of(units_of(paged_length(bt, b, shift)), share); });

@@ -30,12 +30,11 @@
 namespace moss {
 namespace {
 
-constexpr double kOne = 17592186044416.0;  // 2^44: 2^19 entries sum to at most 2^63
 constexpr int kSpan = 46;                  // octaves: smaller weights are 0
 constexpr int kBins = 32 * kSpan;          // 32 an octave
 constexpr int kSegment = 512;              // entries
 constexpr int kSmall = 2048;               // entries of a row that one wave takes
-constexpr int kMaxVocab = 1 << 19;
+constexpr int kMaxVocab = 1 << 19;         // entries of 2^44 at most: a sum is at most 2^63
 constexpr int kMaxChunks = 16;             // workgroups that read a row together
 
 struct SampleArgs {
