@@ -4,8 +4,9 @@
 // h / (QH / KH)); a sequence without rows gives zeros.  One pass with the running maximum m and sum l of each head:
 // scores in the base-2 domain (scale log2(e) in one multiplication), O = sum 2^(s - m) v, rescaled when m grows.
 //
-// What bounds it: the cache's bytes (64 sequences of 4 to 8 thousand rows, 32 / 8 heads of 128: 261 us, 6.2 TB/s; 16 of up to
-// 8000, 58 MB that the last-level cache holds: 16.7 us; one of 509: two launches and the chain of a share, 8.2 us).  Work is laid out on the device from the lengths, so that it is even whatever
+// What bounds it: the cache's bytes (64 sequences of 4 to 8 thousand rows, 32 / 8 heads of 128: 261 us, 6.2 TB/s; 256 of 300 to
+// 2000: 175 to 187 us, 5.2 TB/s; 16 of up to 8000, 58 MB: 16.7 us from the last-level cache, 19.5 from memory; one of 509: two
+// launches and the chain of a share, 8.2 us).  Work is laid out on the device from the lengths, so that it is even whatever
 // they are and a captured graph follows them: rows are counted in units of kUnit, every KV head's units of all
 // sequences are shared out over about kTarget workgroups, and a workgroup takes an even share of one sequence.  A
 // sequence of one share writes its output; the others write (m, l, O) per share and a second launch joins them, which
@@ -25,11 +26,15 @@
 namespace moss {
 namespace {
 
-// Workgroups that the work is shared out over.  512 / 1024 / 1536 / 2048: 300 / 298 / 296 / 299 us for 64 sequences of 4 to 8
-// thousand rows of 8 heads, 23.3 / 22.3 / 21.7 / 21.8 for 48 of up to 2000 rows of 12 heads of 64, no difference for fewer.
+// Workgroups that the work is shared out over.  512 / 1024 / 1536 / 2048: 273 / 265 / 261 / 263 us for 64 sequences of 4 to 8
+// thousand rows of 8 heads, 25.9 / 24.3 / 24.1 / 24.1 for 48 of up to 2000 rows of 12 heads of 64 (six caches in turn), 109 / 99 /
+// 97 / 98 for 128 of 300 to 2000 rows, no difference for 16 sequences.
 constexpr int kTarget = 1536;
-// A cache that the last-level cache (256 MB) cannot hold is read past it: 296 -> 272 us for those 64 sequences (1.6 GB),
-// but 17.0 -> 18.4 for 16 sequences whose 58 MB stay there from call to call.
+// Pages of more than the last-level cache (256 MB) are read past it.  The pages that the call can name decide, since the host
+// does not know the lengths: with a server's pool that is nearly every call, of few rows too, and right for it, as what one
+// layer's call reads is gone by the time of the next step's.  To / past the cache: 287 / 261 us for those 64 sequences (1.6 GB),
+// 103 / 96 for 128 and 192 / 183 for 256 of 300 to 2000 rows; 16 sequences with 58 MB, 36 layers' caches in turn, 19.8 / 19.3, one
+// of 509 rows 9.0 / 8.8; but one cache read again and again, which stays: 16.7 / 17.5, four such 17.0 / 18.6.
 constexpr long long kCached = 256ll << 20;
 
 struct DecodeArgs {

@@ -13,15 +13,18 @@
 //   S^T = K Q^T: 32 keys x 32 rows per matrix instruction, so a lane holds one row and 16 of its keys, and the row's
 //   maximum needs one exchange with the lane 32 away; the running maximum and sum are fp32, base 2.
 //   O^T += V^T P^T: P, rounded to 16 bits, is the B operand as S^T left it.
-// P's rounding is the one step with fewer bits before the output: the largest P of a block is exactly 1 or its
-// share of the running maximum, and the sum adds up the unrounded values.
+// P's rounding is the one step with fewer bits before the output, as in the single request's prompt attention; the sum adds
+// up the unrounded values.  (P = 2^(s scale - m) with m a rounded product: a row's largest P is 1 up to that rounding, which
+// l and O share.)  Split into two 16-bit values as the decode form has it, P adds nothing to the output's own rounding, but
+// costs half as many matrix instructions again where they are what bounds: 8000 tokens 555 -> 724 us, nine prompts 60 -> 67,
+// for an error against 64 bits of 1.65 instead of 1.88 and 1.64 instead of 1.78 10^-3 (heads of 128, bf16; fp16 an eighth).
 // Blocks of 64 keys go from the pages straight into LDS (buffer loads, 16 rows of K and of V a wave, which lie in one page;
 // rows that nobody sees or that have no page are read as zeros: past the buffer's end), into one of two stages while the
 // other is consumed: one barrier per block, no registers.  V is read transposed (ds_read_b64_tr_b16: a lane gets one
 // dim of 4 rows).  16-byte chunk c of row r lies at c ^ f(r), which spreads the rows of one read over the banks.
 // What bounds it: the matrix and vector pipes in turn at the clock that power holds (8000 tokens of 32 / 8 heads of 128:
-// 530 to 550 us, 950 to 990 TFLOP/s, where a matrix product of 8192^3 reaches 1180); with K and V through registers, V transposed on the
-// way, 667 us.
+// 520 to 550 us, 950 to 1010 TFLOP/s, where a large product of bf16 matrices reaches 1640); with K and V through registers, V
+// transposed on the way, 667 us.
 #include "paged.h"
 
 namespace moss {

@@ -22,9 +22,10 @@
 // drawn entry lies in, and one launch in place of the last three finds the border and reads that part alone.  w takes 14
 // operations in 64 bits, of 8 cycles each for a wave.  128 rows of 151,936 bf16 logits, each with its own settings: 53 us;
 // with the last three launches 61 (9 + 18 + 12 + 18 + 6), with linear bins besides 84, of those with a series of ten terms and
-// no table 93, and one workgroup a row 309.  One row: 28 us on the average of its settings, 182 by one workgroup.  A row of up
-// to 2048 entries is one wave's: it holds them and their weights in registers, and needs no barrier (512 rows of 1024: 13.7 us,
-// 46 before).
+// no table 93, and one workgroup a row 309.  One row: 29 us with top-p, 19 without, 182 by one workgroup.  Rows without such
+// bins (fp16, fp32, bf16 with a largest logit below 2^-9, as of log-probabilities) take 46, 48 and 31 us for one row with
+// top-p, 95, 114 and 96 for 128.  A row of up to 2048 entries is one wave's: it holds them and their weights in registers, and
+// needs no barrier (512 rows of 1024: 13.8 us, 46 before; fp32 14.6).
 #include "wave_scan.h"
 
 namespace moss {
@@ -1095,7 +1096,10 @@ long long most_bytes(int rows, int vocab) {
 }
 
 // More bf16 rows than this are drawn by a workgroup each, fewer by several.  Several / one: 28 / 31 us for one row of 151,936
-// with top-p (18 / 29 without), 33.5 / 33.8 for 16, 62 / 53 for 128; 28 / 25 for 40 of 5,000, 62 / 58 for 400 of 30,000.
+// with top-p (18 / 29 without), 33.5 / 33.8 for 16, 34.9 / 35.0 for 17, 43.7 / 40.9 for 40, 62 / 53 for 128; 28 / 25 for 40 of 5,000,
+// 62 / 58 for 400 of 30,000.  Rows without key bins, which the host cannot tell, lose by it while they are long and few: log-
+// probabilities 49.7 / 67.9 for 17, 59.6 / 78.9 for 40 and 84.5 / 96.1 for 128 of 151,936, but 36.4 / 31.5 for 40 of 5,000 and
+// 84.7 / 73.3 for 400 of 30,000.
 constexpr int kFewRows = 16;
 
 template <int TYPE>
