@@ -442,7 +442,9 @@ int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, 
  *             positions lengths[b] - n ..; packed rows from starts[B] on are padding and left alone
  * Table, lengths and starts are read on the device when the kernels run, so a captured graph follows them; their
  * contents cannot lead an access outside the cache or the packed rows.  A call whose grid would pass 2^32 - 1 threads
- * is refused: qk_rope from 2^24 tokens on, the attentions from about 2^24 (sequences + tiles of tokens) x KV heads on. */
+ * is refused: qk_rope from 2^24 tokens on, the attentions from about 2^24 (sequences + tiles of tokens) x KV heads on.
+ * Outputs and workspaces must not overlap the inputs or each other; the cache's keys and values must not share memory
+ * where it is written. */
 
 /* q/k head RMSNorm (weights [d], or both NULL: no norm) + rotary embedding + page write of T packed tokens:
  * qkv [T, (qh + 2 kh) d] (q | k | v), T < 2^24, rows qkv_stride elements apart; cos / sin [table_rows, d] by

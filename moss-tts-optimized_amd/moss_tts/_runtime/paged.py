@@ -95,7 +95,7 @@ def _batch_refuse(table, lengths, starts, rows, index):
 
 
 def _batch(table, lengths, starts, rows, index):
-    """(B, W, table stride) of a checked batch."""
+    """(B, W, table stride, pointers of table, lengths and starts) of a checked batch."""
     try:
         b, w = table.shape
         ts, t1 = table.stride()
@@ -111,7 +111,7 @@ def _batch(table, lengths, starts, rows, index):
     if not ok:
         _batch_refuse(table, lengths, starts, rows, index)
         raise ValueError("table, lengths and starts do not describe a batch")
-    return b, w, ts
+    return b, w, ts, table.data_ptr(), lengths.data_ptr(), None if starts is None else starts.data_ptr()
 
 
 def _query(q):
@@ -174,6 +174,12 @@ def _scale(scale, d: int) -> float:
     return scale
 
 
+def _batch_spans(b, w, ts, table, lengths, starts):
+    """What a batch's tensors cover, as (first, end): results written over them would change the work under the kernels."""
+    spans = (table, table + 4 * ((b - 1) * ts + w)), (lengths, lengths + 4 * b)
+    return spans if starts is None else spans + ((starts, starts + 4 * b + 4),)
+
+
 def _workspace(ws, nbytes: int, like: torch.Tensor, out: torch.Tensor, spans):
     """A new workspace of ``nbytes`` (None for none), or the caller's, checked."""
     if ws is None:
@@ -185,11 +191,12 @@ def _workspace(ws, nbytes: int, like: torch.Tensor, out: torch.Tensor, spans):
     return ws
 
 
-def _output(out, shape, like: torch.Tensor, *spans) -> torch.Tensor:
+def _output(out, shape, like: torch.Tensor, index: int, spans) -> torch.Tensor:
     """A new output (which shares no memory with anything), or the caller's, checked."""
     if out is None:
         return like.new_empty(shape)
-    _cuda_contig("out", out, like.dtype, like.device)
+    if not (isinstance(out, torch.Tensor) and out.dtype is like.dtype and out.get_device() == index and out.is_contiguous()):
+        _cuda_contig("out", out, like.dtype, like.device)
     if out.shape != shape:
         _require(out.numel() == math.prod(shape), f"out must hold {' x '.join(map(str, shape))} values")
         out = out.view(shape)
@@ -220,7 +227,7 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     _require(stride >= width and not (stride & 7 or at & 15), "qkv: rows must be 16-byte aligned and must not overlap")
     c = _Cache(keys, values, dtype, index)
     kh, d = c.kh, c.d
-    b, w, table_stride = _batch(table, lengths, starts, c.rows, index)
+    b, w, table_stride, table_at, lengths_at, starts_at = batch = _batch(table, lengths, starts, c.rows, index)
     qh = width // d - 2 * kh
     _require(width % d == 0 and 0 < qh <= 1024 and qh % kh == 0,
              "qkv must hold a multiple of the KV heads as query heads, then the keys and the values")
@@ -234,10 +241,16 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     if c.k < c.vend and c.v < c.kend:  # interleaved: the keys of a page lie between the values of two
         page, step = 2 * kh * c.rows * d, 2 * c.ks
         _require(c.ks == c.vs and page <= (c.v - c.k) % step <= step - page, "keys and values must not share memory")
-    q = _output(out, (tokens, qh, d), qkv, span, (c.k, c.kend), (c.v, c.vend))
+    spans = ()
+    if out is not None:
+        qw, kw, cos_at, sin_at, f32, rows = norms
+        size = rows * d * (4 if f32 else 2)
+        spans = (span, (c.k, c.kend), (c.v, c.vend), (cos_at, cos_at + size), (sin_at, sin_at + size), *_batch_spans(*batch))
+        if qw is not None:
+            spans += (qw, qw + 2 * d), (kw, kw + 2 * d)
+    q = _output(out, (tokens, qh, d), qkv, index, spans)
     native.call_on(qkv, "moss_paged_qk_rope", at, stride, *norms, q.data_ptr(), c.k, c.v, c.ks, c.vs, c.pages, c.rows,
-                   table.data_ptr(), table_stride, lengths.data_ptr(), None if starts is None else starts.data_ptr(), b,
-                   w, tokens, qh, kh, d, eps, _TYPES[dtype])
+                   table_at, table_stride, lengths_at, starts_at, b, w, tokens, qh, kh, d, eps, _TYPES[dtype])
     return q
 
 
@@ -258,15 +271,17 @@ def decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     n, qh, hd, stride, index = _query(q)
     c = _Cache(keys, values, q.dtype, index)
     kh, d = c.kh, c.d
-    b, w, table_stride = _batch(table, lengths, None, c.rows, index)
+    b, w, table_stride, table_at, lengths_at, _ = batch = _batch(table, lengths, None, c.rows, index)
     _require(n == b and hd == d and qh % kh == 0 and qh <= 1024, "q must be [B, a multiple of the KV heads, head dim]")
     at = q.data_ptr()
-    spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
-    out = _output(out, (b, qh * d), q, *spans)
+    spans = ()
+    if out is not None or ws is not None:
+        spans = (at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend), *_batch_spans(*batch)
+    out = _output(out, (b, qh * d), q, index, spans)
     nbytes = native.lib().moss_paged_decode_workspace_bytes(b, w, c.rows, qh, kh, d)
     ws = _workspace(ws, nbytes, q, out, spans)
-    native.call_on(q, "moss_paged_decode_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),
-                   table_stride, lengths.data_ptr(), b, w, qh, kh, d, _scale(scale, d), out.data_ptr(), ws.data_ptr(),
+    native.call_on(q, "moss_paged_decode_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table_at,
+                   table_stride, lengths_at, b, w, qh, kh, d, _scale(scale, d), out.data_ptr(), ws.data_ptr(),
                    nbytes, _TYPES[q.dtype])
     return out
 
@@ -290,15 +305,17 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     c = _Cache(keys, values, q.dtype, index)
     kh, d = c.kh, c.d
     _require(starts is not None, "starts required")
-    b, w, table_stride = _batch(table, lengths, starts, c.rows, index)
+    b, w, table_stride, table_at, lengths_at, starts_at = batch = _batch(table, lengths, starts, c.rows, index)
     _require(hd == d and qh % kh == 0 and qh <= 1024, "q must be [tokens, a multiple of the KV heads, head dim]")
     _require(n <= 1 << 20, "at most 2^20 packed tokens")
     at = q.data_ptr()
-    spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend))
-    out = _output(out, (n, qh * d), q, *spans)
+    spans = ()
+    if out is not None or ws is not None:
+        spans = (at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend), *_batch_spans(*batch)
+    out = _output(out, (n, qh * d), q, index, spans)
     nbytes = native.lib().moss_paged_prompt_workspace_bytes(b, w, c.rows, n, qh, kh, d)
     ws = _workspace(ws, nbytes, q, out, spans)
-    native.call_on(q, "moss_paged_prompt_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table.data_ptr(),
-                   table_stride, lengths.data_ptr(), starts.data_ptr(), b, w, n, qh, kh, d, _scale(scale, d),
+    native.call_on(q, "moss_paged_prompt_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table_at,
+                   table_stride, lengths_at, starts_at, b, w, n, qh, kh, d, _scale(scale, d),
                    out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _TYPES[q.dtype])
     return out

@@ -43,7 +43,8 @@ def _apart(name: str, t: torch.Tensor, *spans) -> None:
     at = t.data_ptr()
     end = at + t.numel() * t.element_size()
     for first, last in spans:
-        _require(end <= first or last <= at, f"{name} must not overlap the other tensors")
+        if at < last and first < end:
+            raise ValueError(f"{name} must not overlap the other tensors")
 
 
 #: Scales must lie below this bound: the decode GEMV's exact mode and the prefill GEMM form the

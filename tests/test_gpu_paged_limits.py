@@ -56,3 +56,54 @@ def test_rope_refuses_more_tokens_than_a_grid_holds(dev):
     starts = torch.tensor([0, 3], dtype=torch.int32, device=dev)
     with pytest.raises(ValueError, match="2\\^24"):
         paged.qk_rope(qkv, None, None, cos, cos, keys, vals, table, lens, 1e-6, starts=starts)
+
+
+def test_outputs_over_what_the_kernels_read(dev):
+    """An output or a workspace over the table, the lengths, the starts, the head-norm weights or the cos / sin tables is
+    refused: the kernels would find their work changed while they run."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(33)
+    qh, kh, d, n = 4, 2, 64, 2
+    keys, vals, table, lens = cache(dev, g, [20, 700], kh=kh, d=d, page=16, dtype=torch.bfloat16)
+    q = torch.zeros((n, qh, d), dtype=torch.bfloat16, device=dev)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev)
+    memory = torch.zeros(1 << 20, device=dev)
+    width = table.shape[1]
+
+    def over(t, at):  # a copy of t that lies in `memory` from element `at` on
+        part = memory[at:at + t.numel() * t.element_size() // 4].view(t.dtype).view(t.shape)
+        return part.copy_(t)
+
+    out = memory[:n * qh * d // 2].view(torch.bfloat16).view(n, qh * d)
+    last = out.numel() // 2 - 1  # the last word of the output
+    need = paged.decode_workspace(q, keys, table).numel()
+    assert torch.isfinite(paged.decode_attention(q, keys, vals, table, lens, out=out, ws=memory[1024:1024 + need])).all()
+    for at in (0, last):
+        for args in ((over(table, at), lens), (table, over(lens, at))):
+            for more in ((), (starts,)):
+                fn = paged.prompt_attention if more else paged.decode_attention
+                with pytest.raises(ValueError, match="out must not overlap"):
+                    fn(q, keys, vals, *args, *more, out=out)
+                size = (paged.prompt_workspace if more else paged.decode_workspace)(q, keys, table).numel()
+                with pytest.raises(ValueError, match="ws must not overlap"):
+                    fn(q, keys, vals, *args, *more, ws=memory[:max(size, 1024)])
+        with pytest.raises(ValueError, match="out must not overlap"):
+            paged.prompt_attention(q, keys, vals, table, lens, over(starts, at), out=out)
+    # a table whose rows lie apart: its last row counts
+    wide = memory[4096 - width - 3:4096 + width - 3].view(torch.int32).as_strided((2, width), (width, 1), 4096 - width - 3)
+    wide.copy_(table)
+    with pytest.raises(ValueError, match="out must not overlap"):
+        paged.decode_attention(q, keys, vals, wide, lens, out=memory[4096:4096 + n * qh * d // 2].view(torch.bfloat16).view(n, -1))
+
+    qkv = torch.zeros((n, (qh + 2 * kh) * d), dtype=torch.bfloat16, device=dev)
+    weight = torch.ones(d, dtype=torch.bfloat16, device=dev)
+    cos = torch.zeros((1024, d), device=dev)
+    plain = dict(q_weight=weight, k_weight=weight, cos=cos, sin=cos, table=table, lengths=lens, starts=starts)
+    rope_out = out.view(n, qh, d)
+    paged.qk_rope(qkv, keys=keys, values=vals, eps=1e-6, out=rope_out, **plain)
+    torch.cuda.synchronize()
+    for name, t in plain.items():
+        with pytest.raises(ValueError, match="out must not overlap"):
+            paged.qk_rope(qkv, keys=keys, values=vals, eps=1e-6, out=rope_out,
+                          **dict(plain, **{name: over(t, 4 * (last // 4))}))
