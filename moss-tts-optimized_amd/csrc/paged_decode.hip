@@ -44,6 +44,7 @@ struct DecodeArgs {
     float* part;   // [slots, QH, D]: O of each share
     float2* stat;  // [slots, QH]: its m and l
     int qh, group, xdim, shares;  // xdim: head tiles; shares: workgroups per head tile that the units are shared out over
+    long long slots;
     float scale;            // scale log2(e)
 };
 
@@ -290,6 +291,7 @@ __global__ __launch_bounds__(256) void paged_decode_join(DecodeArgs a, PagedCach
     int first = 0;
     for (int s = lane; s < b; s += kWave) first += shares_of(units_of(paged_length(bt, s, c.shift)), su);
     first = wave_total(first);
+    if (!in_slots(first, count, a.slots)) return;  // only when the lengths change between the launches
     // m and l of share 64 i + lane; a share's weight is 2^(m - largest m)
     const float2* st = a.stat + (size_t)first * a.qh + h;
     const float2 own = lane < count ? st[(size_t)lane * a.qh] : make_float2(-INFINITY, 0.f);
@@ -394,7 +396,7 @@ MOSS_API int moss_paged_decode_attention(const void* q, long long q_stride, cons
     const DecodePlan p = decode_plan(B, W, c.shift, qh, kh);
     MOSS_CHECK_ARG(workspace_bytes >= p.slots * qh * (d + 2) * 4 && p.slots * p.xdim * 256 < (1ll << 32));
     DecodeArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, (float*)workspace,
-                 reinterpret_cast<float2*>((float*)workspace + p.slots * qh * d), qh, qh / kh, p.xdim, p.shares,
+                 reinterpret_cast<float2*>((float*)workspace + p.slots * qh * d), qh, qh / kh, p.xdim, p.shares, p.slots,
                  scale * 1.4426950408889634f};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == 0)

@@ -120,6 +120,14 @@ MOSS_HD PromptItem prompt_item(const PromptTiles& t, int share, int index) {
         slot += c;
     }
 }
+// The item stands for a part of a tile: false for a number behind the sequence's items, as starts or lengths that change
+// under the kernel can lead to (its tile is -1 or less, or the part lies behind the tile's blocks).
+MOSS_HD bool is_item(const PromptTiles& t, int share, const PromptItem& it) {
+    return it.tile >= 0 && (it.part == 0 || (long long)it.part * share < t.blocks(it.tile));
+}
+// Partial results first .. first + count - 1 lie in a workspace of `slots` (lengths that change between the launches can name
+// others).
+MOSS_HD bool in_slots(int first, int count, long long slots) { return first >= 0 && count >= 0 && (long long)first + count <= slots; }
 inline long long decode_slots(int B, int W, int shift, int shares) {
     const long long most = (long long)B * ((((long long)W << shift) + kUnit - 1) / kUnit);
     return (long long)B + shares < most ? (long long)B + shares : most;

@@ -145,6 +145,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PromptArgs a, Page
     const int share = f.share, tok0 = f.tok0, pos0 = tiles.pos0;
     const PromptItem found = prompt_item(tiles, share, f.index);
     const PromptItem item{uniform(found.tile), uniform(found.part), uniform(found.slot)};
+    if (!is_item(tiles, share, item)) return;  // only when starts or lengths change under the kernel
     const int row0 = item.tile * HEIGHT, nrows = tiles.rows();
     const int row = min(row0 + 32 * rw + rl, nrows - 1);  // this lane's row (clamped: stores are guarded)
     const int token = tiles.token_of(row), head = kvh * G + row - token * G;
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PromptArgs a, Page
     // O^T element e of d tile dt: d = 32 dt + 8 (e / 4) + 4 half + e % 4
     if (cut) {
         // (starts that do not rise can name more parts than there are tokens for: they have no slot)
-        if (row0 + 32 * rw + rl >= nrows || f.first + item.slot >= a.slots) return;
+        if (row0 + 32 * rw + rl >= nrows || !in_slots(f.first + item.slot, 1, a.slots)) return;
         const size_t at = (size_t)(f.first + item.slot) * c.kh + kvh;
         float4* part = reinterpret_cast<float4*>(a.part) + at * (D / 4) * HEIGHT + 32 * rw + rl;
 #pragma unroll
@@ -399,14 +400,14 @@ __global__ __launch_bounds__(2 * HEIGHT) void paged_prompt_join(PromptArgs a, Pa
     if (f.b < 0) return;
     const int tile = f.tiles.tiles() - 1 - f.index, row = tile * HEIGHT + r;
     const int count = (f.tiles.blocks(tile) + f.share - 1) / f.share;
-    if (row >= f.tiles.rows()) return;
+    if (tile < 0 || row >= f.tiles.rows()) return;  // (tile: as for an item)
     // part k's slot: the cut tiles' parts 0 come first, then those of the tiles of more than 1, 2, .. shares
     float m = -INFINITY, den = 0.f;
     float4 acc[D / 8];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     int slot = f.first + f.index;
-    for (int k = 0; k < count && slot < a.slots; ++k) {
+    for (int k = 0; k < count && in_slots(slot, 1, a.slots); ++k) {
         const size_t at = ((size_t)slot * c.kh + kvh) * HEIGHT + r;
         slot += f.tiles.tiles_over(k ? k * f.share : f.share);
         const float2 st = a.stat[at];
