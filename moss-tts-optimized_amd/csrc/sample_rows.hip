@@ -397,7 +397,8 @@ __global__ __launch_bounds__(512) void sample_bins_kernel(SampleArgs a, Work w) 
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int b = bin_of_key(q, key_of<TYPE>(x[j]));
-                if (b < q.all) atomicAdd(&count[b], 1u);
+                // (a key above the row's largest, as when the logits change under the kernel, has no bin)
+                if ((uint32_t)b < (uint32_t)q.all) atomicAdd(&count[b], 1u);
                 if (b == q.np && (r.by_p || w.finish)) atomicAdd(sum, weight_of(r, x[j], table));
             }
         });
