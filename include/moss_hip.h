@@ -428,6 +428,24 @@ int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, 
                      const void *top_p, float top_p_value, const void *min_p, float min_p_value, void *out,
                      void *workspace, long long workspace_bytes, void *stream);
 
+/* Penalties, biases and a mask on up to 2^21 rows of `vocab` <= 2^19 logits (dtype 0 bf16, 1 fp16, 2 fp32; rows `stride` /
+ * `out_stride` values apart), before they are sampled: in fp32, one rounding, into out (the logits themselves, or memory of
+ * its own).
+ *   tokens    NULL, or int64 / int32 (token_bytes 8 / 4) token i < lengths[row] (int32; NULL: width) of a row at
+ *             row * token_row_stride + i * token_stride; the first prompt[row] (int32; NULL: 0) are the prompt
+ *   repetition, presence, frequency  fp32 [rows], or NULL for the value behind each.  A token among the row's: x > 0 ? x /
+ *             repetition : x * repetition.  Said c > 0 times behind the prompt: x - (c * frequency + presence)
+ *   bias_ids, bias  NULL, or int32 and fp32 [rows, biases] (biases < 65536; rows their strides apart, 0: one for all): x + bias,
+ *             of the last pair that names the entry
+ *   mask      NULL, or int32 words, rows mask_stride apart (0: one for all): -inf where bit v % 32 of word v / 32 is 0
+ * Ids outside [0, vocab) name nothing. */
+int moss_adjust_rows(const void *logits, int dtype, int rows, long long stride, int vocab, const void *tokens, int token_bytes,
+                     long long token_row_stride, long long token_stride, int width, const void *lengths, const void *prompt,
+                     const void *repetition, float repetition_value, const void *presence, float presence_value,
+                     const void *frequency, float frequency_value, const void *bias_ids, long long bias_ids_stride,
+                     const void *bias, long long bias_stride, int biases, const void *mask, long long mask_stride, void *out,
+                     long long out_stride, void *stream);
+
 /* ------------------------------------------- a batch over a paged cache */
 /* The single-request operators' counterparts for B sequences whose keys and values lie in pages that they
  * are handed one by one.  dtype 0 bf16, 1 fp16; head dim d 64 or 128; qh query heads, kh KV heads (qh % kh == 0,
@@ -480,6 +498,36 @@ int moss_paged_prompt_attention(const void *q, long long q_stride, const void *k
                                 long long table_stride, const void *lengths, const void *starts, int B, int W, int T,
                                 int qh, int kh, int d, float scale, void *out, void *workspace,
                                 long long workspace_bytes, int dtype, void *stream);
+
+/* A cache in 8 bits, for the same operators: k, v hold e4m3 codes (page strides in codes, a multiple of 16), and for each row of
+ * a KV head k_scales / v_scales (uint8 [pages, kh, page_rows], pages k_scale_stride / v_scale_stride bytes apart, a multiple of
+ * 16, the rest contiguous; 16-byte aligned) a byte: a value is its code times 2^(byte - 127), bytes 1 to 254.
+ * Written is a row of d values x, fp32, with A the largest |x| that is finite, as codes rounded to nearest even of
+ * x 2^-e with the least e for which A <= 448 2^e, at least -100 and at most 120 (bf16), -15 and 8 (fp16), which keeps what
+ * the codes stand for exact in that type; at the largest e codes end at 240.  NaN and infinities become e4m3's NaN.
+ * dtype is q's and the outputs' type. */
+int moss_paged_qk_rope_fp8(const void *qkv, long long qkv_stride, const void *q_weight, const void *k_weight,
+                           const void *cos, const void *sin, int table_f32, int table_rows, void *q_out, void *k, void *v,
+                           void *k_scales, void *v_scales, long long k_stride, long long v_stride,
+                           long long k_scale_stride, long long v_scale_stride, int pages, int page_rows,
+                           const void *table, long long table_stride, const void *lengths, const void *starts, int B, int W,
+                           int T, int qh, int kh, int d, float eps, int dtype, void *stream);
+int moss_paged_decode_attention_fp8(const void *q, long long q_stride, const void *k, const void *v, const void *k_scales,
+                                    const void *v_scales, long long k_stride, long long v_stride,
+                                    long long k_scale_stride, long long v_scale_stride, int pages, int page_rows,
+                                    const void *table, long long table_stride, const void *lengths, int B, int W, int qh,
+                                    int kh, int d, float scale, void *out, void *workspace, long long workspace_bytes,
+                                    int dtype, void *stream);
+
+/* The K and V rows of T packed tokens (T < 2^24) in order, k_out and v_out [T, kh, d] of the given dtype: a copy from a 16-bit
+ * cache, the values that the codes stand for from one in 8 bits.  A token without a position or a page gives zeros. */
+int moss_paged_gather(const void *k, const void *v, long long k_stride, long long v_stride, int pages, int page_rows,
+                      const void *table, long long table_stride, const void *lengths, const void *starts, int B, int W, int T,
+                      int kh, int d, void *k_out, void *v_out, int dtype, void *stream);
+int moss_paged_gather_fp8(const void *k, const void *v, const void *k_scales, const void *v_scales, long long k_stride,
+                          long long v_stride, long long k_scale_stride, long long v_scale_stride, int pages, int page_rows,
+                          const void *table, long long table_stride, const void *lengths, const void *starts, int B, int W,
+                          int T, int kh, int d, void *k_out, void *v_out, int dtype, void *stream);
 
 /* ------------------------------------------------------- measurement */
 /* No counterpart in the reference: a streaming read for bench.py, which times it on the bytes of a

@@ -1,0 +1,258 @@
+// Penalties for repeated tokens, biases and masks on rows of logits, before they are sampled.
+//
+// For entry v of a row with logit x, with the row's tokens so far h_0 .. h_{n-1}, of which the first `prompt` are the prompt:
+//   said = v among h;  c = how often v is among h_prompt ..
+//   said:   x <- x > 0 ? x / repetition : x repetition
+//   c > 0:  x <- x - (c frequency + presence)
+//   x <- x + bias, of the last of the row's (id, bias) pairs that names v
+//   -inf where the row's mask has a 0 at bit v
+// in fp32, rounded once to the logits' type.  Ids outside the row name nothing.
+//
+// What bounds it: the row's bytes in and out, and for few rows the chain launch, tokens, counts, logits.  A workgroup
+// takes kChunk entries of a row: it has their logits on the way while it goes through the row's tokens, counts those in
+// its range in LDS, with integers (a count, a flag, the largest index of a pair), so that no order of the atomics shows,
+// and then changes and writes its entries.  Tokens are read once for each of a row's chunks, from the cache.
+#include "common.h"
+
+namespace moss {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kChunk = 8192;                     // entries: 16 a thread
+constexpr int kGroups = kChunk / 8 / kThreads;   // of 8 entries, a thread's
+constexpr uint32_t kPrompt = 1u << 31;           // said in the prompt; below it the count
+typedef _Float16 f16_t;
+
+struct AdjustArgs {
+    const void* logits;
+    void* out;
+    long long stride, out_stride;
+    int vocab, chunks;
+    const void* tokens;
+    long long token_row, token_step;  // elements
+    int width;
+    const int* lengths;
+    const int* prompt;
+    const float *repetition, *presence, *frequency;
+    float repetition_v, presence_v, frequency_v;
+    const int* bias_ids;
+    const float* bias;
+    long long bias_ids_stride, bias_stride;
+    int biases;
+    const uint32_t* mask;
+    long long mask_stride;
+};
+
+template <int TYPE>
+struct Logit;
+template <>
+struct Logit<0> {
+    typedef uint16_t Bits;
+    static __device__ __forceinline__ float value(Bits b) { return bf16_bits(b); }
+    static __device__ __forceinline__ Bits bits(float x) { return f32_to_bf16(x); }
+};
+template <>
+struct Logit<1> {
+    typedef uint16_t Bits;
+    static __device__ __forceinline__ float value(Bits b) { return (float)__builtin_bit_cast(f16_t, b); }
+    static __device__ __forceinline__ Bits bits(float x) { return __builtin_bit_cast(Bits, (f16_t)x); }
+};
+template <>
+struct Logit<2> {
+    typedef uint32_t Bits;
+    static __device__ __forceinline__ float value(Bits b) { return __uint_as_float(b); }
+    static __device__ __forceinline__ Bits bits(float x) { return __float_as_uint(x); }
+};
+
+// Eight entries as they lie in memory.
+template <int TYPE>
+struct Group {
+    u32x4_t w[TYPE == 2 ? 2 : 1];
+    __device__ __forceinline__ typename Logit<TYPE>::Bits get(int i) const {
+        if constexpr (TYPE == 2) return w[i / 4][i % 4];
+        else return (uint16_t)(w[0][i / 2] >> (16 * (i & 1)));
+    }
+    __device__ __forceinline__ void set(int i, typename Logit<TYPE>::Bits b) {
+        if constexpr (TYPE == 2) w[i / 4][i % 4] = b;
+        else w[0][i / 2] = i & 1 ? (w[0][i / 2] & 0xffffu) | ((uint32_t)b << 16) : (w[0][i / 2] & 0xffff0000u) | b;
+    }
+};
+
+template <int TYPE, typename Token>
+__global__ __launch_bounds__(kThreads) void adjust_rows_kernel(AdjustArgs a) {
+    typedef Logit<TYPE> L;
+    typedef typename L::Bits Bits;
+    extern __shared__ uint32_t counts[];       // [kChunk]: the tokens; then [kChunk] of 16 bits: the biases
+    uint32_t* last = counts + (a.tokens ? kChunk : 0);  // two entries a word
+    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
+    const Bits* src = reinterpret_cast<const Bits*>(a.logits) + (size_t)row * a.stride;
+    Bits* dst = reinterpret_cast<Bits*>(a.out) + (size_t)row * a.out_stride;
+    // Groups of eight entries that begin at 16 bytes (32 of fp32) in both rows, where both begin at the same place among
+    // them; else one by one.  Entry 0 is entry `shift` of group 0.
+    constexpr int kBytes = 8 * sizeof(Bits);
+    const int shift = (int)((uintptr_t)src % kBytes / sizeof(Bits));
+    const bool wide = (uintptr_t)src % kBytes == (uintptr_t)dst % kBytes;
+    const int from = chunk * kChunk - shift;   // the chunk's first entry (below 0: none)
+    const int e0 = max(from, 0), e1 = min(from + kChunk, a.vocab);
+    Group<TYPE> x[kGroups];
+    auto first_of = [&](int g) { return from + 8 * (g * kThreads + tid); };
+    auto whole = [&](int e) { return wide && e >= 0 && e + 8 <= a.vocab; };
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int e = first_of(g);
+        if (whole(e)) {
+#pragma unroll
+            for (int i = 0; i < (TYPE == 2 ? 2 : 1); ++i) x[g].w[i] = reinterpret_cast<const u32x4_t*>(src + e)[i];
+        }
+    }
+    float rep = 1.f, pres = 0.f, freq = 0.f;
+    if (a.tokens) {
+        rep = a.repetition ? a.repetition[row] : a.repetition_v;
+        pres = a.presence ? a.presence[row] : a.presence_v;
+        freq = a.frequency ? a.frequency[row] : a.frequency_v;
+    }
+    if (a.tokens || a.bias) {
+        const int words = (a.tokens ? kChunk : 0) + (a.bias ? kChunk / 2 : 0);
+        for (int i = 4 * tid; i < words; i += 4 * kThreads) *reinterpret_cast<u32x4_t*>(counts + i) = u32x4_t{0u, 0u, 0u, 0u};
+        __syncthreads();
+        if (a.tokens) {
+            const int n = a.lengths ? min(max(a.lengths[row], 0), a.width) : a.width;
+            const int prompt = a.prompt ? a.prompt[row] : 0;
+            const Token* t = reinterpret_cast<const Token*>(a.tokens) + (long long)row * a.token_row;
+            for (int i = tid; i < n; i += kThreads) {
+                const Token id = t[(long long)i * a.token_step];
+                if (id < e0 || id >= e1) continue;
+                uint32_t* at = counts + ((int)id - from);
+                if (i < prompt) atomicOr(at, kPrompt);
+                else atomicAdd(at, 1u);
+            }
+        }
+        if (a.bias) {
+            // of two pairs that name one entry the later holds: the largest index + 1, in 16 bits, by compare and swap
+            const int* ids = a.bias_ids + (long long)row * a.bias_ids_stride;
+            for (int i = tid; i < a.biases; i += kThreads) {
+                const int id = ids[i];
+                if (id < e0 || id >= e1) continue;
+                uint32_t* at = last + (id - from) / 2;
+                const int up = 16 * ((id - from) & 1);
+                uint32_t old = *at;
+                while (((old >> up) & 0xffffu) < (uint32_t)(i + 1)) {
+                    const uint32_t next = (old & ~(0xffffu << up)) | ((uint32_t)(i + 1) << up);
+                    const uint32_t seen = atomicCAS(at, old, next);
+                    if (seen == old) break;
+                    old = seen;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const float* bias = a.bias + (long long)row * a.bias_stride;
+    const uint32_t* mask = a.mask ? a.mask + (long long)row * a.mask_stride : nullptr;
+    const int last_word = (a.vocab - 1) >> 5;
+    // entry e (from + k) with count word c and bias index b: changed, or as it was
+    auto change = [&](Bits& v, uint32_t c, uint32_t b) {
+        float y = L::value(v);
+        if (c) y = y > 0.f ? y / rep : y * rep;
+        if (c & ~kPrompt) y -= (float)(c & ~kPrompt) * freq + pres;
+        if (b) y += bias[b - 1];
+        v = L::bits(y);
+    };
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int e = first_of(g), k = e - from;
+        if (whole(e)) {
+            if (a.tokens || a.bias) {
+                u32x4_t c[2] = {}, b = {};
+                if (a.tokens) {
+                    c[0] = *reinterpret_cast<const u32x4_t*>(counts + k);
+                    c[1] = *reinterpret_cast<const u32x4_t*>(counts + k + 4);
+                }
+                if (a.bias) b = *reinterpret_cast<const u32x4_t*>(last + k / 2);
+                if (c[0][0] | c[0][1] | c[0][2] | c[0][3] | c[1][0] | c[1][1] | c[1][2] | c[1][3] | b[0] | b[1] | b[2] | b[3]) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t ci = c[i / 4][i % 4], bi = (b[i / 2] >> (16 * (i & 1))) & 0xffffu;
+                        if (ci | bi) {
+                            Bits v = x[g].get(i);
+                            change(v, ci, bi);
+                            x[g].set(i, v);
+                        }
+                    }
+                }
+            }
+            if (mask) {
+                const int w = e >> 5;
+                const uint64_t both = mask[w] | (uint64_t)mask[min(w + 1, last_word)] << 32;
+                const uint32_t bits = (uint32_t)(both >> (e & 31));
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!(bits >> i & 1)) x[g].set(i, L::bits(-INFINITY));
+            }
+#pragma unroll
+            for (int i = 0; i < (TYPE == 2 ? 2 : 1); ++i) reinterpret_cast<u32x4_t*>(dst + e)[i] = x[g].w[i];
+        } else {
+            // a row's ends, or all of a chunk whose rows begin at different places: one entry a lane
+            for (int i = 0; i < 8; ++i) {
+                const int at = wide ? e + i : from + g * 8 * kThreads + i * kThreads + tid;
+                if (at < 0 || at >= a.vocab) continue;
+                Bits v = src[at];
+                const uint32_t ci = a.tokens ? counts[at - from] : 0u;
+                const uint32_t bi = a.bias ? (last[(at - from) / 2] >> (16 * ((at - from) & 1))) & 0xffffu : 0u;
+                if (ci | bi) change(v, ci, bi);
+                if (mask && !(mask[at >> 5] >> (at & 31) & 1)) v = L::bits(-INFINITY);
+                dst[at] = v;
+            }
+        }
+    }
+}
+
+template <int TYPE>
+void launch_adjust(const AdjustArgs& a, int rows, int token_bytes, hipStream_t st) {
+    const dim3 grid((unsigned)(rows * (long long)a.chunks)), block(kThreads);
+    const size_t lds = (a.tokens ? 4 * kChunk : 0) + (a.bias ? 2 * kChunk : 0);
+    if (token_bytes == 8)
+        hipLaunchKernelGGL((adjust_rows_kernel<TYPE, int64_t>), grid, block, lds, st, a);
+    else
+        hipLaunchKernelGGL((adjust_rows_kernel<TYPE, int32_t>), grid, block, lds, st, a);
+}
+
+}  // namespace
+}  // namespace moss
+
+using namespace moss;
+
+MOSS_API int moss_adjust_rows(const void* logits, int dtype, int rows, long long stride, int vocab, const void* tokens,
+                              int token_bytes, long long token_row_stride, long long token_stride, int width, const void* lengths,
+                              const void* prompt, const void* repetition, float repetition_value, const void* presence,
+                              float presence_value, const void* frequency, float frequency_value, const void* bias_ids,
+                              long long bias_ids_stride, const void* bias, long long bias_stride, int biases, const void* mask,
+                              long long mask_stride, void* out, long long out_stride, void* stream) {
+    const int size = dtype == 2 ? 4 : 2;
+    MOSS_CHECK_ARG(logits && out && dtype >= 0 && dtype <= 2 && rows > 0 && rows <= (1 << 21) && vocab > 0 && vocab <= (1 << 19) &&
+                   stride >= vocab && out_stride >= vocab && MOSS_ALIGNED(logits, size) && MOSS_ALIGNED(out, size));
+    MOSS_CHECK_ARG(!tokens || ((token_bytes == 4 || token_bytes == 8) && MOSS_ALIGNED(tokens, token_bytes) && width > 0 &&
+                               token_row_stride >= 0 && token_stride >= 0));
+    MOSS_CHECK_ARG(tokens || (!lengths && !prompt && !repetition && !presence && !frequency));
+    MOSS_CHECK_ARG(MOSS_ALIGNED(lengths, 4) && MOSS_ALIGNED(prompt, 4) && MOSS_ALIGNED(repetition, 4) && MOSS_ALIGNED(presence, 4) &&
+                   MOSS_ALIGNED(frequency, 4));
+    MOSS_CHECK_ARG((bias_ids == nullptr) == (bias == nullptr));
+    MOSS_CHECK_ARG(!bias || (biases > 0 && biases < (1 << 16) && (bias_ids_stride == 0 || bias_ids_stride >= biases) &&
+                             (bias_stride == 0 || bias_stride >= biases) && MOSS_ALIGNED(bias_ids, 4) && MOSS_ALIGNED(bias, 4)));
+    MOSS_CHECK_ARG(!mask || ((mask_stride == 0 || mask_stride >= (vocab + 31) / 32) && MOSS_ALIGNED(mask, 4)));
+    AdjustArgs a;
+    a.logits = logits, a.out = out, a.stride = stride, a.out_stride = out_stride, a.vocab = vocab;
+    // a row that begins inside a group of eight has its last entries one group further
+    a.chunks = (vocab + 7 + kChunk - 1) / kChunk;
+    a.tokens = tokens, a.token_row = token_row_stride, a.token_step = token_stride, a.width = width;
+    a.lengths = (const int*)lengths, a.prompt = (const int*)prompt;
+    a.repetition = (const float*)repetition, a.presence = (const float*)presence, a.frequency = (const float*)frequency;
+    a.repetition_v = repetition_value, a.presence_v = presence_value, a.frequency_v = frequency_value;
+    a.bias_ids = (const int*)bias_ids, a.bias = (const float*)bias, a.bias_ids_stride = bias_ids_stride, a.bias_stride = bias_stride;
+    a.biases = biases, a.mask = (const uint32_t*)mask, a.mask_stride = mask_stride;
+    MOSS_CHECK_ARG((long long)rows * a.chunks * kThreads < (1ll << 32));
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == 0) launch_adjust<0>(a, rows, token_bytes, st);
+    else if (dtype == 1) launch_adjust<1>(a, rows, token_bytes, st);
+    else launch_adjust<2>(a, rows, token_bytes, st);
+    return moss_launch_status();
+}

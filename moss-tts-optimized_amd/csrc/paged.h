@@ -36,7 +36,10 @@ typedef float f32x4_v __attribute__((ext_vector_type(4)));
 typedef float f32x16_v __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x2_v __attribute__((ext_vector_type(2)));
 
+// kLeast, kMost: the exponents of a power of two that e4m3 values may be scaled by and stay exact, 240 2^kMost finite
 struct Bf16 {
+    static constexpr bool kHalf = false;
+    static constexpr int kLeast = -100, kMost = 120;
     static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
@@ -51,6 +54,8 @@ struct Bf16 {
 };
 
 struct F16 {
+    static constexpr bool kHalf = true;
+    static constexpr int kLeast = -15, kMost = 8;
     static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2_v, w)[0]; }
     static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2_v, w)[1]; }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {  // round to nearest even, one value at a time

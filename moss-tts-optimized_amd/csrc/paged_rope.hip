@@ -11,7 +11,10 @@
 // the launch, 2.8 us).  A head is D / 16 lanes, each with 8 values of either half, so every load and store is 16
 // bytes; one workgroup takes 256 / (D / 16) heads of one token, and a wave finds the token's sequence with one ballot
 // per 64 sequences.
-#include "paged.h"
+//
+// Into a cache of 8 bits (paged8.h) K and V go from their fp32 values: the row's largest one over its lanes, its scale byte, the
+// codes.  K is rounded once there too, and not to 16 bits before.
+#include "paged8.h"
 
 namespace moss {
 namespace {
@@ -48,8 +51,29 @@ __device__ __forceinline__ void unpack8(u32x4_t w, float (&v)[8]) {
     for (int i = 0; i < 4; ++i) v[2 * i] = E::lo(w[i]), v[2 * i + 1] = E::hi(w[i]);
 }
 
-template <typename E, int D, bool F32>
-__global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, PagedCache c, PagedBatch bt) {
+// The row of an 8-bit cache that D / 16 lanes hold, 8 values of either half each (all of a row's lanes come here).
+template <typename E, int D>
+__device__ __forceinline__ void store_row8(uint8_t* codes, uint8_t* scale, int j, const float (&x)[8], const float (&y)[8]) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        top = fmaxf(top, x[i] - x[i] == 0.f ? fabsf(x[i]) : 0.f);
+        top = fmaxf(top, y[i] - y[i] == 0.f ? fabsf(y[i]) : 0.f);
+    }
+#pragma unroll
+    for (int m = 1; m < D / 16; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, D / 16));
+    const uint32_t byte = scale_byte<E>(top);
+    const float inverse = scale_of(254 - byte), most = most_of<E>(byte);
+    *reinterpret_cast<uint2*>(codes + 8 * j) = make_uint2(codes4<E>(x[0], x[1], x[2], x[3], inverse, most),
+                                                          codes4<E>(x[4], x[5], x[6], x[7], inverse, most));
+    *reinterpret_cast<uint2*>(codes + D / 2 + 8 * j) = make_uint2(codes4<E>(y[0], y[1], y[2], y[3], inverse, most),
+                                                                  codes4<E>(y[4], y[5], y[6], y[7], inverse, most));
+    if (j == 0) *scale = (uint8_t)byte;
+}
+
+template <typename E, int D, bool F32, typename Cache>
+__global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, Cache c, PagedBatch bt) {
+    constexpr bool EIGHT = std::is_same<Cache, PagedCache8>::value;
     constexpr int LPH = D / 16, HPB = 256 / LPH;  // lanes per head, heads per workgroup
     const int t = blockIdx.x, lane = threadIdx.x & (kWave - 1);
     // the token's sequence: with packed tokens the last one that starts at or before it (empty ones end there too)
@@ -72,12 +96,26 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, PagedCache 
     const u32x4_t wa = *reinterpret_cast<const u32x4_t*>(src), wb = *reinterpret_cast<const u32x4_t*>(src + D / 2);
     // the row's place in the cache; a token without a position (more tokens than the length says) or a page has none
     uint16_t* dst = nullptr;
+    uint8_t *codes = nullptr, *scale = nullptr;
     if (h >= a.qh) {
         const bool is_k = h < a.qh + c.kh;
         const int page = page_of_row(bt.table + (size_t)b * bt.table_stride, position, bt.W, c.shift, c.pages);
-        if (page >= 0)
-            dst = (is_k ? c.k : c.v) + 8 * j +
-                  row_offset(page, is_k ? c.k_stride : c.v_stride, h - a.qh - (is_k ? 0 : c.kh), position, c.shift, D);
+        const int head = h - a.qh - (is_k ? 0 : c.kh);
+        if constexpr (EIGHT) {
+            if (page < 0) return;
+            codes = reinterpret_cast<uint8_t*>(is_k ? c.k : c.v) +
+                    row_offset(page, is_k ? c.k_stride : c.v_stride, head, position, c.shift, D);
+            scale = (is_k ? c.ks : c.vs) + row_offset(page, is_k ? c.ks_stride : c.vs_stride, head, position, c.shift, 1);
+            if (!is_k) {
+                float x[8], y[8];
+                unpack8<E>(wa, x);
+                unpack8<E>(wb, y);
+                store_row8<E, D>(codes, scale, j, x, y);
+                return;
+            }
+        } else if (page >= 0) {
+            dst = (is_k ? c.k : c.v) + 8 * j + row_offset(page, is_k ? c.k_stride : c.v_stride, head, position, c.shift, D);
+        }
         if (h >= a.qh + c.kh) {  // values go as they are
             if (dst) {
                 *reinterpret_cast<u32x4_t*>(dst) = wa;
@@ -114,6 +152,18 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, PagedCache 
     table8<E, F32>(a.cos_t, row + D / 2, cy);
     table8<E, F32>(a.sin_t, row, sx);
     table8<E, F32>(a.sin_t, row + D / 2, sy);
+    if constexpr (EIGHT) {
+        if (h >= a.qh) {
+            float lo[8], hi[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                lo[i] = x[i] * cx[i] - y[i] * sx[i];
+                hi[i] = y[i] * cy[i] + x[i] * sy[i];
+            }
+            store_row8<E, D>(codes, scale, j, lo, hi);
+            return;
+        }
+    }
     if (!dst) return;
     u32x4_t lo, hi;
 #pragma unroll
@@ -127,14 +177,102 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, PagedCache 
     *reinterpret_cast<u32x4_t*>(dst + D / 2) = hi;
 }
 
-template <typename E, int D>
-void launch_rope(const RopeArgs& a, const PagedCache& c, const PagedBatch& bt, bool f32, hipStream_t st) {
+template <typename E, int D, typename Cache>
+void launch_rope(const RopeArgs& a, const Cache& c, const PagedBatch& bt, bool f32, hipStream_t st) {
     constexpr int HPB = 256 / (D / 16);
     const dim3 grid((unsigned)a.T, (unsigned)((a.qh + 2 * c.kh + HPB - 1) / HPB));
     if (f32)
-        hipLaunchKernelGGL((paged_rope_kernel<E, D, true>), grid, dim3(256), 0, st, a, c, bt);
+        hipLaunchKernelGGL((paged_rope_kernel<E, D, true, Cache>), grid, dim3(256), 0, st, a, c, bt);
     else
-        hipLaunchKernelGGL((paged_rope_kernel<E, D, false>), grid, dim3(256), 0, st, a, c, bt);
+        hipLaunchKernelGGL((paged_rope_kernel<E, D, false, Cache>), grid, dim3(256), 0, st, a, c, bt);
+}
+
+template <typename Cache>
+int rope(const RopeArgs& a, const Cache& c, const PagedBatch& bt, int d, int table_f32, int dtype, hipStream_t st) {
+    MOSS_CHECK_ARG(a.qkv && a.cos_t && a.sin_t && a.q_out && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, a.qh, d));
+    // 256 threads a token: from 2^24 tokens on the grid would have more than 2^32 - 1
+    MOSS_CHECK_ARG(a.T > 0 && a.T < (1 << 24) && (bt.starts || a.T == bt.B) && a.table_rows > 0 && a.eps >= 0.f &&
+                   (dtype == 0 || dtype == 1));
+    MOSS_CHECK_ARG((a.qw == nullptr) == (a.kw == nullptr) && a.qkv_stride % 8 == 0 &&
+                   a.qkv_stride >= (long long)(a.qh + 2 * c.kh) * d);
+    MOSS_CHECK_ARG(MOSS_ALIGNED(a.qkv, 16) && MOSS_ALIGNED(a.qw, 16) && MOSS_ALIGNED(a.kw, 16) && MOSS_ALIGNED(a.cos_t, 16) &&
+                   MOSS_ALIGNED(a.sin_t, 16) && MOSS_ALIGNED(a.q_out, 16));
+    if (dtype == 0)
+        d == 128 ? launch_rope<Bf16, 128>(a, c, bt, table_f32 != 0, st) : launch_rope<Bf16, 64>(a, c, bt, table_f32 != 0, st);
+    else
+        d == 128 ? launch_rope<F16, 128>(a, c, bt, table_f32 != 0, st) : launch_rope<F16, 64>(a, c, bt, table_f32 != 0, st);
+    return moss_launch_status();
+}
+
+// ---------------------------------------------------------------- the rows back, in order
+// Token t of a sequence's n newest: the K and V rows at its position, as the 16-bit type; a token without a position or a page
+// gives zeros.  What bounds it: memory.  A row is D / 16 lanes with 8 values of either half, a wave takes 1024 / D rows of one
+// token (K heads, then V heads), so the token's sequence is found with one ballot per 64 sequences.
+struct GatherArgs {
+    uint16_t* k_out;
+    uint16_t* v_out;
+    int T, waves;  // waves a token
+};
+
+template <typename E, int D, typename Cache>
+__global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a, Cache c, PagedBatch bt) {
+    constexpr int LPH = D / 16, RPW = kWave / LPH;
+    const int lane = threadIdx.x & (kWave - 1);
+    const long long wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + threadIdx.x / kWave));
+    const int t = (int)(wave / a.waves), part = (int)(wave % a.waves);
+    if (t >= a.T) return;
+    int at_or_before = 0;
+    for (int b0 = 0; b0 < bt.B; b0 += kWave)
+        at_or_before += __popcll(__ballot(b0 + lane < bt.B && bt.starts[min(b0 + lane, bt.B - 1)] <= t));
+    const int b = at_or_before - 1;
+    if (b < 0) return;
+    const int end = min(bt.starts[b + 1], a.T);
+    if (t >= end) return;  // padding behind the last sequence
+    const int position = paged_length(bt, b, c.shift) - end + t;
+    const int row = part * RPW + lane / LPH, j = lane % LPH;
+    if (row >= 2 * c.kh) return;
+    const bool is_k = row < c.kh;
+    const int head = row - (is_k ? 0 : c.kh);
+    const int page = page_of_row(bt.table + (size_t)b * bt.table_stride, position, bt.W, c.shift, c.pages);
+    u32x4_t lo = {0u, 0u, 0u, 0u}, hi = lo;
+    if (page >= 0) {
+        const size_t at = row_offset(page, is_k ? c.k_stride : c.v_stride, head, position, c.shift, D) + 8 * j;
+        if constexpr (std::is_same<Cache, PagedCache8>::value) {
+            const uint8_t* src = (is_k ? c.kc() : c.vc()) + at;
+            const float scale =
+                scale_of((is_k ? c.ks : c.vs)[row_offset(page, is_k ? c.ks_stride : c.vs_stride, head, position, c.shift, 1)]);
+            const uint2 p = *reinterpret_cast<const uint2*>(src), q = *reinterpret_cast<const uint2*>(src + D / 2);
+            lo = widen8<E>(p.x, p.y, scale);
+            hi = widen8<E>(q.x, q.y, scale);
+        } else {
+            const uint16_t* src = (is_k ? c.k : c.v) + at;
+            lo = *reinterpret_cast<const u32x4_t*>(src);
+            hi = *reinterpret_cast<const u32x4_t*>(src + D / 2);
+        }
+    }
+    uint16_t* dst = (is_k ? a.k_out : a.v_out) + ((size_t)t * c.kh + head) * D + 8 * j;
+    *reinterpret_cast<u32x4_t*>(dst) = lo;
+    *reinterpret_cast<u32x4_t*>(dst + D / 2) = hi;
+}
+
+template <typename E, int D, typename Cache>
+void launch_gather(GatherArgs a, const Cache& c, const PagedBatch& bt, hipStream_t st) {
+    hipLaunchKernelGGL((paged_gather_kernel<E, D, Cache>), dim3((unsigned)(((long long)a.T * a.waves + 3) / 4)), dim3(256), 0, st,
+                       a, c, bt);
+}
+
+template <typename Cache>
+int gather(void* k_out, void* v_out, const Cache& c, const PagedBatch& bt, int T, int d, int dtype, hipStream_t st) {
+    MOSS_CHECK_ARG(k_out && v_out && bt.starts && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, c.kh, d));
+    MOSS_CHECK_ARG(MOSS_ALIGNED(k_out, 16) && MOSS_ALIGNED(v_out, 16) && (dtype == 0 || dtype == 1) && T > 0 && T < (1 << 24));
+    const int rows = 1024 / d;  // of a wave
+    const GatherArgs a{(uint16_t*)k_out, (uint16_t*)v_out, T, (2 * c.kh + rows - 1) / rows};
+    MOSS_CHECK_ARG(((long long)T * a.waves + 3) / 4 * 256 < (1ll << 32));
+    if (dtype == 0)
+        d == 128 ? launch_gather<Bf16, 128>(a, c, bt, st) : launch_gather<Bf16, 64>(a, c, bt, st);
+    else
+        d == 128 ? launch_gather<F16, 128>(a, c, bt, st) : launch_gather<F16, 64>(a, c, bt, st);
+    return moss_launch_status();
 }
 
 }  // namespace
@@ -149,19 +287,40 @@ MOSS_API int moss_paged_qk_rope(const void* qkv, long long qkv_stride, const voi
                                 int W, int T, int qh, int kh, int d, float eps, int dtype, void* stream) {
     const PagedCache c = paged_cache(k, v, k_stride, v_stride, pages, kh, page_rows);
     const PagedBatch bt{(const int*)table, (const int*)lengths, (const int*)starts, B, W, table_stride};
-    MOSS_CHECK_ARG(qkv && cos && sin && q_out && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, qh, d));
-    // 256 threads a token: from 2^24 tokens on the grid would have more than 2^32 - 1
-    MOSS_CHECK_ARG(T > 0 && T < (1 << 24) && (starts || T == B) && table_rows > 0 && eps >= 0.f && (dtype == 0 || dtype == 1));
-    MOSS_CHECK_ARG((q_weight == nullptr) == (k_weight == nullptr) && qkv_stride % 8 == 0 &&
-                   qkv_stride >= (long long)(qh + 2 * kh) * d);
-    MOSS_CHECK_ARG(MOSS_ALIGNED(qkv, 16) && MOSS_ALIGNED(q_weight, 16) && MOSS_ALIGNED(k_weight, 16) && MOSS_ALIGNED(cos, 16) &&
-                   MOSS_ALIGNED(sin, 16) && MOSS_ALIGNED(q_out, 16));
     const RopeArgs a{(const uint16_t*)qkv, qkv_stride, (const uint16_t*)q_weight, (const uint16_t*)k_weight, cos, sin,
                      (uint16_t*)q_out, T, qh, table_rows, eps};
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == 0)
-        d == 128 ? launch_rope<Bf16, 128>(a, c, bt, table_f32 != 0, st) : launch_rope<Bf16, 64>(a, c, bt, table_f32 != 0, st);
-    else
-        d == 128 ? launch_rope<F16, 128>(a, c, bt, table_f32 != 0, st) : launch_rope<F16, 64>(a, c, bt, table_f32 != 0, st);
-    return moss_launch_status();
+    return rope(a, c, bt, d, table_f32, dtype, (hipStream_t)stream);
+}
+
+MOSS_API int moss_paged_qk_rope_fp8(const void* qkv, long long qkv_stride, const void* q_weight, const void* k_weight,
+                                    const void* cos, const void* sin, int table_f32, int table_rows, void* q_out, void* k,
+                                    void* v, void* k_scales, void* v_scales, long long k_stride, long long v_stride,
+                                    long long k_scale_stride, long long v_scale_stride, int pages, int page_rows,
+                                    const void* table, long long table_stride, const void* lengths, const void* starts, int B,
+                                    int W, int T, int qh, int kh, int d, float eps, int dtype, void* stream) {
+    const PagedCache8 c = paged_cache8(k, v, k_scales, v_scales, k_stride, v_stride, k_scale_stride, v_scale_stride, pages, kh, page_rows);
+    const PagedBatch bt{(const int*)table, (const int*)lengths, (const int*)starts, B, W, table_stride};
+    const RopeArgs a{(const uint16_t*)qkv, qkv_stride, (const uint16_t*)q_weight, (const uint16_t*)k_weight, cos, sin,
+                     (uint16_t*)q_out, T, qh, table_rows, eps};
+    MOSS_CHECK_ARG(paged8_ok(c));
+    return rope(a, c, bt, d, table_f32, dtype, (hipStream_t)stream);
+}
+
+MOSS_API int moss_paged_gather(const void* k, const void* v, long long k_stride, long long v_stride, int pages, int page_rows,
+                               const void* table, long long table_stride, const void* lengths, const void* starts, int B, int W,
+                               int T, int kh, int d, void* k_out, void* v_out, int dtype, void* stream) {
+    const PagedCache c = paged_cache(k, v, k_stride, v_stride, pages, kh, page_rows);
+    const PagedBatch bt{(const int*)table, (const int*)lengths, (const int*)starts, B, W, table_stride};
+    return gather(k_out, v_out, c, bt, T, d, dtype, (hipStream_t)stream);
+}
+
+MOSS_API int moss_paged_gather_fp8(const void* k, const void* v, const void* k_scales, const void* v_scales, long long k_stride,
+                                   long long v_stride, long long k_scale_stride, long long v_scale_stride, int pages,
+                                   int page_rows, const void* table, long long table_stride, const void* lengths,
+                                   const void* starts, int B, int W, int T, int kh, int d, void* k_out, void* v_out, int dtype,
+                                   void* stream) {
+    const PagedCache8 c = paged_cache8(k, v, k_scales, v_scales, k_stride, v_stride, k_scale_stride, v_scale_stride, pages, kh, page_rows);
+    const PagedBatch bt{(const int*)table, (const int*)lengths, (const int*)starts, B, W, table_stride};
+    MOSS_CHECK_ARG(paged8_ok(c));
+    return gather(k_out, v_out, c, bt, T, d, dtype, (hipStream_t)stream);
 }

@@ -12,6 +12,12 @@ outside ``[0, pages)`` names no page: its rows take no part and nothing is writt
 ``starts``: int32 ``[B + 1]``, rising from 0: the packed tokens ``starts[b] .. starts[b + 1] - 1`` are the newest ones of
 sequence ``b`` and stand at its last positions.  Packed rows from ``starts[B]`` on are padding and left as they are.
 
+``scales``: None, or for a cache in 8 bits the pair of its keys' and values' scales.  Such a cache holds e4m3 codes
+(``torch.float8_e4m3fn``), and for each row of a KV head one byte, uint8 ``[pages, KV heads, page rows]`` (pages any multiple of
+16 bytes apart): a value is its code times 2^(byte - 127).  :func:`qk_rope` writes both, a row's power of two being the least
+that brings it under 448; the attentions and :func:`gather` read the values that they stand for, which the 16-bit type of ``q``
+holds exactly.  Bytes 0 and 255 are no scale.
+
 Table, lengths and starts are device values, read when the kernels run and not checked by the host: a captured
 graph follows them as sequences grow.  Whatever they hold, no access leaves the cache or the packed rows; what they have
 to hold for results is the caller's to see to: lengths that the table's row can hold (all three operators take a
@@ -78,6 +84,104 @@ class _Cache:
             raise ValueError("keys and values are not a paged cache")
         self.pages, self.kh, self.rows, self.d, self.k, self.v, self.ks, self.vs = n, kh, rows, d, k, v, ks, vs
         self.kend, self.vend = k + 2 * ((n - 1) * ks + page), v + 2 * ((n - 1) * vs + page)
+
+
+    native_name = ""
+
+    def args(self):
+        """What the native entries take to describe the cache."""
+        return self.k, self.v, self.ks, self.vs, self.pages, self.rows
+
+    def spans(self):
+        return (self.k, self.kend), (self.v, self.vend)
+
+    def regions(self):
+        """(first, end, bytes from a page to the next, bytes of a page) of what is written."""
+        page = 2 * self.kh * self.rows * self.d
+        return (self.k, self.kend, 2 * self.ks, page), (self.v, self.vend, 2 * self.vs, page)
+
+
+def _scales_refuse(keys, values, scales, index):
+    for name, t in (("keys", keys), ("values", values)):
+        _require(isinstance(t, torch.Tensor) and t.dtype == torch.float8_e4m3fn,
+                 f"with scales {name} must be a torch.float8_e4m3fn tensor")
+    _cache_refuse(keys, values, torch.float8_e4m3fn, index)
+    n, kh, rows, d = keys.shape
+    for name, t in (("keys", keys), ("values", values)):
+        _require(n == 1 or t.stride(0) % 16 == 0, f"{name}: pages must be 16-byte aligned")
+    _require(isinstance(scales, (tuple, list)) and len(scales) == 2, "scales must be the keys' and the values' scales")
+    for t in scales:
+        _require(isinstance(t, torch.Tensor) and t.dtype == torch.uint8 and t.get_device() == index
+                 and t.shape == (n, kh, rows), f"scales must be uint8 [pages, KV heads, page rows] tensors on cuda:{index}")
+        _require(t.stride(2) == 1 and (kh == 1 or t.stride(1) == rows), "a page of scales must be contiguous")
+        _require(_aligned(t, 16) and (n == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= kh * rows)),
+                 "scales: pages must be 16-byte aligned and must not overlap")
+
+
+class _Cache8:
+    """A checked cache of e4m3 codes and their scales, as numbers."""
+
+    __slots__ = ("pages", "kh", "rows", "d", "k", "v", "ks", "vs", "kend", "vend", "sk", "sv", "sks", "svs", "skend", "svend")
+    native_name = "_fp8"
+
+    def __init__(self, keys, values, scales, index):
+        try:
+            a, b = scales
+            n, kh, rows, d = shape = keys.shape
+            ks, k2, k1, k0 = keys.stride()
+            vs, v2, v1, v0 = values.stride()
+            sks, a1, a0 = a.stride()
+            svs, b1, b0 = b.stride()
+            k, v, sk, sv = keys.data_ptr(), values.data_ptr(), a.data_ptr(), b.data_ptr()
+            few, page = kh * rows, kh * rows * d
+            if n == 1:
+                ks, vs, sks, svs = page, page, few, few
+            if kh == 1:
+                k2 = v2 = rows * d
+                a1 = b1 = rows
+            code = torch.float8_e4m3fn
+            ok = (keys.dtype is code and values.dtype is code and a.dtype is torch.uint8 and b.dtype is torch.uint8
+                  and values.shape == shape and page and a.shape == shape[:3] == b.shape
+                  and keys.get_device() == values.get_device() == a.get_device() == b.get_device() == index
+                  and rows in _PAGE_ROWS and d in _HEAD_DIMS and k0 == v0 == a0 == b0 == 1 and k1 == v1 == d
+                  and k2 == v2 == rows * d and a1 == b1 == rows
+                  and not (ks | vs | sks | svs | k | v | sk | sv) & 15 and ks >= page <= vs and sks >= few <= svs)
+        except (AttributeError, ValueError, TypeError):
+            ok = False
+        if not ok:
+            _scales_refuse(keys, values, scales, index)
+            raise ValueError("keys, values and scales are not a paged cache")
+        self.pages, self.kh, self.rows, self.d, self.k, self.v, self.ks, self.vs = n, kh, rows, d, k, v, ks, vs
+        self.sk, self.sv, self.sks, self.svs = sk, sv, sks, svs
+        n -= 1
+        self.kend, self.vend, self.skend, self.svend = k + n * ks + page, v + n * vs + page, sk + n * sks + few, sv + n * svs + few
+
+    def args(self):
+        return self.k, self.v, self.sk, self.sv, self.ks, self.vs, self.sks, self.svs, self.pages, self.rows
+
+    def spans(self):
+        return (self.k, self.kend), (self.v, self.vend), (self.sk, self.skend), (self.sv, self.svend)
+
+    def regions(self):
+        few, page = self.kh * self.rows, self.kh * self.rows * self.d
+        return ((self.k, self.kend, self.ks, page), (self.v, self.vend, self.vs, page), (self.sk, self.skend, self.sks, few),
+                (self.sv, self.svend, self.svs, few))
+
+
+def _cache_of(keys, values, scales, dtype, index):
+    if scales is not None:
+        return _Cache8(keys, values, scales, index)
+    _require(not (isinstance(keys, torch.Tensor) and keys.dtype == torch.float8_e4m3fn), "a cache in 8 bits needs its scales")
+    return _Cache(keys, values, dtype, index)
+
+
+def _written_apart(regions):
+    """Nothing of a cache that is written lies in another part of it: apart, or pages between pages."""
+    for i, (a, aend, astep, apage) in enumerate(regions):
+        for b, bend, bstep, bpage in regions[i + 1:]:
+            if a < bend and b < aend:
+                _require(astep == bstep and apage <= (b - a) % astep <= astep - bpage,
+                         "keys and values (and their scales) must not share memory")
 
 
 def _batch_refuse(table, lengths, starts, rows, index):
@@ -207,14 +311,18 @@ def _output(out, shape, like: torch.Tensor, index: int, spans) -> torch.Tensor:
 
 def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, cos: torch.Tensor,
             sin: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-            eps: float, *, starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+            eps: float, *, starts: torch.Tensor | None = None, out: torch.Tensor | None = None,
+            scales: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """q/k head RMSNorm + rotary embedding of ``T`` packed tokens, whose K and V rows are written to their pages.
 
     ``qkv`` ``[T, (query heads + 2 KV heads) * head dim]`` (q | k | v; rows may lie apart), head-norm weights ``[head
     dim]`` (both None: no norm), ``cos`` / ``sin`` ``[positions, head dim]`` tables in ``qkv``'s type or fp32.  Without
     ``starts`` every sequence has one token.  Returns ``q`` ``[T, query heads, head dim]``.  The arithmetic is fp32 up
     to one rounding, where ``pointwise.qk_rope`` rounds after every step.  A token at a negative position (more tokens
-    than its length) or without a page is written to no row; a position behind the tables takes their last row."""
+    than its length) or without a page is written to no row; a position behind the tables takes their last row.
+    With ``scales`` the rows are written in 8 bits, straight from fp32: off by at most 2^-4 of a value, or 2^-10 times the
+    row's power of two where that is more; values past 240 times the largest power of two of the type are held at that, and
+    what is not finite is NaN."""
     _require(isinstance(qkv, torch.Tensor) and qkv.dtype in _TYPES, "qkv must be a bf16 or fp16 tensor")
     index, dtype = qkv.get_device(), qkv.dtype
     _require(index >= 0 and qkv.dim() == 2 and qkv.numel() > 0, "qkv must be a CUDA (HIP) tensor [tokens, width]")
@@ -225,7 +333,7 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     at = qkv.data_ptr()
     _require(s0 == 1 or width == 1, "a row of qkv must be contiguous")
     _require(stride >= width and not (stride & 7 or at & 15), "qkv: rows must be 16-byte aligned and must not overlap")
-    c = _Cache(keys, values, dtype, index)
+    c = _cache_of(keys, values, scales, dtype, index)
     kh, d = c.kh, c.d
     b, w, table_stride, table_at, lengths_at, starts_at = batch = _batch(table, lengths, starts, c.rows, index)
     qh = width // d - 2 * kh
@@ -236,22 +344,59 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     _require(eps >= 0, "eps must not be negative")
     _require(tokens < 1 << 24, "fewer than 2^24 packed tokens required")
     span = (at, at + 2 * ((tokens - 1) * stride + width))
-    _require((c.kend <= span[0] or span[1] <= c.k) and (c.vend <= span[0] or span[1] <= c.v),
-             "qkv must not overlap the cache")
-    if c.k < c.vend and c.v < c.kend:  # interleaved: the keys of a page lie between the values of two
-        page, step = 2 * kh * c.rows * d, 2 * c.ks
-        _require(c.ks == c.vs and page <= (c.v - c.k) % step <= step - page, "keys and values must not share memory")
+    regions = c.regions()
+    for first, end, _, _ in regions:
+        _require(end <= span[0] or span[1] <= first, "qkv must not overlap the cache")
+    _written_apart(regions)
     spans = ()
     if out is not None:
         qw, kw, cos_at, sin_at, f32, rows = norms
         size = rows * d * (4 if f32 else 2)
-        spans = (span, (c.k, c.kend), (c.v, c.vend), (cos_at, cos_at + size), (sin_at, sin_at + size), *_batch_spans(*batch))
+        spans = (span, *c.spans(), (cos_at, cos_at + size), (sin_at, sin_at + size), *_batch_spans(*batch))
         if qw is not None:
             spans += (qw, qw + 2 * d), (kw, kw + 2 * d)
     q = _output(out, (tokens, qh, d), qkv, index, spans)
-    native.call_on(qkv, "moss_paged_qk_rope", at, stride, *norms, q.data_ptr(), c.k, c.v, c.ks, c.vs, c.pages, c.rows,
-                   table_at, table_stride, lengths_at, starts_at, b, w, tokens, qh, kh, d, eps, _TYPES[dtype])
+    native.call_on(qkv, "moss_paged_qk_rope" + c.native_name, at, stride, *norms, q.data_ptr(), *c.args(), table_at,
+                   table_stride, lengths_at, starts_at, b, w, tokens, qh, kh, d, eps, _TYPES[dtype])
     return q
+
+
+def gather(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor,
+           tokens: int, *, dtype: torch.dtype | None = None, out: tuple[torch.Tensor, torch.Tensor] | None = None,
+           scales: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached rows of ``tokens`` packed tokens in order: ``(keys, values)``, each ``[tokens, KV heads, head dim]``.
+
+    ``starts`` names each sequence's newest rows, as elsewhere; with the running sums of ``lengths`` they are all of its
+    rows.  From a cache in 8 bits the values that it stands for, in ``dtype`` (bf16 unless it or ``out`` says fp16).  A token
+    without a position or a page gives zeros; rows from ``starts[B]`` on are left as they are."""
+    _require(isinstance(keys, torch.Tensor) and keys.get_device() >= 0, "keys must be a CUDA (HIP) tensor")
+    index = keys.get_device()
+    if out is not None:
+        _require(isinstance(out, (tuple, list)) and len(out) == 2 and all(isinstance(t, torch.Tensor) for t in out),
+                 "out must be a pair of tensors")
+    if dtype is None:
+        dtype = keys.dtype if scales is None else torch.bfloat16 if out is None else out[0].dtype
+    _require(scales is not None or keys.dtype in _TYPES, "keys must be a bf16 or fp16 tensor, or come with scales")
+    _require(dtype in _TYPES and (scales is not None or dtype == keys.dtype), "dtype must be bf16 or fp16, a 16-bit cache's own")
+    c = _cache_of(keys, values, scales, dtype, index)
+    _require(starts is not None, "starts required")
+    b, w, table_stride, table_at, lengths_at, starts_at = batch = _batch(table, lengths, starts, c.rows, index)
+    _require(isinstance(tokens, int) and 0 < tokens < 1 << 24, "tokens must be a whole number below 2^24")
+    shape = (tokens, c.kh, c.d)
+    if out is None:
+        k, v = (torch.empty(shape, dtype=dtype, device=keys.device) for _ in range(2))
+    else:
+        spans = *c.spans(), *_batch_spans(*batch)
+        k, v = out
+        for name, t in (("out[0]", k), ("out[1]", v)):
+            _cuda_contig(name, t, dtype, keys.device)
+            _require(t.shape == shape, f"{name} must be {' x '.join(map(str, shape))}")
+            _require(_aligned(t, 16), f"{name} must be 16-byte aligned")
+            _apart(name, t, *spans)
+        _apart("out[1]", v, (k.data_ptr(), k.data_ptr() + 2 * k.numel()))
+    native.call_on(keys, "moss_paged_gather" + c.native_name, *c.args(), table_at, table_stride, lengths_at, starts_at, b, w,
+                   tokens, c.kh, c.d, k.data_ptr(), v.data_ptr(), _TYPES[dtype])
+    return k, v
 
 
 def decode_workspace(q: torch.Tensor, keys: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
@@ -264,23 +409,24 @@ def decode_workspace(q: torch.Tensor, keys: torch.Tensor, table: torch.Tensor) -
 
 def decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor,
                      lengths: torch.Tensor, *, scale: float | None = None, out: torch.Tensor | None = None,
-                     ws: torch.Tensor | None = None) -> torch.Tensor:
+                     ws: torch.Tensor | None = None,
+                     scales: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """One new token per sequence: ``q`` ``[B, query heads, head dim]`` (rows may lie apart) against the
     ``lengths[b]`` rows of each sequence, the new token's own among them; ``scale`` defaults to head dim ** -0.5.
     Returns ``[B, query heads * head dim]``; a sequence without rows gives zeros."""
     n, qh, hd, stride, index = _query(q)
-    c = _Cache(keys, values, q.dtype, index)
+    c = _cache_of(keys, values, scales, q.dtype, index)
     kh, d = c.kh, c.d
     b, w, table_stride, table_at, lengths_at, _ = batch = _batch(table, lengths, None, c.rows, index)
     _require(n == b and hd == d and qh % kh == 0 and qh <= 1024, "q must be [B, a multiple of the KV heads, head dim]")
     at = q.data_ptr()
     spans = ()
     if out is not None or ws is not None:
-        spans = (at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend), *_batch_spans(*batch)
+        spans = (at, at + 2 * ((n - 1) * stride + qh * d)), *c.spans(), *_batch_spans(*batch)
     out = _output(out, (b, qh * d), q, index, spans)
     nbytes = native.lib().moss_paged_decode_workspace_bytes(b, w, c.rows, qh, kh, d)
     ws = _workspace(ws, nbytes, q, out, spans)
-    native.call_on(q, "moss_paged_decode_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table_at,
+    native.call_on(q, "moss_paged_decode_attention" + c.native_name, at, stride, *c.args(), table_at,
                    table_stride, lengths_at, b, w, qh, kh, d, _scale(scale, d), out.data_ptr(), ws.data_ptr(),
                    nbytes, _TYPES[q.dtype])
     return out
@@ -296,13 +442,14 @@ def prompt_workspace(q: torch.Tensor, keys: torch.Tensor, table: torch.Tensor) -
 
 def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor,
                      lengths: torch.Tensor, starts: torch.Tensor, *, scale: float | None = None,
-                     out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+                     scales: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """Causal attention of packed new tokens whose K and V rows are in the pages already: ``q`` ``[T, query heads,
     head dim]`` (rows may lie apart); each token attends its sequence's rows up to its own position, the cached
     ones before the new among them.  ``scale`` defaults to head dim ** -0.5.  Returns ``[T, query heads * head
     dim]``; a token without a visible row gives zeros."""
     n, qh, hd, stride, index = _query(q)
-    c = _Cache(keys, values, q.dtype, index)
+    c = _cache_of(keys, values, scales, q.dtype, index)
     kh, d = c.kh, c.d
     _require(starts is not None, "starts required")
     b, w, table_stride, table_at, lengths_at, starts_at = batch = _batch(table, lengths, starts, c.rows, index)
@@ -311,11 +458,11 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     at = q.data_ptr()
     spans = ()
     if out is not None or ws is not None:
-        spans = (at, at + 2 * ((n - 1) * stride + qh * d)), (c.k, c.kend), (c.v, c.vend), *_batch_spans(*batch)
+        spans = (at, at + 2 * ((n - 1) * stride + qh * d)), *c.spans(), *_batch_spans(*batch)
     out = _output(out, (n, qh * d), q, index, spans)
     nbytes = native.lib().moss_paged_prompt_workspace_bytes(b, w, c.rows, n, qh, kh, d)
     ws = _workspace(ws, nbytes, q, out, spans)
-    native.call_on(q, "moss_paged_prompt_attention", at, stride, c.k, c.v, c.ks, c.vs, c.pages, c.rows, table_at,
+    native.call_on(q, "moss_paged_prompt_attention" + c.native_name, at, stride, *c.args(), table_at,
                    table_stride, lengths_at, starts_at, b, w, n, qh, kh, d, _scale(scale, d),
                    out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _TYPES[q.dtype])
     return out

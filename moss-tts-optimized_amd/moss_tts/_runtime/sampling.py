@@ -12,6 +12,8 @@ captured in one graph (``src/moss_tts/_runtime/first_audio_graph.py:14-29``).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import native
@@ -174,6 +176,103 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     native.call_on(logits, "moss_sample_rows", logits.data_ptr(), _SAMPLE_TYPES[logits.dtype], rows, stride, vocab,
                    uniform.data_ptr(), t_ptr, float(t), k_ptr, int(k), p_ptr, float(p), m_ptr, float(m), out.data_ptr(),
                    None if ws is None else ws.data_ptr(), 0 if ws is None else 4 * ws.numel())
+    return out
+
+
+def _strided(name: str, t: torch.Tensor, dtypes, rows: int, device):
+    """(pointer, row stride, (first, end)) of a checked [rows, n] tensor whose rows are contiguous, or one row for all."""
+    _require(isinstance(t, torch.Tensor) and t.dtype in dtypes and t.device == device and t.dim() == 2
+             and t.shape[0] in (1, rows) and t.shape[1] > 0,
+             f"{name} must be [rows, n] or [1, n], of {' or '.join(str(d) for d in dtypes)}, on {device}")
+    n = t.shape[1]
+    _require(n == 1 or t.stride(1) == 1, f"a row of {name} must be contiguous")
+    stride = t.stride(0) if t.shape[0] > 1 else 0
+    _require(stride == 0 or stride >= n, f"{name}: rows must not overlap")
+    at = t.data_ptr()
+    return at, stride, (at, at + ((rows - 1) * stride + n) * t.element_size())
+
+
+def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+           prompt: torch.Tensor | None = None, repetition: float | torch.Tensor = 1.0, presence: float | torch.Tensor = 0.0,
+           frequency: float | torch.Tensor = 0.0, bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+           mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 / fp16 / fp32 logits ``[rows, entries]`` (rows any stride apart) with penalties for the tokens said so far, biases
+    and a mask, for :func:`sample`; in the logits' type, from fp32 with one rounding.
+
+    ``tokens`` int64 or int32 ``[rows, width]`` (any strides, so ``ids.T`` of a ``[width, rows]`` history serves): the first
+    ``lengths`` (int32 ``[rows]``; None: all) of a row are its history, of which the first ``prompt`` (int32 ``[rows]``; None:
+    none) are the prompt.  A token of the history divides its logit, where that is positive, by ``repetition`` (> 0) and
+    multiplies it by that elsewhere; one said c > 0 times behind the prompt then loses ``c * frequency + presence``.
+    ``bias`` fp32 and ``bias_ids`` int32, each ``[rows, n]`` or ``[1, n]``: what is added to the entries named; of ids that
+    come twice in a row the last holds.  ``mask`` int32 ``[rows or 1, at least ceil(entries / 32)]``: entry v stays where
+    bit v % 32 of word v // 32 is 1 and becomes ``-inf`` elsewhere.  Tokens and ids outside the row are left out.  Each of the
+    penalties is a number, or an fp32 tensor with one value a row; all are read when the kernel runs.  ``out``: a tensor of
+    the logits' shape, or the logits themselves; it may share memory with nothing else."""
+    _require(isinstance(logits, torch.Tensor) and logits.dtype in _SAMPLE_TYPES, "logits must be a bf16, fp16 or fp32 tensor")
+    _require(logits.is_cuda, "logits must be a CUDA (HIP) tensor")
+    _require(logits.dim() == 2 and logits.shape[0] > 0 and logits.shape[1] > 0, "logits must be [rows, entries]")
+    rows, entries = logits.shape
+    _require(rows <= MAX_SAMPLE_ROWS and entries <= MAX_SAMPLE_VOCAB,
+             f"at most {MAX_SAMPLE_ROWS} rows of {MAX_SAMPLE_VOCAB} entries")
+    _require(entries == 1 or logits.stride(1) == 1, "a row's logits must be contiguous")
+    stride = logits.stride(0) if rows > 1 else entries
+    _require(stride >= entries, "rows must not overlap")
+    dev, size = logits.device, logits.element_size()
+    spans = []
+    history = [None, 8, 0, 0, 0, None, None]
+    if tokens is not None:
+        _require(isinstance(tokens, torch.Tensor) and tokens.dtype in (torch.int64, torch.int32) and tokens.device == dev
+                 and tokens.dim() == 2 and tokens.shape[0] == rows and 0 < tokens.shape[1] < 1 << 31,
+                 f"tokens must be int64 or int32 [rows, width] on {dev}")
+        wide, width = tokens.element_size(), tokens.shape[1]
+        history[:5] = tokens.data_ptr(), wide, tokens.stride(0), tokens.stride(1), width
+        spans.append((history[0], history[0] + wide * ((rows - 1) * history[2] + (width - 1) * history[3] + 1)))
+    for i, (name, t) in enumerate((("lengths", lengths), ("prompt", prompt))):
+        if t is not None:
+            _require(tokens is not None, f"{name} without tokens")
+            _cuda_contig(name, t, torch.int32, dev)
+            _require(t.numel() == rows, f"{name} must hold one value a row")
+            history[5 + i] = t.data_ptr()
+            spans.append((t.data_ptr(), t.data_ptr() + 4 * rows))
+    settings = []
+    for name, value, none in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
+        _require(tokens is not None or (not isinstance(value, torch.Tensor) and value == none), f"{name} without tokens")
+        at, v = _setting(name, value, rows, torch.float32, dev)
+        _require(at is not None or abs(v) < math.inf, f"{name} must be finite")
+        settings += at, float(v)
+        if at is not None:
+            spans.append((at, at + 4 * rows))
+    _require(settings[0] is not None or settings[1] > 0, "repetition must be positive")
+    biases = [None, 0, None, 0, 0]
+    _require((bias is None) == (bias_ids is None), "bias and bias_ids go together")
+    if bias is not None:
+        ids_at, ids_stride, span = _strided("bias_ids", bias_ids, (torch.int32,), rows, dev)
+        at, bias_stride, other = _strided("bias", bias, (torch.float32,), rows, dev)
+        _require(bias.shape[1] == bias_ids.shape[1] < 1 << 16, "as many biases as ids required, fewer than 65536")
+        biases = [ids_at, ids_stride, at, bias_stride, bias.shape[1]]
+        spans += span, other
+    mask_at, mask_stride = None, 0
+    if mask is not None:
+        mask_at, mask_stride, span = _strided("mask", mask, (torch.int32,), rows, dev)
+        _require(32 * mask.shape[1] >= entries, "mask must hold a bit for every entry")
+        spans.append(span)
+    if out is None:
+        out = torch.empty((rows, entries), dtype=logits.dtype, device=dev)
+        out_stride = entries
+    else:
+        _require(isinstance(out, torch.Tensor) and out.dtype == logits.dtype and out.device == dev and out.shape == logits.shape,
+                 "out must have the logits' type, shape and device")
+        _require(entries == 1 or out.stride(1) == 1, "a row of out must be contiguous")
+        out_stride = out.stride(0) if rows > 1 else entries
+        _require(out_stride >= entries, "rows must not overlap")
+        first, end = out.data_ptr(), out.data_ptr() + ((rows - 1) * out_stride + entries) * size
+        at = logits.data_ptr()
+        if first != at or out_stride != stride:
+            spans.append((at, at + ((rows - 1) * stride + entries) * size))
+        for a, z in spans:
+            _require(end <= a or z <= first, "out must not overlap the other tensors")
+    native.call_on(logits, "moss_adjust_rows", logits.data_ptr(), _SAMPLE_TYPES[logits.dtype], rows, stride, entries, *history,
+                   *settings, *biases, mask_at, mask_stride, out.data_ptr(), out_stride)
     return out
 
 

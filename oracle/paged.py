@@ -117,3 +117,67 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
     near = min(near, np.abs(through - goal).min() / through[-1])
     drawn = int((through <= goal).sum())
     return (drawn if drawn < len(x) else int(np.nonzero(kept)[0][-1])), near
+
+
+#: exponents that the scale of an 8-bit row may take, by the 16-bit type that its values stay exact in
+EXPONENTS = {"bf16": (-100, 120), "fp16": (-15, 8)}
+
+
+def quantize_row(x, kind):
+    """(values that the cache holds, scale byte) of one row; NaN where ``x`` is not finite."""
+    low, high = EXPONENTS[kind]
+    fine = np.isfinite(x)
+    top = np.abs(x[fine]).max() if fine.any() else 0.0
+    e = low if top == 0 else min(max(math.ceil(math.log2(top / 448)), low), high)
+    if e > low and top <= 448 * 2.0 ** (e - 1):  # log2 is rounded
+        e -= 1
+    most = (240 if e == high else 448) * 2.0 ** e
+    y = np.clip(np.where(fine, x, 0.0), -most, most)
+    with np.errstate(divide="ignore"):
+        step = 2.0 ** (np.maximum(np.floor(np.log2(np.abs(y))), e - 6) - 3)
+    return np.where(fine, np.round(y / step) * step, np.nan), e + 127
+
+
+def cache_values(codes, scales):
+    """float64 values of e4m3 codes (uint8 ``[.., D]``) and scale bytes ``[..]``."""
+    codes = codes.astype(np.int64)
+    exponent, mantissa = codes >> 3 & 15, codes & 7
+    x = np.where(exponent > 0, (8 + mantissa) * 2.0 ** (exponent - 10), mantissa * 2.0 ** -9)
+    x = np.where((codes & 127) == 127, np.nan, np.where(codes & 128, -x, x))
+    return x * 2.0 ** (scales.astype(np.float64) - 127)[..., None]
+
+
+def gather(pages, table, lengths, starts, before):
+    """The packed rows of ``[n, KH, P, D]`` pages; ``before``: what the output held."""
+    p, out = pages.shape[2], before.copy()
+    for i in range(len(table)):
+        count = starts[i + 1] - starts[i]
+        length = min(max(int(lengths[i]), 0), len(table[i]) * p)
+        for t in range(count):
+            position = length - count + t
+            page = table[i, position // p] if position >= 0 else -1
+            out[starts[i] + t] = pages[page, :, position % p] if 0 <= page < len(pages) else 0.0
+    return out
+
+
+def adjust(logits, tokens, prompt, repetition, presence, frequency, pairs, words):
+    """One row: its tokens so far, how many of them are the prompt, (id, bias) pairs, mask words (None: none)."""
+    x = logits.astype(np.float64).copy()
+    n = len(x)
+    said = {int(t) for t in tokens if 0 <= t < n}
+    count = {}
+    for t in tokens[max(prompt, 0):]:
+        count[int(t)] = count.get(int(t), 0) + 1
+    with np.errstate(invalid="ignore"):
+        for t in said:
+            x[t] = x[t] / repetition if x[t] > 0 else x[t] * repetition
+            if t in count:
+                x[t] -= count[t] * frequency + presence
+        for t, b in dict(pairs).items():
+            if 0 <= t < n:
+                x[t] += b
+    if words is not None:
+        for v in range(n):
+            if not int(words[v // 32]) >> (v % 32) & 1:
+                x[v] = -np.inf
+    return x

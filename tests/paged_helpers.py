@@ -88,3 +88,39 @@ def attend_all(q, keys, vals, table, lengths, starts, before, scale):
             y = torch.matmul(e, v) / torch.where(total == 0, torch.ones_like(total), total)
             out[first:first + n, h * group:(h + 1) * group] = y.view(n, group, d)
     return out.view(before.shape)
+
+
+def cache8(dev, g, lengths, *, kh, d, page, spare=3, width=None, interleaved=False):
+    """(keys, values, scales, table, lengths) of a cache in 8 bits: rows of different sizes where a sequence has them,
+    e4m3's NaN and bytes that are no scale everywhere else."""
+    counts = [-(-n // page) for n in lengths]
+    pages = sum(counts) + spare
+    width = max(max(counts), 1) + 1 if width is None else width
+    order = torch.randperm(pages, generator=g)[:sum(counts)].tolist()
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    both = torch.full((pages, 2, kh, page, d), 0x7f, dtype=torch.uint8)
+    bytes_ = torch.where(torch.rand((pages, 2, kh, page), generator=g) < 0.5, 255, 0).to(torch.uint8)
+    at = 0
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        table[b, :c] = torch.tensor(order[at:at + c], dtype=torch.int32)
+        for j in range(c):
+            m = min(page, n - j * page)
+            both[order[at + j], :, :, :m] = (torch.randn((2, kh, m, d), generator=g) * 100).clamp(-448, 448).to(
+                torch.float8_e4m3fn).view(torch.uint8)
+            bytes_[order[at + j], :, :, :m] = torch.randint(118, 123, (2, kh, m), generator=g).to(torch.uint8)
+        at += c
+    if not interleaved:
+        both, bytes_ = both.transpose(0, 1).contiguous().transpose(0, 1), bytes_.transpose(0, 1).contiguous().transpose(0, 1)
+        keys, vals, ks, vs = (t.contiguous().to(dev) for t in (both[:, 0], both[:, 1], bytes_[:, 0], bytes_[:, 1]))
+    else:
+        both, bytes_ = both.to(dev), bytes_.to(dev)
+        keys, vals, ks, vs = both[:, 0], both[:, 1], bytes_[:, 0], bytes_[:, 1]
+    return keys.view(torch.float8_e4m3fn), vals.view(torch.float8_e4m3fn), (ks, vs), table.to(dev), torch.tensor(
+        lengths, dtype=torch.int32, device=dev)
+
+
+def cache8_values(codes, scales):
+    """What an 8-bit cache holds, as float64."""
+    from oracle import paged as o
+
+    return o.cache_values(codes.view(torch.uint8).cpu().numpy(), scales.cpu().numpy())
