@@ -519,6 +519,13 @@ int moss_paged_decode_attention_fp8(const void *q, long long q_stride, const voi
                                     int kh, int d, float scale, void *out, void *workspace, long long workspace_bytes,
                                     int dtype, void *stream);
 
+int moss_paged_prompt_attention_fp8(const void *q, long long q_stride, const void *k, const void *v, const void *k_scales,
+                                    const void *v_scales, long long k_stride, long long v_stride,
+                                    long long k_scale_stride, long long v_scale_stride, int pages, int page_rows,
+                                    const void *table, long long table_stride, const void *lengths, const void *starts,
+                                    int B, int W, int T, int qh, int kh, int d, float scale, void *out, void *workspace,
+                                    long long workspace_bytes, int dtype, void *stream);
+
 /* The K and V rows of T packed tokens (T < 2^24) in order, k_out and v_out [T, kh, d] of the given dtype: a copy from a 16-bit
  * cache, the values that the codes stand for from one in 8 bits.  A token without a position or a page gives zeros. */
 int moss_paged_gather(const void *k, const void *v, long long k_stride, long long v_stride, int pages, int page_rows,

@@ -90,6 +90,8 @@ SIGNATURES: dict[str, list] = {
     "moss_paged_gather_fp8": [_P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P],
     "moss_paged_decode_attention_fp8": [_P, _L, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _F,
                                         _P, _P, _L, _I, _P],
+    "moss_paged_prompt_attention_fp8": [_P, _L, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I,
+                                        _F, _P, _P, _L, _I, _P],
     "moss_adjust_rows": [_P, _I, _I, _L, _I, _P, _I, _L, _L, _I, _P, _P, _P, _F, _P, _F, _P, _F, _P, _L, _P, _L, _I, _P, _L,
                          _P, _L, _P],
     "moss_stream_read_words": [ctypes.c_longlong],

@@ -57,3 +57,12 @@ def test_adjust_rows(lib):  # noqa: F811
                 dict(bias_ids_stride=3), dict(mask=H), dict(mask_stride=156),
                 dict(rows=1 << 21, vocab=1 << 19, stride=1 << 19, out_stride=1 << 19, mask_stride=0)]:
         assert call(**bad) == 1, bad
+
+
+def test_prompt_attention(lib):  # noqa: F811
+    call = Call(lib.moss_paged_prompt_attention_fp8, q=P, q_stride=4096, **CACHE8, **BATCH, starts=P, B=3, W=4, T=50, qh=32, kh=8, d=128,
+                scale=F(0.1), out=P, workspace=NULL, workspace_bytes=0, dtype=0, stream=NULL)
+    for bad in BAD_CACHE8 + [dict(q=NULL), dict(q=ODD), dict(q_stride=4088), dict(q_stride=4100), dict(scale=F(float("nan"))),
+                             dict(out=NULL), dict(out=ODD), dict(starts=NULL), dict(T=0), dict(T=(1 << 20) + 1), dict(workspace=ODD),
+                             dict(W=100, table_stride=100)]:
+        assert call(**bad) == 1, bad

@@ -329,3 +329,96 @@ def test_captured(dev):
         torch.cuda.synchronize()
         assert torch.equal(step(*mirror), out), i
         assert torch.equal(mirror[0].view(torch.uint8), keys.view(torch.uint8)) and torch.equal(mirror[2][1], scales[1])
+
+
+def _prompt(dev, new, old, layout, dtype, page, *, seed=0, pad=0, edit=None, stride=0, scale=None, interleaved=False):
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(seed)
+    qh, kh, d = layout
+    lengths = [a + b for a, b in zip(new, old)]
+    keys, vals, scales, table, lens = cache8(dev, g, lengths, kh=kh, d=d, page=page, interleaved=interleaved)
+    if edit is not None:
+        table, lens = edit(table.cpu(), lens.cpu())
+        table, lens = table.to(dev), lens.to(dev)
+    starts = torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device=dev)
+    total = sum(new) + pad
+    wide = (torch.randn((total, qh * d + stride), generator=g) * 1.5).to(dtype).to(dev)
+    q = wide[:, :qh * d].unflatten(1, (qh, d))
+    out = torch.full((total, qh * d), 7.0, dtype=dtype, device=dev)
+    before = values(out)
+    print(f"prompt8 new={new} old={old} layout={layout} {dtype} page={page}", flush=True)
+    assert paged.prompt_attention(q, keys, vals, table, lens, starts, scale=scale, out=out, scales=scales) is out
+    torch.cuda.synchronize()
+    args = values(q), cache8_values(keys, scales[0]), cache8_values(vals, scales[1])
+    rest = table.cpu().numpy(), lens.cpu().numpy(), starts.cpu().numpy(), before, scale
+    ref = o.prompt_attention(*args, *rest)
+    ref_abs = o.prompt_attention(args[0], args[1], np.abs(args[2]), *rest)
+    bound = attention_bound(args[0], *(np.where(np.abs(a) < 1e6, a, 0.0) for a in args[1:]), ref, ref_abs,
+                            d ** -0.5 if scale is None else scale, dtype, True)
+    _close(out, ref, bound, "prompt8")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_prompt_layouts(dev, layout, dtype):
+    _prompt(dev, [33, 1, 0, 70], [0, 9, 5, 40], layout, dtype, 16, pad=5)
+
+
+@pytest.mark.parametrize("page", [16, 64, 512])
+@pytest.mark.parametrize("new, old", [([1], [0]), ([1], [130]), ([31, 32, 33, 63, 64, 65], [0] * 6), ([5, 129], [300, 64]),
+                                      ([2, 3, 1, 1, 200], [500, 0, 0, 77, 1])])
+def test_prompt_lengths(dev, new, old, page):
+    _prompt(dev, new, old, (8, 2, 128), torch.bfloat16, page)
+
+
+@pytest.mark.parametrize("layout, dtype", [((32, 8, 128), torch.bfloat16), ((32, 8, 128), torch.float16),
+                                           ((28, 4, 128), torch.bfloat16), ((36, 12, 64), torch.bfloat16)])
+def test_prompt_large(dev, layout, dtype):
+    """Enough rows for the large tiles, with ends inside tiles and blocks."""
+    _prompt(dev, [421, 77, 203], [0, 150, 9], layout, dtype, 32, pad=3)
+
+
+def test_prompt_many_sequences_strides_and_scale(dev):
+    rng = np.random.default_rng(4)
+    new = [int(n) for n in rng.integers(0, 6, 140)]
+    new[0] = new[64] = new[139] = 0
+    _prompt(dev, new, [int(n) for n in rng.integers(0, 40, 140)], (4, 2, 64), torch.bfloat16, 16)
+    _prompt(dev, [40, 3, 20], [0, 8, 100], (8, 4, 128), torch.bfloat16, 32, stride=512, interleaved=True)
+    _prompt(dev, [40, 3, 20], [0, 8, 100], (8, 4, 64), torch.float16, 32, scale=-0.4)
+
+
+def test_prompt_rows_without_keys(dev):
+    def edit(table, lens):
+        table[0, 1] = -1
+        table[1, :] = 10 ** 9
+        table[2, 0] = -3
+        lens[3] = 12
+        lens[4] = -4
+        return table, lens
+
+    _prompt(dev, [20, 10, 70, 30, 5], [60, 20, 0, 0, 0], (8, 2, 128), torch.bfloat16, 16, edit=edit)
+    _prompt(dev, [300, 290, 170, 200, 90], [60, 20, 0, 0, 0], (32, 8, 128), torch.bfloat16, 16, edit=edit)
+
+
+@pytest.mark.parametrize("tokens", [90, 700])
+def test_prompt_values_behind_a_token(dev, tokens):
+    """A row of NaN reaches the tokens at and behind it, and none before it."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(9)
+    qh, kh, d, bad = 32, 8, 128, 37
+    keys, vals, scales, table, lens = cache8(dev, g, [tokens], kh=kh, d=d, page=16)
+    q = torch.randn((tokens, qh, d), generator=g).bfloat16().to(dev)
+    starts = torch.tensor([0, tokens], dtype=torch.int32, device=dev)
+    vals.view(torch.uint8)[int(table[0, bad // 16]), :, bad % 16] = 0x7f
+    got = paged.prompt_attention(q, keys, vals, table, lens, starts, scales=scales)
+    assert torch.isnan(got[bad:]).all()
+    args = values(q), cache8_values(keys, scales[0]), cache8_values(vals, scales[1])
+    table_, lens_ = table.cpu().numpy(), np.array([bad])
+    first = np.array([0, bad])
+    before = np.zeros((bad, qh * d))
+    ref = o.prompt_attention(args[0][:bad], *args[1:], table_, lens_, first, before)
+    ref_abs = o.prompt_attention(args[0][:bad], args[1], np.abs(args[2]), table_, lens_, first, before)
+    bound = attention_bound(args[0], *(np.where(np.abs(a) < 1e6, a, 0.0) for a in args[1:]), ref, ref_abs, d ** -0.5, torch.bfloat16, True)
+    _close(got[:bad], ref, bound, "before the row")
