@@ -536,6 +536,26 @@ int moss_paged_gather_fp8(const void *k, const void *v, const void *k_scales, co
                           const void *table, long long table_stride, const void *lengths, const void *starts, int B, int W,
                           int T, int kh, int d, void *k_out, void *v_out, int dtype, void *stream);
 
+/* moss_paged_decode_attention for sequences that share the first rows of their caches.  groups, shared int32 [B], read on the
+ * device like lengths: neighbouring sequences with the same group number, not below 0, are a run, which a multiple of 64 in
+ * the batch ends too; the first min(shared[b], the first one's shared and length) rows of each of its sequences, whole 16
+ * rows, are the ones that the first sequence's table names, and are read once for all of the run.  Rows beyond, and a sequence
+ * alone, take their own table's.  Where every table names the shared pages too, the result is moss_paged_decode_attention's
+ * up to rounding, whatever groups and shared hold. */
+long long moss_paged_shared_workspace_bytes(int B, int W, int page_rows, int qh, int kh, int d);
+int moss_paged_shared_decode_attention(const void *q, long long q_stride, const void *k, const void *v, long long k_stride,
+                                       long long v_stride, int pages, int page_rows, const void *table,
+                                       long long table_stride, const void *lengths, const void *groups, const void *shared,
+                                       int B, int W, int qh, int kh, int d, float scale, void *out, void *workspace,
+                                       long long workspace_bytes, int dtype, void *stream);
+int moss_paged_shared_decode_attention_fp8(const void *q, long long q_stride, const void *k, const void *v,
+                                           const void *k_scales, const void *v_scales, long long k_stride,
+                                           long long v_stride, long long k_scale_stride, long long v_scale_stride, int pages,
+                                           int page_rows, const void *table, long long table_stride, const void *lengths,
+                                           const void *groups, const void *shared, int B, int W, int qh, int kh, int d,
+                                           float scale, void *out, void *workspace, long long workspace_bytes, int dtype,
+                                           void *stream);
+
 /* ------------------------------------------------------- measurement */
 /* No counterpart in the reference: a streaming read for bench.py, which times it on the bytes of a
  * decode GEMV to measure the ceiling of one launch that only reads those bytes.  Reads `bytes` (a

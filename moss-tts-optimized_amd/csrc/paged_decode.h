@@ -19,6 +19,17 @@
 
 namespace moss {
 
+// Workgroups that the work is shared out over.  512 / 1024 / 1536 / 2048: 273 / 265 / 261 / 263 us for 64 sequences of 4 to 8
+// thousand rows of 8 heads, 25.9 / 24.3 / 24.1 / 24.1 for 48 of up to 2000 rows of 12 heads of 64 (six caches in turn), 109 / 99 /
+// 97 / 98 for 128 of 300 to 2000 rows, no difference for 16 sequences.
+constexpr int kTarget = 1536;
+// Pages of more than the last-level cache (256 MB) are read past it.  The pages that the call can name decide, since the host
+// does not know the lengths: with a server's pool that is nearly every call, of few rows too, and right for it, as what one
+// layer's call reads is gone by the time of the next step's.  To / past the cache: 287 / 261 us for those 64 sequences (1.6 GB),
+// 103 / 96 for 128 and 192 / 183 for 256 of 300 to 2000 rows; 16 sequences with 58 MB, 36 layers' caches in turn, 19.8 / 19.3, one
+// of 509 rows 9.0 / 8.8; but one cache read again and again, which stays: 16.7 / 17.5, four such 17.0 / 18.6.
+constexpr long long kCached = 256ll << 20;
+
 struct DecodeArgs {
     const uint16_t* q;
     long long q_stride;
@@ -28,6 +39,7 @@ struct DecodeArgs {
     int qh, group, xdim, shares;  // xdim: head tiles; shares: workgroups per head tile that the units are shared out over
     long long slots;
     float scale;            // scale log2(e)
+    uint32_t flip;          // its sign where `scale` is without one, for the two values of a word of q
 };
 
 // K or V of a row: 16 bytes or 8, past the last-level cache (NT) or through it.
@@ -156,7 +168,7 @@ __device__ __forceinline__ void decode_share(const DecodeArgs& a, const typename
 #pragma unroll
     for (int i = 0; i < T::NC; ++i) {
         qf[i] = *reinterpret_cast<const u32x4_t*>(qr + T::q_dim(i, g));
-        if (r >= heads) qf[i] = u32x4_t{0u, 0u, 0u, 0u};
+        qf[i] = r < heads ? qf[i] ^ a.flip : u32x4_t{0u, 0u, 0u, 0u};
     }
     f32x4_v o[NJ];
 #pragma unroll

@@ -18,17 +18,6 @@
 namespace moss {
 namespace {
 
-// Workgroups that the work is shared out over.  512 / 1024 / 1536 / 2048: 273 / 265 / 261 / 263 us for 64 sequences of 4 to 8
-// thousand rows of 8 heads, 25.9 / 24.3 / 24.1 / 24.1 for 48 of up to 2000 rows of 12 heads of 64 (six caches in turn), 109 / 99 /
-// 97 / 98 for 128 of 300 to 2000 rows, no difference for 16 sequences.
-constexpr int kTarget = 1536;
-// Pages of more than the last-level cache (256 MB) are read past it.  The pages that the call can name decide, since the host
-// does not know the lengths: with a server's pool that is nearly every call, of few rows too, and right for it, as what one
-// layer's call reads is gone by the time of the next step's.  To / past the cache: 287 / 261 us for those 64 sequences (1.6 GB),
-// 103 / 96 for 128 and 192 / 183 for 256 of 300 to 2000 rows; 16 sequences with 58 MB, 36 layers' caches in turn, 19.8 / 19.3, one
-// of 509 rows 9.0 / 8.8; but one cache read again and again, which stays: 16.7 / 17.5, four such 17.0 / 18.6.
-constexpr long long kCached = 256ll << 20;
-
 // A share's size in units (at most 65535 sequences of 2^23 units).
 __device__ __forceinline__ int share_units(const PagedBatch& bt, int shift, int shares, int lane) {
     long long total = 0;
@@ -173,7 +162,7 @@ int decode(const void* q, long long q_stride, const Cache& c, const PagedBatch& 
     MOSS_CHECK_ARG(workspace_bytes >= p.slots * qh * (d + 2) * 4 && p.slots * p.xdim * 256 < (1ll << 32));
     DecodeArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, (float*)workspace,
                  reinterpret_cast<float2*>((float*)workspace + p.slots * qh * d), qh, qh / c.kh, p.xdim, p.shares, p.slots,
-                 scale * 1.4426950408889634f};
+                 scale * 1.4426950408889634f, 0u};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == 0)
         d == 128 ? launch_decode<Bf16, 128, T<Bf16, 128>>(a, c, bt, p, st) : launch_decode<Bf16, 64, T<Bf16, 64>>(a, c, bt, p, st);

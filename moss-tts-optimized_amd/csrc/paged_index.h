@@ -128,6 +128,27 @@ MOSS_HD bool is_item(const PromptTiles& t, int share, const PromptItem& it) {
 // Partial results first .. first + count - 1 lie in a workspace of `slots` (lengths that change between the launches can name
 // others).
 MOSS_HD bool in_slots(int first, int count, long long slots) { return first >= 0 && count >= 0 && (long long)first + count <= slots; }
+// Shared prefixes (paged_shared.hip).  The rows that a run of sequences shares, whose first one has `length` and shares `want`; where
+// a sequence's own rows begin: behind those, in whole 16 rows (which a page holds all of), or nowhere.
+MOSS_HD int shared_rows(int want, int length) { return (want < length ? want : length) & ~15; }
+MOSS_HD int shared_from(int rows, int want, int length) {
+    const int most = want < rows ? want : rows;
+    return length <= most ? length : most & ~15;
+}
+// Blocks of a part of a tile's keys: the tiles' blocks, `total` of them, in at most `shares` parts and one more a tile.
+constexpr int kPrefixShare = 2;
+MOSS_HD int prefix_share_of(long long total, int shares) {
+    const long long share = (total + shares - 1) / shares;
+    return share < kPrefixShare ? kPrefixShare : share < (1 << 24) ? (int)share : 1 << 24;
+}
+// At most: parts of all tiles, and rows of partial results.  A run has at least two sequences, so there are at most B / 2, and its
+// tiles are size * group / height rounded up; a run's parts hold its rows each, and beyond the first part of each tile the parts
+// are whole shares, so at most `shares` tiles' rows.
+inline void prefix_bounds(int B, int group, int height, int shares, long long& items, long long& rows) {
+    const long long all = (long long)B * group;
+    items = B > 1 ? (all + height - 1) / height + B / 2 + shares : 1;
+    rows = B > 1 ? all + (long long)height * shares : 1;
+}
 inline long long decode_slots(int B, int W, int shift, int shares) {
     const long long most = (long long)B * ((((long long)W << shift) + kUnit - 1) / kUnit);
     return (long long)B + shares < most ? (long long)B + shares : most;

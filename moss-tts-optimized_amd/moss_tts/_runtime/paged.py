@@ -432,6 +432,47 @@ def decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     return out
 
 
+def shared_decode_workspace(q: torch.Tensor, keys: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
+    """A workspace for :func:`shared_decode_attention` calls of these shapes; calls that may overlap need one each."""
+    nbytes = native.lib().moss_paged_shared_workspace_bytes(table.shape[0], table.shape[1], keys.shape[2], q.shape[1],
+                                                            keys.shape[1], keys.shape[3])
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+
+
+def shared_decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor,
+                            lengths: torch.Tensor, groups: torch.Tensor, shared: torch.Tensor, *, scale: float | None = None,
+                            out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+                            scales: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """:func:`decode_attention` of sequences that share a prefix, which is read and multiplied once for all of them.
+
+    ``groups`` int32 ``[B]``: neighbours with the same number, not below 0, share; negative: alone.  ``shared`` int32 ``[B]``:
+    the first rows of a sequence that are those of its run's first one (at most that one's own ``shared`` and length).
+    They are read through the first sequence's table, rounded down to whole 16 rows; every sequence's own table names
+    its pages as well.  Both are device values like ``lengths``: whatever they hold, no access leaves the cache, and as long
+    as the tables agree on the shared rows, they change the time and not the result (beyond rounding).  A run ends at
+    every 64th sequence of the batch, and the prefix's weights are rounded to 16 bits, as :func:`prompt_attention` has them."""
+    n, qh, hd, stride, index = _query(q)
+    c = _cache_of(keys, values, scales, q.dtype, index)
+    kh, d = c.kh, c.d
+    b, w, table_stride, table_at, lengths_at, _ = batch = _batch(table, lengths, None, c.rows, index)
+    _require(n == b and hd == d and qh % kh == 0 and qh <= 1024, "q must be [B, a multiple of the KV heads, head dim]")
+    for name, t in (("groups", groups), ("shared", shared)):
+        _cuda_contig(name, t, torch.int32, q.device)
+        _require(t.numel() == b, f"{name} must hold one value a sequence")
+    at, groups_at, shared_at = q.data_ptr(), groups.data_ptr(), shared.data_ptr()
+    spans = ()
+    if out is not None or ws is not None:
+        spans = ((at, at + 2 * ((n - 1) * stride + qh * d)), *c.spans(), *_batch_spans(*batch), (groups_at, groups_at + 4 * b),
+                 (shared_at, shared_at + 4 * b))
+    out = _output(out, (b, qh * d), q, index, spans)
+    nbytes = native.lib().moss_paged_shared_workspace_bytes(b, w, c.rows, qh, kh, d)
+    ws = _workspace(ws, nbytes, q, out, spans)
+    native.call_on(q, "moss_paged_shared_decode_attention" + c.native_name, at, stride, *c.args(), table_at, table_stride,
+                   lengths_at, groups_at, shared_at, b, w, qh, kh, d, _scale(scale, d), out.data_ptr(), ws.data_ptr(), nbytes,
+                   _TYPES[q.dtype])
+    return out
+
+
 def prompt_workspace(q: torch.Tensor, keys: torch.Tensor, table: torch.Tensor) -> torch.Tensor | None:
     """A workspace for :func:`prompt_attention` calls of these shapes (None: none needed); calls that may overlap need
     one each."""
