@@ -8,26 +8,30 @@
 //   -inf where the row's mask has a 0 at bit v
 // in fp32, rounded once to the logits' type.  Ids outside the row name nothing.
 //
-// What bounds it: the row's bytes in and out, and for few rows the chain launch, tokens, counts, logits.  A workgroup
-// takes kChunk entries of a row: it has their logits on the way while it goes through the row's tokens, counts those in
-// its range in LDS, with integers (a count, a flag, the largest index of a pair), so that no order of the atomics shows,
-// and then changes and writes its entries.  Tokens are read once for each of a row's chunks, from the cache.
+// What bounds it: the row's bytes in and out, and for few rows the chain launch, tokens, counts, logits.  128 rows of 151,936
+// bf16 logits: a copy 16 us (4.8 TB/s), with a mask 17.5, with up to 4096 tokens a row 23, all together 26; 512 rows of 1024
+// with up to 400 tokens 5.3.  A workgroup takes a chunk of a row: it asks for the row's tokens and the chunk's logits and mask
+// bits before it waits for any of them (34 -> 30 us), counts the tokens in its range in LDS, with integers (a count, a flag, the
+// largest index of a pair), so that no order of the atomics shows, and then changes and writes its entries.  A row's
+// tokens are read once for each of its chunks, from the cache: a chunk of 16384 entries with counts of 16 bits, two
+// workgroups of 1024 threads a CU (30 -> 26 us against 8192 with counts of 32 and 512 threads, three a CU, where that only
+// serves for 2^15 tokens and more, which 15 bits and a flag cannot count); a short row is one workgroup of 256 threads (6.1 ->
+// 5.3 us for the 512).
 #include "common.h"
 
 namespace moss {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kChunk = 8192;                     // entries: 16 a thread
-constexpr int kGroups = kChunk / 8 / kThreads;   // of 8 entries, a thread's
-constexpr uint32_t kPrompt = 1u << 31;           // said in the prompt; below it the count
+constexpr int kAhead = 4;        // tokens of a thread on their way together
+constexpr int kSmallRow = 2048;  // entries that one workgroup of 256 threads takes
+constexpr int kNarrow = 1 << 15; // tokens that 15 bits count
 typedef _Float16 f16_t;
 
 struct AdjustArgs {
     const void* logits;
     void* out;
     long long stride, out_stride;
-    int vocab, chunks;
+    int rows, vocab, chunks;
     const void* tokens;
     long long token_row, token_step;  // elements
     int width;
@@ -78,13 +82,26 @@ struct Group {
     }
 };
 
-template <int TYPE, typename Token>
-__global__ __launch_bounds__(kThreads) void adjust_rows_kernel(AdjustArgs a) {
+// COUNT: bits of a count and its flag.
+template <int TYPE, typename Token, int COUNT, int THREADS, int CHUNK>
+__global__ __launch_bounds__(THREADS) void adjust_rows_kernel(AdjustArgs a) {
     typedef Logit<TYPE> L;
     typedef typename L::Bits Bits;
-    extern __shared__ uint32_t counts[];       // [kChunk]: the tokens; then [kChunk] of 16 bits: the biases
-    uint32_t* last = counts + (a.tokens ? kChunk : 0);  // two entries a word
-    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
+    constexpr int kThreads = THREADS, kChunk = CHUNK, kGroups = kChunk / 8 / kThreads;  // groups of 8 entries, a thread's
+    constexpr int kCounts = kChunk * COUNT / 32, kPer = 32 / COUNT;                      // words of all counts, counts of a word
+    constexpr uint32_t kPrompt = 1u << (COUNT - 1);  // said in the prompt; below it the count
+    extern __shared__ uint32_t counts[];       // the tokens; then [kChunk] of 16 bits: the biases
+    uint32_t* last = counts + (a.tokens ? kCounts : 0);  // two entries a word
+    // Workgroups go round the XCDs one by one: of every eight rows each is given to one of them, so that its chunks find its
+    // tokens in one cache.
+    int row, chunk;
+    const int tid = threadIdx.x, eight = blockIdx.x / (8 * a.chunks);
+    if (8 * eight + 8 <= a.rows) {
+        const int at = blockIdx.x - eight * 8 * a.chunks;
+        row = 8 * eight + at % 8, chunk = at / 8;
+    } else {
+        row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    }
     const Bits* src = reinterpret_cast<const Bits*>(a.logits) + (size_t)row * a.stride;
     Bits* dst = reinterpret_cast<Bits*>(a.out) + (size_t)row * a.out_stride;
     // Groups of eight entries that begin at 16 bytes (32 of fp32) in both rows, where both begin at the same place among
@@ -97,58 +114,73 @@ __global__ __launch_bounds__(kThreads) void adjust_rows_kernel(AdjustArgs a) {
     Group<TYPE> x[kGroups];
     auto first_of = [&](int g) { return from + 8 * (g * kThreads + tid); };
     auto whole = [&](int e) { return wide && e >= 0 && e + 8 <= a.vocab; };
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-        const int e = first_of(g);
-        if (whole(e)) {
-#pragma unroll
-            for (int i = 0; i < (TYPE == 2 ? 2 : 1); ++i) x[g].w[i] = reinterpret_cast<const u32x4_t*>(src + e)[i];
-        }
-    }
+    // everything that memory has to be asked for, before anything is waited for, the tokens first: what is asked for later
+    // comes later
+    const Token* tokens = reinterpret_cast<const Token*>(a.tokens) + (long long)row * a.token_row;
+    Token said[kAhead];
+    int n = 0, prompt = 0;
     float rep = 1.f, pres = 0.f, freq = 0.f;
     if (a.tokens) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) said[j] = tokens[(long long)min(j * kThreads + tid, a.width - 1) * a.token_step];
+        n = a.lengths ? min(max(a.lengths[row], 0), a.width) : a.width;
+        prompt = a.prompt ? a.prompt[row] : 0;
         rep = a.repetition ? a.repetition[row] : a.repetition_v;
         pres = a.presence ? a.presence[row] : a.presence_v;
         freq = a.frequency ? a.frequency[row] : a.frequency_v;
     }
+    const int* ids = a.bias_ids + (long long)row * a.bias_ids_stride;
+    int named = a.bias ? ids[min(tid, a.biases - 1)] : -1;
+    const uint32_t* mask = a.mask ? a.mask + (long long)row * a.mask_stride : nullptr;
+    const int last_word = (a.vocab - 1) >> 5;
+    uint32_t bits[kGroups][2];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int e = first_of(g);
+        if (!whole(e)) continue;
+#pragma unroll
+        for (int i = 0; i < (TYPE == 2 ? 2 : 1); ++i) x[g].w[i] = reinterpret_cast<const u32x4_t*>(src + e)[i];
+        if (mask) {
+            bits[g][0] = mask[e >> 5];
+            bits[g][1] = mask[min((e >> 5) + 1, last_word)];
+        }
+    }
     if (a.tokens || a.bias) {
-        const int words = (a.tokens ? kChunk : 0) + (a.bias ? kChunk / 2 : 0);
+        const int words = (a.tokens ? kCounts : 0) + (a.bias ? kChunk / 2 : 0);
         for (int i = 4 * tid; i < words; i += 4 * kThreads) *reinterpret_cast<u32x4_t*>(counts + i) = u32x4_t{0u, 0u, 0u, 0u};
         __syncthreads();
         if (a.tokens) {
-            const int n = a.lengths ? min(max(a.lengths[row], 0), a.width) : a.width;
-            const int prompt = a.prompt ? a.prompt[row] : 0;
-            const Token* t = reinterpret_cast<const Token*>(a.tokens) + (long long)row * a.token_row;
-            for (int i = tid; i < n; i += kThreads) {
-                const Token id = t[(long long)i * a.token_step];
-                if (id < e0 || id >= e1) continue;
-                uint32_t* at = counts + ((int)id - from);
-                if (i < prompt) atomicOr(at, kPrompt);
-                else atomicAdd(at, 1u);
+            for (int i0 = 0; i0 < n; i0 += kAhead * kThreads) {
+                if (i0)
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) said[j] = tokens[(long long)min(i0 + j * kThreads + tid, n - 1) * a.token_step];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const int i = i0 + j * kThreads + tid;
+                    if (i >= n || said[j] < e0 || said[j] >= e1) continue;
+                    const int k = (int)said[j] - from, up = COUNT * (k % kPer);
+                    if (i < prompt) atomicOr(counts + k / kPer, kPrompt << up);
+                    else atomicAdd(counts + k / kPer, 1u << up);
+                }
             }
         }
-        if (a.bias) {
-            // of two pairs that name one entry the later holds: the largest index + 1, in 16 bits, by compare and swap
-            const int* ids = a.bias_ids + (long long)row * a.bias_ids_stride;
-            for (int i = tid; i < a.biases; i += kThreads) {
-                const int id = ids[i];
-                if (id < e0 || id >= e1) continue;
-                uint32_t* at = last + (id - from) / 2;
-                const int up = 16 * ((id - from) & 1);
-                uint32_t old = *at;
-                while (((old >> up) & 0xffffu) < (uint32_t)(i + 1)) {
-                    const uint32_t next = (old & ~(0xffffu << up)) | ((uint32_t)(i + 1) << up);
-                    const uint32_t seen = atomicCAS(at, old, next);
-                    if (seen == old) break;
-                    old = seen;
-                }
+        // of two pairs that name one entry the later holds: the largest index + 1, in 16 bits, by compare and swap
+        for (int i = tid; i < a.biases; i += kThreads) {
+            if (i >= kThreads) named = ids[i];
+            if (named < e0 || named >= e1) continue;
+            uint32_t* at = last + (named - from) / 2;
+            const int up = 16 * ((named - from) & 1);
+            uint32_t old = *at;
+            while (((old >> up) & 0xffffu) < (uint32_t)(i + 1)) {
+                const uint32_t next = (old & ~(0xffffu << up)) | ((uint32_t)(i + 1) << up);
+                const uint32_t seen = atomicCAS(at, old, next);
+                if (seen == old) break;
+                old = seen;
             }
         }
         __syncthreads();
     }
     const float* bias = a.bias + (long long)row * a.bias_stride;
-    const uint32_t* mask = a.mask ? a.mask + (long long)row * a.mask_stride : nullptr;
-    const int last_word = (a.vocab - 1) >> 5;
     // entry e (from + k) with count word c and bias index b: changed, or as it was
     auto change = [&](Bits& v, uint32_t c, uint32_t b) {
         float y = L::value(v);
@@ -162,16 +194,23 @@ __global__ __launch_bounds__(kThreads) void adjust_rows_kernel(AdjustArgs a) {
         const int e = first_of(g), k = e - from;
         if (whole(e)) {
             if (a.tokens || a.bias) {
-                u32x4_t c[2] = {}, b = {};
-                if (a.tokens) {
-                    c[0] = *reinterpret_cast<const u32x4_t*>(counts + k);
-                    c[1] = *reinterpret_cast<const u32x4_t*>(counts + k + 4);
+                u32x4_t c[COUNT / 16] = {}, b = {};
+                uint32_t some = 0;
+                if (a.tokens)
+#pragma unroll
+                    for (int i = 0; i < COUNT / 16; ++i) {
+                        c[i] = *reinterpret_cast<const u32x4_t*>(counts + k / kPer + 4 * i);
+                        some |= c[i][0] | c[i][1] | c[i][2] | c[i][3];
+                    }
+                if (a.bias) {
+                    b = *reinterpret_cast<const u32x4_t*>(last + k / 2);
+                    some |= b[0] | b[1] | b[2] | b[3];
                 }
-                if (a.bias) b = *reinterpret_cast<const u32x4_t*>(last + k / 2);
-                if (c[0][0] | c[0][1] | c[0][2] | c[0][3] | c[1][0] | c[1][1] | c[1][2] | c[1][3] | b[0] | b[1] | b[2] | b[3]) {
+                if (some) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const uint32_t ci = c[i / 4][i % 4], bi = (b[i / 2] >> (16 * (i & 1))) & 0xffffu;
+                        const uint32_t ci = COUNT == 32 ? c[i / 4][i % 4] : (c[0][i / 2] >> (16 * (i & 1))) & 0xffffu;
+                        const uint32_t bi = (b[i / 2] >> (16 * (i & 1))) & 0xffffu;
                         if (ci | bi) {
                             Bits v = x[g].get(i);
                             change(v, ci, bi);
@@ -181,12 +220,10 @@ __global__ __launch_bounds__(kThreads) void adjust_rows_kernel(AdjustArgs a) {
                 }
             }
             if (mask) {
-                const int w = e >> 5;
-                const uint64_t both = mask[w] | (uint64_t)mask[min(w + 1, last_word)] << 32;
-                const uint32_t bits = (uint32_t)(both >> (e & 31));
+                const uint32_t kept = (uint32_t)((bits[g][0] | (uint64_t)bits[g][1] << 32) >> (e & 31));
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (!(bits >> i & 1)) x[g].set(i, L::bits(-INFINITY));
+                    if (!(kept >> i & 1)) x[g].set(i, L::bits(-INFINITY));
             }
 #pragma unroll
             for (int i = 0; i < (TYPE == 2 ? 2 : 1); ++i) reinterpret_cast<u32x4_t*>(dst + e)[i] = x[g].w[i];
@@ -196,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void adjust_rows_kernel(AdjustArgs a) {
                 const int at = wide ? e + i : from + g * 8 * kThreads + i * kThreads + tid;
                 if (at < 0 || at >= a.vocab) continue;
                 Bits v = src[at];
-                const uint32_t ci = a.tokens ? counts[at - from] : 0u;
+                const uint32_t ci = a.tokens ? counts[(at - from) / kPer] >> (COUNT * ((at - from) % kPer)) & (kPrompt | (kPrompt - 1)) : 0u;
                 const uint32_t bi = a.bias ? (last[(at - from) / 2] >> (16 * ((at - from) & 1))) & 0xffffu : 0u;
                 if (ci | bi) change(v, ci, bi);
                 if (mask && !(mask[at >> 5] >> (at & 31) & 1)) v = L::bits(-INFINITY);
@@ -206,14 +243,25 @@ __global__ __launch_bounds__(kThreads) void adjust_rows_kernel(AdjustArgs a) {
     }
 }
 
+template <int TYPE, typename Token, int COUNT, int THREADS, int CHUNK>
+int launch_adjust(AdjustArgs a, hipStream_t st) {
+    a.chunks = (a.vocab + 7 + CHUNK - 1) / CHUNK;  // a row that begins inside a group of eight has its last entries one further
+    const long long groups = (long long)a.rows * a.chunks;
+    MOSS_CHECK_ARG(groups * THREADS < (1ll << 32));
+    const size_t lds = (a.tokens ? COUNT / 8 * CHUNK : 0) + (a.bias ? 2 * CHUNK : 0);
+    hipLaunchKernelGGL((adjust_rows_kernel<TYPE, Token, COUNT, THREADS, CHUNK>), dim3((unsigned)groups), dim3(THREADS), lds, st, a);
+    return moss_launch_status();
+}
+
+template <int TYPE, typename Token>
+int launch_adjust(const AdjustArgs& a, hipStream_t st) {
+    if (a.vocab + 7 <= kSmallRow) return launch_adjust<TYPE, Token, 32, 256, kSmallRow>(a, st);
+    return a.width < kNarrow ? launch_adjust<TYPE, Token, 16, 1024, 16384>(a, st) : launch_adjust<TYPE, Token, 32, 1024, 8192>(a, st);
+}
+
 template <int TYPE>
-void launch_adjust(const AdjustArgs& a, int rows, int token_bytes, hipStream_t st) {
-    const dim3 grid((unsigned)(rows * (long long)a.chunks)), block(kThreads);
-    const size_t lds = (a.tokens ? 4 * kChunk : 0) + (a.bias ? 2 * kChunk : 0);
-    if (token_bytes == 8)
-        hipLaunchKernelGGL((adjust_rows_kernel<TYPE, int64_t>), grid, block, lds, st, a);
-    else
-        hipLaunchKernelGGL((adjust_rows_kernel<TYPE, int32_t>), grid, block, lds, st, a);
+int launch_adjust(const AdjustArgs& a, int token_bytes, hipStream_t st) {
+    return token_bytes == 8 ? launch_adjust<TYPE, int64_t>(a, st) : launch_adjust<TYPE, int32_t>(a, st);
 }
 
 }  // namespace
@@ -240,19 +288,13 @@ MOSS_API int moss_adjust_rows(const void* logits, int dtype, int rows, long long
                              (bias_stride == 0 || bias_stride >= biases) && MOSS_ALIGNED(bias_ids, 4) && MOSS_ALIGNED(bias, 4)));
     MOSS_CHECK_ARG(!mask || ((mask_stride == 0 || mask_stride >= (vocab + 31) / 32) && MOSS_ALIGNED(mask, 4)));
     AdjustArgs a;
-    a.logits = logits, a.out = out, a.stride = stride, a.out_stride = out_stride, a.vocab = vocab;
-    // a row that begins inside a group of eight has its last entries one group further
-    a.chunks = (vocab + 7 + kChunk - 1) / kChunk;
+    a.logits = logits, a.out = out, a.stride = stride, a.out_stride = out_stride, a.rows = rows, a.vocab = vocab;
     a.tokens = tokens, a.token_row = token_row_stride, a.token_step = token_stride, a.width = width;
     a.lengths = (const int*)lengths, a.prompt = (const int*)prompt;
     a.repetition = (const float*)repetition, a.presence = (const float*)presence, a.frequency = (const float*)frequency;
     a.repetition_v = repetition_value, a.presence_v = presence_value, a.frequency_v = frequency_value;
     a.bias_ids = (const int*)bias_ids, a.bias = (const float*)bias, a.bias_ids_stride = bias_ids_stride, a.bias_stride = bias_stride;
     a.biases = biases, a.mask = (const uint32_t*)mask, a.mask_stride = mask_stride;
-    MOSS_CHECK_ARG((long long)rows * a.chunks * kThreads < (1ll << 32));
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == 0) launch_adjust<0>(a, rows, token_bytes, st);
-    else if (dtype == 1) launch_adjust<1>(a, rows, token_bytes, st);
-    else launch_adjust<2>(a, rows, token_bytes, st);
-    return moss_launch_status();
+    return dtype == 0 ? launch_adjust<0>(a, token_bytes, st) : dtype == 1 ? launch_adjust<1>(a, token_bytes, st) : launch_adjust<2>(a, token_bytes, st);
 }

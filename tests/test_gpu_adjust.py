@@ -285,3 +285,15 @@ def test_calls_beside_each_other(dev):
     _check(s, first)
     for _ in range(3):
         assert torch.equal(_run(s), first)
+
+
+@pytest.mark.parametrize("rows, vocab, width", [(19, 2041, 300), (17, 2042, 300), (9, 16377, 33000), (16, 16384, 32768), (3, 33000, 32767), (11, 40001, 70)])
+def test_every_way_of_counting(dev, rows, vocab, width):
+    """Rows of one small workgroup and of several; histories that 15 bits count, and longer ones; more than eight rows, and rows behind
+    the last eight."""
+    s = _inputs(dev, rows, vocab, torch.bfloat16, width=width, seed=rows, token_type=torch.int32 if rows % 2 else torch.int64)
+    s["tokens"][0] = 5
+    s["lengths"][0] = width
+    s["prompt"][0] = 0
+    print(f"adjust {rows} x {vocab}, {width} tokens", flush=True)
+    _check(s, _run(s))
