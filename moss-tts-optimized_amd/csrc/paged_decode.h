@@ -151,12 +151,11 @@ struct ShareOf {
     long long slot;
 };
 
+// ow, mw, lw: LDS for the waves' parts (16-byte aligned).
 template <typename E, int D, typename T, bool NT>
 __device__ __forceinline__ void decode_share(const DecodeArgs& a, const typename T::Cache& c, const PagedBatch& bt,
-                                             const ShareOf& sh) {
+                                             const ShareOf& sh, float (&ow)[4][16][D], float (&mw)[4][16], float (&lw)[4][16]) {
     constexpr int NJ = D / 16;
-    __shared__ __attribute__((aligned(16))) float ow[4][16][D];
-    __shared__ float mw[4][16], lw[4][16];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int g = lane >> 4, r = lane & 15;
     const int kvh = sh.kvh, h0 = sh.h0, heads = sh.heads, r0 = sh.r0, r1 = sh.r1;

@@ -43,6 +43,8 @@ __device__ __forceinline__ Place find_share(const PagedBatch& bt, int shift, int
 
 template <typename E, int D, typename T, bool NT>
 __global__ __launch_bounds__(256, 3) void paged_decode_split(DecodeArgs a, typename T::Cache c, PagedBatch bt) {
+    __shared__ __attribute__((aligned(16))) float ow[4][16][D];
+    __shared__ float mw[4][16], lw[4][16];
     const int tiles = (a.group + 15) / 16;  // head tiles of a KV head
     const int slot = blockIdx.x / a.xdim, x = blockIdx.x % a.xdim;
     const Place pl = find_share(bt, c.shift, a.shares, slot, threadIdx.x & (kWave - 1));
@@ -51,7 +53,7 @@ __global__ __launch_bounds__(256, 3) void paged_decode_split(DecodeArgs a, typen
     sh.b = pl.b, sh.kvh = x / tiles, sh.h0 = 16 * (x % tiles), sh.heads = min(16, a.group - sh.h0);
     share_rows(paged_length(bt, pl.b, c.shift), pl.count, pl.index, sh.r0, sh.r1);
     sh.alone = pl.count == 1, sh.slot = slot;
-    decode_share<E, D, T, NT>(a, c, bt, sh);
+    decode_share<E, D, T, NT>(a, c, bt, sh, ow, mw, lw);
 }
 
 // grid (QH, B), 256 threads: the shares of one head of a sequence, wave w taking w, w + 4, ..; the four waves' sums meet

@@ -154,14 +154,16 @@ struct TileRows {
     bool idle;                  // no row of this wave's exists
 };
 
+// A stage of K | V in LDS.  A workgroup has two, as two variables, so that reading one does not wait for the loads into the other.
+template <int D>
+using Stage = unsigned char[4 * D * kPromptBlock];
+
 // o, m, l of the rows (l summed over the lane's keys and, on return, its partner's).  KS 2: two waves share the rows and halve a
 // block's keys; false: this wave's part went to the other.
 template <typename E, int D, int KS, typename S>
 __device__ __forceinline__ bool attend_rows(const typename S::Cache& c, const TileRows& t, int W, const u32x4_t (&qf)[D / 16], float scale,
-                                            f32x16_v (&o_out)[D / 32], float& m_out, float& l_out) {
+                                            Stage<D>& even, Stage<D>& odd, f32x16_v (&o_out)[D / 32], float& m_out, float& l_out) {
     constexpr int NT = 2 / KS, BK = kPromptBlock, DT = D / 32, DK = D / 16, RB = 2 * D, KB = BK * RB;  // NT: a wave's 32-key tiles
-    // two stages of K | V: two variables, so that reading one does not wait for the loads into the other
-    __shared__ __attribute__((aligned(1024))) unsigned char even[2 * KB], odd[2 * KB];
     const int lane = threadIdx.x & 63, half = lane >> 5, rl = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % (4 / KS), kq = KS == 1 ? 0 : wave / (4 / KS);
     const int kvh = t.kvh, b0 = t.b0, b1 = t.b1, last = t.last, qpos = t.qpos, wave_first = t.wave_first, wave_last = t.wave_last;

@@ -99,6 +99,7 @@ __device__ __forceinline__ Found find_tile(const PromptArgs& a, int shift, const
 template <typename E, int D, int KS, typename S>
 __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PromptArgs a, typename S::Cache c, PagedBatch bt) {
     constexpr int RW = 4 / KS, HEIGHT = 32 * RW, DT = D / 32, DK = D / 16;  // row waves
+    __shared__ __attribute__((aligned(1024))) Stage<D> even, odd;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, rl = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW;
     const int kvh = blockIdx.x % c.kh, G = a.group;  // neighbours in the grid, which lie on different XCDs, differ in it
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PromptArgs a, type
     f32x16_v o[DT];
     float m, l;
     const TileRows rows{bt.table + (size_t)f.b * bt.table_stride, kvh, b0, b1, last, qpos, wave_first, wave_last, idle};
-    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, o, m, l)) return;
+    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, even, odd, o, m, l)) return;
     // O^T element e of d tile dt: d = 32 dt + 8 (e / 4) + 4 half + e % 4
     if (cut) {
         // (starts that do not rise can name more parts than there are tokens for: they have no slot)

@@ -23,8 +23,8 @@ struct SharedArgs {
     DecodeArgs a;             // part and stat: of the sequences' own rows
     const int* groups;        // [B]
     const int* shared;        // [B]
-    float* prefix_part;       // [rows, KH, D]
-    float2* prefix_stat;      // [rows, KH]
+    float* prefix_part;       // [KH, rows, D]
+    float2* prefix_stat;      // [KH, rows]
     long long prefix_rows;
     int prefix_shares;
 };
@@ -60,44 +60,40 @@ __device__ __forceinline__ int tiles_of(const Member& m, int group, int height, 
 }
 __device__ __forceinline__ int blocks_of(const Member& m) { return (m.rows + kPromptBlock - 1) / kPromptBlock; }
 
-// Blocks of a part.
-__device__ __forceinline__ int prefix_share(const SharedArgs& s, const PagedBatch& bt, int shift, int height, int lane) {
-    long long total = 0;
-    for (int b0 = 0; b0 < bt.B; b0 += kWave) {
-        const Member m = member_of(s, bt, shift, b0, lane);
-        total += (long long)tiles_of(m, s.a.group, height, lane) * blocks_of(m);
+// What the batch's work is cut into: blocks of keys of a part of a prefix, units of a share of own rows, parts in all.  `at(b0)`
+// gives the members from sequence b0 on.
+struct Cuts {
+    int share, units;
+    long long items;
+};
+template <int HEIGHT, typename At>
+__device__ __forceinline__ Cuts cuts_of(const SharedArgs& s, int B, int lane, At at) {
+    long long blocks = 0, units = 0, items = 0;
+    for (int b0 = 0; b0 < B; b0 += kWave) {
+        const Member m = at(b0);
+        blocks += (long long)tiles_of(m, s.a.group, HEIGHT, lane) * blocks_of(m);
+        units += units_of(m.own());
     }
-    return prefix_share_of(wave_total(total), s.prefix_shares);
+    Cuts c;
+    c.share = prefix_share_of(wave_total(blocks), s.prefix_shares);
+    c.units = share_of_units(wave_total(units), s.a.shares);
+    for (int b0 = 0; b0 < B; b0 += kWave) {
+        const Member m = at(b0);
+        items += (long long)tiles_of(m, s.a.group, HEIGHT, lane) * shares_of(blocks_of(m), c.share);
+    }
+    c.items = wave_total(items);
+    return c;
 }
 
+// One part of a run's prefix for a tile of its rows.
 template <typename E, int D, int KS, typename S>
-__global__ __launch_bounds__(256, 2) void paged_shared_prefix(SharedArgs s, typename S::Cache c, PagedBatch bt) {
+__device__ __forceinline__ void prefix_part(const SharedArgs& s, const typename S::Cache& c, const PagedBatch& bt, const Member& m, int b0,
+                                            int l, int base, int index, int share, int kvh, Stage<D>& even, Stage<D>& odd) {
     constexpr int HEIGHT = 128 / KS, RW = 4 / KS, DT = D / 32, DK = D / 16;
     const DecodeArgs& a = s.a;
-    const int lane = threadIdx.x & (kWave - 1), half = lane >> 5, rl = lane & 31;
+    const int lane = threadIdx.x & (kWave - 1), half = lane >> 5, rl = lane & 31, G = a.group;
     const int rw = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) % RW;
-    const int kvh = blockIdx.x % c.kh, item = blockIdx.x / c.kh, G = a.group;
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const int share = prefix_share(s, bt, c.shift, HEIGHT, lane);
-    // the item's run: lane `l` of the sequences from b0 on
-    Member m;
-    int b0 = 0, before = 0, base = 0, index = 0, l = -1;
-    for (; b0 < bt.B; b0 += kWave) {
-        m = member_of(s, bt, c.shift, b0, lane);
-        const int tiles = tiles_of(m, G, HEIGHT, lane), parts = shares_of(blocks_of(m), share), n = tiles * parts;
-        const int rows = tiles ? m.size * G * parts : 0;
-        const int through = wave_prefix(n), rows_through = wave_prefix(rows);
-        const unsigned long long past = __ballot(before + through > item);
-        if (past) {
-            l = __builtin_ctzll(past);
-            index = item - before - (lane_value(through, l) - lane_value(n, l));
-            base += lane_value(rows_through, l) - lane_value(rows, l);
-            break;
-        }
-        before += lane_value(through, kWave - 1);
-        base += lane_value(rows_through, kWave - 1);
-    }
-    if (l < 0) return;
     const int size = lane_value(m.size, l), P = lane_value(m.rows, l), blocks = (P + kPromptBlock - 1) / kPromptBlock;
     const int parts = shares_of(blocks, share), tile = uniform(index / parts), part = uniform(index % parts);
     const int nrows = size * G, row = min(tile * HEIGHT + 32 * rw + rl, nrows - 1);  // clamped: stores are guarded
@@ -123,10 +119,10 @@ __global__ __launch_bounds__(256, 2) void paged_shared_prefix(SharedArgs s, type
     rows.idle = tile * HEIGHT + 32 * rw >= nrows;
     f32x16_v o[DT];
     float mx, sum;
-    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, o, mx, sum)) return;
+    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, even, odd, o, mx, sum)) return;
     const int out = base + part * nrows + row;
     if (tile * HEIGHT + 32 * rw + rl >= nrows || !in_slots(out, 1, s.prefix_rows)) return;
-    const size_t at = (size_t)out * c.kh + kvh;
+    const size_t at = (size_t)kvh * s.prefix_rows + out;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -136,25 +132,44 @@ __global__ __launch_bounds__(256, 2) void paged_shared_prefix(SharedArgs s, type
     if (half == 0) s.prefix_stat[at] = make_float2(mx, sum);
 }
 
-// A share's size in units of the sequences' own rows.
-__device__ __forceinline__ int own_share(const SharedArgs& s, const PagedBatch& bt, int shift, int lane) {
-    long long total = 0;
-    for (int b0 = 0; b0 < bt.B; b0 += kWave) total += units_of(member_of(s, bt, shift, b0, lane).own());
-    return share_of_units(wave_total(total), s.a.shares);
-}
-
-template <typename E, int D, typename T, bool NT>
-__global__ __launch_bounds__(256, 3) void paged_shared_own(SharedArgs s, typename T::Cache c, PagedBatch bt) {
+// The parts of the prefixes (matrix cores) and the shares of the rest (memory) side by side in one launch, the parts first.
+template <typename E, int D, int KS, typename S, typename T, bool NT>
+__global__ __launch_bounds__(256, 2) void paged_shared_split(SharedArgs s, typename S::Cache c, PagedBatch bt) {
+    constexpr int HEIGHT = 128 / KS;
+    __shared__ __attribute__((aligned(1024))) Stage<D> even, odd;
     const DecodeArgs& a = s.a;
-    const int tiles = (a.group + 15) / 16, lane = threadIdx.x & (kWave - 1);
-    const int slot = blockIdx.x / a.xdim, x = blockIdx.x % a.xdim;
-    const int share = own_share(s, bt, c.shift, lane);
+    const int lane = threadIdx.x & (kWave - 1), G = a.group;
+    const Member m0 = member_of(s, bt, c.shift, 0, lane);
+    auto at = [&](int b0) { return b0 == 0 ? m0 : member_of(s, bt, c.shift, b0, lane); };
+    const Cuts cuts = cuts_of<HEIGHT>(s, bt.B, lane, at);
+    const long long prefixes = cuts.items * c.kh;
+    if (blockIdx.x < prefixes) {
+        const int kvh = blockIdx.x % c.kh, item = blockIdx.x / c.kh;
+        int before = 0, base = 0;
+        for (int b0 = 0; b0 < bt.B; b0 += kWave) {
+            const Member m = at(b0);
+            const int tiles = tiles_of(m, G, HEIGHT, lane), parts = shares_of(blocks_of(m), cuts.share), n = tiles * parts;
+            const int rows = tiles ? m.size * G * parts : 0;
+            const int through = wave_prefix(n), rows_through = wave_prefix(rows);
+            const unsigned long long past = __ballot(before + through > item);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                prefix_part<E, D, KS, S>(s, c, bt, m, b0, l, base + lane_value(rows_through, l) - lane_value(rows, l),
+                                         item - before - (lane_value(through, l) - lane_value(n, l)), cuts.share, kvh, even, odd);
+                return;
+            }
+            before += lane_value(through, kWave - 1);
+            base += lane_value(rows_through, kWave - 1);
+        }
+        return;
+    }
+    const int tiles = (G + 15) / 16, own = (int)(blockIdx.x - prefixes), slot = own / a.xdim, x = own % a.xdim;
     ShareOf sh;
     int before = 0;
     sh.b = -1;
     for (int b0 = 0; b0 < bt.B; b0 += kWave) {
-        const Member m = member_of(s, bt, c.shift, b0, lane);
-        const int n = shares_of(units_of(m.own()), share), through = wave_prefix(n);
+        const Member m = at(b0);
+        const int n = shares_of(units_of(m.own()), cuts.units), through = wave_prefix(n);
         const unsigned long long past = __ballot(before + through > slot);
         if (past) {
             const int l = __builtin_ctzll(past), count = lane_value(n, l), from = lane_value(m.from, l);
@@ -166,26 +181,31 @@ __global__ __launch_bounds__(256, 3) void paged_shared_own(SharedArgs s, typenam
         }
         before += lane_value(through, kWave - 1);
     }
-    if (sh.b < 0) return;
-    sh.kvh = x / tiles, sh.h0 = 16 * (x % tiles), sh.heads = min(16, a.group - sh.h0), sh.slot = slot;
-    decode_share<E, D, T, NT>(a, c, bt, sh);
+    if (sh.b < 0 || slot >= a.slots) return;
+    sh.kvh = x / tiles, sh.h0 = 16 * (x % tiles), sh.heads = min(16, G - sh.h0), sh.slot = slot;
+    static_assert(sizeof(float[4][16][D]) <= sizeof(Stage<D>) && 2 * sizeof(float[4][16]) <= sizeof(Stage<D>), "");
+    float(&ml)[2][4][16] = *reinterpret_cast<float(*)[2][4][16]>(odd);
+    decode_share<E, D, T, NT>(a, c, bt, sh, *reinterpret_cast<float(*)[4][16][D]>(even), ml[0], ml[1]);
 }
 
 // grid (QH, B), 256 threads: the parts of the prefix and the shares of the rest of one head of a sequence, wave w taking w, w + 4,
 // ..; the four waves' sums meet in LDS.
 template <typename E, int D, int HEIGHT>
-__global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s, int kh, int shift, PagedBatch bt) {
+__global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s, int shift, PagedBatch bt) {
     constexpr int VPL = D / kWave;
     __shared__ float acc_s[4][D];
     const DecodeArgs& a = s.a;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave, G = a.group;
     const int mine = b % kWave;
-    const int share = prefix_share(s, bt, shift, HEIGHT, lane), su = own_share(s, bt, shift, lane);
+    const Member m0 = member_of(s, bt, shift, 0, lane);
+    auto at = [&](int b0) { return b0 == 0 ? m0 : member_of(s, bt, shift, b0, lane); };
+    const Cuts cuts = cuts_of<HEIGHT>(s, bt.B, lane, at);
+    const int share = cuts.share, su = cuts.units;
     // partial results before this sequence's, and its run
     Member m;
     int slots = 0, rows = 0;
     for (int b0 = 0;; b0 += kWave) {
-        m = member_of(s, bt, shift, b0, lane);
+        m = at(b0);
         const int n = shares_of(units_of(m.own()), su);
         const int r = tiles_of(m, G, HEIGHT, lane) ? m.size * G * shares_of(blocks_of(m), share) : 0;
         if (b0 + kWave > b) {
@@ -211,10 +231,10 @@ __global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s, int kh, i
     // only when what says where rows are changes between the launches
     if (!in_slots(slots, own, a.slots) || (parts && !in_slots(row, (parts - 1) * nrows + 1, s.prefix_rows))) return;
     // part i's place among the statistics and results: the prefix's, then the sequence's own
-    const size_t step = (size_t)nrows * kh;
-    const float2* stat0 = s.prefix_stat + (size_t)row * kh + h / G;
+    const size_t step = nrows;
+    const float2* stat0 = s.prefix_stat + (size_t)(h / G) * s.prefix_rows + row;
     const float2* stat1 = a.stat + (size_t)slots * a.qh + h;
-    const float* part0 = s.prefix_part + ((size_t)row * kh + h / G) * D;
+    const float* part0 = s.prefix_part + ((size_t)(h / G) * s.prefix_rows + row) * D;
     const float* part1 = a.part + ((size_t)slots * a.qh + h) * D;
     auto stat = [&](int i) { return i < parts ? stat0[i * step] : stat1[(size_t)(i - parts) * a.qh]; };
     auto part = [&](int i) { return i < parts ? part0 + i * step * D : part1 + (size_t)(i - parts) * a.qh * D; };
@@ -286,26 +306,23 @@ SharedPlan shared_plan(int B, int W, int shift, int qh, int kh) {
     return p;
 }
 
+template <typename E, int D, int KS, typename T, typename S>
+int launch_shared(const SharedArgs& s, const typename S::Cache& c, const PagedBatch& bt, const SharedPlan& p, hipStream_t st) {
+    const long long blocks = p.items * c.kh + p.slots * p.xdim;
+    MOSS_CHECK_ARG(blocks * 256 < (1ll << 32));
+    const long long page = ((long long)c.kh << c.shift) * D * (std::is_same<typename S::Cache, PagedCache>::value ? 2 : 1);
+    const long long named = (long long)bt.B * bt.W;
+    if ((named < c.pages ? named : c.pages) * page * 2 > kCached)
+        hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, true>), dim3((unsigned)blocks), dim3(256), 0, st, s, c, bt);
+    else
+        hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, false>), dim3((unsigned)blocks), dim3(256), 0, st, s, c, bt);
+    hipLaunchKernelGGL((paged_shared_join<E, D, 128 / KS>), dim3((unsigned)s.a.qh, (unsigned)bt.B), dim3(256), 0, st, s, c.shift, bt);
+    return moss_launch_status();
+}
+
 template <typename E, int D, template <typename, int> class T, template <typename, int> class S, typename Cache>
 int launch_shared(const SharedArgs& s, const Cache& c, const PagedBatch& bt, const SharedPlan& p, hipStream_t st) {
-    MOSS_CHECK_ARG(p.slots * p.xdim * 256 < (1ll << 32) && p.items * c.kh * 256 < (1ll << 32));
-    if (p.height == 64)
-        hipLaunchKernelGGL((paged_shared_prefix<E, D, 2, S<E, D>>), dim3((unsigned)(p.items * c.kh)), dim3(256), 0, st, s, c, bt);
-    else
-        hipLaunchKernelGGL((paged_shared_prefix<E, D, 1, S<E, D>>), dim3((unsigned)(p.items * c.kh)), dim3(256), 0, st, s, c, bt);
-    const long long page = ((long long)c.kh << c.shift) * D * (std::is_same<Cache, PagedCache>::value ? 2 : 1);
-    const long long named = (long long)bt.B * bt.W;
-    const dim3 grid((unsigned)(p.xdim * p.slots));
-    if ((named < c.pages ? named : c.pages) * page * 2 > kCached)
-        hipLaunchKernelGGL((paged_shared_own<E, D, T<E, D>, true>), grid, dim3(256), 0, st, s, c, bt);
-    else
-        hipLaunchKernelGGL((paged_shared_own<E, D, T<E, D>, false>), grid, dim3(256), 0, st, s, c, bt);
-    const dim3 joins((unsigned)s.a.qh, (unsigned)bt.B);
-    if (p.height == 64)
-        hipLaunchKernelGGL((paged_shared_join<E, D, 64>), joins, dim3(256), 0, st, s, c.kh, c.shift, bt);
-    else
-        hipLaunchKernelGGL((paged_shared_join<E, D, 128>), joins, dim3(256), 0, st, s, c.kh, c.shift, bt);
-    return moss_launch_status();
+    return p.height == 64 ? launch_shared<E, D, 2, T<E, D>, S<E, D>>(s, c, bt, p, st) : launch_shared<E, D, 1, T<E, D>, S<E, D>>(s, c, bt, p, st);
 }
 
 long long workspace_bytes_of(const SharedPlan& p, int qh, int kh, int d) { return (p.slots * qh + p.rows * kh) * (d + 2) * 4; }
