@@ -151,12 +151,12 @@ struct ShareOf {
     long long slot;
 };
 
-// ow, mw, lw: LDS for the waves' parts (16-byte aligned).
-template <typename E, int D, typename T, bool NT>
+// WAVES: 4, a workgroup's, or 1, each by itself and without LDS.  ow, mw, lw: LDS for the waves' parts (16-byte aligned).
+template <typename E, int D, typename T, bool NT, int WAVES>
 __device__ __forceinline__ void decode_share(const DecodeArgs& a, const typename T::Cache& c, const PagedBatch& bt,
-                                             const ShareOf& sh, float (&ow)[4][16][D], float (&mw)[4][16], float (&lw)[4][16]) {
+                                             const ShareOf& sh, int tid, float (&ow)[4][16][D], float (&mw)[4][16], float (&lw)[4][16]) {
     constexpr int NJ = D / 16;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int g = lane >> 4, r = lane & 15;
     const int kvh = sh.kvh, h0 = sh.h0, heads = sh.heads, r0 = sh.r0, r1 = sh.r1;
     const int qhead = kvh * a.group + h0;
@@ -175,9 +175,10 @@ __device__ __forceinline__ void decode_share(const DecodeArgs& a, const typename
     float m = -INFINITY, l = 0.f;  // l: this lane's rows only
 
     const int* trow = bt.table + (size_t)sh.b * bt.table_stride;
-    const int ntile = r1 > r0 ? ((r1 - r0 + 31) / 32 - w + 3) / 4 : 0;  // this wave's tiles w, w + 4, ..
+    const int w0 = WAVES == 1 ? 0 : w;
+    const int ntile = r1 > r0 ? ((r1 - r0 + 31) / 32 - w0 + WAVES - 1) / WAVES : 0;  // this wave's tiles w0, w0 + WAVES, ..
     // lane i: the page of half tile i of 32 tiles; those of the next 32 replace them when tile 32 k is loaded
-    auto row_of = [&](int i, int h) { return r0 + 32 * (w + 4 * i) + 16 * h; };
+    auto row_of = [&](int i, int h) { return r0 + 32 * (w0 + WAVES * i) + 16 * h; };
     int pages = -1;
     auto fetch_pages = [&](int first) {
         const int row = row_of(first + lane / 2, lane & 1);
@@ -277,8 +278,26 @@ __device__ __forceinline__ void decode_share(const DecodeArgs& a, const typename
         if (i + 1 < ntile) next_v(i + 1);
     }
 
-    // the waves' parts, each against its own m, meet in LDS
     l = sum_xor32(sum_xor16(l));
+    if constexpr (WAVES == 1) {
+        if (r >= heads) return;
+        const float inv = sh.alone ? (l == 0.f ? 0.f : 1.0f / l) : 1.f;
+        const size_t at = (sh.alone ? (size_t)sh.b : (size_t)sh.slot) * a.qh + qhead + r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // dims (D / 16) (4 g + i) + j
+#pragma unroll
+            for (int j = 0; j < NJ; j += 4) {
+                const int d = NJ * (4 * g + i) + j;
+                if (sh.alone)
+                    *reinterpret_cast<uint2*>(a.out + at * D + d) =
+                        make_uint2(E::pack(o[j][i] * inv, o[j + 1][i] * inv), E::pack(o[j + 2][i] * inv, o[j + 3][i] * inv));
+                else
+                    *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
+            }
+        if (!sh.alone && g == 0) a.stat[at] = make_float2(m, l);
+        return;
+    }
+    // the waves' parts, each against its own m, meet in LDS
     if (g == 0) {
         mw[w][r] = m;
         lw[w][r] = l;

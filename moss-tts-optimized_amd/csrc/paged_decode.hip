@@ -29,7 +29,7 @@ __device__ __forceinline__ int share_units(const PagedBatch& bt, int shift, int 
 __device__ __forceinline__ Place find_share(const PagedBatch& bt, int shift, int shares, int slot, int lane) {
     if (bt.B <= kWave) {
         const int units = lane < bt.B ? units_of(paged_length(bt, lane, shift)) : 0;
-        const int share = share_of_units(wave_total((long long)units), shares), n = shares_of(units, share);
+        const int share = share_of_units(wave_total(units), shares), n = shares_of(units, share);  // (at most 2^23 units each)
         const int through = wave_prefix(n);
         const unsigned long long past = __ballot(through > slot);
         if (!past) return Place{-1, 0, 0};
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256, 3) void paged_decode_split(DecodeArgs a, typen
     sh.b = pl.b, sh.kvh = x / tiles, sh.h0 = 16 * (x % tiles), sh.heads = min(16, a.group - sh.h0);
     share_rows(paged_length(bt, pl.b, c.shift), pl.count, pl.index, sh.r0, sh.r1);
     sh.alone = pl.count == 1, sh.slot = slot;
-    decode_share<E, D, T, NT>(a, c, bt, sh, ow, mw, lw);
+    decode_share<E, D, T, NT, 4>(a, c, bt, sh, threadIdx.x, ow, mw, lw);
 }
 
 // grid (QH, B), 256 threads: the shares of one head of a sequence, wave w taking w, w + 4, ..; the four waves' sums meet

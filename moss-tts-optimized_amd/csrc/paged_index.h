@@ -42,8 +42,9 @@ MOSS_HD void clamp_tokens(int s0, int s1, int T, int& first, int& count) {
 // more per sequence; a sequence's units are spread evenly over its own shares.
 constexpr int kUnit = 128;
 MOSS_HD int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
-MOSS_HD int share_of_units(long long total, int shares) {
-    const long long share = total <= shares ? 1 : (total + shares - 1) / shares;
+template <typename N>  // of int (totals up to 2^30) or long long
+MOSS_HD int share_of_units(N total, int shares) {
+    const N share = total <= shares ? 1 : (total + shares - 1) / shares;
     return share < (1 << 24) ? (int)share : 1 << 24;  // no sequence has more units
 }
 MOSS_HD int shares_of(int units, int share) { return (units + share - 1) / share; }
@@ -135,19 +136,22 @@ MOSS_HD int shared_from(int rows, int want, int length) {
     const int most = want < rows ? want : rows;
     return length <= most ? length : most & ~15;
 }
-// Blocks of a part of a tile's keys: the tiles' blocks, `total` of them, in at most `shares` parts and one more a tile.
-constexpr int kPrefixShare = 2;
-MOSS_HD int prefix_share_of(long long total, int shares) {
-    const long long share = (total + shares - 1) / shares;
-    return share < kPrefixShare ? kPrefixShare : share < (1 << 24) ? (int)share : 1 << 24;
+// A line of work, `all` long, in `pieces` equal pieces.  Part (piece w, thing k) of what the line holds in order has the number
+// w + k: either grows along the line, and from a part to the next one of them does.
+MOSS_HD int piece_of(long long all, int pieces) {
+    const long long piece = all < 1ll << 31 ? (long long)(((unsigned)all + (unsigned)pieces - 1) / (unsigned)pieces) : (all + pieces - 1) / pieces;
+    return piece < 1 ? 1 : piece < (1ll << 30) ? (int)piece : 1 << 30;
 }
-// At most: parts of all tiles, and rows of partial results.  A run has at least two sequences, so there are at most B / 2, and its
-// tiles are size * group / height rounded up; a run's parts hold its rows each, and beyond the first part of each tile the parts
-// are whole shares, so at most `shares` tiles' rows.
-inline void prefix_bounds(int B, int group, int height, int shares, long long& items, long long& rows) {
-    const long long all = (long long)B * group;
-    items = B > 1 ? (all + height - 1) / height + B / 2 + shares : 1;
-    rows = B > 1 ? all + (long long)height * shares : 1;
+// Of `workgroups` (2 at least), how many take the prefixes' blocks and not the units of own rows.
+constexpr float kBlockCost = 3.f, kUnitCost = 2.f;
+MOSS_HD int prefix_takers(float blocks, float units, int workgroups) {
+    if (blocks <= 0.f) return 0;
+    if (units <= 0.f) return workgroups;
+    const float share = blocks * kBlockCost / (blocks * kBlockCost + units * kUnitCost);
+    return clamp_int((int)(share * (float)workgroups + 0.5f), 1, workgroups - 1);
+}
+MOSS_HD long long quotient(long long a, int b) {  // of what is not negative; in 32 bits where that is enough
+    return a < 1ll << 32 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
 inline long long decode_slots(int B, int W, int shift, int shares) {
     const long long most = (long long)B * ((((long long)W << shift) + kUnit - 1) / kUnit);

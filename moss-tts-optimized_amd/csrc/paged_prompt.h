@@ -158,14 +158,22 @@ struct TileRows {
 template <int D>
 using Stage = unsigned char[4 * D * kPromptBlock];
 
+// The thread's index for a function that is called in a loop: what such a function computes from it is computed in each call, and
+// not kept in registers from one to the next.
+__device__ __forceinline__ int fresh_thread() {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    return tid;
+}
+
 // o, m, l of the rows (l summed over the lane's keys and, on return, its partner's).  KS 2: two waves share the rows and halve a
 // block's keys; false: this wave's part went to the other.
 template <typename E, int D, int KS, typename S>
 __device__ __forceinline__ bool attend_rows(const typename S::Cache& c, const TileRows& t, int W, const u32x4_t (&qf)[D / 16], float scale,
-                                            Stage<D>& even, Stage<D>& odd, f32x16_v (&o_out)[D / 32], float& m_out, float& l_out) {
+                                            int tid, Stage<D>& even, Stage<D>& odd, f32x16_v (&o_out)[D / 32], float& m_out, float& l_out) {
     constexpr int NT = 2 / KS, BK = kPromptBlock, DT = D / 32, DK = D / 16, RB = 2 * D, KB = BK * RB;  // NT: a wave's 32-key tiles
-    const int lane = threadIdx.x & 63, half = lane >> 5, rl = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % (4 / KS), kq = KS == 1 ? 0 : wave / (4 / KS);
+    const int lane = tid & 63, half = lane >> 5, rl = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % (4 / KS), kq = KS == 1 ? 0 : wave / (4 / KS);
     const int kvh = t.kvh, b0 = t.b0, b1 = t.b1, last = t.last, qpos = t.qpos, wave_first = t.wave_first, wave_last = t.wave_last;
     const bool idle = t.idle;
     const int* trow = t.trow;

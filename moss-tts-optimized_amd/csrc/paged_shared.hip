@@ -8,16 +8,27 @@
 // from its own.  A run of one shares nothing.
 //
 // The prefix: all of a run's query heads of a KV head are the rows of tiles, which go over the keys on the matrix cores
-// (paged_prompt.h), row b up to key n_b; a tile's keys are cut into parts, so that few tiles fill the device.  The rest: paged_decode.h,
-// from row n_b on.  Both leave (m, l, O), and a last launch joins a sequence's.  Who takes what is computed on the device by
-// every wave from groups, shared and lengths, so that a captured graph follows them.
+// (paged_prompt.h), row b up to key n_b.  The rest: paged_decode.h, from row n_b on.  Both leave (m, l, O), and a last launch
+// joins a sequence's.
+//
+// Who takes what follows from groups, shared and lengths on the device, so that a captured graph follows them.  The work of a KV
+// head are two lines: the blocks of 64 keys of every tile, tile after tile, and the units of 128 own rows of every sequence.
+// Of the workgroups (two a CU in all), some take the first, a piece each, and the others the second, a piece a wave, in the
+// proportion of what the lines cost; a piece that passes the end of a tile or a sequence leaves more than one result.
 #include "paged_decode.h"
 #include "paged_prompt.h"
 
 namespace moss {
 namespace {
 
-constexpr int kPrefixTarget = 256;  // workgroups that the prefixes are shared out over
+constexpr int kWorkgroups = 512;  // over all KV heads
+
+// Rows of a KV head that sharing has to save in a batch, over all KV heads.  Alone / shared, us, sequences over 4096 shared rows
+// of 32 / 8 heads: 2 (32768) 15.7 / 19.5, 4 (98304) 19.5 / 21.0, 8 (229376) 25.0 / 23.1, 16 35 / 26, 64 99 / 37; 16 over 640
+// (76800) 17.1 / 17.1, over 1536 (184320) 23.4 / 22.1; 12 / 12 heads of 64, 8 over 1536 (129024) 15.0 / 15.8, over 4096 22 / 19;
+// 16 / 1 heads, 32 over 4096 (126976) 26.2 / 26.2, 64 over 1536 (96768) 24.0 / 26.5.  What the shared rows cost alone is so
+// little because the caches serve all but the first reader.
+constexpr int kWorth = 131072;
 
 struct SharedArgs {
     DecodeArgs a;             // part and stat: of the sequences' own rows
@@ -26,7 +37,9 @@ struct SharedArgs {
     float* prefix_part;       // [KH, rows, D]
     float2* prefix_stat;      // [KH, rows]
     long long prefix_rows;
-    int prefix_shares;
+    struct Found* found;      // [B]
+    int worth;                   // rows in sixteens that have to be saved
+    int workgroups, head_tiles;  // workgroups of a KV head; tiles of 16 of its heads, for the own rows
 };
 
 // Sequence b0 + lane of the batch: where its own rows begin, and its run.
@@ -54,52 +67,126 @@ __device__ __forceinline__ Member member_of(const SharedArgs& s, const PagedBatc
     return m;
 }
 
+// Whether sharing saves enough rows to be worth the prefix's own way; if not, every sequence is taken alone.  (Rows in sixteens,
+// and no more of a run than decide by themselves, so that the sum fits 32 bits.)
+__device__ __forceinline__ int saved_by(const Member& m, int lane) {
+    return m.first == lane ? (m.size - 1) * min(m.rows >> 4, 1 << 14) : 0;
+}
+template <typename At>
+__device__ __forceinline__ bool worth_sharing(const SharedArgs& s, int B, int lane, At at) {
+    if (B <= kWave) return wave_total(saved_by(at(0), lane)) >= s.worth;
+    for (int b0 = 0, saved = 0; b0 < B; b0 += kWave) {
+        saved += wave_total(saved_by(at(b0), lane));  // ends at the first that is enough: no overflow
+        if (saved >= s.worth) return true;
+    }
+    return false;
+}
+// Members as they are taken.
+struct Members {
+    const SharedArgs& s;
+    const PagedBatch& bt;
+    int shift, lane;
+    Member m0;
+    bool worth;
+    __device__ __forceinline__ Members(const SharedArgs& s, const PagedBatch& bt, int shift, int lane)
+        : s(s), bt(bt), shift(shift), lane(lane), m0(member_of(s, bt, shift, 0, lane)) {
+        worth = worth_sharing(s, bt.B, lane, [&](int b0) { return b0 == 0 ? m0 : member_of(s, bt, shift, b0, lane); });
+        if (!worth) m0.from = m0.rows = 0;
+    }
+    __device__ __forceinline__ Member operator()(int b0) const {
+        if (b0 == 0) return m0;
+        Member m = member_of(s, bt, shift, b0, lane);
+        if (!worth) m.from = m.rows = 0;
+        return m;
+    }
+};
+
+__device__ __forceinline__ long long shfl64(long long v, int lane) {
+    return (long long)((unsigned long long)(unsigned)__shfl((int)(v >> 32), lane) << 32 | (unsigned)__shfl((int)v, lane));
+}
+
 // A run's tiles of `height` rows (of its first lane; 0 elsewhere), and their blocks of keys.
 __device__ __forceinline__ int tiles_of(const Member& m, int group, int height, int lane) {
     return m.first == lane && m.rows > 0 ? (m.size * group + height - 1) / height : 0;
 }
 __device__ __forceinline__ int blocks_of(const Member& m) { return (m.rows + kPromptBlock - 1) / kPromptBlock; }
 
-// What the batch's work is cut into: blocks of keys of a part of a prefix, units of a share of own rows, parts in all.  `at(b0)`
-// gives the members from sequence b0 on.
-struct Cuts {
-    int share, units;
-    long long items;
+// The two lines of a KV head's work, how many workgroups take the first, and the pieces' lengths.  `at(b0)` gives the members from
+// sequence b0 on.
+struct Lines {
+    long long blocks, units;
+    int takers, blocks_each, units_each;
 };
 template <int HEIGHT, typename At>
-__device__ __forceinline__ Cuts cuts_of(const SharedArgs& s, int B, int lane, At at) {
-    long long blocks = 0, units = 0, items = 0;
+__device__ __forceinline__ Lines lines_of(const SharedArgs& s, int B, int lane, At at) {
+    long long blocks = 0, units = 0;
     for (int b0 = 0; b0 < B; b0 += kWave) {
         const Member m = at(b0);
         blocks += (long long)tiles_of(m, s.a.group, HEIGHT, lane) * blocks_of(m);
         units += units_of(m.own());
     }
-    Cuts c;
-    c.share = prefix_share_of(wave_total(blocks), s.prefix_shares);
-    c.units = share_of_units(wave_total(units), s.a.shares);
-    for (int b0 = 0; b0 < B; b0 += kWave) {
-        const Member m = at(b0);
-        items += (long long)tiles_of(m, s.a.group, HEIGHT, lane) * shares_of(blocks_of(m), c.share);
-    }
-    c.items = wave_total(items);
-    return c;
+    Lines l;
+    l.blocks = wave_total(blocks), l.units = wave_total(units) * s.head_tiles;
+    l.takers = __builtin_amdgcn_readfirstlane(prefix_takers((float)l.blocks, (float)l.units, s.workgroups));
+    l.blocks_each = piece_of(l.blocks, max(l.takers, 1));
+    l.units_each = piece_of(l.units, 4 * max(s.workgroups - l.takers, 1));
+    return l;
 }
 
-// One part of a run's prefix for a tile of its rows.
+// Where the tiles of the runs that begin at sequences b0 + lane lie.
+struct Places {
+    long long end;  // on the line of blocks; the lane's tiles lie before it
+    int rows_end;   // rows of the tiles so far
+    int tiles, blocks;
+};
+template <int HEIGHT>
+__device__ __forceinline__ Places places_of(const SharedArgs& s, const Member& m, int lane, long long before, int rows_before) {
+    Places p;
+    p.tiles = tiles_of(m, s.a.group, HEIGHT, lane), p.blocks = p.tiles ? blocks_of(m) : 0;
+    p.end = before + wave_prefix((long long)p.tiles * p.blocks);
+    p.rows_end = rows_before + wave_prefix(p.tiles ? m.size * s.a.group : 0);
+    return p;
+}
+// Where the own rows of sequences b0 + lane end on the line of units.
+__device__ __forceinline__ long long units_end(const SharedArgs& s, const Member& m, long long before) {
+    return before + wave_prefix((long long)units_of(m.own()) * s.head_tiles);
+}
+
+// What the join has to know of a sequence, written by the last workgroup: its run's first block on the line, the blocks of a
+// tile (0: nothing shared), its row among the run's and among all partial rows; its first unit and units; the pieces.
+struct Found {
+    long long block, unit;
+    int blocks, in_run, row, units;
+    int blocks_each, units_each;
+};
+
+// The chunk of 64 sequences that a workgroup is at, in LDS: in registers it would lie beside the products' (50 of which went to
+// memory).
+struct Chunk {
+    long long end[kWave];
+    int rows_end[kWave], tiles[kWave], blocks[kWave];
+    int from[kWave], size[kWave], rows[kWave];
+    __device__ __forceinline__ void put(const Member& m, const Places& p, int lane) {  // by one wave
+        end[lane] = p.end, rows_end[lane] = p.rows_end, tiles[lane] = p.tiles, blocks[lane] = p.blocks;
+        from[lane] = m.from, size[lane] = m.size, rows[lane] = m.rows;
+    }
+};
+// A value that is the same in all lanes, in a scalar.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long long scalar(long long v) { return lane_value(v, 0); }
+
+// Some blocks of a tile.
 template <typename E, int D, int KS, typename S>
-__device__ __forceinline__ void prefix_part(const SharedArgs& s, const typename S::Cache& c, const PagedBatch& bt, const Member& m, int b0,
-                                            int l, int base, int index, int share, int kvh, Stage<D>& even, Stage<D>& odd) {
+__device__ __forceinline__ void prefix_part(const SharedArgs& s, const typename S::Cache& c, const PagedBatch& bt, const Chunk& ch, int b0,
+                                            int l, int tile, int from, int to, long long out0, int kvh, Stage<D>& even, Stage<D>& odd) {
     constexpr int HEIGHT = 128 / KS, RW = 4 / KS, DT = D / 32, DK = D / 16;
     const DecodeArgs& a = s.a;
-    const int lane = threadIdx.x & (kWave - 1), half = lane >> 5, rl = lane & 31, G = a.group;
-    const int rw = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) % RW;
-    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const int size = lane_value(m.size, l), P = lane_value(m.rows, l), blocks = (P + kPromptBlock - 1) / kPromptBlock;
-    const int parts = shares_of(blocks, share), tile = uniform(index / parts), part = uniform(index % parts);
-    const int nrows = size * G, row = min(tile * HEIGHT + 32 * rw + rl, nrows - 1);  // clamped: stores are guarded
+    const int tid = fresh_thread(), lane = tid & (kWave - 1), half = lane >> 5, rl = lane & 31, G = a.group;
+    const int rw = scalar(tid >> 6) % RW;
+    const int nrows = scalar(ch.size[l]) * G, row = min(tile * HEIGHT + 32 * rw + rl, nrows - 1);  // clamped: stores are guarded
     const int token = (int)((unsigned)row / (unsigned)G), head = kvh * G + row - token * G;
     TileRows rows;
-    rows.qpos = __shfl(m.from, l + token) - 1;
+    rows.qpos = ch.from[l + token] - 1;
     const int b = b0 + l;
     u32x4_t qf[DK];  // lane: row rl, dims 16 kk + 8 half .. + 7
     {
@@ -114,14 +201,14 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& s, const typename 
         most = max(most, __shfl_xor(most, x));
     }
     rows.trow = bt.table + (size_t)b * bt.table_stride;
-    rows.kvh = kvh, rows.b0 = part * share, rows.b1 = min(blocks, rows.b0 + share), rows.last = P - 1;
-    rows.wave_first = uniform(least), rows.wave_last = uniform(most);
+    rows.kvh = kvh, rows.b0 = from, rows.b1 = to, rows.last = scalar(ch.rows[l]) - 1;
+    rows.wave_first = scalar(least), rows.wave_last = scalar(most);
     rows.idle = tile * HEIGHT + 32 * rw >= nrows;
     f32x16_v o[DT];
     float mx, sum;
-    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, even, odd, o, mx, sum)) return;
-    const int out = base + part * nrows + row;
-    if (tile * HEIGHT + 32 * rw + rl >= nrows || !in_slots(out, 1, s.prefix_rows)) return;
+    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, tid, even, odd, o, mx, sum)) return;
+    const long long out = out0 + 32 * rw + rl;
+    if (tile * HEIGHT + 32 * rw + rl >= nrows || out < 0 || out >= s.prefix_rows) return;
     const size_t at = (size_t)kvh * s.prefix_rows + out;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -132,191 +219,217 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& s, const typename 
     if (half == 0) s.prefix_stat[at] = make_float2(mx, sum);
 }
 
-// The parts of the prefixes (matrix cores) and the shares of the rest (memory) side by side in one launch, the parts first.
+// Grid: workgroups of a KV head * KV heads; neighbours, which lie on different XCDs, differ in the KV head.
 template <typename E, int D, int KS, typename S, typename T, bool NT>
 __global__ __launch_bounds__(256, 2) void paged_shared_split(SharedArgs s, typename S::Cache c, PagedBatch bt) {
     constexpr int HEIGHT = 128 / KS;
     __shared__ __attribute__((aligned(1024))) Stage<D> even, odd;
+    __shared__ Chunk ch;
     const DecodeArgs& a = s.a;
-    const int lane = threadIdx.x & (kWave - 1), G = a.group;
-    const Member m0 = member_of(s, bt, c.shift, 0, lane);
-    auto at = [&](int b0) { return b0 == 0 ? m0 : member_of(s, bt, c.shift, b0, lane); };
-    const Cuts cuts = cuts_of<HEIGHT>(s, bt.B, lane, at);
-    const long long prefixes = cuts.items * c.kh;
-    if (blockIdx.x < prefixes) {
-        const int kvh = blockIdx.x % c.kh, item = blockIdx.x / c.kh;
-        int before = 0, base = 0;
-        for (int b0 = 0; b0 < bt.B; b0 += kWave) {
-            const Member m = at(b0);
-            const int tiles = tiles_of(m, G, HEIGHT, lane), parts = shares_of(blocks_of(m), cuts.share), n = tiles * parts;
-            const int rows = tiles ? m.size * G * parts : 0;
-            const int through = wave_prefix(n), rows_through = wave_prefix(rows);
-            const unsigned long long past = __ballot(before + through > item);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                prefix_part<E, D, KS, S>(s, c, bt, m, b0, l, base + lane_value(rows_through, l) - lane_value(rows, l),
-                                         item - before - (lane_value(through, l) - lane_value(n, l)), cuts.share, kvh, even, odd);
-                return;
+    const int lane = threadIdx.x & (kWave - 1), G = a.group, kvh = blockIdx.x % c.kh, w = blockIdx.x / c.kh;
+    const Members at(s, bt, c.shift, lane);
+    const Member m0 = at(0);
+    const Lines lines = lines_of<HEIGHT>(s, bt.B, lane, at);
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x < kWave) {
+        Member m = m0;
+        Places p = places_of<HEIGHT>(s, m, lane, 0, 0);
+        long long ends = units_end(s, m, 0);
+        for (int b0 = 0;;) {
+            Found f;
+            f.blocks = m.from > 0 ? __shfl(p.blocks, m.first) : 0;
+            f.block = shfl64(p.end, m.first) - (long long)__shfl(p.tiles, m.first) * __shfl(p.blocks, m.first);
+            f.in_run = (lane - m.first) * G;
+            f.row = __shfl(p.rows_end, m.first) - m.size * G + f.in_run;
+            f.units = units_of(m.own());
+            f.unit = ends - (long long)f.units * s.head_tiles;
+            f.blocks_each = lines.blocks_each, f.units_each = lines.units_each;
+            if (b0 + lane < bt.B) s.found[b0 + lane] = f;
+            b0 += kWave;
+            if (b0 >= bt.B) break;
+            const long long before = lane_value(p.end, kWave - 1), units = lane_value(ends, kWave - 1);
+            const int rows = lane_value(p.rows_end, kWave - 1);
+            m = at(b0);
+            p = places_of<HEIGHT>(s, m, lane, before, rows);
+            ends = units_end(s, m, units);
+        }
+    }
+    if (w < lines.takers) {
+        long long pos = (long long)w * lines.blocks_each;
+        const long long end = min(pos + lines.blocks_each, lines.blocks);
+        if (pos >= end) return;
+        const bool writer = threadIdx.x < kWave;
+        {
+            const Places p = places_of<HEIGHT>(s, m0, lane, 0, 0);
+            if (writer) ch.put(m0, p, lane);
+            __syncthreads();
+        }
+        for (int b0 = 0;;) {
+            const unsigned long long past = __ballot(ch.end[lane] > pos);
+            if (!past) {  // further on
+                b0 += kWave;
+                if (b0 >= bt.B) return;
+                const Member m = at(b0);
+                const Places p = places_of<HEIGHT>(s, m, lane, ch.end[kWave - 1], ch.rows_end[kWave - 1]);
+                __syncthreads();
+                if (writer) ch.put(m, p, lane);
+                __syncthreads();
+                continue;
             }
-            before += lane_value(through, kWave - 1);
-            base += lane_value(rows_through, kWave - 1);
+            const int l = __builtin_ctzll(past), blocks = scalar(ch.blocks[l]);
+            const long long in = pos - (scalar(ch.end[l]) - (long long)scalar(ch.tiles[l]) * blocks);
+            const int tile = scalar((int)quotient(in, blocks)), from = scalar((int)(in - (long long)tile * blocks));
+            const int to = scalar((int)min((long long)blocks, from + (end - pos)));
+            const long long out = scalar(ch.rows_end[l]) - scalar(ch.size[l]) * G + tile * HEIGHT + (long long)w * HEIGHT;
+            prefix_part<E, D, KS, S>(s, c, bt, ch, b0, l, tile, from, to, out, kvh, even, odd);
+            pos += to - from;
+            if (pos >= end) return;
+            __syncthreads();  // everyone is done with the LDS
         }
-        return;
     }
-    const int tiles = (G + 15) / 16, own = (int)(blockIdx.x - prefixes), slot = own / a.xdim, x = own % a.xdim;
-    ShareOf sh;
-    int before = 0;
-    sh.b = -1;
-    for (int b0 = 0; b0 < bt.B; b0 += kWave) {
-        const Member m = at(b0);
-        const int n = shares_of(units_of(m.own()), cuts.units), through = wave_prefix(n);
-        const unsigned long long past = __ballot(before + through > slot);
-        if (past) {
-            const int l = __builtin_ctzll(past), count = lane_value(n, l), from = lane_value(m.from, l);
-            sh.b = b0 + l;
-            share_rows(lane_value(m.length, l) - from, count, slot - before - (lane_value(through, l) - count), sh.r0, sh.r1);
-            sh.r0 += from, sh.r1 += from;
-            sh.alone = count == 1 && from == 0;
-            break;
+    const int v = (w - lines.takers) * 4 + scalar((int)threadIdx.x >> 6);
+    long long pos = (long long)v * lines.units_each;
+    const long long end = min(pos + lines.units_each, lines.units);
+    if (pos >= end) return;
+    Member m = m0;
+    long long ends = units_end(s, m, 0);
+    for (int b0 = 0; pos < end;) {
+        const unsigned long long past = __ballot(ends > pos);
+        if (!past) {
+            b0 += kWave;
+            if (b0 >= bt.B) return;
+            m = at(b0);
+            ends = units_end(s, m, lane_value(ends, kWave - 1));
+            continue;
         }
-        before += lane_value(through, kWave - 1);
+        const int l = __builtin_ctzll(past), from = lane_value(m.from, l), rows = lane_value(m.length, l) - from, units = units_of(rows);
+        const long long in = pos - (lane_value(ends, l) - (long long)units * s.head_tiles);
+        const int tile = scalar((int)quotient(in, units)), u0 = scalar((int)(in - (long long)tile * units));
+        const int u1 = scalar((int)min((long long)units, u0 + (end - pos)));
+        pos += u1 - u0;
+        ShareOf sh;
+        sh.b = b0 + l, sh.slot = (long long)v + sh.b;
+        sh.kvh = kvh, sh.h0 = 16 * tile, sh.heads = min(16, G - sh.h0);
+        sh.r0 = from + u0 * kUnit, sh.r1 = from + (int)min((long long)rows, (long long)u1 * kUnit);
+        sh.alone = from == 0 && u0 == 0 && u1 == units;
+        if (sh.slot >= a.slots) return;
+        float(&none)[2][4][16] = *reinterpret_cast<float(*)[2][4][16]>(odd);
+        decode_share<E, D, T, NT, 1>(a, c, bt, sh, fresh_thread(), *reinterpret_cast<float(*)[4][16][D]>(even), none[0], none[1]);
     }
-    if (sh.b < 0 || slot >= a.slots) return;
-    sh.kvh = x / tiles, sh.h0 = 16 * (x % tiles), sh.heads = min(16, G - sh.h0), sh.slot = slot;
-    static_assert(sizeof(float[4][16][D]) <= sizeof(Stage<D>) && 2 * sizeof(float[4][16]) <= sizeof(Stage<D>), "");
-    float(&ml)[2][4][16] = *reinterpret_cast<float(*)[2][4][16]>(odd);
-    decode_share<E, D, T, NT>(a, c, bt, sh, *reinterpret_cast<float(*)[4][16][D]>(even), ml[0], ml[1]);
 }
 
-// grid (QH, B), 256 threads: the parts of the prefix and the shares of the rest of one head of a sequence, wave w taking w, w + 4,
-// ..; the four waves' sums meet in LDS.
+// grid (QH / 4, B) rounded up, a wave a head: the parts of its prefix and of its sequence's own rows.
 template <typename E, int D, int HEIGHT>
-__global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s, int shift, PagedBatch bt) {
+__global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s) {
     constexpr int VPL = D / kWave;
-    __shared__ float acc_s[4][D];
     const DecodeArgs& a = s.a;
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave, G = a.group;
-    const int mine = b % kWave;
-    const Member m0 = member_of(s, bt, shift, 0, lane);
-    auto at = [&](int b0) { return b0 == 0 ? m0 : member_of(s, bt, shift, b0, lane); };
-    const Cuts cuts = cuts_of<HEIGHT>(s, bt.B, lane, at);
-    const int share = cuts.share, su = cuts.units;
-    // partial results before this sequence's, and its run
-    Member m;
-    int slots = 0, rows = 0;
-    for (int b0 = 0;; b0 += kWave) {
-        m = at(b0);
-        const int n = shares_of(units_of(m.own()), su);
-        const int r = tiles_of(m, G, HEIGHT, lane) ? m.size * G * shares_of(blocks_of(m), share) : 0;
-        if (b0 + kWave > b) {
-            const int l = lane_value(m.first, mine);
-            slots += wave_total(lane < mine ? n : 0);
-            rows += wave_total(lane < l ? r : 0);
-            break;
-        }
-        slots += wave_total(n);
-        rows += wave_total(r);
+    const int lane = threadIdx.x & (kWave - 1), b = blockIdx.y, G = a.group;
+    const int h = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + threadIdx.x / kWave));
+    if (h >= a.qh) return;
+    const Found f = s.found[b];
+    // the pieces that hold the tile's blocks, and those that hold the own rows
+    int pieces = 0, pieces_own = 0, w0 = 0, w1 = 0;
+    long long row = 0;
+    if (f.blocks > 0) {
+        const long long start = f.block + (long long)((f.in_run + h % G) / HEIGHT) * f.blocks;
+        w0 = (int)quotient(start, f.blocks_each);
+        pieces = (int)quotient(start + f.blocks - 1, f.blocks_each) - w0 + 1;
+        row = f.row + h % G + (long long)w0 * HEIGHT;
     }
-    const int own = shares_of(units_of(lane_value(m.own(), mine)), su), from = lane_value(m.from, mine);
-    const int parts = from > 0 ? shares_of((lane_value(m.rows, mine) + kPromptBlock - 1) / kPromptBlock, share) : 0;
-    if (parts == 0 && own == 1) return;  // written by its workgroup
-    uint16_t* dst = a.out + ((size_t)b * a.qh + h) * D;
-    const int count = parts + own;
-    if (count == 0) {
-        for (int d = tid; d < D; d += 256) dst[d] = 0;
-        return;
+    if (f.units > 0) {
+        const long long start = f.unit + (long long)f.units * (h % G / 16);
+        w1 = (int)quotient(start, f.units_each);
+        pieces_own = (int)quotient(start + f.units - 1, f.units_each) - w1 + 1;
     }
-    const int first = lane_value(m.first, mine), nrows = lane_value(m.size, mine) * G;
-    const int row = rows + (mine - first) * G + h % G;
-    // only when what says where rows are changes between the launches
-    if (!in_slots(slots, own, a.slots) || (parts && !in_slots(row, (parts - 1) * nrows + 1, s.prefix_rows))) return;
+    if (pieces == 0 && pieces_own == 1) return;  // written by its workgroup
+    uint16_t* dst = a.out + ((size_t)b * a.qh + h) * D + VPL * lane;
+    const int count = pieces + pieces_own;
+    const long long slot = (long long)w1 + b;
+    if (pieces < 0 || pieces_own < 0 || slot < 0 || slot + pieces_own > a.slots || row < 0 ||
+        (pieces && row + (long long)(pieces - 1) * HEIGHT >= s.prefix_rows))
+        return;  // only where another call writes the same workspace
     // part i's place among the statistics and results: the prefix's, then the sequence's own
-    const size_t step = nrows;
-    const float2* stat0 = s.prefix_stat + (size_t)(h / G) * s.prefix_rows + row;
-    const float2* stat1 = a.stat + (size_t)slots * a.qh + h;
-    const float* part0 = s.prefix_part + ((size_t)(h / G) * s.prefix_rows + row) * D;
-    const float* part1 = a.part + ((size_t)slots * a.qh + h) * D;
-    auto stat = [&](int i) { return i < parts ? stat0[i * step] : stat1[(size_t)(i - parts) * a.qh]; };
-    auto part = [&](int i) { return i < parts ? part0 + i * step * D : part1 + (size_t)(i - parts) * a.qh * D; };
-    const float2 mls = lane < count ? stat(lane) : make_float2(-INFINITY, 0.f);
-    float mx = mls.x;
-    for (int i = kWave + lane; i < count; i += kWave) mx = fmaxf(mx, stat(i).x);
-    mx = wave_max(mx);
-    auto weight = [&](float v) { return v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v - mx); };
-    const float f0 = weight(mls.x);
-    float den = f0 * mls.y;
-    for (int i = kWave + lane; i < count; i += kWave) {
-        const float2 v = stat(i);
-        den += weight(v.x) * v.y;
-    }
-    den = wave_sum(den);
+    const long long row0 = (long long)(h / G) * s.prefix_rows + row, row1 = slot * a.qh + h;
+    auto stat = [&](int i) {
+        return i < pieces ? s.prefix_stat[row0 + (long long)i * HEIGHT] : a.stat[row1 + (long long)(i - pieces) * a.qh];
+    };
+    auto part = [&](int i) {
+        return (i < pieces ? s.prefix_part + (row0 + (long long)i * HEIGHT) * D : a.part + (row1 + (long long)(i - pieces) * a.qh) * D) +
+               VPL * lane;
+    };
+    const float2 own = lane < count ? stat(lane) : make_float2(-INFINITY, 0.f);
+    constexpr int N = 16;  // parts on their way together
+    float x[N][VPL];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const float* from_part = part(min(i0 + n, max(count - 1, 0)));
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) x[n][i] = from_part[i];
+        }
+    };
     float acc[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
-    constexpr int N = 8;  // parts on their way together: w, w + 4, ..
-    for (int s0 = w; s0 < count; s0 += 4 * N) {
-        float x[N][VPL], f[N];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const float* p = part(min(s0 + 4 * n, count - 1)) + VPL * lane;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) x[n][i] = p[i];
+    float den = 0.f;
+    if (count) {
+        load(0);
+        float mx = own.x;
+        for (int i = kWave + lane; i < count; i += kWave) mx = fmaxf(mx, stat(i).x);
+        mx = wave_max(mx);
+        auto weight = [&](float v) { return v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v - mx); };
+        const float f0 = weight(own.x);
+        den = f0 * own.y;
+        for (int i = kWave + lane; i < count; i += kWave) {
+            const float2 v = stat(i);
+            den += weight(v.x) * v.y;
         }
+        den = wave_sum(den);
+        for (int i0 = 0; i0 < count; i0 += N) {
+            if (i0) load(i0);
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = min(s0 + 4 * n, count - 1);
-            f[n] = i < kWave ? __uint_as_float(lane_value(__float_as_uint(f0), i)) : weight(stat(i).x);
-            if (s0 + 4 * n >= count) f[n] = 0.f;
+            for (int n = 0; n < N; ++n) {
+                const int i = min(i0 + n, count - 1);
+                float f = i < kWave ? __uint_as_float(lane_value(__float_as_uint(f0), i)) : weight(stat(i).x);
+                if (i0 + n >= count) f = 0.f;
+#pragma unroll
+                for (int k = 0; k < VPL; ++k) acc[k] = f == 0.f ? acc[k] : fmaf(f, x[n][k], acc[k]);
+            }
         }
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) acc[i] = f[n] == 0.f ? acc[i] : fmaf(f[n], x[n][i], acc[i]);
     }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) acc_s[w][VPL * lane + i] = acc[i];
-    __syncthreads();
-    if (tid < D / 2) {
-        const float inv = den == 0.f ? 0.f : 1.0f / den;
-        float x = 0.f, y = 0.f;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            x += acc_s[v][2 * tid];
-            y += acc_s[v][2 * tid + 1];
-        }
-        reinterpret_cast<uint32_t*>(dst)[tid] = E::pack(x * inv, y * inv);
+    const float inv = den == 0.f ? 0.f : 1.0f / den;
+    if constexpr (VPL == 2) {
+        *reinterpret_cast<uint32_t*>(dst) = E::pack(acc[0] * inv, acc[1] * inv);
+    } else {
+        *dst = (uint16_t)E::pack(acc[0] * inv, 0.f);
     }
 }
 
 struct SharedPlan {
-    int xdim, shares, prefix_shares;
-    long long slots, rows, items;  // of the prefixes: rows of partial results, workgroups a KV head at most
-    int height;
+    int workgroups, height, head_tiles;
+    long long slots, rows;  // partial results of own rows, of prefix rows
 };
 
-SharedPlan shared_plan(int B, int W, int shift, int qh, int kh) {
+SharedPlan shared_plan(int B, int qh, int kh) {
     SharedPlan p;
     const long long G = qh / kh;
-    p.xdim = kh * (int)((G + 15) / 16);
-    p.shares = kTarget / p.xdim > 1 ? kTarget / p.xdim : 1;
-    p.slots = decode_slots(B, W, shift, p.shares);
-    p.prefix_shares = kPrefixTarget / kh > 1 ? kPrefixTarget / kh : 1;
+    p.head_tiles = (int)((G + 15) / 16);
+    p.workgroups = kWorkgroups / kh > 2 ? kWorkgroups / kh : 2;
     p.height = B * G * kh <= 1024 ? 64 : 128;
-    prefix_bounds(B, (int)G, p.height, p.prefix_shares, p.items, p.rows);
+    p.slots = 4ll * p.workgroups + B;
+    p.rows = B * G + (long long)p.workgroups * p.height;
     return p;
 }
 
 template <typename E, int D, int KS, typename T, typename S>
 int launch_shared(const SharedArgs& s, const typename S::Cache& c, const PagedBatch& bt, const SharedPlan& p, hipStream_t st) {
-    const long long blocks = p.items * c.kh + p.slots * p.xdim;
-    MOSS_CHECK_ARG(blocks * 256 < (1ll << 32));
     const long long page = ((long long)c.kh << c.shift) * D * (std::is_same<typename S::Cache, PagedCache>::value ? 2 : 1);
     const long long named = (long long)bt.B * bt.W;
+    const dim3 grid((unsigned)(p.workgroups * c.kh)), joins((unsigned)(s.a.qh + 3) / 4, (unsigned)bt.B);
     if ((named < c.pages ? named : c.pages) * page * 2 > kCached)
-        hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, true>), dim3((unsigned)blocks), dim3(256), 0, st, s, c, bt);
+        hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, true>), grid, dim3(256), 0, st, s, c, bt);
     else
-        hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, false>), dim3((unsigned)blocks), dim3(256), 0, st, s, c, bt);
-    hipLaunchKernelGGL((paged_shared_join<E, D, 128 / KS>), dim3((unsigned)s.a.qh, (unsigned)bt.B), dim3(256), 0, st, s, c.shift, bt);
+        hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, false>), grid, dim3(256), 0, st, s, c, bt);
+    hipLaunchKernelGGL((paged_shared_join<E, D, 128 / KS>), joins, dim3(256), 0, st, s);
     return moss_launch_status();
 }
 
@@ -325,7 +438,9 @@ int launch_shared(const SharedArgs& s, const Cache& c, const PagedBatch& bt, con
     return p.height == 64 ? launch_shared<E, D, 2, T<E, D>, S<E, D>>(s, c, bt, p, st) : launch_shared<E, D, 1, T<E, D>, S<E, D>>(s, c, bt, p, st);
 }
 
-long long workspace_bytes_of(const SharedPlan& p, int qh, int kh, int d) { return (p.slots * qh + p.rows * kh) * (d + 2) * 4; }
+long long workspace_bytes_of(const SharedPlan& p, int B, int qh, int kh, int d) {
+    return (p.slots * qh + p.rows * kh) * (d + 2) * 4 + B * (long long)sizeof(Found);
+}
 
 template <template <typename, int> class T, template <typename, int> class S, typename Cache>
 int shared_decode(const void* q, long long q_stride, const Cache& c, const PagedBatch& bt, const void* groups, const void* shared,
@@ -334,16 +449,16 @@ int shared_decode(const void* q, long long q_stride, const Cache& c, const Paged
     MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && q_stride % 8 == 0 && q_stride >= (long long)qh * d && scale == scale);
     MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16) && MOSS_ALIGNED(workspace, 16) && MOSS_ALIGNED(groups, 4) &&
                    MOSS_ALIGNED(shared, 4));
-    const SharedPlan p = shared_plan(bt.B, bt.W, c.shift, qh, c.kh);
-    MOSS_CHECK_ARG(workspace_bytes >= workspace_bytes_of(p, qh, c.kh, d));
+    const SharedPlan p = shared_plan(bt.B, qh, c.kh);
+    MOSS_CHECK_ARG(workspace_bytes >= workspace_bytes_of(p, bt.B, qh, c.kh, d));
     const long long own = p.slots * qh, rows = p.rows * c.kh;
     float* part = (float*)workspace;
     float* prefix_part = part + own * d;
     float2* stat = reinterpret_cast<float2*>(prefix_part + rows * d);
     // the scale is positive in either half, its sign goes to q; never 0, so a masked score stays -inf
-    const DecodeArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, part, stat, qh, qh / c.kh, p.xdim, p.shares, p.slots,
+    const DecodeArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, part, stat, qh, qh / c.kh, 0, 0, p.slots,
                        fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f), scale < 0.f ? 0x80008000u : 0u};
-    const SharedArgs s{a, (const int*)groups, (const int*)shared, prefix_part, stat + own, p.rows, p.prefix_shares};
+    const SharedArgs s{a, (const int*)groups, (const int*)shared, prefix_part, stat + own, p.rows, reinterpret_cast<Found*>(stat + own + rows), (kWorth / 16 + c.kh - 1) / c.kh, p.workgroups, p.head_tiles};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == 0)
         return d == 128 ? launch_shared<Bf16, 128, T, S>(s, c, bt, p, st) : launch_shared<Bf16, 64, T, S>(s, c, bt, p, st);
@@ -360,7 +475,7 @@ MOSS_API long long moss_paged_shared_workspace_bytes(int B, int W, int page_rows
     if (B <= 0 || B > 65535 || W <= 0 || shift < 0 || ((long long)W << shift) > (1ll << 30) || kh <= 0 || qh <= 0 || qh % kh ||
         qh > 1024 || (d != 64 && d != 128))
         return 0;
-    return workspace_bytes_of(shared_plan(B, W, shift, qh, kh), qh, kh, d);
+    return workspace_bytes_of(shared_plan(B, qh, kh), B, qh, kh, d);
 }
 
 MOSS_API int moss_paged_shared_decode_attention(const void* q, long long q_stride, const void* k, const void* v, long long k_stride,
