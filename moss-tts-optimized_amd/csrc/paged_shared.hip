@@ -14,21 +14,28 @@
 // Who takes what follows from groups, shared and lengths on the device, so that a captured graph follows them.  The work of a KV
 // head are two lines: the blocks of 64 keys of every tile, tile after tile, and the units of 128 own rows of every sequence.
 // Of the workgroups (two a CU in all), some take the first, a piece each, and the others the second, a piece a wave, in the
-// proportion of what the lines cost; a piece that passes the end of a tile or a sequence leaves more than one result.
+// proportion of what the lines cost; a piece that passes the end of a tile or a sequence leaves more than one result.  The
+// last workgroup also writes where the join finds a sequence's parts.
+//
+// What bounds it: 64 sequences of 30 to 1500 own rows over 4096 shared ones (32 / 8 heads of 128, bf16) 36 us (decode_attention
+// 102): own rows and parts from and to memory (116 + 28 MB, 27 us at what a copy reaches) beside 0.9 us of matrix work a
+// block and CU; with a launch each for prefix and rest 59, the shares of a sequence as workgroups 50, own rows by whole
+// workgroups 41.  40 in five runs over an 8-bit cache 28 us; four over 640 rows, which are not worth sharing, 11.2.
 #include "paged_decode.h"
 #include "paged_prompt.h"
 
 namespace moss {
 namespace {
 
-constexpr int kWorkgroups = 512;  // over all KV heads
+// Over all KV heads: as many as there are places for.  448 / 512 / 768: 38.9 / 36.3 / 46.2 us for 64 sequences over 4096 shared rows.
+constexpr int kWorkgroups = 512;
 
-// Rows of a KV head that sharing has to save in a batch, over all KV heads.  Alone / shared, us, sequences over 4096 shared rows
-// of 32 / 8 heads: 2 (32768) 15.7 / 19.5, 4 (98304) 19.5 / 21.0, 8 (229376) 25.0 / 23.1, 16 35 / 26, 64 99 / 37; 16 over 640
-// (76800) 17.1 / 17.1, over 1536 (184320) 23.4 / 22.1; 12 / 12 heads of 64, 8 over 1536 (129024) 15.0 / 15.8, over 4096 22 / 19;
-// 16 / 1 heads, 32 over 4096 (126976) 26.2 / 26.2, 64 over 1536 (96768) 24.0 / 26.5.  What the shared rows cost alone is so
-// little because the caches serve all but the first reader.
-constexpr int kWorth = 131072;
+// Rows of a KV head that sharing has to save in a batch, over all KV heads.  Every sequence alone / shared, us, in this kernel: 8
+// sequences over 640 shared rows of 32 / 8 heads (35840) 13.9 / 15.4, 32 over 256 (63488) 18.8 / 18.6, 16 over 640 (76800) 18.0 /
+// 17.1, 4 over 4096 (98304) 21.6 / 21.0, 8 over 4096 (229376) 26 / 20; 16 / 1 heads, 16 over 4096 (61440) 25.5 / 28.3, 32 over
+// 4096 (126976) 31.7 / 26.2; 12 / 12 heads of 64, 8 over 640 (53760) 13.6 / 14.1, 16 over 640 (115200) 16.4 / 14.9.  What the
+// shared rows cost alone is so little because the caches serve all but the first reader.
+constexpr int kWorth = 65536;
 
 struct SharedArgs {
     DecodeArgs a;             // part and stat: of the sequences' own rows
@@ -123,7 +130,7 @@ __device__ __forceinline__ Lines lines_of(const SharedArgs& s, int B, int lane, 
     for (int b0 = 0; b0 < B; b0 += kWave) {
         const Member m = at(b0);
         blocks += (long long)tiles_of(m, s.a.group, HEIGHT, lane) * blocks_of(m);
-        units += units_of(m.own());
+        units += own_units(m.own());
     }
     Lines l;
     l.blocks = wave_total(blocks), l.units = wave_total(units) * s.head_tiles;
@@ -149,7 +156,7 @@ __device__ __forceinline__ Places places_of(const SharedArgs& s, const Member& m
 }
 // Where the own rows of sequences b0 + lane end on the line of units.
 __device__ __forceinline__ long long units_end(const SharedArgs& s, const Member& m, long long before) {
-    return before + wave_prefix((long long)units_of(m.own()) * s.head_tiles);
+    return before + wave_prefix((long long)own_units(m.own()) * s.head_tiles);
 }
 
 // What the join has to know of a sequence, written by the last workgroup: its run's first block on the line, the blocks of a
@@ -240,7 +247,7 @@ __global__ __launch_bounds__(256, 2) void paged_shared_split(SharedArgs s, typen
             f.block = shfl64(p.end, m.first) - (long long)__shfl(p.tiles, m.first) * __shfl(p.blocks, m.first);
             f.in_run = (lane - m.first) * G;
             f.row = __shfl(p.rows_end, m.first) - m.size * G + f.in_run;
-            f.units = units_of(m.own());
+            f.units = own_units(m.own());
             f.unit = ends - (long long)f.units * s.head_tiles;
             f.blocks_each = lines.blocks_each, f.units_each = lines.units_each;
             if (b0 + lane < bt.B) s.found[b0 + lane] = f;
@@ -301,7 +308,7 @@ __global__ __launch_bounds__(256, 2) void paged_shared_split(SharedArgs s, typen
             ends = units_end(s, m, lane_value(ends, kWave - 1));
             continue;
         }
-        const int l = __builtin_ctzll(past), from = lane_value(m.from, l), rows = lane_value(m.length, l) - from, units = units_of(rows);
+        const int l = __builtin_ctzll(past), from = lane_value(m.from, l), rows = lane_value(m.length, l) - from, units = own_units(rows);
         const long long in = pos - (lane_value(ends, l) - (long long)units * s.head_tiles);
         const int tile = scalar((int)quotient(in, units)), u0 = scalar((int)(in - (long long)tile * units));
         const int u1 = scalar((int)min((long long)units, u0 + (end - pos)));
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(256, 2) void paged_shared_split(SharedArgs s, typen
         ShareOf sh;
         sh.b = b0 + l, sh.slot = (long long)v + sh.b;
         sh.kvh = kvh, sh.h0 = 16 * tile, sh.heads = min(16, G - sh.h0);
-        sh.r0 = from + u0 * kUnit, sh.r1 = from + (int)min((long long)rows, (long long)u1 * kUnit);
+        sh.r0 = from + u0 * kOwnUnit, sh.r1 = from + (int)min((long long)rows, (long long)u1 * kOwnUnit);
         sh.alone = from == 0 && u0 == 0 && u1 == units;
         if (sh.slot >= a.slots) return;
         float(&none)[2][4][16] = *reinterpret_cast<float(*)[2][4][16]>(odd);
@@ -317,14 +324,16 @@ __global__ __launch_bounds__(256, 2) void paged_shared_split(SharedArgs s, typen
     }
 }
 
-// grid (QH / 4, B) rounded up, a wave a head: the parts of its prefix and of its sequence's own rows.
-template <typename E, int D, int HEIGHT>
+// grid (QH * WAVES / 4 rounded up, B), 256 threads: the parts of a head's prefix and of its sequence's own rows, by WAVES waves, wave w
+// taking w, w + WAVES, .., whose sums meet in LDS.
+template <typename E, int D, int HEIGHT, int WAVES>
 __global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s) {
     constexpr int VPL = D / kWave;
     const DecodeArgs& a = s.a;
-    const int lane = threadIdx.x & (kWave - 1), b = blockIdx.y, G = a.group;
-    const int h = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + threadIdx.x / kWave));
-    if (h >= a.qh) return;
+    __shared__ float acc_s[4][D];
+    const int lane = threadIdx.x & (kWave - 1), wave = scalar((int)threadIdx.x >> 6), w = wave % WAVES, b = blockIdx.y, G = a.group;
+    const int h = blockIdx.x * (4 / WAVES) + wave / WAVES;
+    if (h >= a.qh) return;  // (WAVES 4: never)
     const Found f = s.found[b];
     // the pieces that hold the tile's blocks, and those that hold the own rows
     int pieces = 0, pieces_own = 0, w0 = 0, w1 = 0;
@@ -341,7 +350,6 @@ __global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s) {
         pieces_own = (int)quotient(start + f.units - 1, f.units_each) - w1 + 1;
     }
     if (pieces == 0 && pieces_own == 1) return;  // written by its workgroup
-    uint16_t* dst = a.out + ((size_t)b * a.qh + h) * D + VPL * lane;
     const int count = pieces + pieces_own;
     const long long slot = (long long)w1 + b;
     if (pieces < 0 || pieces_own < 0 || slot < 0 || slot + pieces_own > a.slots || row < 0 ||
@@ -357,22 +365,20 @@ __global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s) {
                VPL * lane;
     };
     const float2 own = lane < count ? stat(lane) : make_float2(-INFINITY, 0.f);
-    constexpr int N = 16;  // parts on their way together
-    float x[N][VPL];
+    constexpr int N = WAVES == 4 ? 8 : 16;  // parts of a wave on their way together
+    float x[N][VPL], acc[VPL], den = 0.f;
     auto load = [&](int i0) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const float* from_part = part(min(i0 + n, max(count - 1, 0)));
+            const float* from_part = part(min(i0 + WAVES * n, count - 1));
 #pragma unroll
             for (int i = 0; i < VPL; ++i) x[n][i] = from_part[i];
         }
     };
-    float acc[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
-    float den = 0.f;
     if (count) {
-        load(0);
+        if (w < count) load(w);
         float mx = own.x;
         for (int i = kWave + lane; i < count; i += kWave) mx = fmaxf(mx, stat(i).x);
         mx = wave_max(mx);
@@ -384,23 +390,35 @@ __global__ __launch_bounds__(256) void paged_shared_join(SharedArgs s) {
             den += weight(v.x) * v.y;
         }
         den = wave_sum(den);
-        for (int i0 = 0; i0 < count; i0 += N) {
-            if (i0) load(i0);
+        for (int i0 = w; i0 < count; i0 += WAVES * N) {
+            if (i0 != w) load(i0);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int i = min(i0 + n, count - 1);
+                const int i = min(i0 + WAVES * n, count - 1);
                 float f = i < kWave ? __uint_as_float(lane_value(__float_as_uint(f0), i)) : weight(stat(i).x);
-                if (i0 + n >= count) f = 0.f;
+                if (i0 + WAVES * n >= count) f = 0.f;
 #pragma unroll
                 for (int k = 0; k < VPL; ++k) acc[k] = f == 0.f ? acc[k] : fmaf(f, x[n][k], acc[k]);
             }
         }
     }
     const float inv = den == 0.f ? 0.f : 1.0f / den;
-    if constexpr (VPL == 2) {
-        *reinterpret_cast<uint32_t*>(dst) = E::pack(acc[0] * inv, acc[1] * inv);
-    } else {
-        *dst = (uint16_t)E::pack(acc[0] * inv, 0.f);
+    uint16_t* dst = a.out + ((size_t)b * a.qh + h) * D;
+    if constexpr (WAVES == 1) {
+        if constexpr (VPL == 2)
+            reinterpret_cast<uint32_t*>(dst)[lane] = E::pack(acc[0] * inv, acc[1] * inv);
+        else
+            dst[lane] = (uint16_t)E::pack(acc[0] * inv, 0.f);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) acc_s[w][VPL * lane + i] = acc[i];
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+        const int d = 2 * threadIdx.x;
+        const float y0 = (acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d]);
+        const float y1 = (acc_s[0][d + 1] + acc_s[1][d + 1]) + (acc_s[2][d + 1] + acc_s[3][d + 1]);
+        reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = E::pack(y0 * inv, y1 * inv);
     }
 }
 
@@ -414,7 +432,9 @@ SharedPlan shared_plan(int B, int qh, int kh) {
     const long long G = qh / kh;
     p.head_tiles = (int)((G + 15) / 16);
     p.workgroups = kWorkgroups / kh > 2 ? kWorkgroups / kh : 2;
-    p.height = B * G * kh <= 1024 ? 64 : 128;
+    // Tiles of 64 rows, two waves to a row, while there are few.  64 / 128: 64 sequences of 32 / 8 heads over 4096 shared rows and
+    // 30 to 1500 of their own 36.3 / 41.1 us, over 16384 and one 45.4 / 43.8.
+    p.height = B * G * kh <= 4096 ? 64 : 128;
     p.slots = 4ll * p.workgroups + B;
     p.rows = B * G + (long long)p.workgroups * p.height;
     return p;
@@ -424,12 +444,17 @@ template <typename E, int D, int KS, typename T, typename S>
 int launch_shared(const SharedArgs& s, const typename S::Cache& c, const PagedBatch& bt, const SharedPlan& p, hipStream_t st) {
     const long long page = ((long long)c.kh << c.shift) * D * (std::is_same<typename S::Cache, PagedCache>::value ? 2 : 1);
     const long long named = (long long)bt.B * bt.W;
-    const dim3 grid((unsigned)(p.workgroups * c.kh)), joins((unsigned)(s.a.qh + 3) / 4, (unsigned)bt.B);
+    const dim3 grid((unsigned)(p.workgroups * c.kh));
     if ((named < c.pages ? named : c.pages) * page * 2 > kCached)
         hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, true>), grid, dim3(256), 0, st, s, c, bt);
     else
         hipLaunchKernelGGL((paged_shared_split<E, D, KS, S, T, false>), grid, dim3(256), 0, st, s, c, bt);
-    hipLaunchKernelGGL((paged_shared_join<E, D, 128 / KS>), joins, dim3(256), 0, st, s);
+    // A sequence of few has many parts.  A wave a head / four: 2 sequences of 4200 own rows 24.8 / 19.0 us, 4 of 700 11.5 / 11.2, 16
+    // over 4096 shared rows 21.2 / 20.8, 64 of 30 to 1500 own rows 27.5 / 29.2.
+    if (bt.B <= 16)
+        hipLaunchKernelGGL((paged_shared_join<E, D, 128 / KS, 4>), dim3((unsigned)s.a.qh, (unsigned)bt.B), dim3(256), 0, st, s);
+    else
+        hipLaunchKernelGGL((paged_shared_join<E, D, 128 / KS, 1>), dim3((unsigned)(s.a.qh + 3) / 4, (unsigned)bt.B), dim3(256), 0, st, s);
     return moss_launch_status();
 }
 

@@ -65,7 +65,7 @@ int main() {
         }
         for (int b = 0; b < B; ++b)
             for (int t = 0; t < head_tiles; ++t) {
-                owns.push_back({units_all, units_of(length[b] - from[b]), b, t});
+                owns.push_back({units_all, own_units(length[b] - from[b]), b, t});
                 units_all += owns.back().units;
             }
         const int takers = prefix_takers((float)blocks_all, (float)units_all, workgroups);

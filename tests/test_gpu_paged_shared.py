@@ -40,7 +40,7 @@ BALLAST = 4096
 
 
 def _with_ballast(groups, shared, lengths, kh):
-    """Sharing is taken up when it saves enough rows: a run behind the batch that saves as many by itself."""
+    """Sharing is taken up when it saves enough rows: a run behind the batch that saves enough by itself."""
     n = 1 + -(-131072 // (kh * BALLAST))
     return groups + [10 ** 6] * n, shared + [BALLAST] * n, lengths + [BALLAST + 3] + [2 + i for i in range(1, n)], n
 
