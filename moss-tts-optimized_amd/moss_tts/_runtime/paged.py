@@ -385,17 +385,22 @@ def gather(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, length
     shape = (tokens, c.kh, c.d)
     if out is None:
         k, v = (torch.empty(shape, dtype=dtype, device=keys.device) for _ in range(2))
+        k_at, v_at = k.data_ptr(), v.data_ptr()
     else:
-        spans = *c.spans(), *_batch_spans(*batch)
         k, v = out
-        for name, t in (("out[0]", k), ("out[1]", v)):
-            _cuda_contig(name, t, dtype, keys.device)
-            _require(t.shape == shape, f"{name} must be {' x '.join(map(str, shape))}")
-            _require(_aligned(t, 16), f"{name} must be 16-byte aligned")
-            _apart(name, t, *spans)
-        _apart("out[1]", v, (k.data_ptr(), k.data_ptr() + 2 * k.numel()))
+        k_at, v_at, size = k.data_ptr(), v.data_ptr(), 2 * tokens * c.kh * c.d
+        if not (k.dtype is dtype and v.dtype is dtype and k.shape == shape == v.shape and k.get_device() == index == v.get_device()
+                and k.is_contiguous() and v.is_contiguous() and not (k_at | v_at) & 15):
+            for name, t in (("out[0]", k), ("out[1]", v)):
+                _cuda_contig(name, t, dtype, keys.device)
+                _require(t.shape == shape, f"{name} must be {' x '.join(map(str, shape))}")
+                _require(_aligned(t, 16), f"{name} must be 16-byte aligned")
+        apart = k_at + size <= v_at or v_at + size <= k_at
+        for first, end in (*c.spans(), *_batch_spans(*batch)):
+            apart = apart and (end <= k_at or k_at + size <= first) and (end <= v_at or v_at + size <= first)
+        _require(apart, "out must not overlap the other tensors")
     native.call_on(keys, "moss_paged_gather" + c.native_name, *c.args(), table_at, table_stride, lengths_at, starts_at, b, w,
-                   tokens, c.kh, c.d, k.data_ptr(), v.data_ptr(), _TYPES[dtype])
+                   tokens, c.kh, c.d, k_at, v_at, _TYPES[dtype])
     return k, v
 
 

@@ -179,17 +179,19 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | 
     return out
 
 
-def _strided(name: str, t: torch.Tensor, dtypes, rows: int, device):
-    """(pointer, row stride, (first, end)) of a checked [rows, n] tensor whose rows are contiguous, or one row for all."""
-    _require(isinstance(t, torch.Tensor) and t.dtype in dtypes and t.device == device and t.dim() == 2
-             and t.shape[0] in (1, rows) and t.shape[1] > 0,
-             f"{name} must be [rows, n] or [1, n], of {' or '.join(str(d) for d in dtypes)}, on {device}")
-    n = t.shape[1]
-    _require(n == 1 or t.stride(1) == 1, f"a row of {name} must be contiguous")
-    stride = t.stride(0) if t.shape[0] > 1 else 0
-    _require(stride == 0 or stride >= n, f"{name}: rows must not overlap")
+def _strided(name: str, t: torch.Tensor, dtype, rows: int, device):
+    """(pointer, row stride, entries, (first, end)) of a checked [rows, n] tensor whose rows are contiguous, or one row for all."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device.index and t.dim() == 2
+            and t.shape[0] in (1, rows) and t.shape[1] > 0):
+        raise ValueError(f"{name} must be a {dtype} [rows, n] or [1, n] tensor on {device}")
+    many, n = t.shape
+    stride, one = t.stride()
+    _require(n == 1 or one == 1, "a row's entries must be contiguous")
+    if many == 1:
+        stride = 0
+    _require(stride == 0 or stride >= n, "rows must not overlap")
     at = t.data_ptr()
-    return at, stride, (at, at + ((rows - 1) * stride + n) * t.element_size())
+    return at, stride, n, (at, at + 4 * ((rows - 1) * stride + n))
 
 
 def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
@@ -214,31 +216,38 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
     rows, entries = logits.shape
     _require(rows <= MAX_SAMPLE_ROWS and entries <= MAX_SAMPLE_VOCAB,
              f"at most {MAX_SAMPLE_ROWS} rows of {MAX_SAMPLE_VOCAB} entries")
-    _require(entries == 1 or logits.stride(1) == 1, "a row's logits must be contiguous")
-    stride = logits.stride(0) if rows > 1 else entries
+    stride, one = logits.stride()
+    _require(entries == 1 or one == 1, "a row's logits must be contiguous")
+    if rows == 1:
+        stride = entries
     _require(stride >= entries, "rows must not overlap")
-    dev, size = logits.device, logits.element_size()
+    dev, size, index, dtype = logits.device, logits.element_size(), logits.get_device(), logits.dtype
     spans = []
     history = [None, 8, 0, 0, 0, None, None]
     if tokens is not None:
-        _require(isinstance(tokens, torch.Tensor) and tokens.dtype in (torch.int64, torch.int32) and tokens.device == dev
-                 and tokens.dim() == 2 and tokens.shape[0] == rows and 0 < tokens.shape[1] < 1 << 31,
-                 f"tokens must be int64 or int32 [rows, width] on {dev}")
-        wide, width = tokens.element_size(), tokens.shape[1]
-        history[:5] = tokens.data_ptr(), wide, tokens.stride(0), tokens.stride(1), width
-        spans.append((history[0], history[0] + wide * ((rows - 1) * history[2] + (width - 1) * history[3] + 1)))
-    for i, (name, t) in enumerate((("lengths", lengths), ("prompt", prompt))):
+        if not (isinstance(tokens, torch.Tensor) and tokens.dtype in (torch.int64, torch.int32) and tokens.get_device() == index
+                and tokens.dim() == 2 and tokens.shape[0] == rows and 0 < tokens.shape[1] < 1 << 31):
+            raise ValueError(f"tokens must be int64 or int32 [rows, width] on {dev}")
+        wide, width, at = tokens.element_size(), tokens.shape[1], tokens.data_ptr()
+        row_stride, step = tokens.stride()
+        history[:5] = at, wide, row_stride, step, width
+        spans.append((at, at + wide * ((rows - 1) * row_stride + (width - 1) * step + 1)))
+    for i, t in ((5, lengths), (6, prompt)):
         if t is not None:
-            _require(tokens is not None, f"{name} without tokens")
+            name = "lengths" if i == 5 else "prompt"
+            _require(tokens is not None, "lengths or prompt without tokens")
             _cuda_contig(name, t, torch.int32, dev)
-            _require(t.numel() == rows, f"{name} must hold one value a row")
-            history[5 + i] = t.data_ptr()
-            spans.append((t.data_ptr(), t.data_ptr() + 4 * rows))
+            _require(t.numel() == rows, "lengths and prompt must hold one value a row")
+            at = history[i] = t.data_ptr()
+            spans.append((at, at + 4 * rows))
     settings = []
     for name, value, none in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
-        _require(tokens is not None or (not isinstance(value, torch.Tensor) and value == none), f"{name} without tokens")
+        if value is none:
+            settings += None, none
+            continue
+        _require(tokens is not None or (not isinstance(value, torch.Tensor) and value == none), "penalties without tokens")
         at, v = _setting(name, value, rows, torch.float32, dev)
-        _require(at is not None or abs(v) < math.inf, f"{name} must be finite")
+        _require(at is not None or abs(v) < math.inf, "penalties must be finite")
         settings += at, float(v)
         if at is not None:
             spans.append((at, at + 4 * rows))
@@ -246,24 +255,26 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
     biases = [None, 0, None, 0, 0]
     _require((bias is None) == (bias_ids is None), "bias and bias_ids go together")
     if bias is not None:
-        ids_at, ids_stride, span = _strided("bias_ids", bias_ids, (torch.int32,), rows, dev)
-        at, bias_stride, other = _strided("bias", bias, (torch.float32,), rows, dev)
-        _require(bias.shape[1] == bias_ids.shape[1] < 1 << 16, "as many biases as ids required, fewer than 65536")
-        biases = [ids_at, ids_stride, at, bias_stride, bias.shape[1]]
+        ids_at, ids_stride, n, span = _strided("bias_ids", bias_ids, torch.int32, rows, dev)
+        at, bias_stride, many, other = _strided("bias", bias, torch.float32, rows, dev)
+        _require(many == n < 1 << 16, "as many biases as ids required, fewer than 65536")
+        biases = [ids_at, ids_stride, at, bias_stride, n]
         spans += span, other
     mask_at, mask_stride = None, 0
     if mask is not None:
-        mask_at, mask_stride, span = _strided("mask", mask, (torch.int32,), rows, dev)
-        _require(32 * mask.shape[1] >= entries, "mask must hold a bit for every entry")
+        mask_at, mask_stride, n, span = _strided("mask", mask, torch.int32, rows, dev)
+        _require(32 * n >= entries, "mask must hold a bit for every entry")
         spans.append(span)
     if out is None:
-        out = torch.empty((rows, entries), dtype=logits.dtype, device=dev)
+        out = logits.new_empty((rows, entries))
         out_stride = entries
     else:
-        _require(isinstance(out, torch.Tensor) and out.dtype == logits.dtype and out.device == dev and out.shape == logits.shape,
+        _require(isinstance(out, torch.Tensor) and out.dtype is dtype and out.get_device() == index and out.shape == logits.shape,
                  "out must have the logits' type, shape and device")
-        _require(entries == 1 or out.stride(1) == 1, "a row of out must be contiguous")
-        out_stride = out.stride(0) if rows > 1 else entries
+        out_stride, one = out.stride()
+        _require(entries == 1 or one == 1, "a row of out must be contiguous")
+        if rows == 1:
+            out_stride = entries
         _require(out_stride >= entries, "rows must not overlap")
         first, end = out.data_ptr(), out.data_ptr() + ((rows - 1) * out_stride + entries) * size
         at = logits.data_ptr()
@@ -271,7 +282,7 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
             spans.append((at, at + ((rows - 1) * stride + entries) * size))
         for a, z in spans:
             _require(end <= a or z <= first, "out must not overlap the other tensors")
-    native.call_on(logits, "moss_adjust_rows", logits.data_ptr(), _SAMPLE_TYPES[logits.dtype], rows, stride, entries, *history,
+    native.call_on(logits, "moss_adjust_rows", logits.data_ptr(), _SAMPLE_TYPES[dtype], rows, stride, entries, *history,
                    *settings, *biases, mask_at, mask_stride, out.data_ptr(), out_stride)
     return out
 
