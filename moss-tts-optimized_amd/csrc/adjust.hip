@@ -278,7 +278,7 @@ MOSS_API int moss_adjust_rows(const void* logits, int dtype, int rows, long long
     const int size = dtype == 2 ? 4 : 2;
     MOSS_CHECK_ARG(logits && out && dtype >= 0 && dtype <= 2 && rows > 0 && rows <= (1 << 21) && vocab > 0 && vocab <= (1 << 19) &&
                    stride >= vocab && out_stride >= vocab && MOSS_ALIGNED(logits, size) && MOSS_ALIGNED(out, size));
-    MOSS_CHECK_ARG(!tokens || ((token_bytes == 4 || token_bytes == 8) && MOSS_ALIGNED(tokens, token_bytes) && width > 0 &&
+    MOSS_CHECK_ARG(!tokens || ((token_bytes == 4 || token_bytes == 8) && MOSS_ALIGNED(tokens, token_bytes) && width > 0 && width <= (1 << 30) &&
                                token_row_stride >= 0 && token_stride >= 0));
     MOSS_CHECK_ARG(tokens || (!lengths && !prompt && !repetition && !presence && !frequency));
     MOSS_CHECK_ARG(MOSS_ALIGNED(lengths, 4) && MOSS_ALIGNED(prompt, 4) && MOSS_ALIGNED(repetition, 4) && MOSS_ALIGNED(presence, 4) &&

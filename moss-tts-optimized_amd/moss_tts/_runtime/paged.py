@@ -181,7 +181,8 @@ def _written_apart(regions):
         for b, bend, bstep, bpage in regions[i + 1:]:
             if a < bend and b < aend:
                 _require(astep == bstep and apage <= (b - a) % astep <= astep - bpage,
-                         "keys and values (and their scales) must not share memory")
+                         "keys and values must not share memory" if len(regions) == 2 else
+                         "keys, values and scales must not share memory")
 
 
 def _batch_refuse(table, lengths, starts, rows, index):

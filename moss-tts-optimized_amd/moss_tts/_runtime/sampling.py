@@ -226,8 +226,8 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
     history = [None, 8, 0, 0, 0, None, None]
     if tokens is not None:
         if not (isinstance(tokens, torch.Tensor) and tokens.dtype in (torch.int64, torch.int32) and tokens.get_device() == index
-                and tokens.dim() == 2 and tokens.shape[0] == rows and 0 < tokens.shape[1] < 1 << 31):
-            raise ValueError(f"tokens must be int64 or int32 [rows, width] on {dev}")
+                and tokens.dim() == 2 and tokens.shape[0] == rows and 0 < tokens.shape[1] <= 1 << 30):
+            raise ValueError(f"tokens must be int64 or int32 [rows, width <= 2^30] on {dev}")
         wide, width, at = tokens.element_size(), tokens.shape[1], tokens.data_ptr()
         row_stride, step = tokens.stride()
         history[:5] = at, wide, row_stride, step, width

@@ -51,7 +51,7 @@ def test_adjust_rows(lib):  # noqa: F811
     for bad in [dict(logits=NULL), dict(out=NULL), dict(logits=ctypes.c_void_p(4097)), dict(logits=H, dtype=2), dict(out=H, dtype=2),
                 dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=(1 << 21) + 1), dict(vocab=0), dict(stride=4999), dict(out_stride=4999),
                 dict(vocab=(1 << 19) + 1, stride=1 << 20, out_stride=1 << 20, mask_stride=1 << 20), dict(token_bytes=2), dict(tokens=ODD),
-                dict(tokens=NULL), dict(width=0), dict(token_stride=-1), dict(token_row_stride=-1), dict(lengths=H), dict(prompt=H),
+                dict(tokens=NULL), dict(width=0), dict(width=(1 << 30) + 1), dict(token_stride=-1), dict(token_row_stride=-1), dict(lengths=H), dict(prompt=H),
                 dict(repetition=H), dict(presence=H), dict(frequency=H), dict(bias=NULL), dict(bias_ids=NULL), dict(bias=H),
                 dict(bias_ids=H), dict(biases=0), dict(biases=1 << 16, bias_stride=0, bias_ids_stride=0), dict(bias_stride=3),
                 dict(bias_ids_stride=3), dict(mask=H), dict(mask_stride=156),

@@ -297,3 +297,15 @@ def test_every_way_of_counting(dev, rows, vocab, width):
     s["prompt"][0] = 0
     print(f"adjust {rows} x {vocab}, {width} tokens", flush=True)
     _check(s, _run(s))
+
+
+def test_a_width_past_everything(dev):
+    """Tokens that lie at one place can be any number; the rows of a history are 2^30 at most."""
+    from moss_tts._runtime import sampling
+
+    logits = torch.zeros((1, 100), device=dev)
+    one = torch.full((1, 1), 7, device=dev)
+    with pytest.raises(ValueError, match="2\\^30"):
+        sampling.adjust(logits, tokens=one.expand(1, (1 << 30) + 1), frequency=1.0)
+    out = sampling.adjust(logits, tokens=one.expand(1, 1 << 30), lengths=torch.tensor([100000], dtype=torch.int32, device=dev), frequency=1.0)
+    assert float(out[0, 7]) == -100000.0 and float(out.sum()) == -100000.0
