@@ -216,14 +216,18 @@ struct PromptPlan {
 // tokens of 32 / 8 heads, 7.7 / 6.9 for 45, 49.4 / 46.0 for nine prompts of 2800; 56.8 / 58.1 for 2048 tokens, 528 / 641
 // (if it did) for 8000.
 constexpr int kSmallTiles = 1024;
+// From a cache in 8 bits, where halved tiles convert every block of keys twice as often, up to 512.  Halved / not: 9.6 / 10.7 us for
+// 45 tokens, 20.2 / 24.9 for 512, 34.0 / 37.6 for 1024 (256 tiles), 73.0 / 71.6 for 2048 (512), 104 / 89 for 2500, 216 / 174 for
+// 4096 (1024), 59.2 / 59.1 for the nine prompts (700), 40.9 / 34.4 for twelve of 260 (780).
+constexpr int kSmallTiles8 = 512;
 // Parts of the whole call's work, over all KV heads, that a tile is not cut below.  128 / 256 / 512: 29 / 22 / 23 us for 150
 // tokens after 1900, 61 / 46 / 47 for 32 single tokens after 50 to 4000, 46 / 46 / 49 for the nine prompts.
 constexpr int kShares = 256;
 
-PromptPlan prompt_plan(int B, int W, int shift, int T, int qh, int kh) {
+PromptPlan prompt_plan(int B, int W, int shift, int T, int qh, int kh, int small_tiles) {
     PromptPlan p;
     const long long rows = (long long)T * (qh / kh);
-    p.height = (rows + 127) / 128 * kh <= kSmallTiles ? 64 : 128;
+    p.height = (rows + 127) / 128 * kh <= small_tiles ? 64 : 128;
     p.tiles = (rows + p.height - 1) / p.height + (B < T ? B : T);
     p.shares = kShares / kh > 1 ? kShares / kh : 1;
     const long long parts = (((long long)W << shift) + kPromptShare * kPromptBlock - 1) / (kPromptShare * kPromptBlock);
@@ -256,7 +260,7 @@ int prompt(const void* q, long long q_stride, const Cache& c, const PagedBatch& 
     MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && T > 0 && T <= (1 << 20) && q_stride % 8 == 0 &&
                    q_stride >= (long long)qh * d && scale == scale);
     MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16) && MOSS_ALIGNED(workspace, 16));
-    const PromptPlan p = prompt_plan(bt.B, bt.W, c.shift, T, qh, c.kh);
+    const PromptPlan p = prompt_plan(bt.B, bt.W, c.shift, T, qh, c.kh, std::is_same<Cache, PagedCache8>::value ? kSmallTiles8 : kSmallTiles);
     const long long values = p.slots * c.kh * p.height;
     MOSS_CHECK_ARG(p.slots == 0 || (workspace && workspace_bytes >= values * (d + 2) * 4));
     const PromptArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, (float*)workspace,
@@ -278,8 +282,14 @@ MOSS_API long long moss_paged_prompt_workspace_bytes(int B, int W, int page_rows
     if (B <= 0 || W <= 0 || shift < 0 || ((long long)W << shift) > (1ll << 30) || T <= 0 || kh <= 0 || qh <= 0 || qh % kh ||
         (d != 64 && d != 128))
         return 0;
-    const PromptPlan p = prompt_plan(B, W, shift, T, qh, kh);
-    return p.slots * kh * p.height * (d + 2) * 4;
+    // enough for a cache of either kind
+    long long most = 0;
+    for (int small_tiles : {kSmallTiles, kSmallTiles8}) {
+        const PromptPlan p = prompt_plan(B, W, shift, T, qh, kh, small_tiles);
+        const long long need = p.slots * kh * p.height * (d + 2) * 4;
+        most = need > most ? need : most;
+    }
+    return most;
 }
 
 MOSS_API int moss_paged_prompt_attention(const void* q, long long q_stride, const void* k, const void* v,

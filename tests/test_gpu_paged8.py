@@ -422,3 +422,23 @@ def test_prompt_values_behind_a_token(dev, tokens):
     ref_abs = o.prompt_attention(args[0][:bad], args[1], np.abs(args[2]), table_, lens_, first, before)
     bound = attention_bound(args[0], *(np.where(np.abs(a) < 1e6, a, 0.0) for a in args[1:]), ref, ref_abs, d ** -0.5, torch.bfloat16, True)
     _close(got[:bad], ref, bound, "before the row")
+
+
+@pytest.mark.parametrize("layout, new, old", [((32, 8, 128), [1500, 700], [0, 9]), ((36, 12, 64), [1300, 200, 450], [30, 0, 700])])
+def test_prompt_whole_tiles(dev, layout, new, old):
+    """More tokens than the halved tiles are for, with parts of a tile's keys joined."""
+    from moss_tts._runtime import paged
+    from paged_helpers import attend_all
+
+    g = torch.Generator().manual_seed(7)
+    qh, kh, d = layout
+    keys, vals, scales, table, lens = cache8(dev, g, [a + b for a, b in zip(new, old)], kh=kh, d=d, page=64)
+    q = (torch.randn((sum(new), qh, d), generator=g) * 1.5).bfloat16().to(dev)
+    starts = torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device=dev)
+    out = paged.prompt_attention(q, keys, vals, table, lens, starts, scales=scales)
+    wide = [torch.nan_to_num(torch.from_numpy(np.where(np.abs(cache8_values(*t)) < 1e6, cache8_values(*t), 0.0))).to(dev)
+            for t in ((keys, scales[0]), (vals, scales[1]))]
+    rest = table, lens, starts.tolist(), torch.zeros_like(out), d ** -0.5
+    ref, ref_abs = attend_all(q, *wide, *rest), attend_all(q, wide[0], wide[1].abs(), *rest)
+    bound = attention_bound(values(q), values(wide[0]), values(wide[1]), values(ref), values(ref_abs), d ** -0.5, torch.bfloat16, True)
+    _close(out, values(ref), bound, "prompt8")
