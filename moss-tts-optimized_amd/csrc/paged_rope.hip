@@ -12,8 +12,11 @@
 // bytes; one workgroup takes 256 / (D / 16) heads of one token, and a wave finds the token's sequence with one ballot
 // per 64 sequences.
 //
-// Into a cache of 8 bits (paged8.h) K and V go from their fp32 values: the row's largest one over its lanes, its scale byte, the
-// codes.  K is rounded once there too, and not to 16 bits before.
+// Into a cache of 8 bits (paged8.h) go the row's largest value over its lanes as its scale byte, and the codes.  K is rounded
+// once there too, and not to 16 bits before.  Its arithmetic is in 64 bits: a value on the wrong side of a border between two
+// codes is off by 2^-3 of itself, and fp32 sends one in a million there.  The heads with more to do go first, so that
+// the others fill the end: write and gather of 2549 tokens take 20.8 us with fp32, 23.0 in 64 bits, 21.1 in this order
+// (one token 6.4, 6.8, 6.5); the write alone 15.5, 4.0 TB/s.
 #include "paged8.h"
 
 namespace moss {
@@ -49,6 +52,18 @@ template <typename E>
 __device__ __forceinline__ void unpack8(u32x4_t w, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[2 * i] = E::lo(w[i]), v[2 * i + 1] = E::hi(w[i]);
+}
+
+// To fp32 so that rounding again, to fewer bits, gives what one rounding would have given: towards zero, with the last bit set
+// where that left something out.
+__device__ __forceinline__ float to_odd(double x) {
+    const float f = (float)x;
+    uint32_t w = __float_as_uint(f);
+    if ((double)f != x && x == x) {
+        if (fabs((double)f) > fabs(x)) w -= 1;
+        w |= 1u;
+    }
+    return __uint_as_float(w);
 }
 
 // The row of an 8-bit cache that D / 16 lanes hold, 8 values of either half each (all of a row's lanes come here).
@@ -90,7 +105,7 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, Cache c, Pa
     } else {
         position = paged_length(bt, b, c.shift) - 1;
     }
-    const int h = blockIdx.y * HPB + threadIdx.x / LPH, j = threadIdx.x % LPH;
+    const int h = (EIGHT ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * HPB + threadIdx.x / LPH, j = threadIdx.x % LPH;
     if (h >= a.qh + 2 * c.kh) return;  // whole groups of lanes
     const uint16_t* src = a.qkv + (size_t)t * a.qkv_stride + (size_t)h * D + 8 * j;
     const u32x4_t wa = *reinterpret_cast<const u32x4_t*>(src), wb = *reinterpret_cast<const u32x4_t*>(src + D / 2);
@@ -129,6 +144,41 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, Cache c, Pa
     float x[8], y[8];
     unpack8<E>(wa, x);
     unpack8<E>(wb, y);
+    const size_t row = (size_t)min(max(position, 0), a.table_rows - 1) * D + 8 * j;
+    if constexpr (EIGHT) {
+        if (h >= a.qh) {
+            double r = 1.;
+            u32x4_t wx = {}, wy = {};
+            if (a.kw) {
+                double s = 0.;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = fma((double)x[i], (double)x[i], fma((double)y[i], (double)y[i], s));
+#pragma unroll
+                for (int m = 1; m < LPH; m <<= 1) s += __shfl_xor(s, m, LPH);
+                s = s / (double)D + (double)a.eps;
+                r = __builtin_amdgcn_rsq(s);  // about 2^-24 off: one step of Newton's
+                if (s < INFINITY) r = fma(0.5 * r, fma(-s * r, r, 1.), r);
+                wx = *reinterpret_cast<const u32x4_t*>(a.kw + 8 * j), wy = *reinterpret_cast<const u32x4_t*>(a.kw + D / 2 + 8 * j);
+            }
+            float cx[8], cy[8], sx[8], sy[8];
+            table8<E, F32>(a.cos_t, row, cx);
+            table8<E, F32>(a.sin_t, row, sx);
+            table8<E, F32>(a.cos_t, row + D / 2, cy);
+            table8<E, F32>(a.sin_t, row + D / 2, sy);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                double p = x[i], q = y[i];
+                if (a.kw) {
+                    p *= r * (i & 1 ? E::hi(wx[i / 2]) : E::lo(wx[i / 2]));
+                    q *= r * (i & 1 ? E::hi(wy[i / 2]) : E::lo(wy[i / 2]));
+                }
+                x[i] = to_odd(p * cx[i] - q * sx[i]);
+                y[i] = to_odd(q * cy[i] + p * sy[i]);
+            }
+            store_row8<E, D>(codes, scale, j, x, y);
+            return;
+        }
+    }
     const uint16_t* wt = h < a.qh ? a.qw : a.kw;
     if (wt) {
         float s = 0.f;
@@ -146,24 +196,11 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(RopeArgs a, Cache c, Pa
             y[i] = y[i] * r * v[i];
         }
     }
-    const size_t row = (size_t)min(max(position, 0), a.table_rows - 1) * D + 8 * j;
     float cx[8], cy[8], sx[8], sy[8];
     table8<E, F32>(a.cos_t, row, cx);
     table8<E, F32>(a.cos_t, row + D / 2, cy);
     table8<E, F32>(a.sin_t, row, sx);
     table8<E, F32>(a.sin_t, row + D / 2, sy);
-    if constexpr (EIGHT) {
-        if (h >= a.qh) {
-            float lo[8], hi[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                lo[i] = x[i] * cx[i] - y[i] * sx[i];
-                hi[i] = y[i] * cy[i] + x[i] * sy[i];
-            }
-            store_row8<E, D>(codes, scale, j, lo, hi);
-            return;
-        }
-    }
     if (!dst) return;
     u32x4_t lo, hi;
 #pragma unroll
@@ -206,7 +243,7 @@ int rope(const RopeArgs& a, const Cache& c, const PagedBatch& bt, int d, int tab
 
 // ---------------------------------------------------------------- the rows back, in order
 // Token t of a sequence's n newest: the K and V rows at its position, as the 16-bit type; a token without a position or a page
-// gives zeros.  What bounds it: memory.  A row is D / 16 lanes with 8 values of either half, a wave takes 1024 / D rows of one
+// gives zeros.  What bounds it: memory and the launch (2549 tokens from 8 bits 5.5 us, 2.9 TB/s; one 2.4).  A row is D / 16 lanes with 8 values of either half, a wave takes 1024 / D rows of one
 // token (K heads, then V heads), so the token's sequence is found with one ballot per 64 sequences.
 struct GatherArgs {
     uint16_t* k_out;

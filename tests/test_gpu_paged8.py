@@ -146,6 +146,34 @@ def test_write(dev, layout, dtype, normed):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_written_keys_are_the_definitions(dev, dtype):
+    """Keys of a million values, code for code: the kernel's 64-bit steps are off by 2^-44 of |x cos| + |y sin|, and a border
+    lies within that of one value in 10^10."""
+    from moss_tts._runtime import paged
+
+    g = torch.Generator().manual_seed(12)
+    n, d, page = 8192, 128, 64
+    qkv = (torch.randn((n, 3 * d), generator=g) * torch.exp2(torch.randint(-6, 7, (n, 1), generator=g).float())).to(dtype).to(dev)
+    weight = (torch.randn(d, generator=g) * 0.3 + 1).to(dtype).to(dev)
+    cos, sin = _tables(g, n, d, dev)
+    keys, vals = (torch.zeros((n // page, 1, page, d), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
+    scales = tuple(torch.zeros((n // page, 1, page), dtype=torch.uint8, device=dev) for _ in range(2))
+    table = torch.arange(n // page, dtype=torch.int32, device=dev)[None]
+    eps = float(np.float32(1e-6))
+    paged.qk_rope(qkv, weight, weight, cos, sin, keys, vals, table, torch.tensor([n], dtype=torch.int32, device=dev), eps,
+                  starts=torch.tensor([0, n], dtype=torch.int32, device=dev), scales=scales)
+    torch.cuda.synchronize()
+    x = values(qkv)[:, d:2 * d]
+    x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * values(weight)
+    x = x * values(cos) + np.concatenate((-x[:, d // 2:], x[:, :d // 2]), -1) * values(sin)
+    codes, byte = keys.view(torch.uint8).cpu().numpy().reshape(n, d), scales[0].cpu().numpy().reshape(n)
+    got = o.cache_values(codes, byte)
+    for i in range(n):
+        want, want_byte = o.quantize_row(x[i], KIND[dtype])
+        assert byte[i] == want_byte and np.array_equal(got[i], want), i
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_write_values_that_are_not_finite(dev, dtype):
     """NaN and infinities become NaN and leave the rest of the row alone; the largest numbers of the type are held; rows of
     zeros and of the smallest numbers."""
