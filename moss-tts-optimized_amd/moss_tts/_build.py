@@ -2,7 +2,8 @@
 
 ``python -m moss_tts._build`` (with ``moss-tts-optimized_amd`` on ``sys.path``) or
 ``__graft_entry__.build()``.  Each translation unit compiles to its own object in
-parallel; the shared library is linked atomically into ``moss_tts/_lib/``.
+parallel; the shared library is linked atomically into ``moss_tts/_lib/``, and beside it the
+Python module ``_moss_calls.so`` of the batch operators' calls (``csrc/host/calls.cpp``, the host compiler).
 """
 from __future__ import annotations
 
@@ -19,6 +20,8 @@ CSRC = os.path.join(ROOT, "csrc")
 OBJ = os.path.join(ROOT, "_build")
 LIBDIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIBDIR, "libmoss_hip.so")
+CALLS = os.path.join(LIBDIR, "_moss_calls.so")   # csrc/host/calls.cpp: the Python module beside it
+INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 ARCH = "gfx950"
 
 CFLAGS = [
@@ -48,6 +51,30 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _compile_calls(verbose: bool) -> None:
+    """The compiled Python calls, against the torch that is installed."""
+    import sysconfig
+
+    import torch
+
+    top = os.path.dirname(torch.__file__)
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no host compiler; the compiled calls cannot be built")
+    tmp = CALLS + ".tmp"
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-D__HIP_PLATFORM_AMD__", "-I", INCLUDE,
+           "-I", os.path.join(top, "include"), "-I", sysconfig.get_paths()["include"],
+           "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), os.path.join(CSRC, "host", "calls.cpp"), "-o", tmp, "-L", os.path.join(top, "lib"),
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ldl"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"the compiled calls failed to build:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, CALLS)
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -56,7 +83,9 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     jobs = jobs or min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(jobs) as ex:
+        calls = ex.submit(_compile_calls, verbose)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        calls.result()
     tmp = LIB + ".tmp"
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
     if verbose:

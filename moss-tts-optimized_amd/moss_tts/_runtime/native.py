@@ -7,6 +7,9 @@ unloadable library is an error.
 
 ``torch`` is imported before the library so that its ``libamdhip64.so.7`` (same SONAME) is
 the HIP runtime the library binds to; streams and pointers are then shared with torch.
+
+The operators of a batch, whose kernels take less time than Python's checks, are called through a compiled
+module as well (:func:`calls`); it calls the same entries.
 """
 from __future__ import annotations
 
@@ -17,6 +20,8 @@ import os
 import torch  # noqa: F401  (must load torch's HIP runtime first)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_lib", "libmoss_hip.so")
+
+CALLS_PATH = os.path.join(os.path.dirname(LIB_PATH), "_moss_calls.so")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -127,6 +132,21 @@ def lib() -> ctypes.CDLL:
         fn.argtypes = args
         fn.restype = _RESTYPES.get(name, _I)
     return so
+
+
+@functools.lru_cache(maxsize=1)
+def calls():
+    """The compiled form of the batch operators' calls (``csrc/host/calls.cpp``): each of its functions makes a call that is in
+    order and returns what it returns, or None, and then the Python function that asked goes on by itself."""
+    import importlib.util
+
+    if not os.path.exists(CALLS_PATH):
+        raise NativeLibraryMissing(f"{CALLS_PATH} is not built; build it with moss_tts._build.build()")
+    spec = importlib.util.spec_from_file_location("_moss_calls", CALLS_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.init(lib()._handle, check)
+    return module
 
 
 def error_string(code: int) -> str:

@@ -39,9 +39,9 @@ _PAGE_ROWS = tuple(1 << s for s in range(4, 13))
 _HEAD_DIMS = (64, 128)
 
 
-# The checks below read a tensor's shape and strides once and compare plain integers: a call of these operators takes
-# the host longer than most of their kernels take the device (28 us with a torch view or a generator per check, of
-# which 8 are the launches).  What a check finds wrong is named by the slower functions that end in _refuse.
+# A call goes through its compiled form (native.calls), which makes it if all is in order; the checks below are for the rest:
+# what is wrong, another device than the current one.  They read a tensor's shape and strides once and compare plain
+# integers, and what they find wrong is named by the slower functions that end in _refuse.
 def _cache_refuse(keys, values, dtype, index):
     for name, t in (("keys", keys), ("values", values)):
         _require(isinstance(t, torch.Tensor) and t.dtype == dtype, f"{name} must be a {dtype} tensor")
@@ -321,9 +321,12 @@ def qk_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Te
     ``starts`` every sequence has one token.  Returns ``q`` ``[T, query heads, head dim]``.  The arithmetic is fp32 up
     to one rounding, where ``pointwise.qk_rope`` rounds after every step.  A token at a negative position (more tokens
     than its length) or without a page is written to no row; a position behind the tables takes their last row.
-    With ``scales`` the rows are written in 8 bits, straight from fp32: off by at most 2^-4 of a value, or 2^-10 times the
-    row's power of two where that is more; values past 240 times the largest power of two of the type are held at that, and
-    what is not finite is NaN."""
+    With ``scales`` the rows are written in 8 bits, rounded once (keys from 64 bits): off by at most 2^-4 of a value, or
+    2^-10 times the row's power of two where that is more; values past 240 times the largest power of two of the type are
+    held at that, and what is not finite is NaN."""
+    done = native.calls().qk_rope(qkv, q_weight, k_weight, cos, sin, keys, values, scales, table, lengths, starts, eps, out)
+    if done is not None:
+        return done
     _require(isinstance(qkv, torch.Tensor) and qkv.dtype in _TYPES, "qkv must be a bf16 or fp16 tensor")
     index, dtype = qkv.get_device(), qkv.dtype
     _require(index >= 0 and qkv.dim() == 2 and qkv.numel() > 0, "qkv must be a CUDA (HIP) tensor [tokens, width]")
@@ -370,6 +373,10 @@ def gather(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, length
     ``starts`` names each sequence's newest rows, as elsewhere; with the running sums of ``lengths`` they are all of its
     rows.  From a cache in 8 bits the values that it stands for, in ``dtype`` (bf16 unless it or ``out`` says fp16).  A token
     without a position or a page gives zeros; rows from ``starts[B]`` on are left as they are."""
+    if dtype is None:
+        done = native.calls().gather(keys, values, scales, table, lengths, starts, tokens, out)
+        if done is not None:
+            return done
     _require(isinstance(keys, torch.Tensor) and keys.get_device() >= 0, "keys must be a CUDA (HIP) tensor")
     index = keys.get_device()
     if out is not None:
@@ -420,6 +427,9 @@ def decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     """One new token per sequence: ``q`` ``[B, query heads, head dim]`` (rows may lie apart) against the
     ``lengths[b]`` rows of each sequence, the new token's own among them; ``scale`` defaults to head dim ** -0.5.
     Returns ``[B, query heads * head dim]``; a sequence without rows gives zeros."""
+    done = native.calls().decode(q, keys, values, scales, table, lengths, None, None, scale, out, ws)
+    if done is not None:
+        return done
     n, qh, hd, stride, index = _query(q)
     c = _cache_of(keys, values, scales, q.dtype, index)
     kh, d = c.kh, c.d
@@ -457,6 +467,10 @@ def shared_decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.T
     its pages as well.  Both are device values like ``lengths``: whatever they hold, no access leaves the cache, and as long
     as the tables agree on the shared rows, they change the time and not the result (beyond rounding).  A run ends at
     every 64th sequence of the batch, and the prefix's weights are rounded to 16 bits, as :func:`prompt_attention` has them."""
+    if groups is not None:
+        done = native.calls().decode(q, keys, values, scales, table, lengths, groups, shared, scale, out, ws)
+        if done is not None:
+            return done
     n, qh, hd, stride, index = _query(q)
     c = _cache_of(keys, values, scales, q.dtype, index)
     kh, d = c.kh, c.d
@@ -495,6 +509,9 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     head dim]`` (rows may lie apart); each token attends its sequence's rows up to its own position, the cached
     ones before the new among them.  ``scale`` defaults to head dim ** -0.5.  Returns ``[T, query heads * head
     dim]``; a token without a visible row gives zeros."""
+    done = native.calls().prompt(q, keys, values, scales, table, lengths, starts, scale, out, ws)
+    if done is not None:
+        return done
     n, qh, hd, stride, index = _query(q)
     c = _cache_of(keys, values, scales, q.dtype, index)
     kh, d = c.kh, c.d

@@ -210,6 +210,9 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
     bit v % 32 of word v // 32 is 1 and becomes ``-inf`` elsewhere.  Tokens and ids outside the row are left out.  Each of the
     penalties is a number, or an fp32 tensor with one value a row; all are read when the kernel runs.  ``out``: a tensor of
     the logits' shape, or the logits themselves; it may share memory with nothing else."""
+    done = native.calls().adjust(logits, tokens, lengths, prompt, repetition, presence, frequency, bias_ids, bias, mask, out)
+    if done is not None:
+        return done
     _require(isinstance(logits, torch.Tensor) and logits.dtype in _SAMPLE_TYPES, "logits must be a bf16, fp16 or fp32 tensor")
     _require(logits.is_cuda, "logits must be a CUDA (HIP) tensor")
     _require(logits.dim() == 2 and logits.shape[0] > 0 and logits.shape[1] > 0, "logits must be [rows, entries]")
