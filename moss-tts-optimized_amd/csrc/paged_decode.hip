@@ -6,7 +6,11 @@
 //
 // What bounds it: the cache's bytes (64 sequences of 4 to 8 thousand rows, 32 / 8 heads of 128: 261 us, 6.2 TB/s; 256 of 300 to
 // 2000: 175 to 187 us, 5.2 TB/s; 16 of up to 8000, 58 MB: 16.7 us from the last-level cache, 19.5 from memory; one of 509: two
-// launches and the chain of a share, 8.2 us).  Work is laid out on the device from the lengths, so that it is even whatever
+// launches and the chain of a share, 8.2 us).  From 8 bits the same: 64 sequences 147 us, 5.5 TB/s, 16 of up to 3128 15, one of
+// 509 8.8; the conversions (27.3 million vector instructions for 19.5 without them) hide behind the loads, and a fourth
+// workgroup a CU, which spills eight registers, takes 195.
+//
+// Work is laid out on the device from the lengths, so that it is even whatever
 // they are and a captured graph follows them: rows are counted in units of kUnit, every KV head's units of all
 // sequences are shared out over about kTarget workgroups, and a workgroup takes an even share of one sequence.  A
 // sequence of one share writes its output; the others write (m, l, O) per share and a second launch joins them, which

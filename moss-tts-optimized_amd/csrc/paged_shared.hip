@@ -12,15 +12,15 @@
 // joins a sequence's.
 //
 // Who takes what follows from groups, shared and lengths on the device, so that a captured graph follows them.  The work of a KV
-// head are two lines: the blocks of 64 keys of every tile, tile after tile, and the units of 128 own rows of every sequence.
+// head are two lines: the blocks of 64 keys of every tile, tile after tile, and the units of 64 own rows of every sequence.
 // Of the workgroups (two a CU in all), some take the first, a piece each, and the others the second, a piece a wave, in the
 // proportion of what the lines cost; a piece that passes the end of a tile or a sequence leaves more than one result.  The
 // last workgroup also writes where the join finds a sequence's parts.
 //
-// What bounds it: 64 sequences of 30 to 1500 own rows over 4096 shared ones (32 / 8 heads of 128, bf16) 36 us (decode_attention
+// What bounds it: 64 sequences of 30 to 1500 own rows over 4096 shared ones (32 / 8 heads of 128, bf16) 35 us (decode_attention
 // 102): own rows and parts from and to memory (116 + 28 MB, 27 us at what a copy reaches) beside 0.9 us of matrix work a
 // block and CU; with a launch each for prefix and rest 59, the shares of a sequence as workgroups 50, own rows by whole
-// workgroups 41.  40 in five runs over an 8-bit cache 28 us; four over 640 rows, which are not worth sharing, 11.2.
+// workgroups 41.  40 in five runs over an 8-bit cache 26 us; four over 640 rows, which are not worth sharing, 10.8.
 #include "paged_decode.h"
 #include "paged_prompt.h"
 
