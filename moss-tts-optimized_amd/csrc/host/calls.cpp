@@ -376,13 +376,11 @@ PyObject* gather(PyObject* const* v) {
     PyObject* outs[2] = {Py_None, Py_None};
     if (given) {
         if (!PyTuple_CheckExact(v[7]) || PyTuple_GET_SIZE(v[7]) != 2) return nullptr;  // a list may change during the launch
-        for (int i = 0; i < 2; ++i) outs[i] = PyTuple_GET_ITEM(v[7], i);
+        for (int i = 0; i < 2; ++i)
+            if (device_of(outs[i] = PyTuple_GET_ITEM(v[7], i)) != index) return nullptr;  // one of them alone: refused
     }
     at::ScalarType type = none(v[2]) ? THPVariable_Unpack(v[0]).scalar_type() : at::kBFloat16;
-    if (given && !none(v[2])) {
-        if (device_of(outs[0]) != index) return nullptr;
-        type = THPVariable_Unpack(outs[0]).scalar_type();
-    }
+    if (given && !none(v[2])) type = THPVariable_Unpack(outs[0]).scalar_type();
     const int kind = type == at::kBFloat16 ? 0 : type == at::kHalf ? 1 : -1;
     Cache c;
     Batch b;

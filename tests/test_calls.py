@@ -1,11 +1,21 @@
 """The compiled calls without a GPU: what is no call of theirs is left to Python, whatever the arguments are."""
+import os
+
 import pytest
 import torch
+
+from moss_tts import _build
 
 COUNTS = {"decode": 11, "prompt": 10, "qk_rope": 13, "gather": 8, "adjust": 11}
 THINGS = [None, 1, 0, -5, 2.5, float("nan"), True, "x", (), (1, 2), [None, None], object(), 1 << 80, torch.zeros(3),
           torch.zeros((2, 4, 64), dtype=torch.bfloat16), torch.zeros((0, 3)), torch.zeros(2, 3).to_sparse(),
           torch.empty((2, 4, 64), dtype=torch.bfloat16, device="meta"), torch.nn.Parameter(torch.zeros(2, 2))]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    if not (os.path.exists(_build.LIB) and os.path.exists(_build.CALLS)):
+        _build.build()
 
 
 @pytest.mark.parametrize("name", COUNTS)

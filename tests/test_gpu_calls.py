@@ -210,6 +210,15 @@ def test_stream_graph_and_threads(dev, monkeypatch):
     assert not failed, failed
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_one_output_of_two(dev, eight):
+    s = _batch(dev, torch.bfloat16, eight)
+    out = torch.zeros((79, 2, 128), dtype=torch.bfloat16, device=dev)
+    for outs in ((out, None), (None, out), (None, None), (out, out), (out,), (out, out.clone(), out.clone())):
+        with pytest.raises(ValueError):
+            _call(s, "gather", out=outs)
+
+
 def test_lists_are_left_to_python(dev):
     s = _batch(dev, torch.bfloat16, True)
     want = _call(s, "gather")
