@@ -538,4 +538,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_moss_calls", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__moss_calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__moss_calls() {
+    PyObject* m = PyModule_Create(&module);
+    // what reads tensors by the headers of one torch reads another's wrongly: the loader compares
+    if (m && PyModule_AddStringConstant(m, "built_for", MOSS_BUILT_FOR) < 0) Py_CLEAR(m);
+    return m;
+}

@@ -57,12 +57,14 @@ def _compile_calls(verbose: bool) -> None:
 
     import torch
 
+    from ._runtime import native
+
     top = os.path.dirname(torch.__file__)
     cxx = shutil.which("g++") or shutil.which("c++")
     if cxx is None:
         raise RuntimeError("no host compiler; the compiled calls cannot be built")
     tmp = CALLS + ".tmp"
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f'-DMOSS_BUILT_FOR="{native.calls_tag()}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-D__HIP_PLATFORM_AMD__", "-I", INCLUDE,
            "-I", os.path.join(top, "include"), "-I", sysconfig.get_paths()["include"],
            "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), os.path.join(CSRC, "host", "calls.cpp"), "-o", tmp, "-L", os.path.join(top, "lib"),

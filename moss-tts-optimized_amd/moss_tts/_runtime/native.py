@@ -9,13 +9,16 @@ unloadable library is an error.
 the HIP runtime the library binds to; streams and pointers are then shared with torch.
 
 The operators of a batch, whose kernels take less time than Python's checks, are called through a compiled
-module as well (:func:`calls`); it calls the same entries.
+module as well (:func:`calls`); it calls the same entries.  Where that module is missing or was built for another
+Python or torch, Python makes these calls by itself, more slowly, and says so once.
 """
 from __future__ import annotations
 
 import ctypes
 import functools
 import os
+import platform
+import warnings
 
 import torch  # noqa: F401  (must load torch's HIP runtime first)
 
@@ -134,18 +137,41 @@ def lib() -> ctypes.CDLL:
     return so
 
 
+def calls_tag() -> str:
+    """What the compiled calls are built for and depend on: this Python and this torch."""
+    return f"python {platform.python_version()} torch {torch.__version__}"
+
+
+class _NoCalls:
+    """In place of the compiled calls: takes no call."""
+
+    @staticmethod
+    def _none(*args):
+        return None
+
+    decode = prompt = qk_rope = gather = adjust = _none
+
+
 @functools.lru_cache(maxsize=1)
 def calls():
     """The compiled form of the batch operators' calls (``csrc/host/calls.cpp``): each of its functions makes a call that is in
     order and returns what it returns, or None, and then the Python function that asked goes on by itself."""
     import importlib.util
 
-    if not os.path.exists(CALLS_PATH):
-        raise NativeLibraryMissing(f"{CALLS_PATH} is not built; build it with moss_tts._build.build()")
-    spec = importlib.util.spec_from_file_location("_moss_calls", CALLS_PATH)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
-    module.init(lib()._handle, check)
+    try:
+        if not os.path.exists(CALLS_PATH):
+            raise ImportError(f"{CALLS_PATH} is not built")
+        spec = importlib.util.spec_from_file_location("_moss_calls", CALLS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        tag = getattr(module, "built_for", "another")
+        if tag != calls_tag():
+            raise ImportError(f"{CALLS_PATH} was built for {tag}, this is {calls_tag()}")
+        module.init(lib()._handle, check)
+    except ImportError as e:
+        warnings.warn(f"{e}; the batch operators' calls take longer (moss_tts._build.build() builds their compiled form)",
+                      RuntimeWarning, stacklevel=3)
+        return _NoCalls
     return module
 
 

@@ -1,0 +1,72 @@
+"""Without the compiled calls, or with those of another torch, Python makes the batch operators' calls by itself."""
+import os
+
+import pytest
+import torch
+
+from moss_tts import _build
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    if not (os.path.exists(_build.LIB) and os.path.exists(_build.CALLS)):
+        _build.build()
+
+
+@pytest.fixture
+def calls_at(monkeypatch):
+    """``calls`` as a process finds it whose compiled module lies at the path given."""
+    from moss_tts._runtime import native
+
+    def use(path):
+        monkeypatch.setattr(native, "CALLS_PATH", str(path))
+        native.calls.cache_clear()
+        return native.calls
+    yield use
+    monkeypatch.undo()
+    native.calls.cache_clear()
+
+
+def _refused():
+    from moss_tts._runtime import paged, sampling
+
+    x = torch.zeros((2, 4, 64), dtype=torch.bfloat16)
+    for call in (lambda: paged.decode_attention(x, x, x, x, x), lambda: paged.shared_decode_attention(x, x, x, x, x, x, x),
+                 lambda: paged.prompt_attention(x, x, x, x, x, x), lambda: paged.gather(x, x, x, x, x, 3),
+                 lambda: paged.qk_rope(x, None, None, x, x, x, x, x, x, 1e-6), lambda: sampling.adjust(x)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_absent(calls_at, tmp_path):
+    calls = calls_at(tmp_path / "none.so")
+    with pytest.warns(RuntimeWarning, match="not built"):
+        taken = calls()
+    assert taken.decode(*[None] * 11) is None and taken.adjust(*[None] * 11) is None
+    _refused()
+
+
+def test_no_module(calls_at, tmp_path):
+    path = tmp_path / "_moss_calls.so"
+    path.write_bytes(b"\x7fELF and nothing behind it")
+    with pytest.warns(RuntimeWarning):
+        calls_at(path)()
+    _refused()
+
+
+def test_another_torchs(calls_at, monkeypatch):
+    from moss_tts._runtime import native
+
+    tag = native.calls_tag()
+    assert torch.__version__ in tag
+    monkeypatch.setattr(native, "calls_tag", lambda: tag + " of another day")
+    with pytest.warns(RuntimeWarning, match="another day"):
+        calls_at(native.CALLS_PATH)()
+    _refused()
+
+
+def test_this_ones(calls_at):
+    from moss_tts._runtime import native
+
+    calls = calls_at(native.CALLS_PATH)
+    assert calls().built_for == native.calls_tag()
