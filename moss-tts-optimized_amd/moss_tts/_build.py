@@ -61,13 +61,14 @@ def _compile_calls(verbose: bool) -> None:
 
     top = os.path.dirname(torch.__file__)
     cxx = shutil.which("g++") or shutil.which("c++")
-    if cxx is None:
-        raise RuntimeError("no host compiler; the compiled calls cannot be built")
+    # hipcc, which the library needs anyway, is a host compiler too
+    compiler = [cxx] if cxx else [hipcc(), "-x", "c++", "-Wno-unused-command-line-argument"]
     tmp = CALLS + ".tmp"
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f'-DMOSS_BUILT_FOR="{native.calls_tag()}"',
+    cmd = [*compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f'-DMOSS_BUILT_FOR="{native.calls_tag()}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-D__HIP_PLATFORM_AMD__", "-I", INCLUDE,
            "-I", os.path.join(top, "include"), "-I", sysconfig.get_paths()["include"],
-           "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), os.path.join(CSRC, "host", "calls.cpp"), "-o", tmp, "-L", os.path.join(top, "lib"),
+           "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), os.path.join(CSRC, "host", "calls.cpp"),
+           "-o", tmp, "-L", os.path.join(top, "lib"),
            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ldl"]
     if verbose:
         print(" ".join(cmd), flush=True)

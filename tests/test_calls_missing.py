@@ -1,5 +1,6 @@
 """Without the compiled calls, or with those of another torch, Python makes the batch operators' calls by itself."""
 import os
+import shutil
 
 import pytest
 import torch
@@ -70,3 +71,16 @@ def test_this_ones(calls_at):
 
     calls = calls_at(native.CALLS_PATH)
     assert calls().built_for == native.calls_tag()
+
+
+def test_built_without_a_host_compiler(calls_at, monkeypatch, tmp_path):
+    """hipcc alone builds the module, as it does the library."""
+    from moss_tts._runtime import native
+
+    hipcc, which = _build.hipcc(), shutil.which
+    monkeypatch.setattr(_build.shutil, "which", lambda name: None if name in ("g++", "c++") else which(name))
+    monkeypatch.setattr(_build, "hipcc", lambda: hipcc)
+    monkeypatch.setattr(_build, "CALLS", str(tmp_path / "_moss_calls.so"))
+    _build._compile_calls(False)
+    calls = calls_at(_build.CALLS)
+    assert calls().built_for == native.calls_tag() and calls().decode(*[None] * 11) is None
