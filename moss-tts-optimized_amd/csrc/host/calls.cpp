@@ -42,7 +42,7 @@ bool apart(const Span& a, const Span& b) { return a.end <= b.first || b.end <= a
 struct Arg {  // a tensor on device `index`, or not `ok`
     const at::Tensor* t = nullptr;
     Arg(PyObject* o, int index) {
-        if (!THPVariable_Check(o)) return;
+        if (!THPVariable_CheckExact(o)) return;  // a subclass makes its outputs by itself
         const at::Tensor& x = THPVariable_Unpack(o);
         if (x.defined() && x.is_cuda() && x.layout() == at::kStrided && x.get_device() == index) t = &x;
     }
@@ -58,7 +58,7 @@ struct Arg {  // a tensor on device `index`, or not `ok`
 };
 bool none(PyObject* o) { return o == Py_None; }
 int device_of(PyObject* o) {
-    if (!THPVariable_Check(o)) return -1;
+    if (!THPVariable_CheckExact(o)) return -1;
     const at::Tensor& x = THPVariable_Unpack(o);
     return x.defined() && x.is_cuda() ? (int)x.get_device() : -1;
 }
