@@ -90,7 +90,8 @@ struct Region {
 struct Cache {
     ll pages, kh, rows, d, strides[4];  // strides of keys, values and their scales, in elements
     Region regions[4];
-    int n;  // 2, or 4 in 8 bits
+    at::Tensor held[2];  // the scales: other threads may run before the launch, and a list of them may change
+    int n;               // 2, or 4 in 8 bits
     bool eight() const { return n == 4; }
     bool of(PyObject* keys, PyObject* values, PyObject* scales, at::ScalarType type, int index) {
         n = none(scales) ? 2 : 4;
@@ -118,6 +119,7 @@ struct Cache {
             if (step < page || step % (n == 4 ? 16 : 8) || !aligned(a.at())) return false;
             strides[i] = step;
             regions[i] = Region{a.at(), a.at() + wide * ((pages - 1) * step + page), wide * step, wide * page};
+            if (i >= 2) held[i - 2] = *a.t;
         }
         return true;
     }
@@ -183,11 +185,21 @@ bool scale_of(PyObject* o, ll d, double& v) {
     return number(o, v);
 }
 
+// A new tensor.  Device memory may have to be found for it, which can take long: other Python threads run meanwhile.
+struct Unlocked {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, int index) {
+    Unlocked now;
+    return at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, index));
+}
+
 // An output or workspace: a new one, or the caller's, of this shape and apart from the rest.
 bool output(PyObject* given, at::IntArrayRef shape, at::ScalarType type, int index, const Spans& rest, at::Tensor& made, char*& at,
             Span& span) {
     if (none(given)) {
-        made = at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, index));
+        made = fresh(shape, type, index);
         at = static_cast<char*>(made.data_ptr());
         span = Span{at, at + made.numel() * made.element_size()};
         return true;
@@ -201,7 +213,7 @@ bool workspace(PyObject* given, ll bytes, int index, const Spans& rest, const Sp
     if (none(given)) {
         at = nullptr;
         if (bytes) {
-            made = at::empty({bytes / 4}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA, index));
+            made = fresh({bytes / 4}, at::kFloat, index);
             at = static_cast<char*>(made.data_ptr());
         }
         return true;
@@ -375,7 +387,7 @@ PyObject* gather(PyObject* const* v) {
     const bool given = !none(v[7]);
     PyObject* outs[2] = {Py_None, Py_None};
     if (given) {
-        if (!PyTuple_CheckExact(v[7]) || PyTuple_GET_SIZE(v[7]) != 2) return nullptr;  // a list may change during the launch
+        if (!PyTuple_CheckExact(v[7]) || PyTuple_GET_SIZE(v[7]) != 2) return nullptr;  // a list may change meanwhile
         for (int i = 0; i < 2; ++i)
             if (device_of(outs[i] = PyTuple_GET_ITEM(v[7], i)) != index) return nullptr;  // one of them alone: refused
     }
@@ -474,7 +486,7 @@ PyObject* adjust(PyObject* const* v) {
     char* out;
     ll out_stride = entries;
     if (none(v[10])) {
-        made = at::empty({rows, entries}, at::TensorOptions().dtype(type).device(at::kCUDA, index));
+        made = fresh({rows, entries}, type, index);
         out = static_cast<char*>(made.data_ptr());
     } else {
         const Arg o(v[10], index);
