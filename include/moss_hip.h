@@ -519,6 +519,9 @@ int moss_paged_decode_attention_fp8(const void *q, long long q_stride, const voi
                                     int kh, int d, float scale, void *out, void *workspace, long long workspace_bytes,
                                     int dtype, void *stream);
 
+/* The workspace of the prompt form, up to twice the 16-bit one's; one of moss_paged_prompt_workspace_bytes serves too, and some
+ * calls are slower with it. */
+long long moss_paged_prompt_workspace_bytes_fp8(int B, int W, int page_rows, int T, int qh, int kh, int d);
 int moss_paged_prompt_attention_fp8(const void *q, long long q_stride, const void *k, const void *v, const void *k_scales,
                                     const void *v_scales, long long k_stride, long long v_stride,
                                     long long k_scale_stride, long long v_scale_stride, int pages, int page_rows,

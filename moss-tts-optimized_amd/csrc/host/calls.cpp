@@ -23,7 +23,8 @@ namespace {
     X(moss_paged_qk_rope) X(moss_paged_qk_rope_fp8) X(moss_paged_gather) X(moss_paged_gather_fp8)                             \
     X(moss_paged_decode_workspace_bytes) X(moss_paged_decode_attention) X(moss_paged_decode_attention_fp8)                    \
     X(moss_paged_shared_workspace_bytes) X(moss_paged_shared_decode_attention) X(moss_paged_shared_decode_attention_fp8)      \
-    X(moss_paged_prompt_workspace_bytes) X(moss_paged_prompt_attention) X(moss_paged_prompt_attention_fp8) X(moss_adjust_rows)
+    X(moss_paged_prompt_workspace_bytes) X(moss_paged_prompt_workspace_bytes_fp8) X(moss_paged_prompt_attention)              \
+    X(moss_paged_prompt_attention_fp8) X(moss_adjust_rows)
 struct Entries {
 #define X(name) decltype(&::name) name;
     MOSS_ENTRIES(X)
@@ -321,8 +322,11 @@ PyObject* prompt(PyObject* const* v) {
     char *out, *ws;
     Span span;
     if (!output(v[8], {x.tokens, x.heads * x.d}, q.t->scalar_type(), index, s, made, out, span)) return nullptr;
-    const ll bytes = lib.moss_paged_prompt_workspace_bytes(b.b, b.w, (int)c.rows, T, qh, kh, d);
+    // what the cache's form takes at best, or the caller's, which the 16-bit form's is enough for
+    const auto size = c.eight() && none(v[9]) ? lib.moss_paged_prompt_workspace_bytes_fp8 : lib.moss_paged_prompt_workspace_bytes;
+    ll bytes = size(b.b, b.w, (int)c.rows, T, qh, kh, d);
     if (!workspace(v[9], bytes, index, s, span, made_ws, ws)) return nullptr;
+    if (!none(v[9])) bytes = 4 * THPVariable_Unpack(v[9]).numel();
     launch_over(MOSS_OVER(c, moss_paged_prompt_attention), std::make_tuple((const void*)x.at, x.stride),
                 std::make_tuple((const void*)b.table, b.stride, (const void*)b.lengths, (const void*)b.starts, b.b, b.w, T, qh, kh, d,
                                 (float)scale, (void*)out, (void*)ws, bytes, kind_of(*q.t), stream(index)));

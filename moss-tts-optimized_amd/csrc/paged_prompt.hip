@@ -236,6 +236,16 @@ PromptPlan prompt_plan(int B, int W, int shift, int T, int qh, int kh, int small
     return p;
 }
 
+long long workspace_bytes_of(const PromptPlan& p, int kh, int d) { return p.slots * kh * p.height * (d + 2) * 4; }
+
+long long workspace_bytes_for(int B, int W, int page_rows, int T, int qh, int kh, int d, int small_tiles) {
+    const int shift = page_shift(page_rows);
+    if (B <= 0 || W <= 0 || shift < 0 || ((long long)W << shift) > (1ll << 30) || T <= 0 || kh <= 0 || qh <= 0 || qh % kh ||
+        (d != 64 && d != 128))
+        return 0;
+    return workspace_bytes_of(prompt_plan(B, W, shift, T, qh, kh, small_tiles), kh, d);
+}
+
 template <typename E, int D, int KS, typename S>
 int launch_prompt(const PromptArgs& a, const typename S::Cache& c, const PagedBatch& bt, const PromptPlan& p, hipStream_t st) {
     constexpr int HEIGHT = 128 / KS;
@@ -261,9 +271,11 @@ int prompt(const void* q, long long q_stride, const Cache& c, const PagedBatch& 
     MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && T > 0 && T <= (1 << 20) && q_stride % 8 == 0 &&
                    q_stride >= (long long)qh * d && scale == scale);
     MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16) && MOSS_ALIGNED(workspace, 16));
-    const PromptPlan p = prompt_plan(bt.B, bt.W, c.shift, T, qh, c.kh, std::is_same<Cache, PagedCache8>::value ? kSmallTiles8 : kSmallTiles);
+    PromptPlan p = prompt_plan(bt.B, bt.W, c.shift, T, qh, c.kh, std::is_same<Cache, PagedCache8>::value ? kSmallTiles8 : kSmallTiles);
+    // whole tiles' parts need up to twice the halved ones': a workspace of the 16-bit form's size serves with those
+    if (workspace && workspace_bytes < workspace_bytes_of(p, c.kh, d)) p = prompt_plan(bt.B, bt.W, c.shift, T, qh, c.kh, kSmallTiles);
+    MOSS_CHECK_ARG(p.slots == 0 || (workspace && workspace_bytes >= workspace_bytes_of(p, c.kh, d)));
     const long long values = p.slots * c.kh * p.height;
-    MOSS_CHECK_ARG(p.slots == 0 || (workspace && workspace_bytes >= values * (d + 2) * 4));
     const PromptArgs a{(const uint16_t*)q, q_stride, (uint16_t*)out, (float*)workspace,
                        reinterpret_cast<float2*>((float*)workspace + values * d), T, qh, qh / c.kh, p.shares,
                        p.slots, fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f), scale < 0.f ? 0x80008000u : 0u};
@@ -279,18 +291,11 @@ int prompt(const void* q, long long q_stride, const Cache& c, const PagedBatch& 
 using namespace moss;
 
 MOSS_API long long moss_paged_prompt_workspace_bytes(int B, int W, int page_rows, int T, int qh, int kh, int d) {
-    const int shift = page_shift(page_rows);
-    if (B <= 0 || W <= 0 || shift < 0 || ((long long)W << shift) > (1ll << 30) || T <= 0 || kh <= 0 || qh <= 0 || qh % kh ||
-        (d != 64 && d != 128))
-        return 0;
-    // enough for a cache of either kind
-    long long most = 0;
-    for (int small_tiles : {kSmallTiles, kSmallTiles8}) {
-        const PromptPlan p = prompt_plan(B, W, shift, T, qh, kh, small_tiles);
-        const long long need = p.slots * kh * p.height * (d + 2) * 4;
-        most = need > most ? need : most;
-    }
-    return most;
+    return workspace_bytes_for(B, W, page_rows, T, qh, kh, d, kSmallTiles);
+}
+
+MOSS_API long long moss_paged_prompt_workspace_bytes_fp8(int B, int W, int page_rows, int T, int qh, int kh, int d) {
+    return workspace_bytes_for(B, W, page_rows, T, qh, kh, d, kSmallTiles8);
 }
 
 MOSS_API int moss_paged_prompt_attention(const void* q, long long q_stride, const void* k, const void* v,

@@ -92,6 +92,7 @@ SIGNATURES: dict[str, list] = {
     "moss_paged_prompt_attention": [_P, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P,
                                     _L, _I, _P],
     "moss_paged_prompt_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I],
+    "moss_paged_prompt_workspace_bytes_fp8": [_I, _I, _I, _I, _I, _I, _I],
     "moss_paged_qk_rope_fp8": [_P, _L, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _L, _P, _P, _I,
                                _I, _I, _I, _I, _I, _F, _I, _P],
     "moss_paged_gather": [_P, _P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P],
@@ -115,6 +116,7 @@ _RESTYPES = {"moss_error_string": ctypes.c_char_p, "moss_gemm_workspace_bytes": 
              "moss_gemm_qk_rope_workspace_bytes": ctypes.c_longlong,
              "moss_paged_decode_workspace_bytes": ctypes.c_longlong,
              "moss_paged_prompt_workspace_bytes": ctypes.c_longlong,
+             "moss_paged_prompt_workspace_bytes_fp8": ctypes.c_longlong,
              "moss_paged_shared_workspace_bytes": ctypes.c_longlong,
              "moss_sample_rows_workspace_bytes": ctypes.c_longlong,
              "moss_stream_read_words": ctypes.c_longlong}

@@ -495,9 +495,10 @@ def shared_decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.T
 
 def prompt_workspace(q: torch.Tensor, keys: torch.Tensor, table: torch.Tensor) -> torch.Tensor | None:
     """A workspace for :func:`prompt_attention` calls of these shapes (None: none needed); calls that may overlap need
-    one each."""
-    nbytes = native.lib().moss_paged_prompt_workspace_bytes(table.shape[0], table.shape[1], keys.shape[2], q.shape[0],
-                                                            q.shape[1], keys.shape[1], keys.shape[3])
+    one each.  For ``keys`` in 8 bits it may be twice as large; one for 16 bits serves there too, and some calls are slower
+    with it."""
+    size = getattr(native.lib(), "moss_paged_prompt_workspace_bytes" + ("_fp8" if keys.dtype == torch.float8_e4m3fn else ""))
+    nbytes = size(table.shape[0], table.shape[1], keys.shape[2], q.shape[0], q.shape[1], keys.shape[1], keys.shape[3])
     return torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
 
 
@@ -524,8 +525,12 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     if out is not None or ws is not None:
         spans = (at, at + 2 * ((n - 1) * stride + qh * d)), *c.spans(), *_batch_spans(*batch)
     out = _output(out, (n, qh * d), q, index, spans)
-    nbytes = native.lib().moss_paged_prompt_workspace_bytes(b, w, c.rows, n, qh, kh, d)
-    ws = _workspace(ws, nbytes, q, out, spans)
+    # what the cache's form takes at best, or the caller's, which the 16-bit form's is enough for
+    size = native.lib().moss_paged_prompt_workspace_bytes
+    if ws is None:
+        size = getattr(native.lib(), "moss_paged_prompt_workspace_bytes" + c.native_name)
+    ws = _workspace(ws, size(b, w, c.rows, n, qh, kh, d), q, out, spans)
+    nbytes = 0 if ws is None else 4 * ws.numel()
     native.call_on(q, "moss_paged_prompt_attention" + c.native_name, at, stride, *c.args(), table_at,
                    table_stride, lengths_at, starts_at, b, w, n, qh, kh, d, _scale(scale, d),
                    out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _TYPES[q.dtype])
