@@ -31,7 +31,7 @@ struct AdjustArgs {
     const void* logits;
     void* out;
     long long stride, out_stride;
-    int rows, vocab, chunks;
+    int row0, rows, vocab, chunks;  // rows row0 .. row0 + rows - 1
     const void* tokens;
     long long token_row, token_step;  // elements
     int width;
@@ -102,6 +102,7 @@ __global__ __launch_bounds__(THREADS) void adjust_rows_kernel(AdjustArgs a) {
     } else {
         row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     }
+    row += a.row0;
     const Bits* src = reinterpret_cast<const Bits*>(a.logits) + (size_t)row * a.stride;
     Bits* dst = reinterpret_cast<Bits*>(a.out) + (size_t)row * a.out_stride;
     // Groups of eight entries that begin at 16 bytes (32 of fp32) in both rows, where both begin at the same place among
@@ -246,11 +247,16 @@ __global__ __launch_bounds__(THREADS) void adjust_rows_kernel(AdjustArgs a) {
 template <int TYPE, typename Token, int COUNT, int THREADS, int CHUNK>
 int launch_adjust(AdjustArgs a, hipStream_t st) {
     a.chunks = (a.vocab + 7 + CHUNK - 1) / CHUNK;  // a row that begins inside a group of eight has its last entries one further
-    const long long groups = (long long)a.rows * a.chunks;
-    MOSS_CHECK_ARG(groups * THREADS < (1ll << 32));
     const size_t lds = (a.tokens ? COUNT / 8 * CHUNK : 0) + (a.bias ? 2 * CHUNK : 0);
-    hipLaunchKernelGGL((adjust_rows_kernel<TYPE, Token, COUNT, THREADS, CHUNK>), dim3((unsigned)groups), dim3(THREADS), lds, st, a);
-    return moss_launch_status();
+    // a grid has fewer than 2^32 threads: whole eights of rows at a time, all of them but for 2^21 rows of two chunks and the like
+    const int rows = a.rows, most = (int)(((1ll << 32) - 1) / THREADS / a.chunks) & ~7;
+    for (a.row0 = 0; a.row0 < rows; a.row0 += a.rows) {
+        a.rows = rows - a.row0 < most ? rows - a.row0 : most;
+        hipLaunchKernelGGL((adjust_rows_kernel<TYPE, Token, COUNT, THREADS, CHUNK>), dim3((unsigned)a.rows * a.chunks), dim3(THREADS), lds,
+                           st, a);
+        if (const int status = moss_launch_status()) return status;
+    }
+    return 0;
 }
 
 template <int TYPE, typename Token>
@@ -277,7 +283,7 @@ MOSS_API int moss_adjust_rows(const void* logits, int dtype, int rows, long long
                               long long mask_stride, void* out, long long out_stride, void* stream) {
     const int size = dtype == 2 ? 4 : 2;
     MOSS_CHECK_ARG(logits && out && dtype >= 0 && dtype <= 2 && rows > 0 && rows <= (1 << 21) && vocab > 0 && vocab <= (1 << 19) &&
-                   stride >= vocab && out_stride >= vocab && MOSS_ALIGNED(logits, size) && MOSS_ALIGNED(out, size));
+                   (long long)rows * vocab <= (1ll << 38) && stride >= vocab && out_stride >= vocab && MOSS_ALIGNED(logits, size) && MOSS_ALIGNED(out, size));
     MOSS_CHECK_ARG(!tokens || ((token_bytes == 4 || token_bytes == 8) && MOSS_ALIGNED(tokens, token_bytes) && width > 0 && width <= (1 << 30) &&
                                token_row_stride >= 0 && token_stride >= 0));
     MOSS_CHECK_ARG(tokens || (!lengths && !prompt && !repetition && !presence && !frequency));
@@ -288,7 +294,7 @@ MOSS_API int moss_adjust_rows(const void* logits, int dtype, int rows, long long
                              (bias_stride == 0 || bias_stride >= biases) && MOSS_ALIGNED(bias_ids, 4) && MOSS_ALIGNED(bias, 4)));
     MOSS_CHECK_ARG(!mask || ((mask_stride == 0 || mask_stride >= (vocab + 31) / 32) && MOSS_ALIGNED(mask, 4)));
     AdjustArgs a;
-    a.logits = logits, a.out = out, a.stride = stride, a.out_stride = out_stride, a.rows = rows, a.vocab = vocab;
+    a.logits = logits, a.out = out, a.stride = stride, a.out_stride = out_stride, a.row0 = 0, a.rows = rows, a.vocab = vocab;
     a.tokens = tokens, a.token_row = token_row_stride, a.token_step = token_stride, a.width = width;
     a.lengths = (const int*)lengths, a.prompt = (const int*)prompt;
     a.repetition = (const float*)repetition, a.presence = (const float*)presence, a.frequency = (const float*)frequency;

@@ -448,7 +448,7 @@ PyObject* adjust(PyObject* const* v) {
     const at::ScalarType type = x.t->scalar_type();
     const int kind = type == at::kBFloat16 ? 0 : type == at::kHalf ? 1 : type == at::kFloat ? 2 : -1;
     const ll rows = x.size(0), entries = x.size(1), wide = x.t->element_size(), stride = rows == 1 ? entries : x.stride(0);
-    if (kind < 0 || rows > 1 << 21 || entries > 1 << 19 || (entries > 1 && x.stride(1) != 1) || stride < entries) return nullptr;
+    if (kind < 0 || rows > 1 << 21 || entries > 1 << 19 || rows * entries > 1ll << 38 || (entries > 1 && x.stride(1) != 1) || stride < entries) return nullptr;
     Spans s;
     const bool history = !none(v[1]);
     char *tokens = nullptr, *counts[2] = {nullptr, nullptr}, *settings[3] = {nullptr, nullptr, nullptr};

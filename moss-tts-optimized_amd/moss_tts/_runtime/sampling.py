@@ -102,6 +102,7 @@ def sample_topk_pair(a: dict, b: dict, *, seed: torch.Tensor, position: torch.Te
 _SAMPLE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_SAMPLE_VOCAB = 1 << 19
 MAX_SAMPLE_ROWS = 1 << 21
+MAX_ADJUST_LOGITS = 1 << 38
 
 
 def _setting(name: str, value, rows: int, dtype: torch.dtype, device):
@@ -198,8 +199,8 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
            prompt: torch.Tensor | None = None, repetition: float | torch.Tensor = 1.0, presence: float | torch.Tensor = 0.0,
            frequency: float | torch.Tensor = 0.0, bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
            mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """bf16 / fp16 / fp32 logits ``[rows, entries]`` (rows any stride apart) with penalties for the tokens said so far, biases
-    and a mask, for :func:`sample`; in the logits' type, from fp32 with one rounding.
+    """bf16 / fp16 / fp32 logits ``[rows, entries]`` (rows any stride apart; up to 2^21 of 2^19, 2^38 in all) with penalties for
+    the tokens said so far, biases and a mask, for :func:`sample`; in the logits' type, from fp32 with one rounding.
 
     ``tokens`` int64 or int32 ``[rows, width]`` (any strides, so ``ids.T`` of a ``[width, rows]`` history serves): the first
     ``lengths`` (int32 ``[rows]``; None: all) of a row are its history, of which the first ``prompt`` (int32 ``[rows]``; None:
@@ -219,6 +220,7 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
     rows, entries = logits.shape
     _require(rows <= MAX_SAMPLE_ROWS and entries <= MAX_SAMPLE_VOCAB,
              f"at most {MAX_SAMPLE_ROWS} rows of {MAX_SAMPLE_VOCAB} entries")
+    _require(rows * entries <= MAX_ADJUST_LOGITS, f"at most {MAX_ADJUST_LOGITS} logits")
     stride, one = logits.stride()
     _require(entries == 1 or one == 1, "a row's logits must be contiguous")
     if rows == 1:
