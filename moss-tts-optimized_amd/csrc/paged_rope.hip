@@ -248,7 +248,7 @@ int rope(const RopeArgs& a, const Cache& c, const PagedBatch& bt, int d, int tab
 struct GatherArgs {
     uint16_t* k_out;
     uint16_t* v_out;
-    int T, waves;  // waves a token
+    int T, t0, t1, waves;  // tokens in all, those of the launch; waves a token
 };
 
 template <typename E, int D, typename Cache>
@@ -256,8 +256,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a, Cache c
     constexpr int LPH = D / 16, RPW = kWave / LPH;
     const int lane = threadIdx.x & (kWave - 1);
     const long long wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + threadIdx.x / kWave));
-    const int t = (int)(wave / a.waves), part = (int)(wave % a.waves);
-    if (t >= a.T) return;
+    const int t = a.t0 + (int)(wave / a.waves), part = (int)(wave % a.waves);
+    if (t >= a.t1) return;
     int at_or_before = 0;
     for (int b0 = 0; b0 < bt.B; b0 += kWave)
         at_or_before += __popcll(__ballot(b0 + lane < bt.B && bt.starts[min(b0 + lane, bt.B - 1)] <= t));
@@ -294,8 +294,13 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a, Cache c
 
 template <typename E, int D, typename Cache>
 void launch_gather(GatherArgs a, const Cache& c, const PagedBatch& bt, hipStream_t st) {
-    hipLaunchKernelGGL((paged_gather_kernel<E, D, Cache>), dim3((unsigned)(((long long)a.T * a.waves + 3) / 4)), dim3(256), 0, st,
-                       a, c, bt);
+    // a grid has fewer than 2^32 threads: all tokens, or the first of outputs of 137 GB and more
+    const int most = ((1 << 26) - 4) / a.waves;
+    for (; a.t0 < a.T; a.t0 = a.t1) {
+        a.t1 = a.T - a.t0 < most ? a.T : a.t0 + most;
+        hipLaunchKernelGGL((paged_gather_kernel<E, D, Cache>), dim3((unsigned)(((long long)(a.t1 - a.t0) * a.waves + 3) / 4)), dim3(256),
+                           0, st, a, c, bt);
+    }
 }
 
 template <typename Cache>
@@ -303,8 +308,7 @@ int gather(void* k_out, void* v_out, const Cache& c, const PagedBatch& bt, int T
     MOSS_CHECK_ARG(k_out && v_out && bt.starts && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, c.kh, d));
     MOSS_CHECK_ARG(MOSS_ALIGNED(k_out, 16) && MOSS_ALIGNED(v_out, 16) && (dtype == 0 || dtype == 1) && T > 0 && T < (1 << 24));
     const int rows = 1024 / d;  // of a wave
-    const GatherArgs a{(uint16_t*)k_out, (uint16_t*)v_out, T, (2 * c.kh + rows - 1) / rows};
-    MOSS_CHECK_ARG(((long long)T * a.waves + 3) / 4 * 256 < (1ll << 32));
+    const GatherArgs a{(uint16_t*)k_out, (uint16_t*)v_out, T, 0, 0, (2 * c.kh + rows - 1) / rows};
     if (dtype == 0)
         d == 128 ? launch_gather<Bf16, 128>(a, c, bt, st) : launch_gather<Bf16, 64>(a, c, bt, st);
     else
