@@ -3,9 +3,9 @@
 //
 // o_h = sum_t softmax_t(scale q_h . k_t) v_t over the rows t < length, as paged_decode.hip has it.  A run is neighbouring
 // sequences with the same group number (not below 0); runs end at every 64th sequence of the batch, so a wave sees
-// whole ones.  With P the rows that a run's first sequence shares (at most its length, whole 16 rows), sequence b takes
-// n_b = min(P, shared[b]), whole 16 rows, or all of its length if that is no more, from the pages of the first one, and the rest
-// from its own.  A run of one shares nothing.
+// whole ones.  Of the rows that a run's first sequence shares (at most its length, whole 16 rows), sequence b takes the first n_b =
+// shared[b], whole 16 rows, or all of its length if that is no more, from the pages of the first one, and the rest
+// from its own.  P is what the others take at most, which the first one then takes too.  A run of one shares nothing.
 //
 // The prefix: all of a run's query heads of a KV head are the rows of tiles, which go over the keys on the matrix cores
 // (paged_prompt.h), row b up to key n_b.  The rest: paged_decode.h, from row n_b on.  Both leave (m, l, O), and a last launch
@@ -53,7 +53,7 @@ struct SharedArgs {
 struct Member {
     int length, from;  // its rows, of which the first `from` are the run's
     int first, size;   // the run's lanes
-    int rows;          // P; 0 for a run of one
+    int rows;          // P; 0 for a run of one or of which nobody else takes any
     __device__ __forceinline__ int own() const { return length - from; }
 };
 
@@ -69,15 +69,20 @@ __device__ __forceinline__ Member member_of(const SharedArgs& s, const PagedBatc
     m.first = kWave - 1 - __builtin_clzll(heads & up_to);
     const unsigned long long behind = heads & ~up_to;
     m.size = (behind ? __builtin_ctzll(behind) : kWave) - m.first;
-    m.rows = m.size > 1 ? shared_rows(__shfl(want, m.first), __shfl(m.length, m.first)) : 0;
+    const int rows = m.size > 1 ? shared_rows(__shfl(want, m.first), __shfl(m.length, m.first)) : 0;
+    // what those behind the first one take of them: the largest over the run, whose first lane stands above the value, in sixteens
+    const int taken = taken_rows(m.first == lane ? 0 : shared_from(rows, want, m.length)) >> 4;
+    const uint32_t most = wave_prefix_max((uint32_t)m.first << 26 | (uint32_t)min(taken, (1 << 26) - 1));
+    m.rows = (int)(__shfl(most, m.first + m.size - 1) & ((1u << 26) - 1)) << 4;
     m.from = shared_from(m.rows, want, m.length);
     return m;
 }
 
 // Whether sharing saves enough rows to be worth the prefix's own way; if not, every sequence is taken alone.  (Rows in sixteens,
-// and no more of a run than decide by themselves, so that the sum fits 32 bits.)
+// and no more of a sequence than decide by themselves, so that the sum fits 32 bits.)  What is saved is what every sequence but
+// one takes of the prefix: the first takes all that is read.
 __device__ __forceinline__ int saved_by(const Member& m, int lane) {
-    return m.first == lane ? (m.size - 1) * min(m.rows >> 4, 1 << 14) : 0;
+    return m.first == lane ? 0 : min(m.from >> 4, 1 << 14);
 }
 template <typename At>
 __device__ __forceinline__ bool worth_sharing(const SharedArgs& s, int B, int lane, At at) {

@@ -1,4 +1,4 @@
-// Sums over a wave's lanes in lane order, of 32- and 64-bit integers.
+// Sums over a wave's lanes in lane order, of 32- and 64-bit integers, and maxima.
 #pragma once
 
 #include "common.h"
@@ -25,6 +25,16 @@ __device__ __forceinline__ V wave_prefix(V v) {
     v += dpp_before<0x118, 0xf>(v);
     v += dpp_before<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to the rows behind them
     v += dpp_before<0x143, 0xc>(v);  // lane 31 to the upper half
+    return v;
+}
+// Inclusive maximum over the wave's lanes (all of them active), of unsigned values.
+__device__ __forceinline__ uint32_t wave_prefix_max(uint32_t v) {
+    v = max(v, dpp_before<0x111, 0xf>(v));
+    v = max(v, dpp_before<0x112, 0xf>(v));
+    v = max(v, dpp_before<0x114, 0xf>(v));
+    v = max(v, dpp_before<0x118, 0xf>(v));
+    v = max(v, dpp_before<0x142, 0xa>(v));
+    v = max(v, dpp_before<0x143, 0xc>(v));
     return v;
 }
 template <typename V>
