@@ -433,8 +433,9 @@ int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, 
  * its own).
  *   tokens    NULL, or int64 / int32 (token_bytes 8 / 4) token i < lengths[row] (int32; NULL: width <= 2^30) of a row at
  *             row * token_row_stride + i * token_stride; the first prompt[row] (int32; NULL: 0) are the prompt
- *   repetition, presence, frequency  fp32 [rows], or NULL for the value behind each.  A token among the row's: x > 0 ? x /
- *             repetition : x * repetition.  Said c > 0 times behind the prompt: x - (c * frequency + presence)
+ *   repetition, presence, frequency  fp32 [rows], or NULL for the value behind each, which is finite (repetition's
+ *             positive).  A token among the row's: x > 0 ? x / repetition : x * repetition.  Said c > 0 times behind the
+ *             prompt: x - (c * frequency + presence)
  *   bias_ids, bias  NULL, or int32 and fp32 [rows, biases] (biases < 65536; rows their strides apart, 0: one for all): x + bias,
  *             of the last pair that names the entry
  *   mask      NULL, or int32 words, rows mask_stride apart (0: one for all): -inf where bit v % 32 of word v / 32 is 0
@@ -462,7 +463,7 @@ int moss_adjust_rows(const void *logits, int dtype, int rows, long long stride, 
  * contents cannot lead an access outside the cache or the packed rows.  A call whose grid would pass 2^32 - 1 threads
  * is refused: qk_rope from 2^24 tokens on, the attentions from about 2^24 (sequences + tiles of tokens) x KV heads on.
  * Outputs and workspaces must not overlap the inputs or each other; the cache's keys and values must not share memory
- * where it is written. */
+ * where it is written.  An attention's scale is finite and less than 2^127 either way. */
 
 /* q/k head RMSNorm (weights [d], or both NULL: no norm) + rotary embedding + page write of T packed tokens:
  * qkv [T, (qh + 2 kh) d] (q | k | v), T < 2^24, rows qkv_stride elements apart; cos / sin [table_rows, d] by

@@ -289,6 +289,9 @@ MOSS_API int moss_adjust_rows(const void* logits, int dtype, int rows, long long
     MOSS_CHECK_ARG(tokens || (!lengths && !prompt && !repetition && !presence && !frequency));
     MOSS_CHECK_ARG(MOSS_ALIGNED(lengths, 4) && MOSS_ALIGNED(prompt, 4) && MOSS_ALIGNED(repetition, 4) && MOSS_ALIGNED(presence, 4) &&
                    MOSS_ALIGNED(frequency, 4));
+    const bool finite = repetition_value - repetition_value == 0.f && presence_value - presence_value == 0.f &&
+                        frequency_value - frequency_value == 0.f;
+    MOSS_CHECK_ARG(!tokens || (finite && (repetition || repetition_value > 0.f)));
     MOSS_CHECK_ARG((bias_ids == nullptr) == (bias == nullptr));
     MOSS_CHECK_ARG(!bias || (biases > 0 && biases < (1 << 16) && (bias_ids_stride == 0 || bias_ids_stride >= biases) &&
                              (bias_stride == 0 || bias_stride >= biases) && MOSS_ALIGNED(bias_ids, 4) && MOSS_ALIGNED(bias, 4)));

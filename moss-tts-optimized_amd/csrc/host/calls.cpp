@@ -183,7 +183,7 @@ struct Query {
 
 bool scale_of(PyObject* o, ll d, double& v) {
     if (none(o)) return v = std::pow((double)d, -0.5), true;
-    return number(o, v);
+    return number(o, v) && std::fabs((float)v) < 0x1p127f;
 }
 
 // A new tensor.  Device memory may have to be found for it, which can take long: other Python threads run meanwhile.
@@ -476,7 +476,8 @@ PyObject* adjust(PyObject* const* v) {
             settings[i] = t.at();
             s.add(t.all());
             value = 0.0;
-        } else if (!number(v[4 + i], value) || (!history && value != (i == 0 ? 1.0 : 0.0)) || (i == 0 && !(value > 0))) {
+        } else if (!number(v[4 + i], value) || (!history && value != (i == 0 ? 1.0 : 0.0)) || (i == 0 && !((float)value > 0.f)) ||
+                   !std::isfinite((float)value)) {
             return nullptr;
         }
         values[i] = (float)value;

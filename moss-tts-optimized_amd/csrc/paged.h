@@ -123,6 +123,9 @@ static inline bool paged_pointers_ok(const PagedCache& c, const PagedBatch& b) {
            MOSS_ALIGNED(b.lengths, 4) && MOSS_ALIGNED(b.starts, 4);
 }
 
+// Finite, and still so in the base-2 domain.
+static inline bool paged_scale_ok(float scale) { return scale > -0x1p127f && scale < 0x1p127f; }
+
 // log2 of a page's rows, or -1
 static inline int page_shift(int rows) {
     for (int s = 4; s <= 12; ++s)

@@ -162,7 +162,7 @@ template <template <typename, int> class T, typename Cache>
 int decode(const void* q, long long q_stride, const Cache& c, const PagedBatch& bt, int qh, int d, float scale, void* out,
            void* workspace, long long workspace_bytes, int dtype, void* stream) {
     MOSS_CHECK_ARG(q && out && workspace && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, qh, d));
-    MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && q_stride % 8 == 0 && q_stride >= (long long)qh * d && scale == scale);
+    MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && q_stride % 8 == 0 && q_stride >= (long long)qh * d && paged_scale_ok(scale));
     MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16) && MOSS_ALIGNED(workspace, 16));
     const DecodePlan p = decode_plan(bt.B, bt.W, c.shift, qh, c.kh);
     MOSS_CHECK_ARG(workspace_bytes >= p.slots * qh * (d + 2) * 4 && p.slots * p.xdim * 256 < (1ll << 32));

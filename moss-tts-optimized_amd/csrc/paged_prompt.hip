@@ -269,7 +269,7 @@ int prompt(const void* q, long long q_stride, const Cache& c, const PagedBatch& 
            void* workspace, long long workspace_bytes, int dtype, void* stream) {
     MOSS_CHECK_ARG(q && out && bt.starts && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, qh, d));
     MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && T > 0 && T <= (1 << 20) && q_stride % 8 == 0 &&
-                   q_stride >= (long long)qh * d && scale == scale);
+                   q_stride >= (long long)qh * d && paged_scale_ok(scale));
     MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16) && MOSS_ALIGNED(workspace, 16));
     PromptPlan p = prompt_plan(bt.B, bt.W, c.shift, T, qh, c.kh, std::is_same<Cache, PagedCache8>::value ? kSmallTiles8 : kSmallTiles);
     // whole tiles' parts need up to twice the halved ones': a workspace of the 16-bit form's size serves with those

@@ -476,7 +476,7 @@ template <template <typename, int> class T, template <typename, int> class S, ty
 int shared_decode(const void* q, long long q_stride, const Cache& c, const PagedBatch& bt, const void* groups, const void* shared,
                   int qh, int d, float scale, void* out, void* workspace, long long workspace_bytes, int dtype, void* stream) {
     MOSS_CHECK_ARG(q && out && workspace && groups && shared && paged_pointers_ok(c, bt) && paged_shape_ok(c, bt, qh, d));
-    MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && q_stride % 8 == 0 && q_stride >= (long long)qh * d && scale == scale);
+    MOSS_CHECK_ARG((dtype == 0 || dtype == 1) && q_stride % 8 == 0 && q_stride >= (long long)qh * d && paged_scale_ok(scale));
     MOSS_CHECK_ARG(MOSS_ALIGNED(q, 16) && MOSS_ALIGNED(out, 16) && MOSS_ALIGNED(workspace, 16) && MOSS_ALIGNED(groups, 4) &&
                    MOSS_ALIGNED(shared, 4));
     const SharedPlan p = shared_plan(bt.B, qh, c.kh);

@@ -27,6 +27,7 @@ finite makes what it touches not finite; rows that take no part may hold anythin
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -275,7 +276,7 @@ def _scale(scale, d: int) -> float:
     if scale is None:
         return d ** -0.5
     scale = float(scale)
-    _require(scale == scale and abs(scale) != float("inf"), "scale must be finite")
+    _require(abs(ctypes.c_float(scale).value) < 2.0 ** 127, "scale must be finite (and below 2^127, in 32 bits)")
     return scale
 
 

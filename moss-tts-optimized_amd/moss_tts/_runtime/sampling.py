@@ -12,6 +12,7 @@ captured in one graph (``src/moss_tts/_runtime/first_audio_graph.py:14-29``).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -252,8 +253,9 @@ def adjust(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, lengths:
             continue
         _require(tokens is not None or (not isinstance(value, torch.Tensor) and value == none), "penalties without tokens")
         at, v = _setting(name, value, rows, torch.float32, dev)
+        v = ctypes.c_float(v).value  # what the kernel gets
         _require(at is not None or abs(v) < math.inf, "penalties must be finite")
-        settings += at, float(v)
+        settings += at, v
         if at is not None:
             spans.append((at, at + 4 * rows))
     _require(settings[0] is not None or settings[1] > 0, "repetition must be positive")
