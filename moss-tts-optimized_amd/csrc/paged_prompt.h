@@ -3,12 +3,16 @@
 //
 //   S^T = K Q^T: 32 keys x 32 rows per matrix instruction, so a lane holds one row and 16 of its keys, and the row's
 //   maximum needs one exchange with the lane 32 away; the running maximum and sum are fp32, base 2.
-//   O^T += V^T P^T: P, rounded to 16 bits, is the B operand as S^T left it.
-// P's rounding is the one step with fewer bits before the output, as in the single request's prompt attention; the sum adds
-// up the unrounded values.  (P = 2^(s scale - m) with m a rounded product: a row's largest P is 1 up to that rounding, which
-// l and O share.)  Split into two 16-bit values as the decode form has it, P adds nothing to the output's own rounding, but
-// costs half as many matrix instructions again where they are what bounds: 8000 tokens 555 -> 724 us, nine prompts 60 -> 67,
-// for an error against 64 bits of 1.65 instead of 1.88 and 1.64 instead of 1.78 10^-3 (heads of 128, bf16; fp16 an eighth).
+//   O^T += V^T P^T: P, in 16 bits, is the B operand as S^T left it.
+// The prompt form rounds P to 16 bits: the one step with fewer bits before the output, as in the single request's prompt attention;
+// the sum adds up the unrounded values.  (P = 2^(s scale - m) with m a rounded product: a row's largest P is 1 up to that rounding,
+// which l and O share.)  Split into two 16-bit values (SPLIT), as the decode form has it, P adds nothing to the output's own
+// rounding, but costs half as many matrix instructions again where they are what bounds: 8000 tokens 555 -> 724 us, from 8 bits 571
+// -> 770, nine prompts 60 -> 67, from 8 bits 54 -> 67, for an error against 64 bits of 1.65 instead of 1.88 and 1.64 instead of 1.78
+// 10^-3 (heads of 128, bf16; fp16 an eighth).  Shared prefixes split it, since they stand beside rows that the decode form takes, and
+// which rows are whose follows from the rest of the batch: 64 sequences over 4096 rows 35.0 us either way, 40 in groups over 8 bits
+// 25.4 -> 26.9, for an error of 1.66 instead of 1.75 10^-3; there each half of a tile's P is used as soon as it is formed, or its two
+// values would not fit the registers (36.5 and 27.6 us).
 // Blocks of 64 keys lie in LDS in one of two stages while the other is consumed, one barrier per block.  From a 16-bit cache
 // they go there straight from the pages (buffer loads, 16 rows of K and of V a wave, which lie in one page;
 // rows that nobody sees or that have no page are read as zeros: past the buffer's end), without registers.  From one in 8 bits
@@ -181,9 +185,10 @@ __device__ __forceinline__ int fresh_thread() {
     return tid;
 }
 
+// SPLIT: P as the sum of two 16-bit values.
 // o, m, l of the rows (l summed over the lane's keys and, on return, its partner's).  KS 2: two waves share the rows and halve a
 // block's keys; false: this wave's part went to the other.
-template <typename E, int D, int KS, typename S>
+template <typename E, int D, int KS, bool SPLIT, typename S>
 __device__ __forceinline__ bool attend_rows(const typename S::Cache& c, const TileRows& t, int W, const u32x4_t (&qf)[D / 16], float scale,
                                             int tid, Stage<D>& even, Stage<D>& odd, f32x16_v (&o_out)[D / 32], float& m_out, float& l_out) {
     constexpr int NT = 2 / KS, BK = kPromptBlock, DT = D / 32, DK = D / 16, RB = 2 * D, KB = BK * RB;  // NT: a wave's 32-key tiles
@@ -304,25 +309,32 @@ __device__ __forceinline__ bool attend_rows(const typename S::Cache& c, const Ti
         const float mr = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            u32x4_t pf[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            u32x4_t pf[2], pl[2];
+            // keys 16 u + {4 half + 0..3, 8 + 4 half + 0..3} of the tile: their P, and the K step over them
+            auto weights = [&](int u) {
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * v], scale, -mr));
                     const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * v + 1], scale, -mr));
                     l += p0 + p1;
                     pf[u][v] = E::pack(p0, p1);
+                    if constexpr (SPLIT) pl[u][v] = E::pack(p0 - E::lo(pf[u][v]), p1 - E::hi(pf[u][v]));
                 }
-            // K step u: keys 16 u + {4 half + 0..3, 8 + 4 half + 0..3} of the tile
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            };
+            auto step = [&](int u) {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const u32x2_v a0 = read_transposed(vs + vread[0][dt] + (32 * i + 16 * u) * RB);
                     const u32x2_v a1 = read_transposed(vs + vread[1][dt] + (32 * i + 16 * u) * RB);
                     o[dt] = E::mfma32(u32x4_t{a0[0], a0[1], a1[0], a1[1]}, pf[u], o[dt]);
+                    if constexpr (SPLIT) o[dt] = E::mfma32(u32x4_t{a0[0], a0[1], a1[0], a1[1]}, pl[u], o[dt]);
                 }
+            };
+            weights(0);
+            if constexpr (SPLIT) step(0);  // at once: both halves' P in two values would not fit the registers
+            weights(1);
+            if constexpr (!SPLIT) step(0);
+            step(1);
         }
         if (first + 32 * NT - 1 > wave_first) {
             // A P of 0 times a NaN or infinity in V of a key that a row does not see is a NaN all the same.

@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PromptArgs a, type
     f32x16_v o[DT];
     float m, l;
     const TileRows rows{bt.table + (size_t)f.b * bt.table_stride, kvh, b0, b1, last, qpos, wave_first, wave_last, idle};
-    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, tid, even, odd, o, m, l)) return;
+    if (!attend_rows<E, D, KS, false, S>(c, rows, bt.W, qf, a.scale, tid, even, odd, o, m, l)) return;
     // O^T element e of d tile dt: d = 32 dt + 8 (e / 4) + 4 half + e % 4
     if (cut) {
         // (starts that do not rise can name more parts than there are tokens for: they have no slot)

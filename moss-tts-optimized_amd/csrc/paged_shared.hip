@@ -8,7 +8,8 @@
 // from its own.  P is what the others take at most, which the first one then takes too.  A run of one shares nothing.
 //
 // The prefix: all of a run's query heads of a KV head are the rows of tiles, which go over the keys on the matrix cores
-// (paged_prompt.h), row b up to key n_b.  The rest: paged_decode.h, from row n_b on.  Both leave (m, l, O), and a last launch
+// (paged_prompt.h), row b up to key n_b.  The rest: paged_decode.h, from row n_b on.  Both split P into two 16-bit values, so that
+// what a sequence gets is as near to the definition whoever stands beside it; both leave (m, l, O), and a last launch
 // joins a sequence's.
 //
 // Who takes what follows from groups, shared and lengths on the device, so that a captured graph follows them.  The work of a KV
@@ -218,7 +219,7 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& s, const typename 
     rows.idle = tile * HEIGHT + 32 * rw >= nrows;
     f32x16_v o[DT];
     float mx, sum;
-    if (!attend_rows<E, D, KS, S>(c, rows, bt.W, qf, a.scale, tid, even, odd, o, mx, sum)) return;
+    if (!attend_rows<E, D, KS, true, S>(c, rows, bt.W, qf, a.scale, tid, even, odd, o, mx, sum)) return;
     const long long out = out0 + 32 * rw + rl;
     if (tile * HEIGHT + 32 * rw + rl >= nrows || out < 0 || out >= s.prefix_rows) return;
     const size_t at = (size_t)kvh * s.prefix_rows + out;

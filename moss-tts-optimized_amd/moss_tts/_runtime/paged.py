@@ -466,8 +466,8 @@ def shared_decode_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.T
     the first rows of a sequence that are those of its run's first one (at most that one's own ``shared`` and length).
     They are read through the first sequence's table, rounded down to whole 16 rows; every sequence's own table names
     its pages as well.  Both are device values like ``lengths``: whatever they hold, no access leaves the cache, and as long
-    as the tables agree on the shared rows, they change the time and not the result (beyond rounding).  A run ends at
-    every 64th sequence of the batch, and the prefix's weights are rounded to 16 bits, as :func:`prompt_attention` has them."""
+    as the tables agree on the shared rows, they change the time and not the result (beyond the last bits).  A run ends at
+    every 64th sequence of the batch."""
     if groups is not None:
         done = native.calls().decode(q, keys, values, scales, table, lengths, groups, shared, scale, out, ws)
         if done is not None:

@@ -6,6 +6,7 @@ import torch
 
 from oracle import paged as o
 from paged_helpers import cache8, values
+from shared_helpers import prefix_taken, shared_workspace
 from test_gpu_paged8 import KIND, _tables
 from test_gpu_paged_shared import _batch
 
@@ -69,11 +70,12 @@ def test_shared_past_the_cache(dev, layout, count, prefix, dtype, bits):
     want = paged.shared_decode_attention(q, keys, vals, table, lens, ids, most, scales=scales)
     (k2, v2, *s2), wide = _moved(dev, [keys, vals, *(scales or ())], table)
     s2 = tuple(s2) or None
-    got = paged.shared_decode_attention(q, k2, v2, wide, lens, ids, most, scales=s2)
+    ws = shared_workspace(q, k2, wide)
+    got = paged.shared_decode_attention(q, k2, v2, wide, lens, ids, most, scales=s2, ws=ws)
     alone = paged.decode_attention(q, keys, vals, table, lens, scales=scales)
     torch.cuda.synchronize()
-    assert torch.equal(got, want) and not torch.equal(got, alone)  # the prefix was shared: its weights are rounded
-    # either rounds its output, the prefix's weights besides
+    assert torch.equal(got, want) and prefix_taken(ws, q, keys)
+    # either rounds its output
     half = torch.finfo(dtype).eps / 2
     assert float((got.double() - alone.double()).norm() / alone.double().norm()) < 3 * half
 
