@@ -9,8 +9,9 @@
 // in fp32, rounded once to the logits' type.  Ids outside the row name nothing.
 //
 // What bounds it: the row's bytes in and out, and for few rows the chain launch, tokens, counts, logits.  128 rows of 151,936
-// bf16 logits: a copy 16 us (4.8 TB/s), with a mask 17.5, with up to 4096 tokens a row 23, all together 26; 512 rows of 1024
-// with up to 400 tokens 5.3.  A workgroup takes a chunk of a row: it asks for the row's tokens and the chunk's logits and mask
+// bf16 logits, in a graph over three inputs: a copy 14.0 us, with a mask 15.5, with up to 4096 tokens a row 21, all together 24
+// (called one after another 23); 512 rows of 1024 with up to 400 tokens 4.8 (5.1).  Long rows are 1280 workgroups for 512 places, and
+// the last chunk of each is a quarter full.  A workgroup takes a chunk of a row: it asks for the row's tokens and the chunk's logits and mask
 // bits before it waits for any of them (34 -> 30 us), counts the tokens in its range in LDS, with integers (a count, a flag, the
 // largest index of a pair), so that no order of the atomics shows, and then changes and writes its entries.  A row's
 // tokens are read once for each of its chunks, from the cache: a chunk of 16384 entries with counts of 16 bits, two

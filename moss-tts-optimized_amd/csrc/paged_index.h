@@ -139,7 +139,7 @@ MOSS_HD int shared_from(int rows, int want, int length) {
 // The rows of a run that its prefix is read for: what the sequences behind the first one take of them, `most` the largest of their
 // shared_from (whose values stay the same with these rows in place of all that the first one shares).
 MOSS_HD int taken_rows(int most) { return (most + 15) & ~15; }
-// Own rows of a unit.  32 / 64 / 128: four sequences of 700 12.3 / 11.4 / 13.6 us, 64 over 4096 shared rows 43.8 / 41.1 / 40.9.
+// Own rows of a unit.  32 / 64 / 128: four sequences of 700 11.9 / 12.4 / 14.6 us, 64 over 4096 shared rows 41.9 / 37.8 / 42.6.
 constexpr int kOwnUnit = 64;
 MOSS_HD int own_units(int rows) { return (rows + kOwnUnit - 1) / kOwnUnit; }
 // A line of work, `all` long, in `pieces` equal pieces.  Part (piece w, thing k) of what the line holds in order has the number
@@ -149,8 +149,8 @@ MOSS_HD int piece_of(long long all, int pieces) {
     return piece < 1 ? 1 : piece < (1ll << 30) ? (int)piece : 1 << 30;
 }
 // Of `workgroups` (2 at least), how many take the prefixes' blocks and not the units of own rows.
-// (3 : 2 / 2 : 1 / 3 : 1: 64 sequences over 4096 shared rows 36.3 / 40.3 / 41.1 us, 40 in five runs over 8 bits 28.4 / 27.3 / 29.5, 64 over
-// 16384 45.3 / 47.0 / 65.)
+// (1 : 1 / 3 : 2 / 2 : 1 / 3 : 1: 64 sequences over 4096 shared rows 40.5 / 37.8 / 42.1 / 41.5 us, 40 in five runs over 8 bits 28.8 / 28.9 /
+// 28.0 / 29.5, 64 over 16384 74 / 73 / 77 / 90.  One ratio for all forms: 8 bits alone would take 2 : 1.)
 constexpr float kBlockCost = 3.f, kUnitCost = 2.f;
 MOSS_HD int prefix_takers(float blocks, float units, int workgroups) {
     if (blocks <= 0.f) return 0;

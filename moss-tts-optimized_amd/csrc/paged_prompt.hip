@@ -13,8 +13,10 @@
 // A wave's part of it is in paged_prompt.h.
 // What bounds it: the matrix and vector pipes in turn at the clock that power holds (8000 tokens of 32 / 8 heads of 128:
 // 520 to 550 us, 950 to 1010 TFLOP/s, where a large product of bf16 matrices reaches 1640); with K and V through registers, V
-// transposed on the way, 667 us.  From 8 bits 571 us beside 535: the conversion of a block, once a workgroup, is 19 of 137 million
-// vector instructions (118 from 16 bits), and the matrix pipes are as busy.
+// transposed on the way, 667 us.  From 8 bits 572 us beside 539: the conversion of a block, once a workgroup, is 19 of 137 million
+// vector instructions (118 from 16 bits), and the matrix pipes are as busy; six registers of the whole tiles' kernel for heads of
+// 128 are spilled.  Heads of 64, whole tiles, have two waves a SIMD from 8 bits (174 to 187 registers) and three from 16: 8000 tokens
+// of 12 / 12 heads 149 us from 8 bits and 162 from 16, of 16 / 2 heads 197 and 192; 2500 tokens 38 and 33.
 #include "paged_prompt.h"
 
 namespace moss {
@@ -222,7 +224,8 @@ constexpr int kSmallTiles = 1024;
 // 4096 (1024), 59.2 / 59.1 for the nine prompts (700), 40.9 / 34.4 for twelve of 260 (780).
 constexpr int kSmallTiles8 = 512;
 // Parts of the whole call's work, over all KV heads, that a tile is not cut below.  128 / 256 / 512: 29 / 22 / 23 us for 150
-// tokens after 1900, 61 / 46 / 47 for 32 single tokens after 50 to 4000, 46 / 46 / 49 for the nine prompts.
+// tokens after 1900, 61 / 46 / 47 for 32 single tokens after 50 to 4000, 46 / 46 / 49 for the nine prompts.  (All from 16 bits, in
+// halved tiles.  Whole ones of the nine prompts from 8 bits are 95 parts a KV head of up to 25 blocks, where 10.5 are even.)
 constexpr int kShares = 256;
 
 PromptPlan prompt_plan(int B, int W, int shift, int T, int qh, int kh, int small_tiles) {

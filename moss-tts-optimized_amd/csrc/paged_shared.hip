@@ -19,23 +19,33 @@
 // last workgroup also writes where the join finds a sequence's parts.
 //
 // What bounds it: 64 sequences of 30 to 1500 own rows over 4096 shared ones (32 / 8 heads of 128, bf16) 35 us (decode_attention
-// 102): own rows and parts from and to memory (116 + 28 MB, 27 us at what a copy reaches) beside 0.9 us of matrix work a
-// block and CU; with a launch each for prefix and rest 59, the shares of a sequence as workgroups 50, own rows by whole
-// workgroups 41.  40 in five runs over an 8-bit cache 26 us; four over 640 rows, which are not worth sharing, 10.8.
+// 102): the own rows, 92 of the 110 MB that it reads, come by single waves with one tile on its way each, four a CU beside a
+// workgroup of the prefix's; parts are 11.6 MB, written and read again by the join (5 us).  With a launch each for prefix and rest
+// it took 59, with the shares of a sequence as workgroups 50, own rows by whole workgroups 41.  40 in five runs over an 8-bit cache
+// 26.9 us; four over 640 rows, which are not worth sharing, 10.9; sequences that share nothing about as decode_attention does (64
+// of 4 to 8 thousand rows 256 for 273, from 8 bits 148 for 158; 16 of 17 to 8000 rows 20 for 18, from 8 bits 17 for 14).  More than
+// 64 sequences, which every workgroup looks through 64 at a time: 128 over 4096 shared rows 47 us (decode_attention 190), 256 125
+// (429).
+// Registers: the instances for heads of 128 spill 2 / 16 (16 bits, tiles of 64 / 128 rows) or 18 / 34 (8 bits); those for heads of 64
+// none, and of them only the one for 16 bits (bf16) and tiles of 64 rows has three waves a SIMD.
 #include "paged_decode.h"
 #include "paged_prompt.h"
 
 namespace moss {
 namespace {
 
-// Over all KV heads: as many as there are places for.  448 / 512 / 768: 38.9 / 36.3 / 46.2 us for 64 sequences over 4096 shared rows.
+// Over all KV heads: as many as there are places for.  448 / 512 / 768: 39.8 / 37.8 / 49.9 us for 64 sequences over 4096 shared rows
+// (in a graph over three caches in turn).
 constexpr int kWorkgroups = 512;
 
 // Rows of a KV head that sharing has to save in a batch, over all KV heads.  Every sequence alone / shared, us, in this kernel: 8
 // sequences over 640 shared rows of 32 / 8 heads (35840) 13.9 / 15.4, 32 over 256 (63488) 18.8 / 18.6, 16 over 640 (76800) 18.0 /
 // 17.1, 4 over 4096 (98304) 21.6 / 21.0, 8 over 4096 (229376) 26 / 20; 16 / 1 heads, 16 over 4096 (61440) 25.5 / 28.3, 32 over
 // 4096 (126976) 31.7 / 26.2; 12 / 12 heads of 64, 8 over 640 (53760) 13.6 / 14.1, 16 over 640 (115200) 16.4 / 14.9.  What the
-// shared rows cost alone is so little because the caches serve all but the first reader.
+// shared rows cost alone is so little because the caches serve all but the first reader.  Those were small caches; from pools past
+// kCached, up to 40 in turn, with 50 own rows each: 32 / 8 heads, 8 over 640 12.4 / 13.8, 32 over 256 16.5 / 14.1, 16 over 640 17.3 /
+// 17.1, 4 over 4096 22.8 / 18.9, 8 over 4096 35 / 19; 16 / 1 heads, 16 over 4096 24.0 / 21.1; from 8 bits 16 over 640 15.5 / 16.0,
+// 4 over 4096 18.4 / 17.2, 8 over 4096 23.6 / 17.8.
 constexpr int kWorth = 65536;
 
 struct SharedArgs {
@@ -439,7 +449,7 @@ SharedPlan shared_plan(int B, int qh, int kh) {
     p.head_tiles = (int)((G + 15) / 16);
     p.workgroups = kWorkgroups / kh > 2 ? kWorkgroups / kh : 2;
     // Tiles of 64 rows, two waves to a row, while there are few.  64 / 128: 64 sequences of 32 / 8 heads over 4096 shared rows and
-    // 30 to 1500 of their own 36.3 / 41.1 us, over 16384 and one 45.4 / 43.8.
+    // 30 to 1500 of their own 37.8 / 42.8 us, over 16384 73 / 70, over 16384 and one 57.0 / 56.7.
     p.height = B * G * kh <= 4096 ? 64 : 128;
     p.slots = 4ll * p.workgroups + B;
     p.rows = B * G + (long long)p.workgroups * p.height;
