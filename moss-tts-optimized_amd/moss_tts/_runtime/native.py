@@ -17,7 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-import platform
+import sys
 import warnings
 
 import torch  # noqa: F401  (must load torch's HIP runtime first)
@@ -141,7 +141,7 @@ def lib() -> ctypes.CDLL:
 
 def calls_tag() -> str:
     """What the compiled calls are built for and depend on: this Python and this torch."""
-    return f"python {platform.python_version()} torch {torch.__version__}"
+    return f"python {sys.version_info[0]}.{sys.version_info[1]} torch {torch.__version__}"
 
 
 class _NoCalls:

@@ -66,6 +66,16 @@ def test_another_torchs(calls_at, monkeypatch):
     _refused()
 
 
+def test_a_patch_release_is_the_same_python(monkeypatch):
+    from moss_tts._runtime import native
+
+    tag = native.calls_tag()
+    monkeypatch.setattr(native.sys, "version_info", (*native.sys.version_info[:2], 99, "final", 0))
+    assert native.calls_tag() == tag
+    monkeypatch.setattr(native.sys, "version_info", (3, 99, 0, "final", 0))
+    assert native.calls_tag() != tag
+
+
 def test_this_ones(calls_at):
     from moss_tts._runtime import native
 
