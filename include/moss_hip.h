@@ -428,9 +428,9 @@ int moss_sample_rows(const void *logits, int dtype, int rows, long long stride, 
                      const void *top_p, float top_p_value, const void *min_p, float min_p_value, void *out,
                      void *workspace, long long workspace_bytes, void *stream);
 
-/* Penalties, biases and a mask on up to 2^21 rows of `vocab` <= 2^19 logits, 2^38 in all (dtype 0 bf16, 1 fp16, 2 fp32; rows `stride` /
- * `out_stride` values apart), before they are sampled: in fp32, one rounding, into out (the logits themselves, or memory of
- * its own).
+/* Penalties, biases and a mask on up to 2^21 rows of `vocab` <= 2^19 logits, 2^38 in all (dtype 0 bf16, 1 fp16, 2 fp32;
+ * rows `stride` / `out_stride` values apart), before they are sampled: in fp32, one rounding, into out (the logits
+ * themselves, or memory of its own).
  *   tokens    NULL, or int64 / int32 (token_bytes 8 / 4) token i < lengths[row] (int32; NULL: width <= 2^30) of a row at
  *             row * token_row_stride + i * token_stride; the first prompt[row] (int32; NULL: 0) are the prompt
  *   repetition, presence, frequency  fp32 [rows], or NULL for the value behind each, which is finite (repetition's
